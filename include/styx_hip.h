@@ -302,6 +302,75 @@ int styx_op_attn_decode_noalloc(styx_gpu *gpu, const float *q, const float *k, c
                                 const int32_t *page_table, int page_tokens, const int32_t *pos,
                                 float *out, int nh, int nkv, int hd, int chunk, int max_chunks,
                                 float scale);
+/* Decode attention of one new token for each sequence of a batch over one
+ * paged KV cache (no counterpart in the reference, which decodes one
+ * sequence), with the per-head q/k RMSNorm, NEOX rope and K/V append of
+ * styx_op_attn_decode, and with the attention weight of every row added to an
+ * accumulator, by which styx_op_kv_evict chooses the rows that leave. */
+typedef struct styx_kv_cache {
+    int type;          /* of the rows: STYX_F32 or STYX_F16 */
+    int n_seq;         /* sequences */
+    int nkv, hd;       /* kv heads; head_dim 64, 128 or 256 */
+    int page_tokens;   /* rows of a page, any number */
+    int n_pages;       /* pages of the pools */
+    int table_len;     /* page-table entries of a sequence */
+    void *kpool, *vpool;       /* [n_pages][page_tokens][nkv*hd], 16-byte aligned */
+    const int32_t *page_table; /* [n_seq][table_len] physical pages */
+} styx_kv_cache;
+/* Slot t of a sequence is row t % page_tokens of its page t / page_tokens;
+ * cap = table_len * page_tokens slots.  Rows in pages that are not one of the
+ * pool's (an entry outside [0, n_pages)) are neither read nor written and not
+ * attended to; no page may hold two pages' slots that are in use.
+ *
+ * Sequence b has rows in slots [0, len[b]); its new token is at position
+ * pos[b] (its rope angle, rope [n_rope][hd/2][2] from styx_rope_table) and
+ * its row goes to slot len[b].  A sequence with len[b] outside [0, cap) or
+ * pos[b] outside [0, n_rope) is skipped: nothing of it is read or written
+ * (padding).  The lengths are the caller's to advance.
+ * q [n_seq][nh*hd], k and v [n_seq][nkv*hd] f32 raw projections, q_norm and
+ * k_norm [hd] or NULL, out [n_seq][nh*hd]; nh / nkv from 1 to 16.  An f16
+ * cache holds k and v rounded once; scores, sums and outputs are f32 (a V
+ * value that is not finite makes its dimension of the outputs infinite, or,
+ * in an f16 cache, infinite or NaN).  No row seen: out is 0.
+ * acc_in / acc_out [n_seq][nkv][cap] f32: for the rows t <= len[b]
+ *   acc_out[t] = decay * acc_in[t] + sum over the kv head's query heads of
+ *                the softmax weight of row t
+ * with 0 in place of acc_in[len[b]] (a new row); slots past it stay as they
+ * are.  acc_in NULL: zeros; acc_in == acc_out is fine; both NULL: attention
+ * alone.  slot_pos [n_seq][nkv][cap] or NULL: slot len[b] gets pos[b].
+ * ws: styx_op_attn_batch_ws_bytes() bytes, 16-byte aligned, which no other
+ * call uses meanwhile (its contents need not be kept).  Allocates nothing;
+ * the lengths and positions are read on the device. */
+int styx_op_attn_decode_batch(styx_gpu *gpu, const styx_kv_cache *kv, const int32_t *len,
+                              const int32_t *pos, int nh, const float *q, const float *k,
+                              const float *v, const float *q_norm, const float *k_norm, float eps,
+                              const double *rope, int n_rope, float scale, float decay,
+                              const float *acc_in, float *acc_out, int32_t *slot_pos, float *out,
+                              void *ws, uint64_t ws_bytes);
+/* scored: with acc_out.  0: a shape that the call refuses. */
+uint64_t styx_op_attn_batch_ws_bytes(const styx_kv_cache *kv, int nh, int scored);
+/* The rows of least accumulated attention weight leave the cache (no
+ * counterpart in the reference).  For each sequence with len[b] > trigger
+ * rows (trigger >= keep), by itself for each kv head: the `keep` rows of the
+ * largest acc_in stay, before all others the rows whose position slot_pos is
+ * one of the `recent` last up to pos[b] (> pos[b] - recent) or below `sinks`;
+ * NaN counts least, ties go to the lower slot; recent + sinks <= keep.  Rows
+ * that stay in slots below keep lie still; the slots below keep that lose
+ * their row, ascending, take the rows that stay in slots at or past keep,
+ * ascending: K and V, weight and position (attention does not depend on the
+ * order of the slots).  len_out[b] = keep, and pages past it are free for
+ * the caller to hand on.  Sequences with fewer rows, and those with len[b]
+ * < 0 or > cap, keep their rows and len_out[b] = len[b].
+ * acc_out and slot_pos_out [n_seq][nkv][cap] get slots [0, len_out[b]) of
+ * every sequence (those past it stay as they are); each may be its input,
+ * and len_out may be len, else they may not overlap.  ws:
+ * styx_op_kv_evict_ws_bytes() bytes, 16-byte aligned, which no other call
+ * uses meanwhile.  Allocates nothing. */
+int styx_op_kv_evict(styx_gpu *gpu, const styx_kv_cache *kv, const int32_t *len,
+                     const int32_t *pos, int trigger, int keep, int recent, int sinks,
+                     const float *acc_in, float *acc_out, const int32_t *slot_pos_in,
+                     int32_t *slot_pos_out, int32_t *len_out, void *ws, uint64_t ws_bytes);
+uint64_t styx_op_kv_evict_ws_bytes(const styx_kv_cache *kv, int keep);
 /* Host-side NEOX rope table: out[p][i] = (cos, sin)(p * base^(-2i/hd)) in
  * f64 for p < n_pos, i < hd/2 (crates/vk-backend/tests/ops2.rs:426-442).
  * out holds n_pos * hd doubles.  Needs no GPU. */
@@ -316,6 +385,38 @@ int styx_op_gather_slabs(styx_gpu *gpu, const void *const src[3], const int64_t 
  * 64 f32 + 64 u32. */
 int styx_op_argmax(styx_gpu *gpu, const float *v, int n, uint32_t *out, float *scratch_val,
                    uint32_t *scratch_idx);
+/* The next token of each row of logits by temperature, top-k, top-p and
+ * min-p (no counterpart in the reference, which is greedy).  With T the
+ * temperature and max the row's largest logit, a word's weight is
+ * e^((x - max) / T), held in whole units of 2^-44 (so sums are exact and no
+ * result depends on an order; a word below half a unit is no candidate).
+ * Words are ordered by logit, larger first, then by index.  In this order:
+ *   top_k   > 0: only the first top_k words stay
+ *   top_p   < 1: of those the shortest run from the first whose weight is at
+ *           least top_p of theirs
+ *   min_p   > 0: of those the words of at least min_p of the largest weight
+ * and the first word always stays.  A temperature that is not above 0 takes
+ * the first word (ties: the lowest index; styx_op_argmax takes the highest);
+ * a NaN top_p or min_p is off. */
+typedef struct styx_sample_params {
+    float temperature;
+    int32_t top_k;
+    float top_p, min_p;
+} styx_sample_params;
+/* logits [rows] of n f32, `ld` floats apart (ld >= n), n up to 2^19 - 1, rows
+ * up to 65535; params on the device, n_params = rows of them or 1 for all
+ * rows; u [rows] random numbers of [0, 1).  token[r] is, with S the weight
+ * that is left, the first word at which the running sum in the order of the
+ * indices exceeds floor(u[r] S); logprob[r] (or NULL) = ln(its weight / S),
+ * n_kept[r] (or NULL) the words that are left.  A logit of NaN counts as
+ * -infinity and is never chosen; +infinity leaves only its like.  A row
+ * without a logit above -infinity: token STYX_SKIP, logprob -infinity, none
+ * left.  ws: styx_op_sample_ws_bytes() bytes, 16-byte aligned, which no other
+ * call uses meanwhile.  Allocates nothing. */
+int styx_op_sample(styx_gpu *gpu, const float *logits, int64_t ld, int rows, int n,
+                   const styx_sample_params *params, int n_params, const float *u,
+                   uint32_t *token, float *logprob, uint32_t *n_kept, void *ws, uint64_t ws_bytes);
+uint64_t styx_op_sample_ws_bytes(int rows, int n);
 /* Measurement helper with no counterpart in the reference: reads every
  * 16-byte word of [p, p + bytes) once with grid x 256 threads (each
  * workgroup a contiguous chunk, 8 non-temporal 16-byte loads in flight per

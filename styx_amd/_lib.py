@@ -75,6 +75,17 @@ class ExpertSrc(C.Structure):
     ]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("type", C.c_int), ("n_seq", C.c_int), ("nkv", C.c_int), ("hd", C.c_int),
+                ("page_tokens", C.c_int), ("n_pages", C.c_int), ("table_len", C.c_int),
+                ("kpool", C.c_void_p), ("vpool", C.c_void_p), ("page_table", C.c_void_p)]
+
+
+class SampleParams(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float),
+                ("min_p", C.c_float)]
+
+
 class KernelStat(C.Structure):
     _fields_ = [("name", C.c_char * 32), ("launches", C.c_uint64), ("total_ms", C.c_double),
                 ("bytes", C.c_double)]
@@ -155,6 +166,13 @@ _SIGS = {
     "styx_op_attn_decode_noalloc": (i32, [vp, vp, vp, vp, vp, vp, C.c_float, vp, vp, vp, vp, i32,
                                           vp, vp, i32, i32, i32, i32, i32, C.c_float]),
     "styx_op_attn_part_floats": (i64, [i32, i32, i32, i32]),
+    "styx_op_attn_decode_batch": (i32, [vp, vp, vp, vp, i32, vp, vp, vp, vp, vp, C.c_float, vp,
+                                        i32, C.c_float, C.c_float, vp, vp, vp, vp, vp, u64]),
+    "styx_op_attn_batch_ws_bytes": (u64, [vp, i32, i32]),
+    "styx_op_kv_evict": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, u64]),
+    "styx_op_kv_evict_ws_bytes": (u64, [vp, i32]),
+    "styx_op_sample": (i32, [vp, vp, i64, i32, i32, vp, i32, vp, vp, vp, vp, vp, u64]),
+    "styx_op_sample_ws_bytes": (u64, [i32, i32]),
     "styx_rope_table": (None, [C.c_float, i32, i32, vp]),
     "styx_op_read_probe": (i32, [vp, vp, i64, vp, i32]),
     "styx_residency_plan": (i32, [C.c_char_p, i32, i32, vp, i64, vp, vp]),

@@ -25,6 +25,9 @@ SOURCES = [
     "kernels_aux.hip",
     "kernels_ref.hip",
     "attn.hip",
+    "attn_batch.hip",
+    "kv_evict.hip",
+    "sample.hip",
     "moe_block.hip",
     "prompt.hip",
     "capi.cpp",

@@ -1,0 +1,89 @@
+// attn_batch.h -- what the operators on a batch's paged KV cache share: the
+// cache as the kernels see it, and the arguments of the launches
+// (attn_batch.hip, kv_evict.hip).
+#pragma once
+
+#include "common.h"
+
+namespace styx {
+
+// Quotients by the page size without a division: t / d = umulhi(2 t, mul) >> sh
+// for 0 <= t < 2^31 (sh = ceil(log2 d), mul = ceil(2^(31 + sh) / d) <= 2^32 - 1
+// but for d = 1, where mul = 2^31: the error t (mul d - 2^(31+sh)) < 2^31 d
+// <= 2^(31+sh) never carries the quotient over).
+struct PageDiv {
+    uint32_t mul;
+    int sh;
+};
+inline PageDiv page_div(uint32_t d)
+{
+    PageDiv p{0, 0};
+    while ((1ull << p.sh) < d) p.sh++;
+    p.mul = (uint32_t)(((1ull << (31 + p.sh)) + d - 1) / d);
+    return p;
+}
+
+struct KvView {
+    void *kpool, *vpool;  // [n_pages][page_tokens][nkv][hd] f32 or f16
+    const int32_t *table; // [n_seq][table_len]
+    int f16, n_seq, nkv, hd, page_tokens, n_pages, table_len;
+    int cap;              // slots of a sequence: table_len * page_tokens
+    PageDiv div;
+
+    // Row of the pools that holds slot t of sequence b, -1 where its page is
+    // not one of the pool's.
+    __device__ __forceinline__ int row(const int32_t *tab, int t) const
+    {
+        const int pg = (int)(__umulhi(2u * (uint32_t)t, div.mul) >> div.sh);
+        const int e = tab[pg];
+        return (uint32_t)e < (uint32_t)n_pages ? e * page_tokens + (t - pg * page_tokens) : -1;
+    }
+};
+
+struct AttnBatchArgs {
+    KvView kv;
+    const int32_t *len, *pos;
+    const float *q, *k, *v, *q_norm, *k_norm;
+    const double2 *rope;
+    int n_rope, nh, gqa;
+    float eps, scale, decay;
+    const float *acc_in;
+    float *acc_out;
+    int32_t *slot_pos;
+    float *out;
+    // workspace: partials of the chunks, scores of every query head
+    float *part_ml, *part_o, *score;
+    int stride;  // slots of a score row (a multiple of 64)
+    int target;  // workgroups that the rows are spread over
+    int n_merge, tiles;  // the joining launch's workgroups (filled by the launch)
+};
+
+// Sizes of the workspace's pieces in floats for a cache of this shape.
+struct AttnBatchWs {
+    int64_t chunks, ml, o, score;  // chunks: workgroups of the first launch
+    int64_t join;                  // workgroups of the second
+    int stride, target, tiles;
+};
+AttnBatchWs attn_batch_ws(int n_seq, int nkv, int hd, int cap, int gqa, bool scored);
+hipError_t launch_attn_batch(hipStream_t st, AttnBatchArgs a, float *ws);
+
+struct KvEvictArgs {
+    KvView kv;
+    const int32_t *len, *pos;
+    int trigger, keep, recent, sinks;
+    const float *acc_in;
+    float *acc_out;
+    const int32_t *pos_in;
+    int32_t *pos_out;
+    int32_t *len_out;
+    // workspace
+    int32_t *map;    // [n_seq][nkv][keep] slot whose row comes to each place
+    int32_t *holes;  // [n_seq][nkv][keep] places whose own row leaves
+    int copy_tiles;  // the moving launch's workgroups per kv head (filled by the launch)
+};
+inline uint64_t kv_evict_ws_bytes(int n_seq, int nkv, int keep) { return 8ull * n_seq * nkv * keep; }
+// Workgroups of the moving launch.
+int64_t kv_evict_grid(const KvEvictArgs &a);
+hipError_t launch_kv_evict(hipStream_t st, KvEvictArgs a, void *ws);
+
+}  // namespace styx

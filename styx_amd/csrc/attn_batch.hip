@@ -1,0 +1,687 @@
+// attn_batch.hip -- decode attention of one new token for each sequence of a
+// batch over one paged KV cache of f32 or f16 rows, which also adds every
+// row's attention weight to an accumulator (what kv_evict.hip goes by).
+//
+// Per sequence b with n = len[b] rows, new token at position p = pos[b], and
+// query head h of kv head j = h / gqa:
+//   q^ = rope_p(rmsnorm(q)), k^ = rope_p(rmsnorm(k)), rows K[n] = k^, V[n] = v
+//   s_t = scale q^ . K[t], M = max_t s_t, L = sum_t e^(s_t - M), t = 0 .. n
+//   out = sum_t e^(s_t - M) V[t] / L
+//   acc_out[j][t] = decay acc_in[j][t] + sum_{h of j} e^(s_t - M_h) / L_h
+//
+// Bound: HBM.  A row of a kv head is read once for its gqa query heads, 2 to
+// 16 flop per byte in f32 and twice that in f16, far below what the matrix
+// cores give.  All products are on the matrix cores all the same, 16 query
+// rows at a time (fewer heads are padded): they take the per-row reductions
+// away, which would cost the VALU more than the products.
+//
+// Split: a workgroup takes one chunk of one sequence's rows for one kv head.
+// The chunk length is the same for all sequences of the batch and spreads
+// their rows evenly over the chip whatever their lengths (a split by a fixed
+// count per sequence leaves a ragged batch waiting for its longest); every
+// workgroup finds its sequence from the lengths itself.  A second launch
+// merges the chunks' (M, L, o) and turns the stored scores into weights: the
+// weights need M and L of the whole context, and the scores (4 gqa bytes
+// per row) are cheaper to keep than K is to read again (up to 1024 bytes).
+#include <algorithm>
+#include <type_traits>
+
+#include "attn16.h"
+#include "attn_batch.h"
+
+namespace styx {
+
+constexpr int AB_WG = 256, AB_WAVES = AB_WG / 64;
+// Shortest chunk: one 16-row tile (f32) or two (f16) per wave.
+constexpr int AB_MIN = 64;
+// Slots per workgroup of the joining launch's weights, dims of its merges.
+constexpr int AB_WTILE = 1024, AB_DIMS = 32;
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ int wave_scan(int v)  // inclusive, over the wave
+{
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+__device__ __forceinline__ int64_t wave_total(int64_t v)
+{
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+    return v;
+}
+__device__ __forceinline__ double wave_sum64(double v)
+{
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+    return v;
+}
+
+// Rows that the new token of sequence b sees, itself among them; 0: skipped.
+__device__ __forceinline__ int rows_of(const AttnBatchArgs &a, int b)
+{
+    if (b >= a.kv.n_seq) return 0;
+    const int n = a.len[b], p = a.pos[b];
+    return n >= 0 && n < a.kv.cap && p >= 0 && p < a.n_rope ? n + 1 : 0;
+}
+
+// Rows per chunk: the batch's rows over `target` workgroups.
+__device__ __forceinline__ int chunk_rows(const AttnBatchArgs &a)
+{
+    const int lane = threadIdx.x & 63;
+    int64_t rows = 0;
+    for (int b = lane; b < a.kv.n_seq; b += 64) rows += rows_of(a, b);
+    rows = wave_total(rows) * a.kv.nkv;
+    const int64_t c = (rows + a.target - 1) / a.target;
+    return max(AB_MIN, (int)((c + 63) / 64 * 64));
+}
+
+struct ChunkAt {
+    int b, first, count, rows;  // sequence, its first chunk and their count, its rows
+};
+// The sequence of chunk `c` (BY_SEQ: of sequence `c`); count 0: there is none.
+template <bool BY_SEQ> __device__ __forceinline__ ChunkAt chunk_find(const AttnBatchArgs &a, int chunk, int c)
+{
+    const int lane = threadIdx.x & 63;
+    int base = 0;
+    for (int b0 = 0; b0 < a.kv.n_seq; b0 += 64) {
+        const int rows = rows_of(a, b0 + lane), cnt = (rows + chunk - 1) / chunk;
+        const int incl = base + wave_scan(cnt);
+        const unsigned long long hit = BY_SEQ ? (c - b0 < 64 ? 1ull << (c - b0) : 0ull) : __ballot(incl > c);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            const int n = __builtin_amdgcn_readlane(cnt, l);
+            return {b0 + l, __builtin_amdgcn_readlane(incl, l) - n, n, __builtin_amdgcn_readlane(rows, l)};
+        }
+        base = __builtin_amdgcn_readlane(incl, 63);
+    }
+    return {0, 0, 0, 0};
+}
+
+// One head's RMSNorm and rotation by a wave, in f64 to the end, so that the
+// cache's rounding of k does not depend on how a sum was ordered:
+// emit(dim, value) once per dimension.
+template <int HD, typename Emit>
+__device__ __forceinline__ void head64(const float *x, const float *w, const double2 *cs, float eps, Emit emit)
+{
+    constexpr int HALF = HD / 2, PPL = (HALF + 63) / 64;
+    const int lane = threadIdx.x & 63;
+    double x0[PPL], x1[PPL], ss = 0.0;
+#pragma unroll
+    for (int j = 0; j < PPL; j++) {
+        const int i = lane + 64 * j;
+        x0[j] = i < HALF ? (double)x[i] : 0.0;
+        x1[j] = i < HALF ? (double)x[i + HALF] : 0.0;
+        ss += x0[j] * x0[j] + x1[j] * x1[j];
+    }
+    const double f = w ? 1.0 / sqrt(wave_sum64(ss) / HD + (double)eps) : 1.0;
+#pragma unroll
+    for (int j = 0; j < PPL; j++) {
+        const int i = lane + 64 * j;
+        if (i >= HALF) continue;
+        const double2 r = cs[i];
+        const double a = w ? x0[j] * f * (double)w[i] : x0[j], b = w ? x1[j] * f * (double)w[i + HALF] : x1[j];
+        emit(i, (float)(a * r.x - b * r.y));
+        emit(i + HALF, (float)(a * r.y + b * r.x));
+    }
+}
+
+// Lane (n = lane & 15, g = lane >> 4) holds query row n.  Scores are formed
+// transposed, keys x queries, so a lane has its own query's scores of keys
+// 4 g + i of a 16-key tile: the softmax factors are lane-local, and the
+// scores already are the operand of the value product.
+template <typename T, int HD, bool WIDE> struct Tile;
+
+// f32 rows: v_mfma_f32_16x16x4_f32, 16 keys a step.  The head's dimensions
+// are permuted alike on both sides of each product, for 16-byte loads.
+template <int HD, bool WIDE> struct Tile<float, HD, WIDE> {
+    static constexpr int KEYS = 16, NS = 4, NQ = HD / 16, NV = HD / 64, QROWS = 16;
+    f4 q[NQ], kf[NQ], vf[4][NV], o[NV][4];
+
+    __device__ __forceinline__ void init(const float *qs, const float *)  // qs [16][HD + 4]
+    {
+        const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int i = 0; i < NQ; i++) q[i] = *(const f4 *)(qs + n * (HD + 4) + 16 * i + 4 * g);
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[j][e] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    __device__ __forceinline__ static int key_of(int i) { return 4 * ((threadIdx.x & 63) >> 4) + i; }
+    // row[0]: the pool row of key n
+    __device__ __forceinline__ void load_k(const float *pool, const int *row, int64_t stride)
+    {
+        const float *p = pool + max(row[0], 0) * stride + 4 * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+        for (int i = 0; i < NQ; i++) kf[i] = *(const f4 *)(p + 16 * i);
+    }
+    __device__ __forceinline__ void load_v(const float *pool, const int *row, int64_t stride)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float *p = pool + max(__shfl(row[0], key_of(i)), 0) * stride + 4 * (threadIdx.x & 15);
+#pragma unroll
+            for (int j = 0; j < NV; j++) vf[i][j] = *(const f4 *)(p + 64 * j);
+        }
+    }
+    // the new row, at key `at` of the tile, from LDS; values of keys that
+    // are not seen become 0 (their factor is 0, but 0 times an infinity that
+    // a stale row may hold is not)
+    __device__ __forceinline__ void patch_k(const float *knew, int at)
+    {
+        if ((int)(threadIdx.x & 15) != at) return;
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int i = 0; i < NQ; i++) kf[i] = *(const f4 *)(knew + 16 * i + 4 * g);
+    }
+    __device__ __forceinline__ void patch_v(const float *vnew, int at, uint32_t seen)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                if (key_of(i) == at) vf[i][j] = *(const f4 *)(vnew + 64 * j + 4 * (threadIdx.x & 15));
+                if (!((seen >> key_of(i)) & 1u)) vf[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+    }
+    __device__ __forceinline__ void scores(float (&s)[NS], float scale)
+    {
+        const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        f4 c[4];
+#pragma unroll
+        for (int i = 0; i < NQ; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                c[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[i][e], q[i][e], i ? c[e] : zero, 0, 0, 0);
+        const f4 t = (c[0] + c[1]) + (c[2] + c[3]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) s[i] = t[i] * scale;
+    }
+    __device__ __forceinline__ void values(const float (&p)[NS], float corr)
+    {
+#pragma unroll
+        for (int j = 0; j < NV; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                o[j][e] *= corr;
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    o[j][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(vf[i][j][e], p[i], o[j][e], 0, 0, 0);
+            }
+    }
+    // values 64 j + 4 (4 g + r) .. + 3 of query n, r < 4
+    __device__ __forceinline__ void put(int j, float *dst) const  // dst: 64 values of query n
+    {
+        const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            *(f4 *)(dst + 4 * (4 * g + r)) = f4{o[j][0][r], o[j][1][r], o[j][2][r], o[j][3][r]};
+    }
+};
+
+// f16 rows: v_mfma_f32_16x16x32_f16, 32 keys a step.  Queries and factors are
+// f32 values in two f16 pieces, hi + lo with |x - hi - lo| <= 2^-22 |x| (each
+// rounding is off by half a step, 2^-11, of what it rounds), so the products
+// are as exact as f32 ones; queries are brought to [2^9, 2^10) by a power of
+// two per head and factors (at most 1) to 2^10, so that the low pieces of
+// all that count are normal numbers.  With up to 8 query heads the two
+// pieces are the two halves of the 16 query rows (WIDE: two products).
+// Lane group g's keys are 4 g + i and 16 + 4 g + i on both sides of the value
+// product; its V operand, 8 keys of one dimension, is made of 16-byte pieces
+// of 8 rows by lane-local byte permutes.
+template <int HD, bool WIDE> struct Tile<_Float16, HD, WIDE> {
+    static constexpr int KEYS = 32, NS = 8, NQ = HD / 32, DPL = HD / 16, QROWS = WIDE ? 16 : 8;
+    static constexpr int NB = DPL > 8 ? DPL / 8 : 1, ND = DPL > 8 ? 4 : DPL / 2;  // 16-byte blocks, dwords of each
+    static constexpr int EB = 2 * ND;  // dims of a lane in a block
+    static constexpr float PSCALE = 1024.0f;
+    h8 q[NQ], ql[WIDE ? NQ : 1], kf[2][NQ];
+    uint32_t vf[8][NB][ND];
+    f4 o[NB][EB];
+    float qscale;
+
+    __device__ __forceinline__ void init(const float *qs, const float *qmax)
+    {
+        const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4, row = n & (QROWS - 1);
+        const float m = qmax[row];
+        const int e = m > 0.0f && m < INFINITY ? (int)((__float_as_uint(m) >> 23) & 255) - 127 : 9;
+        // 2^(9 - e), in range for every exponent: 9 - e within [-118, 136]
+        const float up = e < -100 ? ldexpf(1.0f, 109) : ldexpf(1.0f, 9 - e);
+        qscale = 1.0f / up;
+#pragma unroll
+        for (int i = 0; i < NQ; i++)
+#pragma unroll
+            for (int x = 0; x < 8; x++) {
+                const float v = qs[row * (HD + 4) + 32 * i + 8 * g + x] * up;
+                const _Float16 hi = (_Float16)v, lo = (_Float16)(v - (float)hi);
+                q[i][x] = WIDE || n < 8 ? hi : lo;
+                if constexpr (WIDE) ql[i][x] = lo;
+            }
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e2 = 0; e2 < EB; e2++) o[b][e2] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    __device__ __forceinline__ static int key_of(int i)
+    {
+        return (i & 4) * 4 + 4 * ((threadIdx.x & 63) >> 4) + (i & 3);
+    }
+    // row[0], row[1]: the pool rows of keys n and 16 + n
+    __device__ __forceinline__ void load_k(const _Float16 *pool, const int *row, int64_t stride)
+    {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const _Float16 *p = pool + max(row[t], 0) * stride + 8 * ((threadIdx.x & 63) >> 4);
+#pragma unroll
+            for (int i = 0; i < NQ; i++) kf[t][i] = *(const h8 *)(p + 32 * i);
+        }
+    }
+    __device__ __forceinline__ void load_v_row(int i, const _Float16 *p)
+    {
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            const uint32_t *s = (const uint32_t *)(p + 128 * b + EB * (threadIdx.x & 15));
+            if constexpr (ND == 4) {
+                const styx_u4 v = *(const styx_u4 *)s;
+#pragma unroll
+                for (int d = 0; d < 4; d++) vf[i][b][d] = v[d];
+            } else {
+                const styx_u2 v = *(const styx_u2 *)s;
+                vf[i][b][0] = v[0];
+                vf[i][b][1] = v[1];
+            }
+        }
+    }
+    __device__ __forceinline__ void load_v(const _Float16 *pool, const int *row, int64_t stride)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            load_v_row(i, pool + max(__shfl(row[i >> 2], key_of(i & 3)), 0) * stride);
+    }
+    __device__ __forceinline__ void patch_k(const _Float16 *knew, int at)
+    {
+        const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+            if (16 * t + n == at) {
+#pragma unroll
+                for (int i = 0; i < NQ; i++) kf[t][i] = *(const h8 *)(knew + 32 * i + 8 * g);
+            }
+    }
+    __device__ __forceinline__ void patch_v(const _Float16 *vnew, int at, uint32_t seen)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (key_of(i) == at) load_v_row(i, vnew);
+            if (!((seen >> key_of(i)) & 1u)) {
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int d = 0; d < ND; d++) vf[i][b][d] = 0;
+            }
+        }
+    }
+    __device__ __forceinline__ void scores(float (&s)[NS], float scale)
+    {
+        const f4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        scale *= qscale;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            f4 c = zero, d = zero;
+#pragma unroll
+            for (int i = 0; i < NQ; i++) {
+                c = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][i], q[i], c, 0, 0, 0);
+                if constexpr (WIDE) d = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[t][i], ql[i], d, 0, 0, 0);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                // rows n and n + 8 (row_ror:8) are the two pieces of a query
+                const float other = WIDE ? d[i] : dpp_f<0x128>(c[i]);
+                s[4 * t + i] = (c[i] + other) * scale;
+            }
+        }
+    }
+    __device__ __forceinline__ void values(const float (&p)[NS], float corr)
+    {
+        const bool low = !WIDE && (threadIdx.x & 8);
+        h8 hi, lo;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float v = p[i] * PSCALE;
+            const _Float16 h = (_Float16)v, l = (_Float16)(v - (float)h);
+            hi[i] = low ? l : h;
+            lo[i] = l;
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int e = 0; e < EB; e++) {
+                // 8 keys of dimension e: halves e & 1 of dword e / 2 of 8 rows
+                const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
+                styx_u4 w;
+#pragma unroll
+                for (int x = 0; x < 4; x++)
+                    w[x] = __builtin_amdgcn_perm(vf[2 * x + 1][b][e >> 1], vf[2 * x][b][e >> 1], sel);
+                const h8 vo = __builtin_bit_cast(h8, w);
+                o[b][e] *= corr;
+                o[b][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vo, hi, o[b][e], 0, 0, 0);
+                if constexpr (WIDE) o[b][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vo, lo, o[b][e], 0, 0, 0);
+            }
+    }
+    // values 64 j .. + 63 of query n; a lane has dims 128 b + EB (4 g + r) + e
+    __device__ __forceinline__ void put(int j, float *dst) const
+    {
+        const int g = (threadIdx.x & 63) >> 4;
+        constexpr int PER = 64 / EB;  // lanes' rows (4 g + r) that make 64 values
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int m = 4 * g + r;
+#pragma unroll
+                for (int e = 0; e < EB; e++) {
+                    float v = o[b][e][r];
+                    if constexpr (!WIDE) v += dpp_f<0x128>(v);
+                    if (128 * b / 64 + m / PER == j) dst[m % PER * EB + e] = v * (1.0f / PSCALE);
+                }
+            }
+    }
+};
+
+template <typename T, int HD, bool WIDE, bool SCORED>
+__global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
+{
+    using Tl = Tile<T, HD, WIDE>;
+    constexpr int KEYS = Tl::KEYS, NS = Tl::NS, QROWS = Tl::QROWS, NR = KEYS / 16;
+    __shared__ __align__(16) float s_q[QROWS][HD + 4];
+    __shared__ float s_qmax[QROWS];
+    __shared__ __align__(16) T s_k[HD], s_v[HD];
+    __shared__ __align__(16) float s_o[AB_WAVES][QROWS][68];
+    __shared__ float s_m[AB_WAVES][16], s_l[AB_WAVES][16];
+    const KvView &kv = a.kv;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.x % kv.nkv, cidx = blockIdx.x / kv.nkv;
+    const int chunk = chunk_rows(a);
+    const ChunkAt at = chunk_find<false>(a, chunk, cidx);
+    if (at.count == 0) return;
+    const int b = at.b, rows = at.rows, last = rows - 1;
+    const int t0 = (cidx - at.first) * chunk, t1 = min(rows, t0 + chunk);
+    const int32_t *tab = kv.table + (int64_t)b * kv.table_len;
+    const int64_t stride = (int64_t)kv.nkv * HD;
+    const T *kp = (const T *)kv.kpool + kvh * HD, *vp = (const T *)kv.vpool + kvh * HD;
+    Tl x;
+    int row[NR];  // pool rows of this lane's keys of a tile
+    auto rows_at = [&](int tb) {
+#pragma unroll
+        for (int r = 0; r < NR; r++) row[r] = kv.row(tab, min(tb + 16 * r + n, last));
+    };
+    const int step = AB_WAVES * KEYS;
+    int tb = t0 + wave * KEYS;
+    // the first tile's rows are in flight while the heads are formed
+    if (tb < t1) {
+        rows_at(tb);
+        x.load_k(kp, row, stride);
+        x.load_v(vp, row, stride);
+    }
+    const double2 *cs = a.rope + (int64_t)a.pos[b] * (HD / 2);
+    for (int h = wave; h < QROWS; h += AB_WAVES) {
+        float big = 0.0f;
+        if (h < a.gqa)
+            head64<HD>(a.q + ((int64_t)b * a.nh + kvh * a.gqa + h) * HD, a.q_norm, cs, a.eps, [&](int i, float v) {
+                s_q[h][i] = v;
+                big = fmaxf(big, fabsf(v));
+            });
+        else
+            for (int i = lane; i < HD; i += 64) s_q[h][i] = 0.0f;
+        big = wave_max(big);
+        if (lane == 0) s_qmax[h] = big;
+    }
+    const bool own = t1 == rows;  // this chunk holds the new row
+    if (own && wave == AB_WAVES - 1) {
+        const int64_t in = ((int64_t)b * kv.nkv + kvh) * HD;
+        head64<HD>(a.k + in, a.k_norm, cs, a.eps, [&](int i, float v) { s_k[i] = (T)v; });
+        for (int i = lane; i < HD; i += 64) s_v[i] = (T)a.v[in + i];
+    }
+    __syncthreads();
+    x.init(&s_q[0][0], s_qmax);
+    float m = -INFINITY, l = 0.0f;  // l: this lane group's share
+    float *score = nullptr;
+    if constexpr (SCORED)
+        score = a.score + (((int64_t)b * kv.nkv + kvh) * a.gqa + min(n, a.gqa - 1)) * a.stride;
+    for (; tb < t1; tb += step) {
+        // keys seen: of the tile's, those of the chunk whose page is there
+        uint32_t seen = 0;
+#pragma unroll
+        for (int r = 0; r < NR; r++)
+            seen |= (uint32_t)(__ballot(row[r] >= 0 && tb + 16 * r + n < t1) & 0xFFFFu) << (16 * r);
+        const bool whole = seen == (KEYS == 32 ? 0xFFFFFFFFu : 0xFFFFu) && !(own && last < tb + KEYS);
+        const int fresh = own ? last - tb : -1;
+        if (!whole) x.patch_k(s_k, fresh);
+        float s[NS], mn = m;
+        x.scores(s, a.scale);
+        const int tn = tb + step;
+        if (tn < t1) {
+            rows_at(tn);
+            x.load_k(kp, row, stride);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+                if (!((seen >> Tl::key_of(i)) & 1u)) s[i] = -INFINITY;
+            x.patch_v(s_v, fresh, seen);
+        }
+        if constexpr (SCORED) {
+            if (n < a.gqa) {
+#pragma unroll
+                for (int r = 0; r < NR; r++)
+                    *(f4 *)(score + tb + 16 * r + 4 * g) = f4{s[4 * r], s[4 * r + 1], s[4 * r + 2], s[4 * r + 3]};
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < NS; i++) mn = fmaxf(mn, s[i]);
+        mn = groups_max(mn);
+        const float mz = mn == -INFINITY ? 0.0f : mn;  // nothing seen yet
+        const float corr = expf(m - mz);
+        m = mn;
+        float lb = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            s[i] = expf(s[i] - mz);
+            lb += s[i];
+        }
+        l = l * corr + lb;
+        x.values(s, corr);
+        if (tn < t1) x.load_v(vp, row, stride);
+    }
+    // the new row goes to the pools (the tiles took it from LDS)
+    if (own && wave == 0) {
+        const int r = kv.row(tab, last);
+        if (r >= 0)
+            for (int i = lane; i < HD; i += 64) {
+                ((T *)kv.kpool)[r * stride + kvh * HD + i] = s_k[i];
+                ((T *)kv.vpool)[r * stride + kvh * HD + i] = s_v[i];
+            }
+        if (a.slot_pos && lane == 0) a.slot_pos[((int64_t)b * kv.nkv + kvh) * kv.cap + last] = a.pos[b];
+    }
+    // the waves' results of each head merged, one partial per chunk and head
+    l = groups_sum(l);
+    if (g == 0 && n < QROWS) {
+        s_m[wave][n] = m;
+        s_l[wave][n] = l;
+    }
+    const int64_t pc = (int64_t)blockIdx.x * a.gqa;
+#pragma unroll
+    for (int j = 0; j < HD / 64; j++) {
+        __syncthreads();
+        // (every lane takes part: pieces of a query come from two lanes)
+        x.put(j, s_o[wave][n & (QROWS - 1)]);
+        __syncthreads();
+        for (int i = threadIdx.x; i < a.gqa * 64; i += AB_WG) {
+            const int h = i >> 6, d = i & 63;
+            float M = s_m[0][h];
+#pragma unroll
+            for (int w = 1; w < AB_WAVES; w++) M = fmaxf(M, s_m[w][h]);
+            float L = 0.0f, O = 0.0f;
+#pragma unroll
+            for (int w = 0; w < AB_WAVES; w++) {
+                const float f = s_m[w][h] == -INFINITY ? 0.0f : expf(s_m[w][h] - M);
+                L += s_l[w][h] * f;
+                O += f == 0.0f ? 0.0f : s_o[w][h][d] * f;
+            }
+            a.part_o[(pc + h) * HD + 64 * j + d] = O;
+            if (j == 0 && d == 0) {
+                a.part_ml[2 * (pc + h)] = M;
+                a.part_ml[2 * (pc + h) + 1] = L;
+            }
+        }
+    }
+}
+
+// The chunks joined.  Workgroups below n_merge: one query head of one
+// sequence and 32 of its dimensions, half wave w taking every eighth chunk.
+// The others: 1024 slots of one kv head's weights, M and L of its heads
+// formed from the chunks' first.
+__global__ void __launch_bounds__(AB_WG) k_attn_batch_join(AttnBatchArgs a)
+{
+    __shared__ float s_o[8][AB_DIMS], s_m[16][8], s_l[16][8], s_M[16], s_R[16];
+    const KvView &kv = a.kv;
+    const int chunk = chunk_rows(a), tid = threadIdx.x;
+    if ((int)blockIdx.x < a.n_merge) {
+        const int nd = kv.hd / AB_DIMS, bh = blockIdx.x / nd, d0 = blockIdx.x % nd * AB_DIMS;
+        const int b = bh / a.nh, h = bh % a.nh, kvh = h / a.gqa, hg = h % a.gqa;
+        const ChunkAt at = chunk_find<true>(a, chunk, b);
+        if (at.count == 0) return;
+        const int part = tid >> 5, d = tid & 31;
+        float m = -INFINITY, l = 0.0f, o = 0.0f;
+        for (int c = part; c < at.count; c += 8) {
+            const int64_t p = ((int64_t)(at.first + c) * kv.nkv + kvh) * a.gqa + hg;
+            const float mc = a.part_ml[2 * p], lc = a.part_ml[2 * p + 1], oc = a.part_o[p * kv.hd + d0 + d];
+            if (mc == -INFINITY) continue;
+            const float mn = fmaxf(m, mc), fa = expf(m - mn), fb = expf(mc - mn);
+            l = l * fa + lc * fb;
+            o = o * fa + oc * fb;
+            m = mn;
+        }
+        s_o[part][d] = o;
+        if (d == 0) {
+            s_m[0][part] = m;
+            s_l[0][part] = l;
+        }
+        __syncthreads();
+        if (tid < AB_DIMS) {
+            float M = -INFINITY, L = 0.0f, O = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 8; w++) M = fmaxf(M, s_m[0][w]);
+#pragma unroll
+            for (int w = 0; w < 8; w++) {
+                const float f = s_m[0][w] == -INFINITY ? 0.0f : expf(s_m[0][w] - M);
+                L += s_l[0][w] * f;
+                O += s_o[w][tid] * f;
+            }
+            // no row seen (M = -inf): 0
+            a.out[((int64_t)b * a.nh + h) * kv.hd + d0 + tid] = M == -INFINITY ? 0.0f : O / L;
+        }
+        return;
+    }
+    const int w = blockIdx.x - a.n_merge, tile = w % a.tiles, bk = w / a.tiles;
+    const int b = bk / kv.nkv, kvh = bk % kv.nkv, t0 = tile * AB_WTILE;
+    const ChunkAt at = chunk_find<true>(a, chunk, b);
+    if (t0 >= at.rows) return;
+    // 16 heads x 16 lanes
+    {
+        const int h = tid >> 4, i = tid & 15;
+        float m = -INFINITY, l = 0.0f;
+        if (h < a.gqa)
+            for (int c = i; c < at.count; c += 16) {
+                const int64_t p = ((int64_t)(at.first + c) * kv.nkv + kvh) * a.gqa + h;
+                const float mc = a.part_ml[2 * p], lc = a.part_ml[2 * p + 1];
+                if (mc == -INFINITY) continue;
+                const float mn = fmaxf(m, mc);
+                l = l * expf(m - mn) + lc * expf(mc - mn);
+                m = mn;
+            }
+        const float M = bfly<16>(m, [](float x, float y) { return fmaxf(x, y); });
+        const float L = bfly_sum<16>(m == -INFINITY ? 0.0f : l * expf(m - M));
+        if (i == 0) {
+            s_M[h] = M;
+            s_R[h] = M == -INFINITY ? 0.0f : 1.0f / L;
+        }
+    }
+    __syncthreads();
+    const int64_t base = (int64_t)b * kv.nkv + kvh;
+    for (int t = t0 + tid; t < min(at.rows, t0 + AB_WTILE); t += AB_WG) {
+        const float *s = a.score + base * a.gqa * a.stride + t;
+        float sum = 0.0f;
+        for (int h = 0; h < a.gqa; h++) {
+            const float v = s[(int64_t)h * a.stride];
+            sum += v == -INFINITY ? 0.0f : expf(v - s_M[h]) * s_R[h];
+        }
+        const float old = a.acc_in && t < at.rows - 1 ? a.acc_in[base * kv.cap + t] : 0.0f;
+        a.acc_out[base * kv.cap + t] = a.decay * old + sum;
+    }
+}
+
+AttnBatchWs attn_batch_ws(int n_seq, int nkv, int hd, int cap, int gqa, bool scored)
+{
+    AttnBatchWs w{};
+    // two four-wave workgroups per CU
+    w.target = 512;
+    const int64_t heads = (int64_t)n_seq * nkv, most = ((int64_t)cap + AB_MIN - 1) / AB_MIN * heads;
+    // sum over sequences of ceil(rows / chunk) <= target / nkv + n_seq
+    w.chunks = std::min(most, w.target + heads);
+    w.stride = (cap + 63) / 64 * 64;
+    w.ml = (2 * w.chunks * gqa + 63) / 64 * 64;
+    w.o = w.chunks * gqa * hd;
+    w.score = scored ? heads * gqa * w.stride : 0;
+    w.tiles = scored ? (cap + AB_WTILE - 1) / AB_WTILE : 0;
+    w.join = heads * gqa * (hd / AB_DIMS) + heads * w.tiles;
+    return w;
+}
+
+template <typename T, int HD, bool WIDE>
+static void launch_ab(hipStream_t st, const AttnBatchArgs &a, int64_t grid)
+{
+    if (a.acc_out)
+        hipLaunchKernelGGL((k_attn_batch<T, HD, WIDE, true>), dim3((unsigned)grid), dim3(AB_WG), 0, st, a);
+    else
+        hipLaunchKernelGGL((k_attn_batch<T, HD, WIDE, false>), dim3((unsigned)grid), dim3(AB_WG), 0, st, a);
+}
+
+template <int HD> static void launch_ab_hd(hipStream_t st, const AttnBatchArgs &a, int64_t grid)
+{
+    if (!a.kv.f16)
+        launch_ab<float, HD, true>(st, a, grid);
+    else if (a.gqa > 8)
+        launch_ab<_Float16, HD, true>(st, a, grid);
+    else
+        launch_ab<_Float16, HD, false>(st, a, grid);
+}
+
+hipError_t launch_attn_batch(hipStream_t st, AttnBatchArgs a, float *ws)
+{
+    const KvView &kv = a.kv;
+    const AttnBatchWs w = attn_batch_ws(kv.n_seq, kv.nkv, kv.hd, kv.cap, a.gqa, a.acc_out != nullptr);
+    a.stride = w.stride;
+    a.target = w.target;
+    a.n_merge = kv.n_seq * a.nh * (kv.hd / AB_DIMS);
+    a.tiles = w.tiles;
+    a.part_ml = ws;
+    a.part_o = a.part_ml + w.ml;
+    a.score = a.part_o + w.o;
+    switch (kv.hd) {
+    case 64: launch_ab_hd<64>(st, a, w.chunks); break;
+    case 128: launch_ab_hd<128>(st, a, w.chunks); break;
+    default: launch_ab_hd<256>(st, a, w.chunks); break;
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(k_attn_batch_join, dim3((unsigned)w.join), dim3(AB_WG), 0, st, a);
+    return hipGetLastError();
+}
+
+}  // namespace styx

@@ -6,8 +6,10 @@
 #include <vector>
 #include <string>
 
+#include "attn_batch.h"
 #include "kernels.h"
 #include "runtime.h"
+#include "sample.h"
 
 namespace styx {
 
@@ -479,6 +481,177 @@ int styx_op_argmax(styx_gpu *g, const float *v, int n, uint32_t *out, float *sv,
 {
     OP_GPU(g);
     OP_RUN(launch_argmax(g->stream, v, n, out, sv, si, nullptr, 0, nullptr), "styx_op_argmax");
+    return STYX_OK;
+}
+
+// The gpu's device current for a call, whatever device the caller has current.
+struct DeviceScope {
+    int before = -1, now;
+    explicit DeviceScope(int device) : now(device)
+    {
+        if (hipGetDevice(&before) == hipSuccess && before != now) hipSetDevice(now);
+    }
+    ~DeviceScope()
+    {
+        if (before >= 0 && before != now) hipSetDevice(before);
+    }
+};
+
+// A launch's workgroups times its threads stay below 2^32.
+static constexpr int64_t MAX_WG_256 = (1 << 24) - 1;
+
+static bool kv_shape_ok(const styx_kv_cache *kv)
+{
+    return kv && (kv->type == STYX_F32 || kv->type == STYX_F16) && kv->n_seq >= 1 && kv->nkv >= 1 &&
+           (kv->hd == 64 || kv->hd == 128 || kv->hd == 256) && kv->page_tokens >= 1 && kv->n_pages >= 1 &&
+           kv->table_len >= 1 && (int64_t)kv->table_len * kv->page_tokens <= (1 << 30) &&
+           (int64_t)kv->n_pages * kv->page_tokens <= INT32_MAX && (int64_t)kv->n_seq * kv->nkv <= MAX_WG_256 / 4;
+}
+
+static int kv_view(const styx_kv_cache *kv, KvView *v, const char *who)
+{
+    if (!kv_shape_ok(kv))
+        return fail(STYX_E_INVALID, std::string(who) + ": unsupported cache type or shape");
+    if (!kv->kpool || !kv->vpool || !kv->page_table)
+        return fail(STYX_E_INVALID, std::string(who) + ": NULL pointer in the cache");
+    if (((uintptr_t)kv->kpool | (uintptr_t)kv->vpool) & 15)
+        return fail(STYX_E_INVALID, std::string(who) + ": pools must be 16-byte aligned");
+    *v = KvView{kv->kpool, kv->vpool, kv->page_table, kv->type == STYX_F16, kv->n_seq, kv->nkv, kv->hd,
+                kv->page_tokens, kv->n_pages, kv->table_len, kv->table_len * kv->page_tokens,
+                page_div((uint32_t)kv->page_tokens)};
+    return STYX_OK;
+}
+
+static int ws_ok(const void *ws, uint64_t have, uint64_t need, const char *who)
+{
+    if (!ws || have < need)
+        return fail(STYX_E_INVALID, std::string(who) + ": workspace of " + std::to_string(have) + " bytes, " +
+                                        std::to_string(need) + " needed");
+    if ((uintptr_t)ws & 15) return fail(STYX_E_INVALID, std::string(who) + ": workspace must be 16-byte aligned");
+    return STYX_OK;
+}
+
+uint64_t styx_op_attn_batch_ws_bytes(const styx_kv_cache *kv, int nh, int scored)
+{
+    if (!kv_shape_ok(kv) || nh < 1 || nh % kv->nkv || nh / kv->nkv > 16) return 0;
+    const AttnBatchWs w = attn_batch_ws(kv->n_seq, kv->nkv, kv->hd, kv->table_len * kv->page_tokens,
+                                        nh / kv->nkv, scored != 0);
+    if (w.chunks > MAX_WG_256 || w.join > MAX_WG_256) return 0;
+    return 4ull * (uint64_t)(w.ml + w.o + w.score);
+}
+
+int styx_op_attn_decode_batch(styx_gpu *g, const styx_kv_cache *kv, const int32_t *len, const int32_t *pos,
+                              int nh, const float *q, const float *k, const float *v, const float *q_norm,
+                              const float *k_norm, float eps, const double *rope, int n_rope, float scale,
+                              float decay, const float *acc_in, float *acc_out, int32_t *slot_pos, float *out,
+                              void *ws, uint64_t ws_bytes)
+{
+    const char *who = "styx_op_attn_decode_batch";
+    OP_GPU(g);
+    AttnBatchArgs a{};
+    if (int r = kv_view(kv, &a.kv, who)) return r;
+    if (nh < 1 || nh % kv->nkv || nh / kv->nkv > 16)
+        return fail(STYX_E_INVALID, std::string(who) + ": nh must be 1 to 16 times nkv");
+    if (!len || !pos || !q || !k || !v || !rope || !out || n_rope < 1)
+        return fail(STYX_E_INVALID, std::string(who) + ": NULL pointer");
+    if (acc_in && !acc_out) return fail(STYX_E_INVALID, std::string(who) + ": acc_in without acc_out");
+    const uint64_t need = styx_op_attn_batch_ws_bytes(kv, nh, acc_out != nullptr);
+    if (!need) return fail(STYX_E_INVALID, std::string(who) + ": too many sequences, heads or slots");
+    if (int r = ws_ok(ws, ws_bytes, need, who)) return r;
+    a.len = len;
+    a.pos = pos;
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.q_norm = q_norm;
+    a.k_norm = k_norm;
+    a.rope = (const double2 *)rope;
+    a.n_rope = n_rope;
+    a.nh = nh;
+    a.gqa = nh / kv->nkv;
+    a.eps = eps;
+    a.scale = scale;
+    a.decay = decay;
+    a.acc_in = acc_in;
+    a.acc_out = acc_out;
+    a.slot_pos = slot_pos;
+    a.out = out;
+    const DeviceScope on(g->device);
+    OP_RUN(launch_attn_batch(g->stream, a, (float *)ws), who);
+    return STYX_OK;
+}
+
+uint64_t styx_op_kv_evict_ws_bytes(const styx_kv_cache *kv, int keep)
+{
+    if (!kv_shape_ok(kv) || keep < 1 || keep > kv->table_len * kv->page_tokens) return 0;
+    return kv_evict_ws_bytes(kv->n_seq, kv->nkv, keep);
+}
+
+int styx_op_kv_evict(styx_gpu *g, const styx_kv_cache *kv, const int32_t *len, const int32_t *pos, int trigger,
+                     int keep, int recent, int sinks, const float *acc_in, float *acc_out,
+                     const int32_t *slot_pos_in, int32_t *slot_pos_out, int32_t *len_out, void *ws,
+                     uint64_t ws_bytes)
+{
+    const char *who = "styx_op_kv_evict";
+    OP_GPU(g);
+    KvEvictArgs a{};
+    if (int r = kv_view(kv, &a.kv, who)) return r;
+    if (keep < 1 || keep > a.kv.cap || trigger < keep)
+        return fail(STYX_E_INVALID, std::string(who) + ": keep must be 1 to cap rows and trigger at least keep");
+    if (recent < 0 || sinks < 0 || (int64_t)recent + sinks > keep)
+        return fail(STYX_E_INVALID, std::string(who) + ": recent and sinks must together be at most keep");
+    if (!len || !pos || !acc_in || !acc_out || !slot_pos_in || !slot_pos_out || !len_out)
+        return fail(STYX_E_INVALID, std::string(who) + ": NULL pointer");
+    const uint64_t need = styx_op_kv_evict_ws_bytes(kv, keep);
+    if (int r = ws_ok(ws, ws_bytes, need, who)) return r;
+    a.len = len;
+    a.pos = pos;
+    a.trigger = trigger;
+    a.keep = keep;
+    a.recent = recent;
+    a.sinks = sinks;
+    a.acc_in = acc_in;
+    a.acc_out = acc_out;
+    a.pos_in = slot_pos_in;
+    a.pos_out = slot_pos_out;
+    a.len_out = len_out;
+    if (kv_evict_grid(a) > MAX_WG_256)
+        return fail(STYX_E_INVALID, std::string(who) + ": too many sequences, heads or slots");
+    const DeviceScope on(g->device);
+    OP_RUN(launch_kv_evict(g->stream, a, ws), who);
+    return STYX_OK;
+}
+
+uint64_t styx_op_sample_ws_bytes(int rows, int n)
+{
+    if (rows < 1 || rows > 65535 || n < 1 || n > SAMPLE_MAX_N) return 0;
+    return (uint64_t)sample_ws(rows, n).bytes;
+}
+
+int styx_op_sample(styx_gpu *g, const float *logits, int64_t ld, int rows, int n,
+                   const styx_sample_params *params, int n_params, const float *u, uint32_t *token,
+                   float *logprob, uint32_t *n_kept, void *ws, uint64_t ws_bytes)
+{
+    const char *who = "styx_op_sample";
+    OP_GPU(g);
+    const uint64_t need = styx_op_sample_ws_bytes(rows, n);
+    if (!need || ld < n || (n_params != 1 && n_params != rows))
+        return fail(STYX_E_INVALID, std::string(who) + ": bad rows, n, ld or n_params");
+    if (!logits || !params || !u || !token) return fail(STYX_E_INVALID, std::string(who) + ": NULL pointer");
+    if (int r = ws_ok(ws, ws_bytes, need, who)) return r;
+    SampleArgs a{};
+    a.logits = logits;
+    a.ld = ld;
+    a.rows = rows;
+    a.n = n;
+    a.params = params;
+    a.one_params = n_params == 1;
+    a.u = u;
+    a.token = token;
+    a.logprob = logprob;
+    a.n_kept = n_kept;
+    const DeviceScope on(g->device);
+    OP_RUN(launch_sample(g->stream, a, ws), who);
     return STYX_OK;
 }
 
