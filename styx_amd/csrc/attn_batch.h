@@ -30,14 +30,18 @@ struct KvView {
     int cap;              // slots of a sequence: table_len * page_tokens
     PageDiv div;
 
-    // Row of the pools that holds slot t of sequence b, -1 where its page is
-    // not one of the pool's.
-    __device__ __forceinline__ int row(const int32_t *tab, int t) const
+    // Page-table entry of slot t, and the row of the pools that it makes: -1
+    // where the page is not one of the pool's.
+    __device__ __forceinline__ int page_of(int t) const
     {
-        const int pg = (int)(__umulhi(2u * (uint32_t)t, div.mul) >> div.sh);
-        const int e = tab[pg];
-        return (uint32_t)e < (uint32_t)n_pages ? e * page_tokens + (t - pg * page_tokens) : -1;
+        return (int)(__umulhi(2u * (uint32_t)t, div.mul) >> div.sh);
     }
+    __device__ __forceinline__ int entry(const int32_t *tab, int t) const { return tab[page_of(t)]; }
+    __device__ __forceinline__ int row_of(int e, int t) const
+    {
+        return (uint32_t)e < (uint32_t)n_pages ? e * page_tokens + (t - page_of(t) * page_tokens) : -1;
+    }
+    __device__ __forceinline__ int row(const int32_t *tab, int t) const { return row_of(entry(tab, t), t); }
 };
 
 struct AttnBatchArgs {
@@ -54,7 +58,6 @@ struct AttnBatchArgs {
     // workspace: partials of the chunks, scores of every query head
     float *part_ml, *part_o, *score;
     int stride;  // slots of a score row (a multiple of 64)
-    int target;  // workgroups that the rows are spread over
     int n_merge, tiles;  // the joining launch's workgroups (filled by the launch)
 };
 
@@ -62,7 +65,7 @@ struct AttnBatchArgs {
 struct AttnBatchWs {
     int64_t chunks, ml, o, score;  // chunks: workgroups of the first launch
     int64_t join;                  // workgroups of the second
-    int stride, target, tiles;
+    int stride, tiles;
 };
 AttnBatchWs attn_batch_ws(int n_seq, int nkv, int hd, int cap, int gqa, bool scored);
 hipError_t launch_attn_batch(hipStream_t st, AttnBatchArgs a, float *ws);

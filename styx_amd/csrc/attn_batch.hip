@@ -32,10 +32,18 @@
 namespace styx {
 
 constexpr int AB_WG = 256, AB_WAVES = AB_WG / 64;
-// Shortest chunk: one 16-row tile (f32) or two (f16) per wave.
+// Workgroups that the rows are spread over: two of four waves per CU.
+constexpr int AB_LOG_TARGET = 9;
+// Shortest chunk: one 16-row tile (f32), or half of a 32-row one, per wave.
 constexpr int AB_MIN = 64;
 // Slots per workgroup of the joining launch's weights, dims of its merges.
-constexpr int AB_WTILE = 1024, AB_DIMS = 32;
+constexpr int AB_WTILE = 512, AB_DIMS = 32;
+// Chunks whose partials a thread of the joining launch has in flight.
+constexpr int AB_BATCH = 8;
+
+// Scores are in units of ln 2 (the caller's scale times log2 e, one rounding):
+// v_exp_f32 is then the exponential, good to a unit in the last place.
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
@@ -49,17 +57,40 @@ __device__ __forceinline__ int wave_scan(int v)  // inclusive, over the wave
     }
     return v;
 }
-__device__ __forceinline__ int64_t wave_total(int64_t v)
+// Sums over the wave by lane permutes (bfly's steps, qdot.h), every lane
+// getting the result.
+template <int CTRL> __device__ __forceinline__ uint32_t dpp_u(uint32_t v)
 {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+}
+template <typename T, typename Step> __device__ __forceinline__ T wave_sum_by(T v, Step step)
+{
+    v += step(v, [](uint32_t x) { return dpp_u<0xB1>(x); });
+    v += step(v, [](uint32_t x) { return dpp_u<0x4E>(x); });
+    v += step(v, [](uint32_t x) { return dpp_u<0x141>(x); });
+    v += step(v, [](uint32_t x) { return dpp_u<0x140>(x); });
+    // the other of a pair of rows, then of halves: the two words that a swap
+    // returns are one's own and the partner's
+    v += step(v, [](uint32_t x) {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        return (threadIdx.x & 16) ? r[0] : r[1];
+    });
+    v += step(v, [](uint32_t x) {
+        const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        return (threadIdx.x & 32) ? r[0] : r[1];
+    });
     return v;
 }
 __device__ __forceinline__ double wave_sum64(double v)
 {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-    return v;
+    return wave_sum_by(v, [](double x, auto f) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, x);
+        return __builtin_bit_cast(double, (uint64_t)f((uint32_t)(u >> 32)) << 32 | f((uint32_t)u));
+    });
+}
+__device__ __forceinline__ uint32_t wave_sum_u(uint32_t v)
+{
+    return wave_sum_by(v, [](uint32_t x, auto f) { return f(x); });
 }
 
 // Rows that the new token of sequence b sees, itself among them; 0: skipped.
@@ -70,27 +101,37 @@ __device__ __forceinline__ int rows_of(const AttnBatchArgs &a, int b)
     return n >= 0 && n < a.kv.cap && p >= 0 && p < a.n_rope ? n + 1 : 0;
 }
 
-// Rows per chunk: the batch's rows over `target` workgroups.
-__device__ __forceinline__ int chunk_rows(const AttnBatchArgs &a)
+// The batch's split: the rows over 2^AB_LOG_TARGET workgroups.  `mine`: the
+// rows of sequence `lane`.
+struct RowSplit {
+    int chunk, mine;
+};
+__device__ __forceinline__ RowSplit split_rows(const AttnBatchArgs &a)
 {
-    const int lane = threadIdx.x & 63;
-    int64_t rows = 0;
-    for (int b = lane; b < a.kv.n_seq; b += 64) rows += rows_of(a, b);
-    rows = wave_total(rows) * a.kv.nkv;
-    const int64_t c = (rows + a.target - 1) / a.target;
-    return max(AB_MIN, (int)((c + 63) / 64 * 64));
+    const int lane = threadIdx.x & 63, mine = rows_of(a, lane);
+    uint64_t rows = mine;
+    for (int b = lane + 64; b < a.kv.n_seq; b += 64) rows += rows_of(a, b);
+    // (in two parts: each of 64 lanes' is below 2^26 and below 2^24 * 2^k)
+    const uint64_t all = (((uint64_t)wave_sum_u((uint32_t)(rows >> 24)) << 24) +
+                          wave_sum_u((uint32_t)rows & 0xFFFFFFu)) * a.kv.nkv;
+    const uint64_t c = (all + (1 << AB_LOG_TARGET) - 1) >> AB_LOG_TARGET;
+    return {max(AB_MIN, (int)((c + 63) / 64 * 64)), mine};
 }
 
 struct ChunkAt {
     int b, first, count, rows;  // sequence, its first chunk and their count, its rows
 };
 // The sequence of chunk `c` (BY_SEQ: of sequence `c`); count 0: there is none.
-template <bool BY_SEQ> __device__ __forceinline__ ChunkAt chunk_find(const AttnBatchArgs &a, int chunk, int c)
+template <bool BY_SEQ> __device__ __forceinline__ ChunkAt chunk_find(const AttnBatchArgs &a, const RowSplit &sp, int c)
 {
+    if (a.kv.n_seq == 1) {
+        const int rows = __builtin_amdgcn_readfirstlane(sp.mine), n = (rows + sp.chunk - 1) / sp.chunk;
+        return {0, 0, BY_SEQ || c < n ? n : 0, rows};
+    }
     const int lane = threadIdx.x & 63;
     int base = 0;
     for (int b0 = 0; b0 < a.kv.n_seq; b0 += 64) {
-        const int rows = rows_of(a, b0 + lane), cnt = (rows + chunk - 1) / chunk;
+        const int rows = b0 ? rows_of(a, b0 + lane) : sp.mine, cnt = (rows + sp.chunk - 1) / sp.chunk;
         const int incl = base + wave_scan(cnt);
         const unsigned long long hit = BY_SEQ ? (c - b0 < 64 ? 1ull << (c - b0) : 0ull) : __ballot(incl > c);
         if (hit) {
@@ -104,32 +145,45 @@ template <bool BY_SEQ> __device__ __forceinline__ ChunkAt chunk_find(const AttnB
 }
 
 // One head's RMSNorm and rotation by a wave, in f64 to the end, so that the
-// cache's rounding of k does not depend on how a sum was ordered:
-// emit(dim, value) once per dimension.
-template <int HD, typename Emit>
-__device__ __forceinline__ void head64(const float *x, const float *w, const double2 *cs, float eps, Emit emit)
-{
-    constexpr int HALF = HD / 2, PPL = (HALF + 63) / 64;
-    const int lane = threadIdx.x & 63;
-    double x0[PPL], x1[PPL], ss = 0.0;
+// cache's rounding of k does not depend on how a sum was ordered.  In two
+// phases, so that all of a wave's heads are in flight at once.  Lane l has
+// the rope pairs (i, i + HD/2), i = l + 64 j.
+template <int HD> struct HeadRow {
+    static constexpr int HALF = HD / 2, PPL = (HALF + 63) / 64;
+    float x0[PPL], x1[PPL];
+    __device__ __forceinline__ void load(const float *x)
+    {
+        const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int j = 0; j < PPL; j++) {
-        const int i = lane + 64 * j;
-        x0[j] = i < HALF ? (double)x[i] : 0.0;
-        x1[j] = i < HALF ? (double)x[i + HALF] : 0.0;
-        ss += x0[j] * x0[j] + x1[j] * x1[j];
+        for (int j = 0; j < PPL; j++) {
+            const int i = HALF < 64 ? min(lane, HALF - 1) : lane + 64 * j;
+            x0[j] = x[i];
+            x1[j] = x[i + HALF];
+        }
     }
-    const double f = w ? 1.0 / sqrt(wave_sum64(ss) / HD + (double)eps) : 1.0;
+    // emit(dim, value) once per dimension
+    template <typename Emit>
+    __device__ __forceinline__ void turn(const HeadRow &w, bool norm, const double2 *cs, float eps, Emit emit) const
+    {
+        const int lane = threadIdx.x & 63;
+        double f = 1.0;
+        if (norm) {
+            double ss = 0.0;
 #pragma unroll
-    for (int j = 0; j < PPL; j++) {
-        const int i = lane + 64 * j;
-        if (i >= HALF) continue;
-        const double2 r = cs[i];
-        const double a = w ? x0[j] * f * (double)w[i] : x0[j], b = w ? x1[j] * f * (double)w[i + HALF] : x1[j];
-        emit(i, (float)(a * r.x - b * r.y));
-        emit(i + HALF, (float)(a * r.y + b * r.x));
+            for (int j = 0; j < PPL; j++)
+                if (HALF >= 64 || lane < HALF) ss += (double)x0[j] * x0[j] + (double)x1[j] * x1[j];
+            f = 1.0 / sqrt(wave_sum64(ss) * (1.0 / HD) + (double)eps);
+        }
+#pragma unroll
+        for (int j = 0; j < PPL; j++) {
+            if (HALF < 64 && lane >= HALF) continue;
+            const int i = lane + 64 * j;
+            const double a = norm ? x0[j] * f * w.x0[j] : x0[j], b = norm ? x1[j] * f * w.x1[j] : x1[j];
+            emit(i, (float)(a * cs[j].x - b * cs[j].y));
+            emit(i + HALF, (float)(a * cs[j].y + b * cs[j].x));
+        }
     }
-}
+};
 
 // Lane (n = lane & 15, g = lane >> 4) holds query row n.  Scores are formed
 // transposed, keys x queries, so a lane has its own query's scores of keys
@@ -406,8 +460,9 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
     const KvView &kv = a.kv;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x % kv.nkv, cidx = blockIdx.x / kv.nkv;
-    const int chunk = chunk_rows(a);
-    const ChunkAt at = chunk_find<false>(a, chunk, cidx);
+    const RowSplit sp = split_rows(a);
+    const int chunk = sp.chunk;
+    const ChunkAt at = chunk_find<false>(a, sp, cidx);
     if (at.count == 0) return;
     const int b = at.b, rows = at.rows, last = rows - 1;
     const int t0 = (cidx - at.first) * chunk, t1 = min(rows, t0 + chunk);
@@ -415,37 +470,68 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
     const int64_t stride = (int64_t)kv.nkv * HD;
     const T *kp = (const T *)kv.kpool + kvh * HD, *vp = (const T *)kv.vpool + kvh * HD;
     Tl x;
-    int row[NR];  // pool rows of this lane's keys of a tile
+    // pool rows of this lane's keys of a tile: page-table entries are asked
+    // for one tile ahead of the rows, the rows one tile ahead of their use
+    int entry[NR], row[NR];
+    auto entries_at = [&](int tb) {
+#pragma unroll
+        for (int r = 0; r < NR; r++) entry[r] = kv.entry(tab, min(tb + 16 * r + n, last));
+    };
     auto rows_at = [&](int tb) {
 #pragma unroll
-        for (int r = 0; r < NR; r++) row[r] = kv.row(tab, min(tb + 16 * r + n, last));
+        for (int r = 0; r < NR; r++) row[r] = kv.row_of(entry[r], min(tb + 16 * r + n, last));
     };
     const int step = AB_WAVES * KEYS;
     int tb = t0 + wave * KEYS;
-    // the first tile's rows are in flight while the heads are formed
-    if (tb < t1) {
-        rows_at(tb);
-        x.load_k(kp, row, stride);
-        x.load_v(vp, row, stride);
+    const bool own = t1 == rows;  // this chunk holds the new row
+    // Everything that does not wait for the page table is asked for behind
+    // it: loads are counted in order, and the rows of K and V after them
+    // then do not hold up the heads.
+    entries_at(tb);
+    constexpr int PPL = HeadRow<HD>::PPL;
+    const int pos = a.pos[b];
+    double2 cs[PPL];
+    HeadRow<HD> hq[QROWS / AB_WAVES], qw, hk, kw, hv;
+#pragma unroll
+    for (int j = 0; j < PPL; j++) cs[j] = a.rope[(int64_t)pos * (HD / 2) + (HD < 128 ? lane & (HD / 2 - 1) : lane + 64 * j)];
+    const float *qb = a.q + ((int64_t)b * a.nh + kvh * a.gqa) * HD;
+#pragma unroll
+    for (int i = 0; i < QROWS / AB_WAVES; i++) hq[i].load(qb + min(wave + AB_WAVES * i, a.gqa - 1) * HD);
+    qw.load(a.q_norm ? a.q_norm : qb);
+    const int64_t in = ((int64_t)b * kv.nkv + kvh) * HD;
+    if (own && wave == AB_WAVES - 1) {
+        hk.load(a.k + in);
+        kw.load(a.k_norm ? a.k_norm : a.k + in);
+        hv.load(a.v + in);
     }
-    const double2 *cs = a.rope + (int64_t)a.pos[b] * (HD / 2);
-    for (int h = wave; h < QROWS; h += AB_WAVES) {
+    rows_at(tb);
+    x.load_k(kp, row, stride);
+    x.load_v(vp, row, stride);
+    entries_at(tb + step);
+#pragma unroll
+    for (int i = 0; i < QROWS / AB_WAVES; i++) {
+        const int h = wave + AB_WAVES * i;
         float big = 0.0f;
         if (h < a.gqa)
-            head64<HD>(a.q + ((int64_t)b * a.nh + kvh * a.gqa + h) * HD, a.q_norm, cs, a.eps, [&](int i, float v) {
-                s_q[h][i] = v;
+            hq[i].turn(qw, a.q_norm != nullptr, cs, a.eps, [&](int d, float v) {
+                s_q[h][d] = v;
                 big = fmaxf(big, fabsf(v));
             });
         else
-            for (int i = lane; i < HD; i += 64) s_q[h][i] = 0.0f;
-        big = wave_max(big);
-        if (lane == 0) s_qmax[h] = big;
+            for (int d = lane; d < HD; d += 64) s_q[h][d] = 0.0f;
+        if constexpr (!std::is_same<T, float>::value) {
+            big = wave_max(big);
+            if (lane == 0) s_qmax[h] = big;
+        }
     }
-    const bool own = t1 == rows;  // this chunk holds the new row
     if (own && wave == AB_WAVES - 1) {
-        const int64_t in = ((int64_t)b * kv.nkv + kvh) * HD;
-        head64<HD>(a.k + in, a.k_norm, cs, a.eps, [&](int i, float v) { s_k[i] = (T)v; });
-        for (int i = lane; i < HD; i += 64) s_v[i] = (T)a.v[in + i];
+        hk.turn(kw, a.k_norm != nullptr, cs, a.eps, [&](int d, float v) { s_k[d] = (T)v; });
+#pragma unroll
+        for (int j = 0; j < PPL; j++)
+            if (HD >= 128 || lane < HD / 2) {
+                s_v[lane + 64 * j] = (T)hv.x0[j];
+                s_v[lane + 64 * j + HD / 2] = (T)hv.x1[j];
+            }
     }
     __syncthreads();
     x.init(&s_q[0][0], s_qmax);
@@ -464,11 +550,12 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
         if (!whole) x.patch_k(s_k, fresh);
         float s[NS], mn = m;
         x.scores(s, a.scale);
+        // the next tile's K (issued after the last tile too, of clamped rows:
+        // every trip then issues the same loads)
         const int tn = tb + step;
-        if (tn < t1) {
-            rows_at(tn);
-            x.load_k(kp, row, stride);
-        }
+        rows_at(tn);
+        x.load_k(kp, row, stride);
+        entries_at(tn + step);
         if (!whole) {
 #pragma unroll
             for (int i = 0; i < NS; i++)
@@ -486,17 +573,17 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
         for (int i = 0; i < NS; i++) mn = fmaxf(mn, s[i]);
         mn = groups_max(mn);
         const float mz = mn == -INFINITY ? 0.0f : mn;  // nothing seen yet
-        const float corr = expf(m - mz);
+        const float corr = exp2_(m - mz);
         m = mn;
         float lb = 0.0f;
 #pragma unroll
         for (int i = 0; i < NS; i++) {
-            s[i] = expf(s[i] - mz);
+            s[i] = exp2_(s[i] - mz);
             lb += s[i];
         }
         l = l * corr + lb;
         x.values(s, corr);
-        if (tn < t1) x.load_v(vp, row, stride);
+        x.load_v(vp, row, stride);
     }
     // the new row goes to the pools (the tiles took it from LDS)
     if (own && wave == 0) {
@@ -506,7 +593,7 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
                 ((T *)kv.kpool)[r * stride + kvh * HD + i] = s_k[i];
                 ((T *)kv.vpool)[r * stride + kvh * HD + i] = s_v[i];
             }
-        if (a.slot_pos && lane == 0) a.slot_pos[((int64_t)b * kv.nkv + kvh) * kv.cap + last] = a.pos[b];
+        if (a.slot_pos && lane == 0) a.slot_pos[((int64_t)b * kv.nkv + kvh) * kv.cap + last] = pos;
     }
     // the waves' results of each head merged, one partial per chunk and head
     l = groups_sum(l);
@@ -529,7 +616,7 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
             float L = 0.0f, O = 0.0f;
 #pragma unroll
             for (int w = 0; w < AB_WAVES; w++) {
-                const float f = s_m[w][h] == -INFINITY ? 0.0f : expf(s_m[w][h] - M);
+                const float f = s_m[w][h] == -INFINITY ? 0.0f : exp2_(s_m[w][h] - M);
                 L += s_l[w][h] * f;
                 O += f == 0.0f ? 0.0f : s_o[w][h][d] * f;
             }
@@ -542,45 +629,79 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
     }
 }
 
+// Partials of every STEP-th chunk from c0 on of one head merged by a thread:
+// the loads of AB_BATCH chunks in flight at once, their maximum first, then
+// independent factors.  o: of the value at dim (null: M and L alone).
+template <int STEP, bool O>
+__device__ __forceinline__ void merge_chunks(const AttnBatchArgs &a, const ChunkAt &at, int c0, int kvh, int hg, int dim,
+                                             float &m, float &l, float &o)
+{
+    m = -INFINITY;
+    l = o = 0.0f;
+    for (int c = c0; c < at.count; c += STEP * AB_BATCH) {
+        float2 ml[AB_BATCH];
+        float oc[AB_BATCH];
+#pragma unroll
+        for (int i = 0; i < AB_BATCH; i++) {
+            const int cc = min(c + STEP * i, at.count - 1);
+            const int64_t p = ((int64_t)(at.first + cc) * a.kv.nkv + kvh) * a.gqa + hg;
+            ml[i] = ((const float2 *)a.part_ml)[p];
+            if (O) oc[i] = a.part_o[p * a.kv.hd + dim];
+        }
+        float mn = m;
+#pragma unroll
+        for (int i = 0; i < AB_BATCH; i++) {
+            if (c + STEP * i >= at.count) ml[i].x = -INFINITY;
+            mn = fmaxf(mn, ml[i].x);
+        }
+        if (mn == -INFINITY) continue;  // nothing seen in these
+        const float fa = exp2_(m - mn);
+        l *= fa;
+        o *= fa;
+#pragma unroll
+        for (int i = 0; i < AB_BATCH; i++) {
+            if (ml[i].x == -INFINITY) continue;
+            const float f = exp2_(ml[i].x - mn);
+            l += ml[i].y * f;
+            if (O) o += oc[i] * f;
+        }
+        m = mn;
+    }
+}
+
 // The chunks joined.  Workgroups below n_merge: one query head of one
-// sequence and 32 of its dimensions, half wave w taking every eighth chunk.
-// The others: 1024 slots of one kv head's weights, M and L of its heads
-// formed from the chunks' first.
+// sequence and 32 of its dimensions, a half wave taking every eighth chunk.
+// The others: AB_WTILE slots of one kv head's weights, M and L of its heads
+// formed from the chunks' first (16 lanes a head), the scores in flight
+// meanwhile.
 __global__ void __launch_bounds__(AB_WG) k_attn_batch_join(AttnBatchArgs a)
 {
-    __shared__ float s_o[8][AB_DIMS], s_m[16][8], s_l[16][8], s_M[16], s_R[16];
+    __shared__ float s_o[8][AB_DIMS], s_m[8], s_l[8], s_M[16], s_R[16];
     const KvView &kv = a.kv;
-    const int chunk = chunk_rows(a), tid = threadIdx.x;
+    const int tid = threadIdx.x;
+    const RowSplit sp = split_rows(a);
     if ((int)blockIdx.x < a.n_merge) {
         const int nd = kv.hd / AB_DIMS, bh = blockIdx.x / nd, d0 = blockIdx.x % nd * AB_DIMS;
         const int b = bh / a.nh, h = bh % a.nh, kvh = h / a.gqa, hg = h % a.gqa;
-        const ChunkAt at = chunk_find<true>(a, chunk, b);
+        const ChunkAt at = chunk_find<true>(a, sp, b);
         if (at.count == 0) return;
         const int part = tid >> 5, d = tid & 31;
-        float m = -INFINITY, l = 0.0f, o = 0.0f;
-        for (int c = part; c < at.count; c += 8) {
-            const int64_t p = ((int64_t)(at.first + c) * kv.nkv + kvh) * a.gqa + hg;
-            const float mc = a.part_ml[2 * p], lc = a.part_ml[2 * p + 1], oc = a.part_o[p * kv.hd + d0 + d];
-            if (mc == -INFINITY) continue;
-            const float mn = fmaxf(m, mc), fa = expf(m - mn), fb = expf(mc - mn);
-            l = l * fa + lc * fb;
-            o = o * fa + oc * fb;
-            m = mn;
-        }
+        float m, l, o;
+        merge_chunks<8, true>(a, at, part, kvh, hg, d0 + d, m, l, o);
         s_o[part][d] = o;
         if (d == 0) {
-            s_m[0][part] = m;
-            s_l[0][part] = l;
+            s_m[part] = m;
+            s_l[part] = l;
         }
         __syncthreads();
         if (tid < AB_DIMS) {
             float M = -INFINITY, L = 0.0f, O = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 8; w++) M = fmaxf(M, s_m[0][w]);
+            for (int w = 0; w < 8; w++) M = fmaxf(M, s_m[w]);
 #pragma unroll
             for (int w = 0; w < 8; w++) {
-                const float f = s_m[0][w] == -INFINITY ? 0.0f : expf(s_m[0][w] - M);
-                L += s_l[0][w] * f;
+                const float f = s_m[w] == -INFINITY ? 0.0f : exp2_(s_m[w] - M);
+                L += s_l[w] * f;
                 O += s_o[w][tid] * f;
             }
             // no row seen (M = -inf): 0
@@ -590,50 +711,48 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch_join(AttnBatchArgs a)
     }
     const int w = blockIdx.x - a.n_merge, tile = w % a.tiles, bk = w / a.tiles;
     const int b = bk / kv.nkv, kvh = bk % kv.nkv, t0 = tile * AB_WTILE;
-    const ChunkAt at = chunk_find<true>(a, chunk, b);
+    const ChunkAt at = chunk_find<true>(a, sp, b);
     if (t0 >= at.rows) return;
-    // 16 heads x 16 lanes
+    constexpr int PER = AB_WTILE / AB_WG;
+    const int64_t base = (int64_t)b * kv.nkv + kvh;
+    const float *sc = a.score + base * a.gqa * a.stride;
+    float s[PER][16], old[PER];
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        const int t = min(t0 + tid + AB_WG * j, at.rows - 1);
+#pragma unroll
+        for (int h = 0; h < 16; h++) s[j][h] = h < a.gqa ? sc[(int64_t)h * a.stride + t] : -INFINITY;
+        old[j] = a.acc_in && t < at.rows - 1 ? a.acc_in[base * kv.cap + t] : 0.0f;
+    }
     {
-        const int h = tid >> 4, i = tid & 15;
-        float m = -INFINITY, l = 0.0f;
-        if (h < a.gqa)
-            for (int c = i; c < at.count; c += 16) {
-                const int64_t p = ((int64_t)(at.first + c) * kv.nkv + kvh) * a.gqa + h;
-                const float mc = a.part_ml[2 * p], lc = a.part_ml[2 * p + 1];
-                if (mc == -INFINITY) continue;
-                const float mn = fmaxf(m, mc);
-                l = l * expf(m - mn) + lc * expf(mc - mn);
-                m = mn;
-            }
+        const int h = tid >> 4;
+        float m = -INFINITY, l = 0.0f, o;
+        if (h < a.gqa) merge_chunks<16, false>(a, at, tid & 15, kvh, h, 0, m, l, o);
         const float M = bfly<16>(m, [](float x, float y) { return fmaxf(x, y); });
-        const float L = bfly_sum<16>(m == -INFINITY ? 0.0f : l * expf(m - M));
-        if (i == 0) {
-            s_M[h] = M;
+        const float L = bfly_sum<16>(m == -INFINITY ? 0.0f : l * exp2_(m - M));
+        if ((tid & 15) == 0) {
+            s_M[h] = M == -INFINITY ? 0.0f : M;
             s_R[h] = M == -INFINITY ? 0.0f : 1.0f / L;
         }
     }
     __syncthreads();
-    const int64_t base = (int64_t)b * kv.nkv + kvh;
-    for (int t = t0 + tid; t < min(at.rows, t0 + AB_WTILE); t += AB_WG) {
-        const float *s = a.score + base * a.gqa * a.stride + t;
+#pragma unroll
+    for (int j = 0; j < PER; j++) {
+        const int t = t0 + tid + AB_WG * j;
         float sum = 0.0f;
-        for (int h = 0; h < a.gqa; h++) {
-            const float v = s[(int64_t)h * a.stride];
-            sum += v == -INFINITY ? 0.0f : expf(v - s_M[h]) * s_R[h];
-        }
-        const float old = a.acc_in && t < at.rows - 1 ? a.acc_in[base * kv.cap + t] : 0.0f;
-        a.acc_out[base * kv.cap + t] = a.decay * old + sum;
+#pragma unroll
+        for (int h = 0; h < 16; h++)
+            if (h < a.gqa) sum += exp2_(s[j][h] - s_M[h]) * s_R[h];
+        if (t < at.rows) a.acc_out[base * kv.cap + t] = a.decay * old[j] + sum;
     }
 }
 
 AttnBatchWs attn_batch_ws(int n_seq, int nkv, int hd, int cap, int gqa, bool scored)
 {
     AttnBatchWs w{};
-    // two four-wave workgroups per CU
-    w.target = 512;
     const int64_t heads = (int64_t)n_seq * nkv, most = ((int64_t)cap + AB_MIN - 1) / AB_MIN * heads;
-    // sum over sequences of ceil(rows / chunk) <= target / nkv + n_seq
-    w.chunks = std::min(most, w.target + heads);
+    // sum over sequences of ceil(rows / chunk) <= 2^AB_LOG_TARGET / nkv + n_seq
+    w.chunks = std::min(most, (1 << AB_LOG_TARGET) + heads);
     w.stride = (cap + 63) / 64 * 64;
     w.ml = (2 * w.chunks * gqa + 63) / 64 * 64;
     w.o = w.chunks * gqa * hd;
@@ -667,7 +786,7 @@ hipError_t launch_attn_batch(hipStream_t st, AttnBatchArgs a, float *ws)
     const KvView &kv = a.kv;
     const AttnBatchWs w = attn_batch_ws(kv.n_seq, kv.nkv, kv.hd, kv.cap, a.gqa, a.acc_out != nullptr);
     a.stride = w.stride;
-    a.target = w.target;
+    a.scale = (float)((double)a.scale * 1.4426950408889634);  // log2 e
     a.n_merge = kv.n_seq * a.nh * (kv.hd / AB_DIMS);
     a.tiles = w.tiles;
     a.part_ml = ws;
