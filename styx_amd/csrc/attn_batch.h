@@ -55,17 +55,18 @@ struct AttnBatchArgs {
     float *acc_out;
     int32_t *slot_pos;
     float *out;
-    // workspace: partials of the chunks, scores of every query head
+    // workspace: partials of the pieces, scores of every query head, the split
     float *part_ml, *part_o, *score;
+    uint32_t *plan;
     int stride;  // slots of a score row (a multiple of 64)
     int n_merge, tiles;  // the joining launch's workgroups (filled by the launch)
 };
 
 // Sizes of the workspace's pieces in floats for a cache of this shape.
 struct AttnBatchWs {
-    int64_t chunks, ml, o, score;  // chunks: workgroups of the first launch
-    int64_t join;                  // workgroups of the second
-    int stride, tiles;
+    int64_t ml, o, plan, score;
+    int64_t units, grid, join;  // units of rows at most, workgroups of the two launches
+    int stride, tiles, dims;
 };
 AttnBatchWs attn_batch_ws(int n_seq, int nkv, int hd, int cap, int gqa, bool scored);
 hipError_t launch_attn_batch(hipStream_t st, AttnBatchArgs a, float *ws);

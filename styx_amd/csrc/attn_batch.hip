@@ -15,14 +15,15 @@
 // rows at a time (fewer heads are padded): they take the per-row reductions
 // away, which would cost the VALU more than the products.
 //
-// Split: a workgroup takes one chunk of one sequence's rows for one kv head.
-// The chunk length is the same for all sequences of the batch and spreads
-// their rows evenly over the chip whatever their lengths (a split by a fixed
-// count per sequence leaves a ragged batch waiting for its longest); every
-// workgroup finds its sequence from the lengths itself.  A second launch
-// merges the chunks' (M, L, o) and turns the stored scores into weights: the
-// weights need M and L of the whole context, and the scores (4 gqa bytes
-// per row) are cheaper to keep than K is to read again (up to 1024 bytes).
+// Split: the rows of all sequences and kv heads, in units of 64, lie one
+// after another and every workgroup takes the same number of them, as many
+// workgroups as run at once: a ragged batch keeps the whole chip busy to the
+// end, where a split by sequence waits for the longest, or for the rounds of
+// a grid that does not fit.  A workgroup's share may end one (sequence, head)
+// and go on with the next; each such piece is a partial result (M, L, o).
+// A second launch merges the pieces and turns the stored scores into
+// weights: these need M and L of the whole context, and the scores (4 gqa
+// bytes per row) are cheaper to keep than K is to read again (up to 1024).
 #include <algorithm>
 #include <type_traits>
 
@@ -32,13 +33,15 @@
 namespace styx {
 
 constexpr int AB_WG = 256, AB_WAVES = AB_WG / 64;
-// Workgroups that the rows are spread over: two of four waves per CU.
-constexpr int AB_LOG_TARGET = 9;
-// Shortest chunk: one 16-row tile (f32), or half of a 32-row one, per wave.
-constexpr int AB_MIN = 64;
-// Slots per workgroup of the joining launch's weights, dims of its merges.
-constexpr int AB_WTILE = 512, AB_DIMS = 32;
-// Chunks whose partials a thread of the joining launch has in flight.
+// Workgroups of a 256-CU chip that run at once: by their registers (about
+// 148, 232 and 371 per lane), three, two and one of four waves per CU.
+__host__ __device__ constexpr int ab_slots(int hd) { return hd == 64 ? 768 : hd == 128 ? 512 : 256; }
+// Rows of a unit: a 16-row tile (f32), or half of a 32-row one, per wave.
+constexpr int AB_UNIT = 64;
+// Slots of a step of the joining launch's weights: 8 of a thread's in flight
+// with up to 4 query heads per kv head, 2 with more.
+__host__ __device__ constexpr int ab_wper(int gqa) { return gqa <= 4 ? 8 : 2; }
+// Pieces whose partials a thread of the joining launch has in flight.
 constexpr int AB_BATCH = 8;
 
 // Scores are in units of ln 2 (the caller's scale times log2 e, one rounding):
@@ -101,47 +104,124 @@ __device__ __forceinline__ int rows_of(const AttnBatchArgs &a, int b)
     return n >= 0 && n < a.kv.cap && p >= 0 && p < a.n_rope ? n + 1 : 0;
 }
 
-// The batch's split: the rows over 2^AB_LOG_TARGET workgroups.  `mine`: the
-// rows of sequence `lane`.
+// The batch's split.  Unit u of the batch belongs to workgroup u / share.
+// A share that ends one head and begins another costs its workgroup a second
+// start and end, about 10 us on a busy chip; where a slightly larger share
+// does without, every head is padded to whole shares (24 ragged f16
+// conversations, 8 units instead of 7: 25 us against 36; six f32 documents,
+// 10 instead of 9: 62 against 68).  It does not pay where the heads are too
+// many for the workgroups (40 sequences of 8 heads, 45 units instead of 27:
+// 105 us against 81).  AB_MORE: units of a share that cost about as much as
+// a second start.
+// `mine`, `upto`: rows of sequence `lane` and units of the sequences up to it.
+constexpr int AB_MORE_F16 = 3, AB_MORE_F32 = 1;
 struct RowSplit {
-    int chunk, mine;
+    uint32_t units, share, upto;
+    int mine, padded;
 };
+__device__ __forceinline__ uint32_t head_units(const RowSplit &sp, int rows)
+{
+    const uint32_t u = (uint32_t)(rows + AB_UNIT - 1) / AB_UNIT;
+    return sp.padded ? (u + sp.share - 1) / sp.share * sp.share : u;
+}
 __device__ __forceinline__ RowSplit split_rows(const AttnBatchArgs &a)
 {
-    const int lane = threadIdx.x & 63, mine = rows_of(a, lane);
-    uint64_t rows = mine;
-    for (int b = lane + 64; b < a.kv.n_seq; b += 64) rows += rows_of(a, b);
-    // (in two parts: each of 64 lanes' is below 2^26 and below 2^24 * 2^k)
-    const uint64_t all = (((uint64_t)wave_sum_u((uint32_t)(rows >> 24)) << 24) +
-                          wave_sum_u((uint32_t)rows & 0xFFFFFFu)) * a.kv.nkv;
-    const uint64_t c = (all + (1 << AB_LOG_TARGET) - 1) >> AB_LOG_TARGET;
-    return {max(AB_MIN, (int)((c + 63) / 64 * 64)), mine};
+    const int lane = threadIdx.x & 63;
+    const uint32_t nkv = a.kv.nkv, slots = ab_slots(a.kv.hd);
+    RowSplit sp;
+    sp.padded = 0;
+    sp.mine = rows_of(a, lane);
+    if (a.kv.n_seq == 1) {
+        sp.mine = __builtin_amdgcn_readfirstlane(sp.mine);
+        const uint32_t u = (uint32_t)(sp.mine + AB_UNIT - 1) / AB_UNIT;
+        // whole shares for every head, if there are workgroups for the heads
+        sp.padded = nkv <= slots;
+        sp.share = sp.padded ? (u + slots / nkv - 1) / (slots / nkv) : (u * nkv + slots - 1) / slots;
+        sp.share += sp.share == 0;
+        sp.units = sp.upto = head_units(sp, sp.mine) * nkv;
+        return sp;
+    }
+    const uint32_t u = head_units(sp, sp.mine);
+    uint32_t all = u, seqs = sp.mine > 0;
+    for (int b = lane + 64; b < a.kv.n_seq; b += 64) {
+        const int r = rows_of(a, b);
+        all += head_units(sp, r);
+        seqs += r > 0;
+    }
+    all = wave_sum_u(all) * nkv;
+    const uint32_t heads = wave_sum_u(seqs) * nkv, least = (all + slots - 1) / slots;
+    sp.share = least + (least == 0);
+    if (heads < slots) {
+        // at most all / share and one for every head
+        const uint32_t most = (all + slots - heads - 1) / (slots - heads);
+        uint32_t at = most;
+        if (a.kv.n_seq <= 64)
+            for (at = sp.share; at < most && wave_sum_u((u + at - 1) / at) * nkv > slots; at++)
+                ;
+        if (at <= least + (a.kv.f16 ? AB_MORE_F16 : AB_MORE_F32)) {
+            sp.padded = 1;
+            sp.share = at;
+        }
+    }
+    sp.upto = wave_scan(head_units(sp, sp.mine) * nkv);
+    sp.units = __builtin_amdgcn_readlane(sp.upto, 63);
+    if (a.kv.n_seq > 64) {
+        uint32_t more = 0;
+        for (int b = lane + 64; b < a.kv.n_seq; b += 64) more += head_units(sp, rows_of(a, b)) * nkv;
+        sp.units += wave_sum_u(more);
+    }
+    return sp;
 }
 
-struct ChunkAt {
-    int b, first, count, rows;  // sequence, its first chunk and their count, its rows
+// A sequence, its rows, and the unit at which its first kv head begins.
+struct SeqAt {
+    int b, rows;
+    uint32_t first;
 };
-// The sequence of chunk `c` (BY_SEQ: of sequence `c`); count 0: there is none.
-template <bool BY_SEQ> __device__ __forceinline__ ChunkAt chunk_find(const AttnBatchArgs &a, const RowSplit &sp, int c)
+// The sequence of unit u.
+__device__ __forceinline__ SeqAt seq_find(const AttnBatchArgs &a, const RowSplit &sp, uint32_t u)
 {
-    if (a.kv.n_seq == 1) {
-        const int rows = __builtin_amdgcn_readfirstlane(sp.mine), n = (rows + sp.chunk - 1) / sp.chunk;
-        return {0, 0, BY_SEQ || c < n ? n : 0, rows};
-    }
+    if (a.kv.n_seq == 1) return {0, sp.mine, 0};
     const int lane = threadIdx.x & 63;
-    int base = 0;
-    for (int b0 = 0; b0 < a.kv.n_seq; b0 += 64) {
-        const int rows = b0 ? rows_of(a, b0 + lane) : sp.mine, cnt = (rows + sp.chunk - 1) / sp.chunk;
-        const int incl = base + wave_scan(cnt);
-        const unsigned long long hit = BY_SEQ ? (c - b0 < 64 ? 1ull << (c - b0) : 0ull) : __ballot(incl > c);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            const int n = __builtin_amdgcn_readlane(cnt, l);
-            return {b0 + l, __builtin_amdgcn_readlane(incl, l) - n, n, __builtin_amdgcn_readlane(rows, l)};
+    uint32_t base = 0;
+    for (int b0 = 0;; b0 += 64) {
+        const int rows = b0 ? rows_of(a, b0 + lane) : sp.mine;
+        const uint32_t upto = b0 ? base + wave_scan(head_units(sp, rows) * a.kv.nkv) : sp.upto;
+        if (const unsigned long long hit = __ballot(upto > u)) {
+            const int l = __builtin_ctzll(hit), r = __builtin_amdgcn_readlane(rows, l);
+            return {b0 + l, r, __builtin_amdgcn_readlane(upto, l) - head_units(sp, r) * a.kv.nkv};
         }
-        base = __builtin_amdgcn_readlane(incl, 63);
+        base = __builtin_amdgcn_readlane(upto, 63);
     }
-    return {0, 0, 0, 0};
+}
+
+// The split for the joining launch, by one wave: a.plan = {share, padded,
+// first unit of every sequence}.
+__device__ __forceinline__ void split_store(const AttnBatchArgs &a, const RowSplit &sp)
+{
+    const int lane = threadIdx.x & 63;
+    if (lane == 0) {
+        a.plan[0] = sp.share;
+        a.plan[1] = sp.padded;
+    }
+    if (a.kv.n_seq == 1) {
+        if (lane == 0) a.plan[2] = 0;
+        return;
+    }
+    uint32_t base = 0;
+    for (int b0 = 0; b0 < a.kv.n_seq; b0 += 64) {
+        const int rows = b0 ? rows_of(a, b0 + lane) : sp.mine;
+        const uint32_t mine = head_units(sp, rows) * a.kv.nkv;
+        const uint32_t upto = b0 ? base + wave_scan(mine) : sp.upto;
+        if (b0 + lane < a.kv.n_seq) a.plan[2 + b0 + lane] = upto - mine;
+        base = __builtin_amdgcn_readlane(upto, 63);
+    }
+}
+__device__ __forceinline__ SeqAt seq_load(const AttnBatchArgs &a, RowSplit &sp, int b)
+{
+    sp.share = a.plan[0];
+    sp.padded = (int)a.plan[1];
+    return {b, rows_of(a, b), a.plan[2 + b]};
 }
 
 // One head's RMSNorm and rotation by a wave, in f64 to the end, so that the
@@ -151,9 +231,8 @@ template <bool BY_SEQ> __device__ __forceinline__ ChunkAt chunk_find(const AttnB
 template <int HD> struct HeadRow {
     static constexpr int HALF = HD / 2, PPL = (HALF + 63) / 64;
     float x0[PPL], x1[PPL];
-    __device__ __forceinline__ void load(const float *x)
+    __device__ __forceinline__ void load(const float *x, int lane)
     {
-        const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int j = 0; j < PPL; j++) {
             const int i = HALF < 64 ? min(lane, HALF - 1) : lane + 64 * j;
@@ -163,9 +242,8 @@ template <int HD> struct HeadRow {
     }
     // emit(dim, value) once per dimension
     template <typename Emit>
-    __device__ __forceinline__ void turn(const HeadRow &w, bool norm, const double2 *cs, float eps, Emit emit) const
+    __device__ __forceinline__ void turn(const HeadRow &w, bool norm, const double2 *cs, float eps, int lane, Emit emit) const
     {
-        const int lane = threadIdx.x & 63;
         double f = 1.0;
         if (norm) {
             double ss = 0.0;
@@ -195,11 +273,12 @@ template <typename T, int HD, bool WIDE> struct Tile;
 // are permuted alike on both sides of each product, for 16-byte loads.
 template <int HD, bool WIDE> struct Tile<float, HD, WIDE> {
     static constexpr int KEYS = 16, NS = 4, NQ = HD / 16, NV = HD / 64, QROWS = 16;
+    int lane;
     f4 q[NQ], kf[NQ], vf[4][NV], o[NV][4];
 
     __device__ __forceinline__ void init(const float *qs, const float *)  // qs [16][HD + 4]
     {
-        const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+        const int n = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int i = 0; i < NQ; i++) q[i] = *(const f4 *)(qs + n * (HD + 4) + 16 * i + 4 * g);
 #pragma unroll
@@ -207,11 +286,11 @@ template <int HD, bool WIDE> struct Tile<float, HD, WIDE> {
 #pragma unroll
             for (int e = 0; e < 4; e++) o[j][e] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    __device__ __forceinline__ static int key_of(int i) { return 4 * ((threadIdx.x & 63) >> 4) + i; }
+    __device__ __forceinline__ int key_of(int i) const { return 4 * (lane >> 4) + i; }
     // row[0]: the pool row of key n
     __device__ __forceinline__ void load_k(const float *pool, const int *row, int64_t stride)
     {
-        const float *p = pool + max(row[0], 0) * stride + 4 * ((threadIdx.x & 63) >> 4);
+        const float *p = pool + max(row[0], 0) * stride + 4 * (lane >> 4);
 #pragma unroll
         for (int i = 0; i < NQ; i++) kf[i] = *(const f4 *)(p + 16 * i);
     }
@@ -219,7 +298,7 @@ template <int HD, bool WIDE> struct Tile<float, HD, WIDE> {
     {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float *p = pool + max(__shfl(row[0], key_of(i)), 0) * stride + 4 * (threadIdx.x & 15);
+            const float *p = pool + max(__shfl(row[0], key_of(i)), 0) * stride + 4 * (lane & 15);
 #pragma unroll
             for (int j = 0; j < NV; j++) vf[i][j] = *(const f4 *)(p + 64 * j);
         }
@@ -229,8 +308,8 @@ template <int HD, bool WIDE> struct Tile<float, HD, WIDE> {
     // a stale row may hold is not)
     __device__ __forceinline__ void patch_k(const float *knew, int at)
     {
-        if ((int)(threadIdx.x & 15) != at) return;
-        const int g = (threadIdx.x & 63) >> 4;
+        if ((lane & 15) != at) return;
+        const int g = lane >> 4;
 #pragma unroll
         for (int i = 0; i < NQ; i++) kf[i] = *(const f4 *)(knew + 16 * i + 4 * g);
     }
@@ -240,7 +319,7 @@ template <int HD, bool WIDE> struct Tile<float, HD, WIDE> {
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int j = 0; j < NV; j++) {
-                if (key_of(i) == at) vf[i][j] = *(const f4 *)(vnew + 64 * j + 4 * (threadIdx.x & 15));
+                if (key_of(i) == at) vf[i][j] = *(const f4 *)(vnew + 64 * j + 4 * (lane & 15));
                 if (!((seen >> key_of(i)) & 1u)) vf[i][j] = f4{0.0f, 0.0f, 0.0f, 0.0f};
             }
     }
@@ -272,7 +351,7 @@ template <int HD, bool WIDE> struct Tile<float, HD, WIDE> {
     // values 64 j + 4 (4 g + r) .. + 3 of query n, r < 4
     __device__ __forceinline__ void put(int j, float *dst) const  // dst: 64 values of query n
     {
-        const int g = (threadIdx.x & 63) >> 4;
+        const int g = lane >> 4;
 #pragma unroll
         for (int r = 0; r < 4; r++)
             *(f4 *)(dst + 4 * (4 * g + r)) = f4{o[j][0][r], o[j][1][r], o[j][2][r], o[j][3][r]};
@@ -298,10 +377,11 @@ template <int HD, bool WIDE> struct Tile<_Float16, HD, WIDE> {
     uint32_t vf[8][NB][ND];
     f4 o[NB][EB];
     float qscale;
+    int lane;
 
     __device__ __forceinline__ void init(const float *qs, const float *qmax)
     {
-        const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4, row = n & (QROWS - 1);
+        const int n = lane & 15, g = lane >> 4, row = n & (QROWS - 1);
         const float m = qmax[row];
         const int e = m > 0.0f && m < INFINITY ? (int)((__float_as_uint(m) >> 23) & 255) - 127 : 9;
         // 2^(9 - e), in range for every exponent: 9 - e within [-118, 136]
@@ -321,16 +401,16 @@ template <int HD, bool WIDE> struct Tile<_Float16, HD, WIDE> {
 #pragma unroll
             for (int e2 = 0; e2 < EB; e2++) o[b][e2] = f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    __device__ __forceinline__ static int key_of(int i)
+    __device__ __forceinline__ int key_of(int i) const
     {
-        return (i & 4) * 4 + 4 * ((threadIdx.x & 63) >> 4) + (i & 3);
+        return (i & 4) * 4 + 4 * (lane >> 4) + (i & 3);
     }
     // row[0], row[1]: the pool rows of keys n and 16 + n
     __device__ __forceinline__ void load_k(const _Float16 *pool, const int *row, int64_t stride)
     {
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            const _Float16 *p = pool + max(row[t], 0) * stride + 8 * ((threadIdx.x & 63) >> 4);
+            const _Float16 *p = pool + max(row[t], 0) * stride + 8 * (lane >> 4);
 #pragma unroll
             for (int i = 0; i < NQ; i++) kf[t][i] = *(const h8 *)(p + 32 * i);
         }
@@ -339,7 +419,7 @@ template <int HD, bool WIDE> struct Tile<_Float16, HD, WIDE> {
     {
 #pragma unroll
         for (int b = 0; b < NB; b++) {
-            const uint32_t *s = (const uint32_t *)(p + 128 * b + EB * (threadIdx.x & 15));
+            const uint32_t *s = (const uint32_t *)(p + 128 * b + EB * (lane & 15));
             if constexpr (ND == 4) {
                 const styx_u4 v = *(const styx_u4 *)s;
 #pragma unroll
@@ -359,7 +439,7 @@ template <int HD, bool WIDE> struct Tile<_Float16, HD, WIDE> {
     }
     __device__ __forceinline__ void patch_k(const _Float16 *knew, int at)
     {
-        const int n = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
+        const int n = lane & 15, g = lane >> 4;
 #pragma unroll
         for (int t = 0; t < 2; t++)
             if (16 * t + n == at) {
@@ -402,7 +482,7 @@ template <int HD, bool WIDE> struct Tile<_Float16, HD, WIDE> {
     }
     __device__ __forceinline__ void values(const float (&p)[NS], float corr)
     {
-        const bool low = !WIDE && (threadIdx.x & 8);
+        const bool low = !WIDE && (lane & 8);
         h8 hi, lo;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -430,7 +510,7 @@ template <int HD, bool WIDE> struct Tile<_Float16, HD, WIDE> {
     // values 64 j .. + 63 of query n; a lane has dims 128 b + EB (4 g + r) + e
     __device__ __forceinline__ void put(int j, float *dst) const
     {
-        const int g = (threadIdx.x & 63) >> 4;
+        const int g = lane >> 4;
         constexpr int PER = 64 / EB;  // lanes' rows (4 g + r) that make 64 values
 #pragma unroll
         for (int b = 0; b < NB; b++)
@@ -448,28 +528,39 @@ template <int HD, bool WIDE> struct Tile<_Float16, HD, WIDE> {
 };
 
 template <typename T, int HD, bool WIDE, bool SCORED>
-__global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
+__global__ void __launch_bounds__(AB_WG, ab_slots(HD) / 256) k_attn_batch(AttnBatchArgs a)
 {
     using Tl = Tile<T, HD, WIDE>;
     constexpr int KEYS = Tl::KEYS, NS = Tl::NS, QROWS = Tl::QROWS, NR = KEYS / 16;
     __shared__ __align__(16) float s_q[QROWS][HD + 4];
     __shared__ float s_qmax[QROWS];
     __shared__ __align__(16) T s_k[HD], s_v[HD];
-    __shared__ __align__(16) float s_o[AB_WAVES][QROWS][68];
+    constexpr int DR = HD < 128 ? HD : 128;  // dimensions merged at a time
+    __shared__ __align__(16) float s_o[AB_WAVES][QROWS][DR + 4];
     __shared__ float s_m[AB_WAVES][16], s_l[AB_WAVES][16];
     const KvView &kv = a.kv;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
-    const int kvh = blockIdx.x % kv.nkv, cidx = blockIdx.x / kv.nkv;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const RowSplit sp = split_rows(a);
-    const int chunk = sp.chunk;
-    const ChunkAt at = chunk_find<false>(a, sp, cidx);
-    if (at.count == 0) return;
+    if (blockIdx.x == 0 && wave == 0) split_store(a, sp);
+    const uint32_t end = min(sp.units, (blockIdx.x + 1) * sp.share);
+    for (uint32_t u = blockIdx.x * sp.share; u < end;) {
+    // (a lane number that the compiler takes for a new one in every trip:
+    // what is computed from it would else be kept in registers over the
+    // trips, a wave less of them per SIMD)
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int n = lane & 15, g = lane >> 4;
+    const SeqAt at = seq_find(a, sp, u);
     const int b = at.b, rows = at.rows, last = rows - 1;
-    const int t0 = (cidx - at.first) * chunk, t1 = min(rows, t0 + chunk);
+    const uint32_t per_head = head_units(sp, rows), in_seq = u - at.first;
+    const int kvh = in_seq / per_head, u0 = in_seq - kvh * per_head, nu = min(per_head - u0, end - u);
+    u += nu;
+    const int t0 = u0 * AB_UNIT, t1 = min(rows, t0 + nu * AB_UNIT);
     const int32_t *tab = kv.table + (int64_t)b * kv.table_len;
     const int64_t stride = (int64_t)kv.nkv * HD;
     const T *kp = (const T *)kv.kpool + kvh * HD, *vp = (const T *)kv.vpool + kvh * HD;
     Tl x;
+    x.lane = lane;
     // pool rows of this lane's keys of a tile: page-table entries are asked
     // for one tile ahead of the rows, the rows one tile ahead of their use
     int entry[NR], row[NR];
@@ -483,7 +574,7 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
     };
     const int step = AB_WAVES * KEYS;
     int tb = t0 + wave * KEYS;
-    const bool own = t1 == rows;  // this chunk holds the new row
+    const bool own = t1 == rows;  // this piece holds the new row
     // Everything that does not wait for the page table is asked for behind
     // it: loads are counted in order, and the rows of K and V after them
     // then do not hold up the heads.
@@ -496,13 +587,13 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
     for (int j = 0; j < PPL; j++) cs[j] = a.rope[(int64_t)pos * (HD / 2) + (HD < 128 ? lane & (HD / 2 - 1) : lane + 64 * j)];
     const float *qb = a.q + ((int64_t)b * a.nh + kvh * a.gqa) * HD;
 #pragma unroll
-    for (int i = 0; i < QROWS / AB_WAVES; i++) hq[i].load(qb + min(wave + AB_WAVES * i, a.gqa - 1) * HD);
-    qw.load(a.q_norm ? a.q_norm : qb);
+    for (int i = 0; i < QROWS / AB_WAVES; i++) hq[i].load(qb + min(wave + AB_WAVES * i, a.gqa - 1) * HD, lane);
+    qw.load(a.q_norm ? a.q_norm : qb, lane);
     const int64_t in = ((int64_t)b * kv.nkv + kvh) * HD;
     if (own && wave == AB_WAVES - 1) {
-        hk.load(a.k + in);
-        kw.load(a.k_norm ? a.k_norm : a.k + in);
-        hv.load(a.v + in);
+        hk.load(a.k + in, lane);
+        kw.load(a.k_norm ? a.k_norm : a.k + in, lane);
+        hv.load(a.v + in, lane);
     }
     rows_at(tb);
     x.load_k(kp, row, stride);
@@ -513,7 +604,7 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
         const int h = wave + AB_WAVES * i;
         float big = 0.0f;
         if (h < a.gqa)
-            hq[i].turn(qw, a.q_norm != nullptr, cs, a.eps, [&](int d, float v) {
+            hq[i].turn(qw, a.q_norm != nullptr, cs, a.eps, lane, [&](int d, float v) {
                 s_q[h][d] = v;
                 big = fmaxf(big, fabsf(v));
             });
@@ -525,7 +616,7 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
         }
     }
     if (own && wave == AB_WAVES - 1) {
-        hk.turn(kw, a.k_norm != nullptr, cs, a.eps, [&](int d, float v) { s_k[d] = (T)v; });
+        hk.turn(kw, a.k_norm != nullptr, cs, a.eps, lane, [&](int d, float v) { s_k[d] = (T)v; });
 #pragma unroll
         for (int j = 0; j < PPL; j++)
             if (HD >= 128 || lane < HD / 2) {
@@ -540,7 +631,7 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
     if constexpr (SCORED)
         score = a.score + (((int64_t)b * kv.nkv + kvh) * a.gqa + min(n, a.gqa - 1)) * a.stride;
     for (; tb < t1; tb += step) {
-        // keys seen: of the tile's, those of the chunk whose page is there
+        // keys seen: of the tile's, those of the piece whose page is there
         uint32_t seen = 0;
 #pragma unroll
         for (int r = 0; r < NR; r++)
@@ -559,7 +650,7 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
         if (!whole) {
 #pragma unroll
             for (int i = 0; i < NS; i++)
-                if (!((seen >> Tl::key_of(i)) & 1u)) s[i] = -INFINITY;
+                if (!((seen >> x.key_of(i)) & 1u)) s[i] = -INFINITY;
             x.patch_v(s_v, fresh, seen);
         }
         if constexpr (SCORED) {
@@ -595,21 +686,22 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
             }
         if (a.slot_pos && lane == 0) a.slot_pos[((int64_t)b * kv.nkv + kvh) * kv.cap + last] = pos;
     }
-    // the waves' results of each head merged, one partial per chunk and head
+    // the waves' results of each head merged, one partial per piece and head
     l = groups_sum(l);
     if (g == 0 && n < QROWS) {
         s_m[wave][n] = m;
         s_l[wave][n] = l;
     }
-    const int64_t pc = (int64_t)blockIdx.x * a.gqa;
+    const int64_t pc = ((int64_t)blockIdx.x + b * kv.nkv + kvh) * a.gqa;
 #pragma unroll
-    for (int j = 0; j < HD / 64; j++) {
+    for (int d0 = 0; d0 < HD; d0 += DR) {
         __syncthreads();
         // (every lane takes part: pieces of a query come from two lanes)
-        x.put(j, s_o[wave][n & (QROWS - 1)]);
+#pragma unroll
+        for (int j = 0; j < DR / 64; j++) x.put(d0 / 64 + j, s_o[wave][n & (QROWS - 1)] + 64 * j);
         __syncthreads();
-        for (int i = threadIdx.x; i < a.gqa * 64; i += AB_WG) {
-            const int h = i >> 6, d = i & 63;
+        for (int i = threadIdx.x; i < a.gqa * DR; i += AB_WG) {
+            const int h = i / DR, d = i % DR;
             float M = s_m[0][h];
 #pragma unroll
             for (int w = 1; w < AB_WAVES; w++) M = fmaxf(M, s_m[w][h]);
@@ -620,20 +712,34 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch(AttnBatchArgs a)
                 L += s_l[w][h] * f;
                 O += f == 0.0f ? 0.0f : s_o[w][h][d] * f;
             }
-            a.part_o[(pc + h) * HD + 64 * j + d] = O;
-            if (j == 0 && d == 0) {
+            a.part_o[(pc + h) * HD + d0 + d] = O;
+            if (d0 == 0 && d == 0) {
                 a.part_ml[2 * (pc + h)] = M;
                 a.part_ml[2 * (pc + h) + 1] = L;
             }
         }
     }
+    }
 }
 
-// Partials of every STEP-th chunk from c0 on of one head merged by a thread:
-// the loads of AB_BATCH chunks in flight at once, their maximum first, then
-// independent factors.  o: of the value at dim (null: M and L alone).
+// The pieces of one kv head: their partials lie one after another (piece i of
+// the batch is workgroup w's of the p-th head with w + p = i).
+struct Pieces {
+    int64_t first;
+    int count;
+};
+__device__ __forceinline__ Pieces pieces_of(const AttnBatchArgs &a, const RowSplit &sp, const SeqAt &at, int kvh)
+{
+    const uint32_t per_head = head_units(sp, at.rows), u = at.first + kvh * per_head;
+    const uint32_t w0 = u / sp.share, w1 = (u + per_head - 1) / sp.share;
+    return {(int64_t)w0 + at.b * a.kv.nkv + kvh, (int)(w1 - w0) + 1};
+}
+
+// Partials of every STEP-th piece from c0 on of one head merged by a thread:
+// the loads of AB_BATCH pieces in flight at once, their maximum first, then
+// independent factors.  O: of the value at dim; else M and L alone.
 template <int STEP, bool O>
-__device__ __forceinline__ void merge_chunks(const AttnBatchArgs &a, const ChunkAt &at, int c0, int kvh, int hg, int dim,
+__device__ __forceinline__ void merge_pieces(const AttnBatchArgs &a, const Pieces &at, int c0, int hg, int dim,
                                              float &m, float &l, float &o)
 {
     m = -INFINITY;
@@ -644,7 +750,7 @@ __device__ __forceinline__ void merge_chunks(const AttnBatchArgs &a, const Chunk
 #pragma unroll
         for (int i = 0; i < AB_BATCH; i++) {
             const int cc = min(c + STEP * i, at.count - 1);
-            const int64_t p = ((int64_t)(at.first + cc) * a.kv.nkv + kvh) * a.gqa + hg;
+            const int64_t p = (at.first + cc) * a.gqa + hg;
             ml[i] = ((const float2 *)a.part_ml)[p];
             if (O) oc[i] = a.part_o[p * a.kv.hd + dim];
         }
@@ -669,37 +775,39 @@ __device__ __forceinline__ void merge_chunks(const AttnBatchArgs &a, const Chunk
     }
 }
 
-// The chunks joined.  Workgroups below n_merge: one query head of one
-// sequence and 32 of its dimensions, a half wave taking every eighth chunk.
-// The others: AB_WTILE slots of one kv head's weights, M and L of its heads
-// formed from the chunks' first (16 lanes a head), the scores in flight
-// meanwhile.
+// The pieces joined.  Workgroups below n_merge: one query head of one
+// sequence and DIMS of its dimensions, each part of the workgroup taking
+// every AB_WG / DIMS-th piece.  The others: every a.tiles-th step of one kv
+// head's weights, M and L of its heads formed from the pieces' first (16
+// lanes a head), the first step's scores in flight meanwhile.
+template <int DIMS, int HM>
 __global__ void __launch_bounds__(AB_WG) k_attn_batch_join(AttnBatchArgs a)
 {
-    __shared__ float s_o[8][AB_DIMS], s_m[8], s_l[8], s_M[16], s_R[16];
+    constexpr int PARTS = AB_WG / DIMS, PER = ab_wper(HM);
+    __shared__ float s_o[PARTS][DIMS], s_m[PARTS], s_l[PARTS], s_M[16], s_R[16];
     const KvView &kv = a.kv;
     const int tid = threadIdx.x;
-    const RowSplit sp = split_rows(a);
+    RowSplit sp;
     if ((int)blockIdx.x < a.n_merge) {
-        const int nd = kv.hd / AB_DIMS, bh = blockIdx.x / nd, d0 = blockIdx.x % nd * AB_DIMS;
+        const int nd = kv.hd / DIMS, bh = blockIdx.x / nd, d0 = blockIdx.x % nd * DIMS;
         const int b = bh / a.nh, h = bh % a.nh, kvh = h / a.gqa, hg = h % a.gqa;
-        const ChunkAt at = chunk_find<true>(a, sp, b);
-        if (at.count == 0) return;
-        const int part = tid >> 5, d = tid & 31;
+        const SeqAt at = seq_load(a, sp, b);
+        if (at.rows == 0) return;
+        const int part = tid / DIMS, d = tid % DIMS;
         float m, l, o;
-        merge_chunks<8, true>(a, at, part, kvh, hg, d0 + d, m, l, o);
+        merge_pieces<PARTS, true>(a, pieces_of(a, sp, at, kvh), part, hg, d0 + d, m, l, o);
         s_o[part][d] = o;
         if (d == 0) {
             s_m[part] = m;
             s_l[part] = l;
         }
         __syncthreads();
-        if (tid < AB_DIMS) {
+        if (tid < DIMS) {
             float M = -INFINITY, L = 0.0f, O = 0.0f;
 #pragma unroll
-            for (int w = 0; w < 8; w++) M = fmaxf(M, s_m[w]);
+            for (int w = 0; w < PARTS; w++) M = fmaxf(M, s_m[w]);
 #pragma unroll
-            for (int w = 0; w < 8; w++) {
+            for (int w = 0; w < PARTS; w++) {
                 const float f = s_m[w] == -INFINITY ? 0.0f : exp2_(s_m[w] - M);
                 L += s_l[w] * f;
                 O += s_o[w][tid] * f;
@@ -710,24 +818,27 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch_join(AttnBatchArgs a)
         return;
     }
     const int w = blockIdx.x - a.n_merge, tile = w % a.tiles, bk = w / a.tiles;
-    const int b = bk / kv.nkv, kvh = bk % kv.nkv, t0 = tile * AB_WTILE;
-    const ChunkAt at = chunk_find<true>(a, sp, b);
-    if (t0 >= at.rows) return;
-    constexpr int PER = AB_WTILE / AB_WG;
+    const int b = bk / kv.nkv, kvh = bk % kv.nkv;
+    const SeqAt at = seq_load(a, sp, b);
+    constexpr int STEP = PER * AB_WG;
+    if (tile * STEP >= at.rows) return;
     const int64_t base = (int64_t)b * kv.nkv + kvh;
     const float *sc = a.score + base * a.gqa * a.stride;
-    float s[PER][16], old[PER];
+    float s[PER][HM], old[PER];
+    auto load = [&](int t0) {
 #pragma unroll
-    for (int j = 0; j < PER; j++) {
-        const int t = min(t0 + tid + AB_WG * j, at.rows - 1);
+        for (int j = 0; j < PER; j++) {
+            const int t = min(t0 + tid + AB_WG * j, at.rows - 1);
 #pragma unroll
-        for (int h = 0; h < 16; h++) s[j][h] = h < a.gqa ? sc[(int64_t)h * a.stride + t] : -INFINITY;
-        old[j] = a.acc_in && t < at.rows - 1 ? a.acc_in[base * kv.cap + t] : 0.0f;
-    }
+            for (int h = 0; h < HM; h++) s[j][h] = h < a.gqa ? sc[(int64_t)h * a.stride + t] : -INFINITY;
+            old[j] = a.acc_in && t < at.rows - 1 ? a.acc_in[base * kv.cap + t] : 0.0f;
+        }
+    };
+    load(tile * STEP);
     {
         const int h = tid >> 4;
         float m = -INFINITY, l = 0.0f, o;
-        if (h < a.gqa) merge_chunks<16, false>(a, at, tid & 15, kvh, h, 0, m, l, o);
+        if (h < a.gqa) merge_pieces<16, false>(a, pieces_of(a, sp, at, kvh), tid & 15, h, 0, m, l, o);
         const float M = bfly<16>(m, [](float x, float y) { return fmaxf(x, y); });
         const float L = bfly_sum<16>(m == -INFINITY ? 0.0f : l * exp2_(m - M));
         if ((tid & 15) == 0) {
@@ -736,29 +847,49 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch_join(AttnBatchArgs a)
         }
     }
     __syncthreads();
+    for (int t0 = tile * STEP;;) {
 #pragma unroll
-    for (int j = 0; j < PER; j++) {
-        const int t = t0 + tid + AB_WG * j;
-        float sum = 0.0f;
+        for (int j = 0; j < PER; j++) {
+            const int t = t0 + tid + AB_WG * j;
+            float sum = 0.0f;
 #pragma unroll
-        for (int h = 0; h < 16; h++)
-            if (h < a.gqa) sum += exp2_(s[j][h] - s_M[h]) * s_R[h];
-        if (t < at.rows) a.acc_out[base * kv.cap + t] = a.decay * old[j] + sum;
+            for (int h = 0; h < HM; h++)
+                if (h < a.gqa) sum += exp2_(s[j][h] - s_M[h]) * s_R[h];
+            if (t < at.rows) a.acc_out[base * kv.cap + t] = a.decay * old[j] + sum;
+        }
+        t0 += a.tiles * STEP;
+        if (t0 >= at.rows) break;
+        load(t0);
     }
+}
+
+// Dimensions of a merging workgroup: all of a head's where that makes two
+// workgroups per CU, else as few as it takes (32 at least), so that many
+// pieces of few heads are read by many.
+static int merge_dims(int64_t heads, int hd)
+{
+    int d = hd;
+    while (d > 32 && heads * (hd / d) < 512) d /= 2;
+    return d;
 }
 
 AttnBatchWs attn_batch_ws(int n_seq, int nkv, int hd, int cap, int gqa, bool scored)
 {
     AttnBatchWs w{};
-    const int64_t heads = (int64_t)n_seq * nkv, most = ((int64_t)cap + AB_MIN - 1) / AB_MIN * heads;
-    // sum over sequences of ceil(rows / chunk) <= 2^AB_LOG_TARGET / nkv + n_seq
-    w.chunks = std::min(most, (1 << AB_LOG_TARGET) + heads);
+    const int64_t heads = (int64_t)n_seq * nkv;
+    w.units = ((int64_t)cap + AB_UNIT - 1) / AB_UNIT * heads;
+    w.grid = std::min<int64_t>(w.units, ab_slots(hd));
+    const int64_t pieces = w.grid + heads;
     w.stride = (cap + 63) / 64 * 64;
-    w.ml = (2 * w.chunks * gqa + 63) / 64 * 64;
-    w.o = w.chunks * gqa * hd;
+    w.ml = (2 * pieces * gqa + 63) / 64 * 64;
+    w.o = pieces * gqa * hd;
+    w.plan = ((int64_t)n_seq + 2 + 63) / 64 * 64;
     w.score = scored ? heads * gqa * w.stride : 0;
-    w.tiles = scored ? (cap + AB_WTILE - 1) / AB_WTILE : 0;
-    w.join = heads * gqa * (hd / AB_DIMS) + heads * w.tiles;
+    w.dims = merge_dims(heads * gqa, hd);
+    // weights: eight workgroups per CU, or one for every step
+    const int step = ab_wper(gqa) * AB_WG;
+    w.tiles = scored ? (int)std::min<int64_t>((cap - 1) / step + 1, std::max<int64_t>(1, 2048 / heads)) : 0;
+    w.join = heads * gqa * (hd / w.dims) + heads * w.tiles;
     return w;
 }
 
@@ -781,25 +912,39 @@ template <int HD> static void launch_ab_hd(hipStream_t st, const AttnBatchArgs &
         launch_ab<_Float16, HD, false>(st, a, grid);
 }
 
+template <int DIMS> static void launch_join(hipStream_t st, const AttnBatchArgs &a, int64_t grid)
+{
+    if (a.gqa <= 4)
+        hipLaunchKernelGGL((k_attn_batch_join<DIMS, 4>), dim3((unsigned)grid), dim3(AB_WG), 0, st, a);
+    else
+        hipLaunchKernelGGL((k_attn_batch_join<DIMS, 16>), dim3((unsigned)grid), dim3(AB_WG), 0, st, a);
+}
+
 hipError_t launch_attn_batch(hipStream_t st, AttnBatchArgs a, float *ws)
 {
     const KvView &kv = a.kv;
     const AttnBatchWs w = attn_batch_ws(kv.n_seq, kv.nkv, kv.hd, kv.cap, a.gqa, a.acc_out != nullptr);
     a.stride = w.stride;
     a.scale = (float)((double)a.scale * 1.4426950408889634);  // log2 e
-    a.n_merge = kv.n_seq * a.nh * (kv.hd / AB_DIMS);
+    a.n_merge = kv.n_seq * a.nh * (kv.hd / w.dims);
     a.tiles = w.tiles;
     a.part_ml = ws;
     a.part_o = a.part_ml + w.ml;
-    a.score = a.part_o + w.o;
+    a.plan = (uint32_t *)(a.part_o + w.o);
+    a.score = a.part_o + w.o + w.plan;
     switch (kv.hd) {
-    case 64: launch_ab_hd<64>(st, a, w.chunks); break;
-    case 128: launch_ab_hd<128>(st, a, w.chunks); break;
-    default: launch_ab_hd<256>(st, a, w.chunks); break;
+    case 64: launch_ab_hd<64>(st, a, w.grid); break;
+    case 128: launch_ab_hd<128>(st, a, w.grid); break;
+    default: launch_ab_hd<256>(st, a, w.grid); break;
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_attn_batch_join, dim3((unsigned)w.join), dim3(AB_WG), 0, st, a);
+    switch (w.dims) {
+    case 32: launch_join<32>(st, a, w.join); break;
+    case 64: launch_join<64>(st, a, w.join); break;
+    case 128: launch_join<128>(st, a, w.join); break;
+    default: launch_join<256>(st, a, w.join); break;
+    }
     return hipGetLastError();
 }
 

@@ -536,8 +536,8 @@ uint64_t styx_op_attn_batch_ws_bytes(const styx_kv_cache *kv, int nh, int scored
     if (!kv_shape_ok(kv) || nh < 1 || nh % kv->nkv || nh / kv->nkv > 16) return 0;
     const AttnBatchWs w = attn_batch_ws(kv->n_seq, kv->nkv, kv->hd, kv->table_len * kv->page_tokens,
                                         nh / kv->nkv, scored != 0);
-    if (w.chunks > MAX_WG_256 || w.join > MAX_WG_256) return 0;
-    return 4ull * (uint64_t)(w.ml + w.o + w.score);
+    if (w.units > INT32_MAX || w.join > MAX_WG_256) return 0;
+    return 4ull * (uint64_t)(w.ml + w.o + w.plan + w.score);
 }
 
 int styx_op_attn_decode_batch(styx_gpu *g, const styx_kv_cache *kv, const int32_t *len, const int32_t *pos,
