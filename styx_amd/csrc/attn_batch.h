@@ -80,14 +80,17 @@ struct KvEvictArgs {
     const int32_t *pos_in;
     int32_t *pos_out;
     int32_t *len_out;
-    // workspace
-    int32_t *map;    // [n_seq][nkv][keep] slot whose row comes to each place
-    int32_t *holes;  // [n_seq][nkv][keep] places whose own row leaves
-    int copy_tiles;  // the moving launch's workgroups per kv head (filled by the launch)
+    // workspace (filled by the launch)
+    unsigned long long *stay; // [n_seq][nkv][stay_words] whether a slot below keep keeps its row
+    int2 *left;               // [n_seq] new length, whether rows leave
+    int32_t *moves;           // [n_seq][nkv] how many holes and movers
+    int32_t *holes, *movers;  // [n_seq][nkv][keep] ascending
+    uint32_t *bins;           // long caches: of every part
+    int stay_words, parts, move_tiles, copy_tiles;
 };
-inline uint64_t kv_evict_ws_bytes(int n_seq, int nkv, int keep) { return 8ull * n_seq * nkv * keep; }
-// Workgroups of the moving launch.
-int64_t kv_evict_grid(const KvEvictArgs &a);
+uint64_t kv_evict_ws_bytes(int n_seq, int nkv, int cap, int keep);
+// Workgroups of the largest launch, in such of 256 threads.
+int64_t kv_evict_grid(KvEvictArgs a);
 hipError_t launch_kv_evict(hipStream_t st, KvEvictArgs a, void *ws);
 
 }  // namespace styx

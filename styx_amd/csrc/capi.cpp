@@ -584,7 +584,7 @@ int styx_op_attn_decode_batch(styx_gpu *g, const styx_kv_cache *kv, const int32_
 uint64_t styx_op_kv_evict_ws_bytes(const styx_kv_cache *kv, int keep)
 {
     if (!kv_shape_ok(kv) || keep < 1 || keep > kv->table_len * kv->page_tokens) return 0;
-    return kv_evict_ws_bytes(kv->n_seq, kv->nkv, keep);
+    return kv_evict_ws_bytes(kv->n_seq, kv->nkv, kv->table_len * kv->page_tokens, keep);
 }
 
 int styx_op_kv_evict(styx_gpu *g, const styx_kv_cache *kv, const int32_t *len, const int32_t *pos, int trigger,

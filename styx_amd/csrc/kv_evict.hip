@@ -13,181 +13,485 @@
 // Bound: latency (a selection has to see all weights before its first
 // move) and, for long caches, HBM: 8 bytes of weight and position per row
 // read, 2 rows of K and V read and written per move.
+//
+// A selecting launch (four for caches of more than 16K slots) leaves lists of
+// holes and movers, and which slots stay; a moving launch does the rest.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_batch.h"
 
 namespace styx {
 
 constexpr int EV_WG = 1024, EV_WAVES = EV_WG / 64;
-constexpr int MV_WG = 256, MV_SLOTS = 256;
+constexpr int EV_KPT = 16;                // keys of a thread, in registers
+constexpr int EV_PART = EV_WG * EV_KPT;   // slots that a workgroup selects from
+constexpr int EV_BINS = 2048, EV_COPIES = 4;
+constexpr int EV_LDS = (EV_COPIES + 2) * EV_BINS;
+constexpr int EV_HIST = 2 * EV_BINS + EV_BINS / 2;  // bins of a part's three passes
+constexpr int MV_WG = 256, MV_DEEP = 4, CP_SLOTS = 1024;
+typedef unsigned long long u64;
+// for the lambdas that touch a thread's array of keys, which a call would
+// put into memory
+#define EV_INLINE __attribute__((always_inline))
 
 // A row's key: weights in order, NaN below all; rows that stay anyway above all.
-__device__ __forceinline__ uint32_t evict_key(const KvEvictArgs &a, int64_t base, int t, int64_t newest)
+__device__ __forceinline__ uint32_t evict_key(const KvEvictArgs &a, float weight, int32_t pos, int64_t newest)
 {
-    const int64_t p = a.pos_in[base + t];
-    const float w = a.acc_in[base + t] + 0.0f;  // -0 is 0
-    if (p > newest - a.recent || p < a.sinks) return 0xFFFFFFFFu;
+    const float w = weight + 0.0f;  // -0 is 0
+    if (pos > newest - a.recent || pos < a.sinks) return 0xFFFFFFFFu;
     if (w != w) return 0;
     const uint32_t u = __float_as_uint(w);
     return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
-// Over a workgroup's threads in order: how many of those before this one
-// have f set, and the total.  Every thread takes part.
-struct Before {
-    int rank, total;
-};
-__device__ __forceinline__ Before count_before(bool f, int *s)  // s [EV_WAVES]
+// Inclusive sums over the wave by lane permutes: within rows of 16, then the
+// rows' last lanes passed on (row_bcast:15 to rows 1 and 3, :31 to the upper
+// half).
+__device__ __forceinline__ int scan_add(int v)
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const unsigned long long m = __ballot(f);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+__device__ __forceinline__ int last_lane(int v) { return __builtin_amdgcn_readlane(v, 63); }
+
+// Sum of the earlier waves' v (uniform in a wave), *total that of all.  Every
+// thread takes part.
+__device__ __forceinline__ int waves_before(int v, int wave, int *s, int *total = nullptr)  // s [EV_WAVES]
+{
     __syncthreads();
-    if (lane == 0) s[wave] = __popcll(m);
+    if ((threadIdx.x & 63) == 0) s[wave] = v;
     __syncthreads();
-    Before r{(int)__popcll(m & ((1ull << lane) - 1)), 0};
+    int sum = 0, all = 0;
+#pragma unroll
     for (int w = 0; w < EV_WAVES; w++) {
-        if (w < wave) r.rank += s[w];
-        r.total += s[w];
+        sum += w < wave ? s[w] : 0;
+        all += s[w];
     }
-    return r;
+    if (total) *total = all;
+    return sum;
 }
 
-// One workgroup per sequence and kv head: the keep-th largest key by a radix
-// selection of 8 bits a pass, then holes and movers in slot order.
+// f(I) for I = 0 .. N - 1, each a constant of its own: arrays indexed by it
+// stay in registers.
+template <int N, int I = 0, typename F> __device__ __forceinline__ void unrolled(F f)
+{
+    if constexpr (I < N) {
+        f(std::integral_constant<int, I>{});
+        unrolled<N, I + 1>(f);
+    }
+}
+
+// The radix selection's passes: 11, 11 and 10 bits.
+__host__ __device__ constexpr int pass_shift(int p) { return p == 0 ? 21 : p == 1 ? 10 : 0; }
+__host__ __device__ constexpr int pass_bins(int p) { return p == 2 ? EV_BINS / 2 : EV_BINS; }
+__host__ __device__ constexpr uint32_t pass_mask(int p) { return p == 0 ? 0u : p == 1 ? 0xFFE00000u : 0xFFFFFC00u; }
+
+// The keys of up to EV_PART slots from t0 on, the waves each a contiguous run
+// of rows of 64 slots, a lane one slot of each row.
+struct EvKeys {
+    uint32_t key[EV_KPT];
+    int per, first, end, lane;  // rows of a wave, its first slot, the slots' end
+    __device__ __forceinline__ void load(const KvEvictArgs &a, int64_t base, int t0, int t1, int wave, int64_t newest)
+    {
+        lane = threadIdx.x & 63;
+        per = (t1 - t0 + EV_WG - 1) / EV_WG;
+        first = t0 + wave * per * 64;
+        end = t1;
+        float w[EV_KPT];
+        int32_t p[EV_KPT];
+#pragma unroll
+        for (int j = 0; j < EV_KPT; j++) {
+            if (j >= per) break;
+            const int t = min(first + 64 * j + lane, t1 - 1);
+            w[j] = a.acc_in[base + t];
+            p[j] = a.pos_in[base + t];
+        }
+#pragma unroll
+        for (int j = 0; j < EV_KPT; j++) key[j] = j < per ? evict_key(a, w[j], p[j], newest) : 0;
+    }
+    // f(row, key, whether there is one), the wave's lanes together
+    template <typename F> __device__ __forceinline__ void each(F f) const
+    {
+        unrolled<EV_KPT>([&](auto j) EV_INLINE {
+            if (j < per) f((int)j, key[j], first + 64 * j + lane < end);
+        });
+    }
+    // Keys that match the prefix counted by their next digit.
+    __device__ __forceinline__ void count(int pass, uint32_t prefix, uint32_t *h) const
+    {
+        const int shift = pass_shift(pass), bins = pass_bins(pass);
+        const uint32_t mask = pass_mask(pass);
+        each([&](int, uint32_t k, bool there) EV_INLINE {
+            if (there && (k & mask) == prefix) atomicAdd(&h[(k >> shift) & (bins - 1)], 1u);
+        });
+    }
+    // Lane j: the mask of row j's slots that stay: keys above the prefix, and
+    // of those that equal it the first `need` (`ties` were before these).
+    __device__ __forceinline__ u64 masks(uint32_t prefix, bool all_ties, int need, int ties) const
+    {
+        u64 mine = 0;
+        const u64 below = (1ull << lane) - 1;
+        each([&](int j, uint32_t k, bool there) EV_INLINE {
+            bool stays = there && k >= prefix;
+            if (!all_ties) {
+                const bool tie = there && k == prefix;
+                const u64 m = __ballot(tie);
+                stays = stays && (!tie || ties + __popcll(m & below) < need);
+                ties += __popcll(m);
+            }
+            const u64 m = __ballot(stays);
+            if (lane == j) mine = m;
+        });
+        return mine;
+    }
+    // The slots below `keep` of lane j's row, and those that there are.
+    __device__ __forceinline__ u64 low(int keep) const
+    {
+        const int k = keep - (first + 64 * lane);
+        return lane >= per || k <= 0 ? 0ull : k >= 64 ? ~0ull : (1ull << k) - 1;
+    }
+    // f(slot, rank) for the bits of the rows' masks (lane j's: row j's), ranks
+    // from `rank` on.
+    template <typename F> __device__ __forceinline__ void emit(u64 p, int rank, F f) const
+    {
+        const int c = __popcll(p), before = scan_add(c) - c + rank;
+        u64 rows = __ballot(c > 0);
+        while (rows) {
+            const int j = __builtin_ctzll(rows);
+            rows &= rows - 1;
+            const u64 m = (u64)(uint32_t)__builtin_amdgcn_readlane((int)(p >> 32), j) << 32 |
+                          (uint32_t)__builtin_amdgcn_readlane((int)p, j);
+            const int r = __builtin_amdgcn_readlane(before, j) + __popcll(m & ((1ull << lane) - 1));
+            if ((m >> lane) & 1) f(first + 64 * j + lane, r);
+        }
+    }
+};
+
+// The selection so far: the need-th largest of the `equal` keys that match
+// the prefix is looked for.
+struct EvPick {
+    uint32_t prefix;
+    int need, equal;
+    // One digit: c0, c1 the numbers in thread i's bins 2 i and 2 i + 1 from
+    // the top.  Every thread takes part; s [EV_WAVES], o [3].
+    __device__ __forceinline__ int digit(int pass, int c0, int c1, int wave, int *s, int *o)
+    {
+        const int top = pass_bins(pass) - 1 - 2 * (int)threadIdx.x, incl = scan_add(c0 + c1);
+        const int above = waves_before(last_lane(incl), wave, s) + incl - c0 - c1;
+        if (above < need && above + c0 + c1 >= need) {
+            const bool second = above + c0 < need;
+            o[0] = second ? top - 1 : top;
+            o[1] = second ? above + c0 : above;
+            o[2] = second ? c1 : c0;
+        }
+        __syncthreads();
+        prefix |= (uint32_t)o[0] << pass_shift(pass);
+        need -= o[1];
+        equal = o[2];
+        return o[0];
+    }
+};
+
+// Sequence and kv head of a selecting workgroup; keeps for the moving launch
+// what it may not read any more, as it overwrites the lengths.
+struct EvHead {
+    int bk, b, n;
+    bool act;
+};
+__device__ __forceinline__ EvHead evict_head(const KvEvictArgs &a, int bk, bool store)
+{
+    EvHead h;
+    h.bk = bk;
+    h.b = bk / a.kv.nkv;
+    h.n = a.len[h.b];
+    h.act = h.n > a.trigger && h.n <= a.kv.cap;
+    if (store && threadIdx.x == 0) {
+        if (bk % a.kv.nkv == 0) a.left[h.b] = make_int2(h.act ? a.keep : h.n, h.act);
+        if (!h.act) a.moves[bk] = 0;
+    }
+    return h;
+}
+
+// Caches of up to EV_PART slots: one workgroup per sequence and kv head.  One
+// CU does all of a head's work, so what counts are instructions per key and
+// barriers.  The first pass counts every key, and weights of one size crowd
+// into few bins: four copies of them, by lane, keep the adds of a wave apart.
 __global__ void __launch_bounds__(EV_WG) k_evict_select(KvEvictArgs a)
 {
-    __shared__ uint32_t hist[256];
-    __shared__ int cnt[EV_WAVES];
-    __shared__ uint32_t s_digit;
-    __shared__ int s_above;
-    const KvView &kv = a.kv;
-    const int bk = blockIdx.x, b = bk / kv.nkv, n = a.len[b], tid = threadIdx.x;
-    if (n <= a.trigger || n > kv.cap) return;
-    const int64_t base = (int64_t)bk * kv.cap, newest = a.pos[b];
-    uint32_t prefix = 0, mask = 0;
-    int need = a.keep;  // the need-th largest of the keys that match the prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
+    // bins of the three passes
+    __shared__ uint32_t hist[EV_LDS];
+    __shared__ int s_cnt[EV_WAVES], s_out[3];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const EvHead hd = evict_head(a, blockIdx.x, true);
+    if (!hd.act) return;
+    for (int i = tid; i < EV_LDS; i += EV_WG) hist[i] = 0;
+    EvKeys k;
+    k.load(a, (int64_t)hd.bk * a.kv.cap, 0, hd.n, wave, a.pos[hd.b]);
+    EvPick pick{0, a.keep, 0};
+#pragma unroll 1
+    for (int pass = 0; pass < 3; pass++) {
+        const int copies = pass == 0 ? EV_COPIES : 1;
+        uint32_t *bin = hist + (pass == 0 ? 0 : (EV_COPIES + pass - 1) * EV_BINS);
         __syncthreads();
-        for (int t = tid; t < n; t += EV_WG) {
-            const uint32_t k = evict_key(a, base, t, newest);
-            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
+        k.count(pass, pick.prefix, bin + (pass == 0 ? lane % EV_COPIES * EV_BINS : 0));
+        __syncthreads();
+        const int top = pass_bins(pass) - 1 - 2 * tid;
+        int c0 = 0, c1 = 0;
+        if (top > 0)
+            for (int c = 0; c < copies; c++) {
+                c0 += bin[c * EV_BINS + top];
+                c1 += bin[c * EV_BINS + top - 1];
+            }
+        pick.digit(pass, c0, c1, wave, s_cnt, s_out);
+    }
+    const bool all_ties = pick.equal == pick.need;
+    int ties = 0;
+    if (!all_ties) {
+        int eq = 0;
+        k.each([&](int, uint32_t v, bool there) EV_INLINE { eq += __popcll(__ballot(there && v == pick.prefix)); });
+        ties = waves_before(eq, wave, s_cnt);
+    }
+    const u64 stay = k.masks(pick.prefix, all_ties, pick.need, ties), low = k.low(a.keep);
+    if (low) a.stay[(int64_t)hd.bk * a.stay_words + k.first / 64 + lane] = stay;
+    const u64 holes = ~stay & low, movers = stay & ~low;
+    // both counts in one sum: each is below 2^15
+    int total;
+    const int before = waves_before(last_lane(scan_add(__popcll(holes) | __popcll(movers) << 16)), wave, s_cnt, &total);
+    int32_t *to = a.holes + (int64_t)hd.bk * a.keep, *from = a.movers + (int64_t)hd.bk * a.keep;
+    k.emit(holes, before & 0xFFFF, [&](int t, int r) EV_INLINE { to[r] = t; });
+    k.emit(movers, before >> 16, [&](int t, int r) EV_INLINE { from[r] = t; });
+    if (tid == 0) a.moves[hd.bk] = total & 0xFFFF;
+}
+
+// Longer caches: a workgroup per part of EV_PART slots, the slots below keep
+// and those from it on each in parts of their own, and a launch per pass of
+// the selection (STAGE 0 to 2: the part's bins go to memory), with a last one
+// for the lists.  Every workgroup forms the digits found so far from all
+// parts' bins; from them also follow the numbers of rows that stay in the
+// parts before its own, and with these the ranks of its holes or movers.
+template <int STAGE> __global__ void __launch_bounds__(EV_WG) k_evict_part(KvEvictArgs a)
+{
+    __shared__ uint32_t hist[STAGE == 0 ? EV_COPIES * EV_BINS : EV_BINS];
+    __shared__ int s_cnt[EV_WAVES], s_out[3];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int part = blockIdx.x % a.parts, n_low = (a.keep + EV_PART - 1) / EV_PART;
+    const EvHead hd = evict_head(a, blockIdx.x / a.parts, STAGE == 3 && part == 0);
+    if (!hd.act) return;
+    const bool lower = part < n_low;
+    const int64_t t0 = lower ? (int64_t)part * EV_PART : a.keep + (int64_t)(part - n_low) * EV_PART;
+    if (t0 >= hd.n) return;
+    const int t1 = min((int64_t)(lower ? a.keep : hd.n), t0 + EV_PART);
+    const int parts = n_low + (hd.n - a.keep + EV_PART - 1) / EV_PART;  // of this head
+    EvKeys k;
+    k.load(a, (int64_t)hd.bk * a.kv.cap, t0, t1, wave, a.pos[hd.b]);
+    if constexpr (STAGE < 3)
+        for (int i = tid; i < (STAGE == 0 ? EV_COPIES : 1) * EV_BINS; i += EV_WG) hist[i] = 0;
+    uint32_t *mine = a.bins + ((int64_t)hd.bk * a.parts + part) * EV_HIST;
+    const uint32_t *all = a.bins + (int64_t)hd.bk * a.parts * EV_HIST;
+    EvPick pick{0, a.keep, 0};
+    // rows above the prefix in the parts of this part's kind before it; ties
+    // in all parts before it, and in those before its kind
+    int above = 0, ties = 0, ties_low = 0;
+    const int kind = lower ? 0 : n_low;
+#pragma unroll
+    for (int pass = 0; pass < STAGE; pass++) {
+        const int top = pass_bins(pass) - 1 - 2 * tid;
+        int c[2] = {0, 0}, bef[2] = {0, 0}, lo[2] = {0, 0};
+        if (top > 0)
+            for (int q = 0; q < parts; q++) {
+                const uint2 v = *(const uint2 *)(all + (int64_t)q * EV_HIST + pass * EV_BINS + top - 1);
+                const int w[2] = {(int)v.y, (int)v.x};
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    c[i] += w[i];
+                    bef[i] += q < part ? w[i] : 0;
+                    lo[i] += q < kind ? w[i] : 0;
+                }
+            }
+        const int d = pick.digit(pass, c[0], c[1], wave, s_cnt, s_out);
+        if (STAGE == 3) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                above += top - i > d ? bef[i] - lo[i] : 0;
+                if (pass == 2 && top - i == d) {
+                    ties += bef[i];
+                    ties_low += lo[i];
+                }
+            }
         }
-        __syncthreads();
-        if (tid == 0) {
-            int above = 0, d = 255;
-            for (; d > 0 && above + (int)hist[d] < need; d--) above += hist[d];
-            s_digit = d;
-            s_above = above;
-        }
-        __syncthreads();
-        prefix |= s_digit << shift;
-        mask |= 255u << shift;
-        need -= s_above;
         __syncthreads();
     }
-    // keys above the prefix stay, and the first `need` that equal it
-    int32_t *map = a.map + (int64_t)bk * a.keep, *holes = a.holes + (int64_t)bk * a.keep;
-    int ties = 0, n_holes = 0, n_moved = 0;
-    for (int t0 = 0; t0 < n; t0 += EV_WG) {
-        const int t = t0 + tid;
-        const uint32_t k = t < n ? evict_key(a, base, t, newest) : 0;
-        const Before eq = count_before(t < n && k == prefix, cnt);
-        const bool stays = t < n && (k > prefix || (k == prefix && ties + eq.rank < need));
-        ties += eq.total;
-        const bool hole = t < a.keep && !stays, mover = stays && t >= a.keep;
-        const Before h = count_before(hole, cnt);
-        if (hole) holes[n_holes + h.rank] = t;
-        if (t < a.keep && stays) map[t] = t;
-        n_holes += h.total;
-        // (a mover's hole is below keep, so it has been written: in an
-        // earlier round, or in this one before the barrier)
-        const Before mv = count_before(mover, cnt);
-        if (mover) map[holes[n_moved + mv.rank]] = t;
-        n_moved += mv.total;
+    if constexpr (STAGE < 3) {
+        __syncthreads();
+        k.count(STAGE, pick.prefix, hist + (STAGE == 0 ? lane % EV_COPIES * EV_BINS : 0));
+        __syncthreads();
+        for (int i = tid; i < pass_bins(STAGE); i += EV_WG) {
+            uint32_t v = hist[i];
+            if (STAGE == 0)
+                for (int c = 1; c < EV_COPIES; c++) v += hist[c * EV_BINS + i];
+            mine[STAGE * EV_BINS + i] = v;
+        }
+    } else {
+        int all_above, all_ties_before, all_ties_low;
+        waves_before(last_lane(scan_add(above)), wave, s_cnt, &all_above);
+        waves_before(last_lane(scan_add(ties)), wave, s_cnt, &all_ties_before);
+        waves_before(last_lane(scan_add(ties_low)), wave, s_cnt, &all_ties_low);
+        const bool all_ties = pick.equal == pick.need;
+        int eq = 0;
+        if (!all_ties)
+            k.each([&](int, uint32_t v, bool there) EV_INLINE { eq += __popcll(__ballot(there && v == pick.prefix)); });
+        const int eq_before = waves_before(eq, wave, s_cnt);
+        const u64 stay = k.masks(pick.prefix, all_ties, pick.need, all_ties_before + eq_before), low = k.low(a.keep);
+        if (low) a.stay[(int64_t)hd.bk * a.stay_words + k.first / 64 + lane] = stay;
+        // rows that stay in this kind's parts before this one
+        const int stays = all_above + min(pick.need, all_ties_before) - min(pick.need, all_ties_low);
+        const u64 out = lower ? ~stay & low : stay;
+        int total;
+        const int before = waves_before(last_lane(scan_add(__popcll(out))), wave, s_cnt, &total);
+        const int rank = lower ? (int)t0 - stays : stays;
+        int32_t *list = (lower ? a.holes : a.movers) + (int64_t)hd.bk * a.keep;
+        k.emit(out, rank + before, [&](int t, int r) EV_INLINE { list[r] = t; });
+        if (part == parts - 1 && tid == 0) a.moves[hd.bk] = rank + total;
     }
 }
 
-// 256 places of one kv head: weights and positions, then the rows of the
-// places whose row changes, one after another by a wave.
+// The moves of a list: weight and position by one lane, the rows of K and V
+// by ROW16 lanes, MV_DEEP moves in flight for each; workgroups past
+// move_tiles per head: weights and positions of the rows that lie still,
+// where these go to other buffers.
 template <int ROW16>  // 16-byte pieces of a row
 __global__ void __launch_bounds__(MV_WG) k_evict_move(KvEvictArgs a)
 {
+    constexpr int GROUPS = MV_WG / ROW16, STEP = GROUPS * MV_DEEP;
     const KvView &kv = a.kv;
-    const int bk = blockIdx.x / a.copy_tiles, tile = blockIdx.x % a.copy_tiles;
-    const int b = bk / kv.nkv, kvh = bk % kv.nkv, n = a.len[b];
-    const bool act = n > a.trigger && n <= kv.cap;
-    const int left = act ? a.keep : n > kv.cap ? 0 : n;
-    const int lane = threadIdx.x & 63, s = tile * MV_SLOTS + threadIdx.x;
-    if (tile * MV_SLOTS >= left) return;
+    const int tiles = a.move_tiles + a.copy_tiles, bk = blockIdx.x / tiles, tile = blockIdx.x % tiles;
+    const int b = bk / kv.nkv, kvh = bk % kv.nkv, tid = threadIdx.x;
     const int64_t base = (int64_t)bk * kv.cap;
-    int src = s;
-    if (s < left) {
-        if (act) src = a.map[(int64_t)bk * a.keep + s];
-        a.acc_out[base + s] = a.acc_in[base + src];
-        a.pos_out[base + s] = a.pos_in[base + src];
-    }
-    const int32_t *tab = kv.table + (int64_t)b * kv.table_len;
-    int from = -1, to = -1;
-    if (src != s) {
-        from = kv.row(tab, src);
-        to = kv.row(tab, s);
-    }
-    unsigned long long todo = __ballot(from >= 0 && to >= 0);
-    const int64_t stride = (int64_t)kv.nkv * ROW16;
-    while (todo) {
-        const int l = __builtin_ctzll(todo);
-        todo &= todo - 1;
-        const int64_t f = __builtin_amdgcn_readlane(from, l) * stride + kvh * ROW16;
-        const int64_t d = __builtin_amdgcn_readlane(to, l) * stride + kvh * ROW16;
-        if (lane < ROW16) {
-            const styx_u4 k = ((const styx_u4 *)kv.kpool)[f + lane], v = ((const styx_u4 *)kv.vpool)[f + lane];
-            ((styx_u4 *)kv.kpool)[d + lane] = k;
-            ((styx_u4 *)kv.vpool)[d + lane] = v;
+    if (tile >= a.move_tiles) {
+        const int2 left = a.left[b];  // the new length, whether rows leave
+        const int n = left.x > kv.cap ? 0 : left.x;
+        const u64 *stay = a.stay + (int64_t)bk * a.stay_words;
+        const int s0 = (tile - a.move_tiles) * CP_SLOTS + tid;
+#pragma unroll
+        for (int j = 0; j < CP_SLOTS / MV_WG; j++) {
+            const int s = s0 + j * MV_WG;
+            if (s < n && (!left.y || (stay[s / 64] >> (s & 63)) & 1)) {
+                a.acc_out[base + s] = a.acc_in[base + s];
+                a.pos_out[base + s] = a.pos_in[base + s];
+            }
         }
+        return;
+    }
+    if (tile == 0 && kvh == 0 && tid == 0) a.len_out[b] = a.left[b].x;
+    const int moves = a.moves[bk];
+    const int32_t *tab = kv.table + (int64_t)b * kv.table_len;
+    const int32_t *to = a.holes + (int64_t)bk * a.keep, *from = a.movers + (int64_t)bk * a.keep;
+    const int64_t stride = (int64_t)kv.nkv * ROW16;
+    const int group = tid / ROW16, piece = kvh * ROW16 + tid % ROW16;
+    const styx_u4 *kp = (const styx_u4 *)kv.kpool + piece, *vp = (const styx_u4 *)kv.vpool + piece;
+    styx_u4 *kd = (styx_u4 *)kv.kpool + piece, *vd = (styx_u4 *)kv.vpool + piece;
+    for (int i0 = tile * STEP; i0 < moves; i0 += a.move_tiles * STEP) {
+        if (tid < STEP && i0 + tid < moves) {
+            const int f = from[i0 + tid], t = to[i0 + tid];
+            a.acc_out[base + t] = a.acc_in[base + f];
+            a.pos_out[base + t] = a.pos_in[base + f];
+        }
+        int f[MV_DEEP], t[MV_DEEP];
+        styx_u4 k[MV_DEEP], v[MV_DEEP];
+#pragma unroll
+        for (int j = 0; j < MV_DEEP; j++) {
+            const int i = min(i0 + group + j * GROUPS, moves - 1);
+            f[j] = from[i];
+            t[j] = to[i];
+        }
+#pragma unroll
+        for (int j = 0; j < MV_DEEP; j++) {
+            f[j] = kv.row(tab, f[j]);
+            t[j] = i0 + group + j * GROUPS < moves ? kv.row(tab, t[j]) : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < MV_DEEP; j++) {
+            k[j] = kp[max(f[j], 0) * stride];
+            v[j] = vp[max(f[j], 0) * stride];
+        }
+#pragma unroll
+        for (int j = 0; j < MV_DEEP; j++)
+            if (f[j] >= 0 && t[j] >= 0) {
+                kd[t[j] * stride] = k[j];
+                vd[t[j] * stride] = v[j];
+            }
     }
 }
 
-// Last, when no workgroup reads the lengths any more: they may be the
-// caller's own.
-__global__ void __launch_bounds__(256) k_evict_len(KvEvictArgs a)
+static int parts_of(int cap, int keep)
 {
-    const int b = blockIdx.x * 256 + threadIdx.x;
-    if (b >= a.kv.n_seq) return;
-    const int n = a.len[b];
-    a.len_out[b] = n > a.trigger && n <= a.kv.cap ? a.keep : n;
+    return cap <= EV_PART ? 1 : (keep + EV_PART - 1) / EV_PART + (cap - keep + EV_PART - 1) / EV_PART;
 }
 
-static int copy_tiles(const KvEvictArgs &a)
+// In 4-byte words: the lists, the masks of what stays, lengths, moves, bins.
+uint64_t kv_evict_ws_bytes(int n_seq, int nkv, int cap, int keep)
 {
-    // sequences that stay as they are are copied only into other buffers
-    const bool apart = a.acc_out != a.acc_in || a.pos_out != a.pos_in;
-    const int most = apart && a.trigger > a.keep ? std::min(a.trigger, a.kv.cap) : a.keep;
-    return (most - 1) / MV_SLOTS + 1;
+    const uint64_t heads = (uint64_t)n_seq * nkv, parts = parts_of(cap, keep);
+    return 4 * (2 * heads * ((keep + 63) / 64) + 2 * (uint64_t)n_seq + (heads + 1) / 2 * 2 + 2 * heads * keep +
+                (parts > 1 ? heads * parts * EV_HIST : 0));
 }
-int64_t kv_evict_grid(const KvEvictArgs &a) { return (int64_t)a.kv.n_seq * a.kv.nkv * copy_tiles(a); }
+
+static void evict_tiles(KvEvictArgs &a)
+{
+    const KvView &kv = a.kv;
+    const int heads = kv.n_seq * kv.nkv, most = std::min(a.keep, kv.cap - a.keep);
+    const int step = MV_WG / (kv.hd * (kv.f16 ? 2 : 4) / 16) * MV_DEEP;
+    // sixteen workgroups per CU, or one for every step of the longest list
+    a.move_tiles = std::max(1, std::min((most + step - 1) / step, 4096 / heads));
+    // rows that lie still are copied only into other buffers
+    const bool apart = a.acc_out != a.acc_in || a.pos_out != a.pos_in;
+    a.copy_tiles = apart ? (std::min(a.trigger, kv.cap) + CP_SLOTS - 1) / CP_SLOTS : 0;
+    a.parts = parts_of(kv.cap, a.keep);
+}
+int64_t kv_evict_grid(KvEvictArgs a)
+{
+    evict_tiles(a);
+    const int64_t heads = (int64_t)a.kv.n_seq * a.kv.nkv;
+    // (a part's workgroup is four of the others' size)
+    return heads * std::max<int64_t>(a.move_tiles + a.copy_tiles, 4 * (int64_t)a.parts);
+}
 
 hipError_t launch_kv_evict(hipStream_t st, KvEvictArgs a, void *ws)
 {
     const KvView &kv = a.kv;
-    const int heads = kv.n_seq * kv.nkv;
-    a.copy_tiles = copy_tiles(a);
-    a.map = (int32_t *)ws;
-    a.holes = a.map + (int64_t)heads * a.keep;
-    hipLaunchKernelGGL(k_evict_select, dim3(heads), dim3(EV_WG), 0, st, a);
+    const int64_t heads = (int64_t)kv.n_seq * kv.nkv;
+    evict_tiles(a);
+    a.stay_words = (a.keep + 63) / 64;
+    a.stay = (u64 *)ws;
+    a.left = (int2 *)(a.stay + heads * a.stay_words);
+    a.moves = (int32_t *)(a.left + kv.n_seq);
+    a.holes = a.moves + (heads + 1) / 2 * 2;
+    a.movers = a.holes + heads * a.keep;
+    a.bins = (uint32_t *)(a.movers + heads * a.keep);
+    if (a.parts == 1) {
+        hipLaunchKernelGGL(k_evict_select, dim3((unsigned)heads), dim3(EV_WG), 0, st, a);
+    } else {
+        const dim3 grid((unsigned)(heads * a.parts));
+        hipLaunchKernelGGL(k_evict_part<0>, grid, dim3(EV_WG), 0, st, a);
+        hipLaunchKernelGGL(k_evict_part<1>, grid, dim3(EV_WG), 0, st, a);
+        hipLaunchKernelGGL(k_evict_part<2>, grid, dim3(EV_WG), 0, st, a);
+        hipLaunchKernelGGL(k_evict_part<3>, grid, dim3(EV_WG), 0, st, a);
+    }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const dim3 grid((unsigned)(heads * a.copy_tiles));
+    const dim3 grid((unsigned)(heads * (a.move_tiles + a.copy_tiles)));
     switch (kv.hd * (kv.f16 ? 2 : 4) / 16) {
     case 8: hipLaunchKernelGGL(k_evict_move<8>, grid, dim3(MV_WG), 0, st, a); break;
     case 16: hipLaunchKernelGGL(k_evict_move<16>, grid, dim3(MV_WG), 0, st, a); break;
     case 32: hipLaunchKernelGGL(k_evict_move<32>, grid, dim3(MV_WG), 0, st, a); break;
     default: hipLaunchKernelGGL(k_evict_move<64>, grid, dim3(MV_WG), 0, st, a); break;
     }
-    e = hipGetLastError();
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(k_evict_len, dim3((kv.n_seq + 255) / 256), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 

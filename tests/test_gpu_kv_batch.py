@@ -452,6 +452,23 @@ def test_evict_long(gpu):
     same(run_evict(gpu, c, 10000, 10000, 500, 4), want_evict(c, 10000, 10000, 500, 4))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("keep,in_place", [(1, False), (100, True), (16384, False), (16385, True), (25000, False),
+                                           (36000, True)])
+@pytest.mark.parametrize("weights", ["drawn", "few", "equal"])
+def test_evict_caches_of_several_parts(gpu, keep, in_place, weights):
+    """Past 16K slots a head is selected by several workgroups: ties that run
+    over their borders, sequences that end inside a part or do not reach it."""
+    rng = np.random.default_rng(keep)
+    c = evict_case(rng, True, [36863, 100, keep + 1, 16384 * 2 + 3, 20000], 1, 64, 512, table_len=72)
+    if weights == "few":
+        c.acc = rng.integers(0, 3, c.acc.shape).astype(np.float32)
+    elif weights == "equal":
+        c.acc[:] = 1.5
+    recent, sinks = min(keep // 2, 300), min(keep // 4, 4)
+    same(run_evict(gpu, c, keep, keep, recent, sinks, in_place), want_evict(c, keep, keep, recent, sinks, in_place))
+
+
 # ------------------------------------------------------------ refusals -----
 def cache(**kw):
     d = dict(type=L.F32, n_seq=2, nkv=2, hd=128, page_tokens=16, n_pages=4, table_len=2, kpool=256, vpool=256,
