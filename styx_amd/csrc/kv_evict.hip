@@ -24,8 +24,8 @@
 namespace styx {
 
 constexpr int EV_WG = 1024, EV_WAVES = EV_WG / 64;
-constexpr int EV_KPT = 16;                // keys of a thread, in registers
-constexpr int EV_PART = EV_WG * EV_KPT;   // slots that a workgroup selects from
+constexpr int EV_KPT = 16;                // most keys of a thread, in registers
+constexpr int EV_PART = EV_WG * EV_KPT;   // most slots that a workgroup selects from
 constexpr int EV_BINS = 2048, EV_COPIES = 4;
 constexpr int EV_LDS = (EV_COPIES + 2) * EV_BINS;
 constexpr int EV_HIST = 2 * EV_BINS + EV_BINS / 2;  // bins of a part's three passes
@@ -92,10 +92,10 @@ __host__ __device__ constexpr int pass_shift(int p) { return p == 0 ? 21 : p == 
 __host__ __device__ constexpr int pass_bins(int p) { return p == 2 ? EV_BINS / 2 : EV_BINS; }
 __host__ __device__ constexpr uint32_t pass_mask(int p) { return p == 0 ? 0u : p == 1 ? 0xFFE00000u : 0xFFFFFC00u; }
 
-// The keys of up to EV_PART slots from t0 on, the waves each a contiguous run
+// The keys of up to EV_WG * KPT slots from t0 on, the waves each a contiguous run
 // of rows of 64 slots, a lane one slot of each row.
-struct EvKeys {
-    uint32_t key[EV_KPT];
+template <int KPT> struct EvKeys {
+    uint32_t key[KPT];
     int per, first, end, lane;  // rows of a wave, its first slot, the slots' end
     __device__ __forceinline__ void load(const KvEvictArgs &a, int64_t base, int t0, int t1, int wave, int64_t newest)
     {
@@ -103,22 +103,22 @@ struct EvKeys {
         per = (t1 - t0 + EV_WG - 1) / EV_WG;
         first = t0 + wave * per * 64;
         end = t1;
-        float w[EV_KPT];
-        int32_t p[EV_KPT];
+        float w[KPT];
+        int32_t p[KPT];
 #pragma unroll
-        for (int j = 0; j < EV_KPT; j++) {
+        for (int j = 0; j < KPT; j++) {
             if (j >= per) break;
             const int t = min(first + 64 * j + lane, t1 - 1);
             w[j] = a.acc_in[base + t];
             p[j] = a.pos_in[base + t];
         }
 #pragma unroll
-        for (int j = 0; j < EV_KPT; j++) key[j] = j < per ? evict_key(a, w[j], p[j], newest) : 0;
+        for (int j = 0; j < KPT; j++) key[j] = j < per ? evict_key(a, w[j], p[j], newest) : 0;
     }
     // f(row, key, whether there is one), the wave's lanes together
     template <typename F> __device__ __forceinline__ void each(F f) const
     {
-        unrolled<EV_KPT>([&](auto j) EV_INLINE {
+        unrolled<KPT>([&](auto j) EV_INLINE {
             if (j < per) f((int)j, key[j], first + 64 * j + lane < end);
         });
     }
@@ -218,11 +218,11 @@ __device__ __forceinline__ EvHead evict_head(const KvEvictArgs &a, int bk, bool 
     return h;
 }
 
-// Caches of up to EV_PART slots: one workgroup per sequence and kv head.  One
+// Caches of up to EV_WG * KPT slots: one workgroup per sequence and kv head.  One
 // CU does all of a head's work, so what counts are instructions per key and
 // barriers.  The first pass counts every key, and weights of one size crowd
 // into few bins: four copies of them, by lane, keep the adds of a wave apart.
-__global__ void __launch_bounds__(EV_WG) k_evict_select(KvEvictArgs a)
+template <int KPT> __global__ void __launch_bounds__(EV_WG) k_evict_select(KvEvictArgs a)
 {
     // bins of the three passes
     __shared__ uint32_t hist[EV_LDS];
@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(EV_WG) k_evict_select(KvEvictArgs a)
     const EvHead hd = evict_head(a, blockIdx.x, true);
     if (!hd.act) return;
     for (int i = tid; i < EV_LDS; i += EV_WG) hist[i] = 0;
-    EvKeys k;
+    EvKeys<KPT> k;
     k.load(a, (int64_t)hd.bk * a.kv.cap, 0, hd.n, wave, a.pos[hd.b]);
     EvPick pick{0, a.keep, 0};
 #pragma unroll 1
@@ -269,26 +269,27 @@ __global__ void __launch_bounds__(EV_WG) k_evict_select(KvEvictArgs a)
     if (tid == 0) a.moves[hd.bk] = total & 0xFFFF;
 }
 
-// Longer caches: a workgroup per part of EV_PART slots, the slots below keep
+// Longer caches: a workgroup per part of EV_WG * KPT slots, the slots below keep
 // and those from it on each in parts of their own, and a launch per pass of
 // the selection (STAGE 0 to 2: the part's bins go to memory), with a last one
 // for the lists.  Every workgroup forms the digits found so far from all
 // parts' bins; from them also follow the numbers of rows that stay in the
 // parts before its own, and with these the ranks of its holes or movers.
-template <int STAGE> __global__ void __launch_bounds__(EV_WG) k_evict_part(KvEvictArgs a)
+template <int STAGE, int KPT> __global__ void __launch_bounds__(EV_WG) k_evict_part(KvEvictArgs a)
 {
+    constexpr int PART = EV_WG * KPT;
     __shared__ uint32_t hist[STAGE == 0 ? EV_COPIES * EV_BINS : EV_BINS];
     __shared__ int s_cnt[EV_WAVES], s_out[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int part = blockIdx.x % a.parts, n_low = (a.keep + EV_PART - 1) / EV_PART;
+    const int part = blockIdx.x % a.parts, n_low = (a.keep + PART - 1) / PART;
     const EvHead hd = evict_head(a, blockIdx.x / a.parts, STAGE == 3 && part == 0);
     if (!hd.act) return;
     const bool lower = part < n_low;
-    const int64_t t0 = lower ? (int64_t)part * EV_PART : a.keep + (int64_t)(part - n_low) * EV_PART;
+    const int64_t t0 = lower ? (int64_t)part * PART : a.keep + (int64_t)(part - n_low) * PART;
     if (t0 >= hd.n) return;
-    const int t1 = min((int64_t)(lower ? a.keep : hd.n), t0 + EV_PART);
-    const int parts = n_low + (hd.n - a.keep + EV_PART - 1) / EV_PART;  // of this head
-    EvKeys k;
+    const int t1 = min((int64_t)(lower ? a.keep : hd.n), t0 + PART);
+    const int parts = n_low + (hd.n - a.keep + PART - 1) / PART;  // of this head
+    EvKeys<KPT> k;
     k.load(a, (int64_t)hd.bk * a.kv.cap, t0, t1, wave, a.pos[hd.b]);
     if constexpr (STAGE < 3)
         for (int i = tid; i < (STAGE == 0 ? EV_COPIES : 1) * EV_BINS; i += EV_WG) hist[i] = 0;
@@ -304,14 +305,20 @@ template <int STAGE> __global__ void __launch_bounds__(EV_WG) k_evict_part(KvEvi
         const int top = pass_bins(pass) - 1 - 2 * tid;
         int c[2] = {0, 0}, bef[2] = {0, 0}, lo[2] = {0, 0};
         if (top > 0)
-            for (int q = 0; q < parts; q++) {
-                const uint2 v = *(const uint2 *)(all + (int64_t)q * EV_HIST + pass * EV_BINS + top - 1);
-                const int w[2] = {(int)v.y, (int)v.x};
+            for (int q0 = 0; q0 < parts; q0 += 8) {
+                uint2 v[8];
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    c[i] += w[i];
-                    bef[i] += q < part ? w[i] : 0;
-                    lo[i] += q < kind ? w[i] : 0;
+                for (int j = 0; j < 8; j++)
+                    v[j] = *(const uint2 *)(all + (int64_t)min(q0 + j, parts - 1) * EV_HIST + pass * EV_BINS + top - 1);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int q = q0 + j, w[2] = {q < parts ? (int)v[j].y : 0, q < parts ? (int)v[j].x : 0};
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        c[i] += w[i];
+                        bef[i] += q < part ? w[i] : 0;
+                        lo[i] += q < kind ? w[i] : 0;
+                    }
                 }
             }
         const int d = pick.digit(pass, c[0], c[1], wave, s_cnt, s_out);
@@ -429,15 +436,24 @@ __global__ void __launch_bounds__(MV_WG) k_evict_move(KvEvictArgs a)
     }
 }
 
-static int parts_of(int cap, int keep)
+// Keys of a selecting thread, and parts of a head.  Parts of 4K slots where
+// 16K would not give every CU one: 16 heads of 64K rows, 61 us with 16K in
+// the four launches, 41 with 4K.
+static int parts_in(int cap, int keep, int part) { return (keep - 1) / part + (cap - keep + part - 1) / part + 1; }
+static int keys_of(int64_t heads, int cap, int keep)
 {
-    return cap <= EV_PART ? 1 : (keep + EV_PART - 1) / EV_PART + (cap - keep + EV_PART - 1) / EV_PART;
+    if (cap <= EV_PART) return cap <= 4 * EV_WG ? 4 : 16;
+    return heads * parts_in(cap, keep, EV_PART) < 256 ? 4 : 16;
+}
+static int parts_of(int64_t heads, int cap, int keep)
+{
+    return cap <= EV_PART ? 1 : parts_in(cap, keep, keys_of(heads, cap, keep) * EV_WG);
 }
 
 // In 4-byte words: the lists, the masks of what stays, lengths, moves, bins.
 uint64_t kv_evict_ws_bytes(int n_seq, int nkv, int cap, int keep)
 {
-    const uint64_t heads = (uint64_t)n_seq * nkv, parts = parts_of(cap, keep);
+    const uint64_t heads = (uint64_t)n_seq * nkv, parts = parts_of(heads, cap, keep);
     return 4 * (2 * heads * ((keep + 63) / 64) + 2 * (uint64_t)n_seq + (heads + 1) / 2 * 2 + 2 * heads * keep +
                 (parts > 1 ? heads * parts * EV_HIST : 0));
 }
@@ -452,7 +468,7 @@ static void evict_tiles(KvEvictArgs &a)
     // rows that lie still are copied only into other buffers
     const bool apart = a.acc_out != a.acc_in || a.pos_out != a.pos_in;
     a.copy_tiles = apart ? (std::min(a.trigger, kv.cap) + CP_SLOTS - 1) / CP_SLOTS : 0;
-    a.parts = parts_of(kv.cap, a.keep);
+    a.parts = parts_of(heads, kv.cap, a.keep);
 }
 int64_t kv_evict_grid(KvEvictArgs a)
 {
@@ -460,6 +476,15 @@ int64_t kv_evict_grid(KvEvictArgs a)
     const int64_t heads = (int64_t)a.kv.n_seq * a.kv.nkv;
     // (a part's workgroup is four of the others' size)
     return heads * std::max<int64_t>(a.move_tiles + a.copy_tiles, 4 * (int64_t)a.parts);
+}
+
+template <int KPT> static void launch_parts(hipStream_t st, const KvEvictArgs &a, int64_t heads)
+{
+    const dim3 grid((unsigned)(heads * a.parts));
+    hipLaunchKernelGGL((k_evict_part<0, KPT>), grid, dim3(EV_WG), 0, st, a);
+    hipLaunchKernelGGL((k_evict_part<1, KPT>), grid, dim3(EV_WG), 0, st, a);
+    hipLaunchKernelGGL((k_evict_part<2, KPT>), grid, dim3(EV_WG), 0, st, a);
+    hipLaunchKernelGGL((k_evict_part<3, KPT>), grid, dim3(EV_WG), 0, st, a);
 }
 
 hipError_t launch_kv_evict(hipStream_t st, KvEvictArgs a, void *ws)
@@ -474,14 +499,16 @@ hipError_t launch_kv_evict(hipStream_t st, KvEvictArgs a, void *ws)
     a.holes = a.moves + (heads + 1) / 2 * 2;
     a.movers = a.holes + heads * a.keep;
     a.bins = (uint32_t *)(a.movers + heads * a.keep);
+    const int keys = keys_of(heads, kv.cap, a.keep);
     if (a.parts == 1) {
-        hipLaunchKernelGGL(k_evict_select, dim3((unsigned)heads), dim3(EV_WG), 0, st, a);
+        if (keys == 4)
+            hipLaunchKernelGGL(k_evict_select<4>, dim3((unsigned)heads), dim3(EV_WG), 0, st, a);
+        else
+            hipLaunchKernelGGL(k_evict_select<16>, dim3((unsigned)heads), dim3(EV_WG), 0, st, a);
+    } else if (keys == 4) {
+        launch_parts<4>(st, a, heads);
     } else {
-        const dim3 grid((unsigned)(heads * a.parts));
-        hipLaunchKernelGGL(k_evict_part<0>, grid, dim3(EV_WG), 0, st, a);
-        hipLaunchKernelGGL(k_evict_part<1>, grid, dim3(EV_WG), 0, st, a);
-        hipLaunchKernelGGL(k_evict_part<2>, grid, dim3(EV_WG), 0, st, a);
-        hipLaunchKernelGGL(k_evict_part<3>, grid, dim3(EV_WG), 0, st, a);
+        launch_parts<16>(st, a, heads);
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;

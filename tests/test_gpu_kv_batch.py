@@ -460,7 +460,8 @@ def test_evict_caches_of_several_parts(gpu, keep, in_place, weights):
     """Past 16K slots a head is selected by several workgroups: ties that run
     over their borders, sequences that end inside a part or do not reach it."""
     rng = np.random.default_rng(keep)
-    c = evict_case(rng, True, [36863, 100, keep + 1, 16384 * 2 + 3, 20000], 1, 64, 512, table_len=72)
+    lens = [36863, 100, keep + 1, 16384 * 2 + 3, 20000]
+    c = evict_case(rng, True, lens * (20 if keep == 25000 and weights == "few" else 1), 1, 64, 512, table_len=72)
     if weights == "few":
         c.acc = rng.integers(0, 3, c.acc.shape).astype(np.float32)
     elif weights == "equal":
