@@ -29,6 +29,7 @@
 
 #include "attn16.h"
 #include "attn_batch.h"
+#include "lanes.h"
 
 namespace styx {
 
@@ -49,52 +50,6 @@ constexpr int AB_BATCH = 8;
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-
-__device__ __forceinline__ int wave_scan(int v)  // inclusive, over the wave
-{
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
-}
-// Sums over the wave by lane permutes (bfly's steps, qdot.h), every lane
-// getting the result.
-template <int CTRL> __device__ __forceinline__ uint32_t dpp_u(uint32_t v)
-{
-    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
-}
-template <typename T, typename Step> __device__ __forceinline__ T wave_sum_by(T v, Step step)
-{
-    v += step(v, [](uint32_t x) { return dpp_u<0xB1>(x); });
-    v += step(v, [](uint32_t x) { return dpp_u<0x4E>(x); });
-    v += step(v, [](uint32_t x) { return dpp_u<0x141>(x); });
-    v += step(v, [](uint32_t x) { return dpp_u<0x140>(x); });
-    // the other of a pair of rows, then of halves: the two words that a swap
-    // returns are one's own and the partner's
-    v += step(v, [](uint32_t x) {
-        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-        return (threadIdx.x & 16) ? r[0] : r[1];
-    });
-    v += step(v, [](uint32_t x) {
-        const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-        return (threadIdx.x & 32) ? r[0] : r[1];
-    });
-    return v;
-}
-__device__ __forceinline__ double wave_sum64(double v)
-{
-    return wave_sum_by(v, [](double x, auto f) {
-        const uint64_t u = __builtin_bit_cast(uint64_t, x);
-        return __builtin_bit_cast(double, (uint64_t)f((uint32_t)(u >> 32)) << 32 | f((uint32_t)u));
-    });
-}
-__device__ __forceinline__ uint32_t wave_sum_u(uint32_t v)
-{
-    return wave_sum_by(v, [](uint32_t x, auto f) { return f(x); });
-}
 
 // Rows that the new token of sequence b sees, itself among them; 0: skipped.
 __device__ __forceinline__ int rows_of(const AttnBatchArgs &a, int b)
@@ -148,27 +103,27 @@ __device__ __forceinline__ RowSplit split_rows(const AttnBatchArgs &a)
         all += head_units(sp, r);
         seqs += r > 0;
     }
-    all = wave_sum_u(all) * nkv;
-    const uint32_t heads = wave_sum_u(seqs) * nkv, least = (all + slots - 1) / slots;
+    all = wave_total(all) * nkv;
+    const uint32_t heads = wave_total(seqs) * nkv, least = (all + slots - 1) / slots;
     sp.share = least + (least == 0);
     if (heads < slots) {
         // at most all / share and one for every head
         const uint32_t most = (all + slots - heads - 1) / (slots - heads);
         uint32_t at = most;
         if (a.kv.n_seq <= 64)
-            for (at = sp.share; at < most && wave_sum_u((u + at - 1) / at) * nkv > slots; at++)
+            for (at = sp.share; at < most && wave_total((u + at - 1) / at) * nkv > slots; at++)
                 ;
         if (at <= least + (a.kv.f16 ? AB_MORE_F16 : AB_MORE_F32)) {
             sp.padded = 1;
             sp.share = at;
         }
     }
-    sp.upto = wave_scan(head_units(sp, sp.mine) * nkv);
+    sp.upto = wave_upto(head_units(sp, sp.mine) * nkv);
     sp.units = __builtin_amdgcn_readlane(sp.upto, 63);
     if (a.kv.n_seq > 64) {
         uint32_t more = 0;
         for (int b = lane + 64; b < a.kv.n_seq; b += 64) more += head_units(sp, rows_of(a, b)) * nkv;
-        sp.units += wave_sum_u(more);
+        sp.units += wave_total(more);
     }
     return sp;
 }
@@ -186,7 +141,7 @@ __device__ __forceinline__ SeqAt seq_find(const AttnBatchArgs &a, const RowSplit
     uint32_t base = 0;
     for (int b0 = 0;; b0 += 64) {
         const int rows = b0 ? rows_of(a, b0 + lane) : sp.mine;
-        const uint32_t upto = b0 ? base + wave_scan(head_units(sp, rows) * a.kv.nkv) : sp.upto;
+        const uint32_t upto = b0 ? base + wave_upto(head_units(sp, rows) * a.kv.nkv) : sp.upto;
         if (const unsigned long long hit = __ballot(upto > u)) {
             const int l = __builtin_ctzll(hit), r = __builtin_amdgcn_readlane(rows, l);
             return {b0 + l, r, __builtin_amdgcn_readlane(upto, l) - head_units(sp, r) * a.kv.nkv};
@@ -212,7 +167,7 @@ __device__ __forceinline__ void split_store(const AttnBatchArgs &a, const RowSpl
     for (int b0 = 0; b0 < a.kv.n_seq; b0 += 64) {
         const int rows = b0 ? rows_of(a, b0 + lane) : sp.mine;
         const uint32_t mine = head_units(sp, rows) * a.kv.nkv;
-        const uint32_t upto = b0 ? base + wave_scan(mine) : sp.upto;
+        const uint32_t upto = b0 ? base + wave_upto(mine) : sp.upto;
         if (b0 + lane < a.kv.n_seq) a.plan[2 + b0 + lane] = upto - mine;
         base = __builtin_amdgcn_readlane(upto, 63);
     }
@@ -250,7 +205,7 @@ template <int HD> struct HeadRow {
 #pragma unroll
             for (int j = 0; j < PPL; j++)
                 if (HALF >= 64 || lane < HALF) ss += (double)x0[j] * x0[j] + (double)x1[j] * x1[j];
-            f = 1.0 / sqrt(wave_sum64(ss) * (1.0 / HD) + (double)eps);
+            f = 1.0 / sqrt(wave_total(ss) * (1.0 / HD) + (double)eps);
         }
 #pragma unroll
         for (int j = 0; j < PPL; j++) {

@@ -20,6 +20,7 @@
 #include <type_traits>
 
 #include "attn_batch.h"
+#include "lanes.h"
 
 namespace styx {
 
@@ -44,21 +45,6 @@ __device__ __forceinline__ uint32_t evict_key(const KvEvictArgs &a, float weight
     const uint32_t u = __float_as_uint(w);
     return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
-
-// Inclusive sums over the wave by lane permutes: within rows of 16, then the
-// rows' last lanes passed on (row_bcast:15 to rows 1 and 3, :31 to the upper
-// half).
-__device__ __forceinline__ int scan_add(int v)
-{
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-    return v;
-}
-__device__ __forceinline__ int last_lane(int v) { return __builtin_amdgcn_readlane(v, 63); }
 
 // Sum of the earlier waves' v (uniform in a wave), *total that of all.  Every
 // thread takes part.
@@ -160,7 +146,7 @@ template <int KPT> struct EvKeys {
     // from `rank` on.
     template <typename F> __device__ __forceinline__ void emit(u64 p, int rank, F f) const
     {
-        const int c = __popcll(p), before = scan_add(c) - c + rank;
+        const int c = (int)__popcll(p), before = wave_upto(c) - c + rank;
         u64 rows = __ballot(c > 0);
         while (rows) {
             const int j = __builtin_ctzll(rows);
@@ -182,8 +168,8 @@ struct EvPick {
     // the top.  Every thread takes part; s [EV_WAVES], o [3].
     __device__ __forceinline__ int digit(int pass, int c0, int c1, int wave, int *s, int *o)
     {
-        const int top = pass_bins(pass) - 1 - 2 * (int)threadIdx.x, incl = scan_add(c0 + c1);
-        const int above = waves_before(last_lane(incl), wave, s) + incl - c0 - c1;
+        const int top = pass_bins(pass) - 1 - 2 * (int)threadIdx.x, incl = wave_upto(c0 + c1);
+        const int above = waves_before(of_lane(incl, 63), wave, s) + incl - c0 - c1;
         if (above < need && above + c0 + c1 >= need) {
             const bool second = above + c0 < need;
             o[0] = second ? top - 1 : top;
@@ -262,7 +248,7 @@ template <int KPT> __global__ void __launch_bounds__(EV_WG) k_evict_select(KvEvi
     const u64 holes = ~stay & low, movers = stay & ~low;
     // both counts in one sum: each is below 2^15
     int total;
-    const int before = waves_before(last_lane(scan_add(__popcll(holes) | __popcll(movers) << 16)), wave, s_cnt, &total);
+    const int before = waves_before(wave_total((int)(__popcll(holes) | __popcll(movers) << 16)), wave, s_cnt, &total);
     int32_t *to = a.holes + (int64_t)hd.bk * a.keep, *from = a.movers + (int64_t)hd.bk * a.keep;
     k.emit(holes, before & 0xFFFF, [&](int t, int r) EV_INLINE { to[r] = t; });
     k.emit(movers, before >> 16, [&](int t, int r) EV_INLINE { from[r] = t; });
@@ -346,9 +332,9 @@ template <int STAGE, int KPT> __global__ void __launch_bounds__(EV_WG) k_evict_p
         }
     } else {
         int all_above, all_ties_before, all_ties_low;
-        waves_before(last_lane(scan_add(above)), wave, s_cnt, &all_above);
-        waves_before(last_lane(scan_add(ties)), wave, s_cnt, &all_ties_before);
-        waves_before(last_lane(scan_add(ties_low)), wave, s_cnt, &all_ties_low);
+        waves_before(wave_total(above), wave, s_cnt, &all_above);
+        waves_before(wave_total(ties), wave, s_cnt, &all_ties_before);
+        waves_before(wave_total(ties_low), wave, s_cnt, &all_ties_low);
         const bool all_ties = pick.equal == pick.need;
         int eq = 0;
         if (!all_ties)
@@ -360,7 +346,7 @@ template <int STAGE, int KPT> __global__ void __launch_bounds__(EV_WG) k_evict_p
         const int stays = all_above + min(pick.need, all_ties_before) - min(pick.need, all_ties_low);
         const u64 out = lower ? ~stay & low : stay;
         int total;
-        const int before = waves_before(last_lane(scan_add(__popcll(out))), wave, s_cnt, &total);
+        const int before = waves_before(wave_total((int)__popcll(out)), wave, s_cnt, &total);
         const int rank = lower ? (int)t0 - stays : stays;
         int32_t *list = (lower ? a.holes : a.movers) + (int64_t)hd.bk * a.keep;
         k.emit(out, rank + before, [&](int t, int r) EV_INLINE { list[r] = t; });

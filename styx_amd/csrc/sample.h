@@ -19,15 +19,18 @@ struct SampleArgs {
     uint32_t *token;
     float *logprob;   // or null
     uint32_t *n_kept; // or null
-    // workspace, per row: the chunks' largest keys, sums and counts of kept
-    // words; weights and counts of the bins; border words
-    unsigned long long *cmax, *csum, *hw;
-    uint32_t *ccnt, *hc, *nlist, *list;
-    int G, ch;  // chunks of a row, words of a chunk
+    // workspace (filled by the launch), per row: the workgroups' largest keys;
+    // per block of words the sum and number of those that surely stay and the
+    // number of border words; weights and numbers of the bins; border words,
+    // each block's at its own place
+    unsigned long long *top, *sum, *hw;
+    uint32_t *cnt, *lcnt, *hc;
+    uint16_t *list;
+    int blocks, per, G;  // blocks of a row, of a workgroup; workgroups of a row
 };
 
 struct SampleWs {
-    int G, ch;
+    int blocks, per, G;
     int64_t bytes;
 };
 SampleWs sample_ws(int rows, int n);

@@ -11,18 +11,19 @@
 // left and t = floor(u S), the token is the first word, in the order of the
 // indices, at which the running sum exceeds t.
 //
-// Nothing is sorted.  Four launches over chunks of the rows:
+// Nothing is sorted.  Four launches over blocks of 2048 words:
 //   1 the rows' largest logits
 //   2 weight and number of the words in bins of 1/64 of (max - x) / T
 //   3 from these, the bins in which the k-th word and the end of the top-p
-//     run lie: the words of those bins go to a list, the weight that surely
-//     stays is summed per chunk
+//     run lie: the words of those bins are listed, the weight that surely
+//     stays is summed per block
 //   4 one workgroup per row: the border words in their order, which of them
-//     stay, and the token in its chunk
+//     stay, and the token in its block
 // Bound: latency for a few rows (each launch waits for all of the one
-// before), reads of the logits from HBM once and from the Infinity Cache
-// twice more for many.
+// before); for many, the f64 exponentials of launches 2 and 3 and one read of
+// the logits from HBM (the other two hit the Infinity Cache).
 #include "../../include/styx_hip.h"
+#include "lanes.h"
 #include "sample.h"
 
 #include <algorithm>
@@ -30,7 +31,10 @@
 namespace styx {
 
 constexpr int SA_WG = 256, FI_WG = 1024, FI_WAVES = FI_WG / 64;
-constexpr int SA_MIN = 2048;        // fewest words of a chunk
+constexpr int SA_BLOCK = 2048, SA_PER = SA_BLOCK / SA_WG;  // words of a block, of a thread
+constexpr int FI_BLOCKS = (SAMPLE_MAX_N + SA_BLOCK - 1) / SA_BLOCK;
+constexpr int FI_LIST = 2048;       // border words that are kept in LDS
+constexpr int FI_PAIRS = 256;       // words that are ranked each against all
 constexpr double SA_ONE = 17592186044416.0;  // 2^44
 typedef unsigned long long u64;
 
@@ -51,101 +55,97 @@ __device__ __forceinline__ uint32_t key_index(u64 k) { return ~(uint32_t)k; }
 
 struct RowAt {
     const float *x;
-    styx_sample_params p;
     u64 kmax;       // the first word
     float mx;
-    double inv_t;
+    double inv_t, p, min_w;
     bool greedy, top_p, min_p;
     int k;          // 0: all
 };
 
-__device__ __forceinline__ u64 wave_max64(u64 v)
-{
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const u64 o = __shfl_xor(v, d);
-        v = o > v ? o : v;
-    }
-    return v;
-}
-__device__ __forceinline__ u64 wave_add64(u64 v)
-{
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-    return v;
-}
-__device__ __forceinline__ u64 wave_scan64(u64 v)  // inclusive
-{
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const u64 o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
-}
-
-// The row's settings and, from the chunks, its first word; every wave by itself.
+// The row's settings and, from the workgroups, its first word; every wave by
+// itself.
 __device__ __forceinline__ RowAt row_at(const SampleArgs &a, int r)
 {
     RowAt w;
-    w.x = a.logits + r * a.ld;
-    w.p = a.params[a.one_params ? 0 : r];
+    const styx_sample_params p = a.params[a.one_params ? 0 : r];
     u64 k = 0;
     for (int c = threadIdx.x & 63; c < a.G; c += 64) {
-        const u64 o = a.cmax[(int64_t)r * a.G + c];
+        const u64 o = a.top[(int64_t)r * a.G + c];
         k = o > k ? o : k;
     }
-    w.kmax = wave_max64(k);
+    w.x = a.logits + r * a.ld;
+    w.kmax = wave_most(k);
     w.mx = key_value(w.kmax);
-    w.greedy = !(w.p.temperature > 0.0f);
-    w.inv_t = 1.0 / (double)w.p.temperature;
-    w.top_p = w.p.top_p < 1.0f;
-    w.min_p = w.p.min_p > 0.0f;
-    w.k = w.p.top_k > 0 && w.p.top_k < a.n ? w.p.top_k : 0;
+    w.greedy = !(p.temperature > 0.0f);
+    w.inv_t = 1.0 / (double)p.temperature;
+    w.top_p = p.top_p < 1.0f;
+    w.p = p.top_p;
+    w.min_p = p.min_p > 0.0f;
+    w.min_w = (double)p.min_p * SA_ONE;
+    w.k = p.top_k > 0 && p.top_k < a.n ? p.top_k : 0;
     return w;
 }
 
-__device__ __forceinline__ double word_dist(const RowAt &w, float x) { return ((double)w.mx - (double)x) * w.inv_t; }
 // Weight of a candidate, and its bin.
 __device__ __forceinline__ u64 word_weight(const RowAt &w, float x, int *bin)
 {
     *bin = 0;
     if (x == w.mx) return (u64)SA_ONE;
     if (!(x > -INFINITY) || w.mx == INFINITY) return 0;
-    const double d = word_dist(w, x);
+    const double d = ((double)w.mx - (double)x) * w.inv_t;
     if (!(d < 31.5)) return 0;
     *bin = (int)(d * 64.0);
     return (u64)rint(exp(-d) * SA_ONE);
 }
-__device__ __forceinline__ bool min_p_stays(const RowAt &w, u64 weight, u64 key)
+__device__ __forceinline__ bool min_p_stays(const RowAt &w, u64 weight, float x, uint32_t i)
 {
-    return !w.min_p || (double)weight >= (double)w.p.min_p * SA_ONE || key == w.kmax;
+    return !w.min_p || (double)weight >= w.min_w || word_key(x, i) == w.kmax;
+}
+
+// f(block) for the blocks of this workgroup.
+template <typename F> __device__ __forceinline__ void my_blocks(const SampleArgs &a, F f)
+{
+    const int b1 = min(a.blocks, (int)(blockIdx.x + 1) * a.per);
+    for (int b = blockIdx.x * a.per; b < b1; b++) f(b);
+}
+// A thread's words of a block, all in flight at once: word SA_WG j + thread;
+// words past the row are NaN.
+__device__ __forceinline__ void load_block(const SampleArgs &a, const float *x, int b, float (&v)[SA_PER])
+{
+    const int i0 = b * SA_BLOCK + threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < SA_PER; j++) v[j] = x[min(i0 + j * SA_WG, a.n - 1)];
+#pragma unroll
+    for (int j = 0; j < SA_PER; j++)
+        if (i0 + j * SA_WG >= a.n) v[j] = __int_as_float(0x7FC00000);
 }
 
 // ------------------------------------------------------------- 1: largest --
 __global__ void __launch_bounds__(SA_WG) k_sample_max(SampleArgs a)
 {
     __shared__ u64 s[SA_WG / 64];
-    const int c = blockIdx.x, r = blockIdx.y, c0 = c * a.ch, c1 = min(a.n, c0 + a.ch);
-    const float *x = a.logits + r * a.ld;
+    const int r = blockIdx.y;
     u64 k = 0;
-    for (int i = c0 + threadIdx.x; i < c1; i += SA_WG) {
-        const u64 o = word_key(x[i], i);
-        k = o > k ? o : k;
-    }
-    k = wave_max64(k);
+    my_blocks(a, [&](int b) {
+        float v[SA_PER];
+        load_block(a, a.logits + r * a.ld, b, v);
+#pragma unroll
+        for (int j = 0; j < SA_PER; j++) {
+            const u64 o = word_key(v[j], b * SA_BLOCK + j * SA_WG + threadIdx.x);
+            k = o > k ? o : k;
+        }
+    });
+    k = wave_most(k);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = k;
-    // the bins and the list of the row, emptied by its chunks together
-    for (int i = c * SA_WG + threadIdx.x; i < SAMPLE_BINS; i += a.G * SA_WG) {
+    // the row's bins, emptied by its workgroups together
+    for (int i = blockIdx.x * SA_WG + threadIdx.x; i < SAMPLE_BINS; i += a.G * SA_WG) {
         a.hw[(int64_t)r * SAMPLE_BINS + i] = 0;
         a.hc[(int64_t)r * SAMPLE_BINS + i] = 0;
     }
-    if (c == 0 && threadIdx.x == 0) a.nlist[r] = 0;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < SA_WG / 64; w++) k = s[w] > k ? s[w] : k;
-        a.cmax[(int64_t)r * a.G + c] = k;
+        a.top[(int64_t)r * a.G + blockIdx.x] = k;
     }
 }
 
@@ -154,18 +154,23 @@ __global__ void __launch_bounds__(SA_WG) k_sample_bins(SampleArgs a)
 {
     __shared__ u64 hw[SAMPLE_BINS];
     __shared__ uint32_t hc[SAMPLE_BINS];
-    const int c = blockIdx.x, r = blockIdx.y, c0 = c * a.ch, c1 = min(a.n, c0 + a.ch);
+    const int r = blockIdx.y;
     const RowAt w = row_at(a, r);
     if (w.kmax == 0 || w.greedy || !(w.top_p || w.k)) return;
     for (int i = threadIdx.x; i < SAMPLE_BINS; i += SA_WG) hw[i] = hc[i] = 0;
     __syncthreads();
-    for (int i = c0 + threadIdx.x; i < c1; i += SA_WG) {
-        int bin;
-        const u64 v = word_weight(w, w.x[i], &bin);
-        if (v == 0) continue;
-        atomicAdd(&hw[bin], v);
-        if (w.k) atomicAdd(&hc[bin], 1u);
-    }
+    my_blocks(a, [&](int b) {
+        float v[SA_PER];
+        load_block(a, w.x, b, v);
+#pragma unroll
+        for (int j = 0; j < SA_PER; j++) {
+            int bin;
+            const u64 m = word_weight(w, v[j], &bin);
+            if (m == 0) continue;
+            atomicAdd(&hw[bin], m);
+            if (w.k) atomicAdd(&hc[bin], 1u);
+        }
+    });
     __syncthreads();
     for (int i = threadIdx.x; i < SAMPLE_BINS; i += SA_WG)
         if (hw[i]) {
@@ -180,9 +185,10 @@ __global__ void __launch_bounds__(SA_WG) k_sample_bins(SampleArgs a)
 // are looked at one by one; all others leave.
 struct Border {
     int sure, p_end, k_bin;
-    u64 k_weight;   // weight and number of the bins before k_bin
     uint32_t k_count;
+    u64 k_weight;   // weight and number (k_count) of the bins before k_bin
     u64 p_weight;   // weight of the bins before `sure`
+    u64 total;      // of all bins
 };
 
 // All threads of the workgroup (NT of them) take part.
@@ -193,7 +199,7 @@ template <int NT> __device__ Border find_border(const SampleArgs &a, const RowAt
     __shared__ uint32_t s_c[NW];
     __shared__ Border s_b;
     __shared__ u64 s_lo, s_hi;
-    if (!(w.top_p || w.k)) return {SAMPLE_BINS, -1, -1, 0, 0, 0};
+    if (!(w.top_p || w.k)) return {SAMPLE_BINS, -1, -1, 0, 0, 0, 0};
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     u64 vw[PER], aw = 0;
     uint32_t vc[PER], ac = 0;
@@ -204,13 +210,12 @@ template <int NT> __device__ Border find_border(const SampleArgs &a, const RowAt
         aw += vw[j];
         ac += vc[j];
     }
-    u64 iw = wave_scan64(aw);
-    uint32_t ic = (uint32_t)wave_scan64(ac);
+    u64 iw = wave_upto(aw);
+    uint32_t ic = wave_upto(ac);
     if (lane == 63) {
         s_w[wave] = iw;
         s_c[wave] = ic;
     }
-    if (tid == 0) s_b = {SAMPLE_BINS, -1, -1, 0, 0, 0};
     __syncthreads();
     u64 total = 0;
     for (int q = 0; q < NW; q++) {
@@ -223,7 +228,10 @@ template <int NT> __device__ Border find_border(const SampleArgs &a, const RowAt
     // running sums before this thread's first bin
     const u64 w0 = iw - aw;
     const uint32_t k0 = ic - ac;
-    if (tid == 0) s_lo = s_hi = total;
+    if (tid == 0) {
+        s_b = {SAMPLE_BINS, -1, -1, 0, 0, 0, total};
+        s_lo = s_hi = total;
+    }
     __syncthreads();
     if (w.k) {
         u64 rw = w0;
@@ -243,12 +251,12 @@ template <int NT> __device__ Border find_border(const SampleArgs &a, const RowAt
             rw += vw[j];
             rc += vc[j];
         }
+        __syncthreads();
     }
-    __syncthreads();
     if (w.top_p) {
         // the run ends at the first word before which at least top_p S lies;
         // S is between s_lo and s_hi
-        const double lo = (double)w.p.top_p * (double)s_lo, hi = (double)w.p.top_p * (double)s_hi;
+        const double lo = w.p * (double)s_lo, hi = w.p * (double)s_hi;
         u64 rw = w0;
 #pragma unroll
         for (int j = 0; j < PER; j++) {
@@ -262,163 +270,238 @@ template <int NT> __device__ Border find_border(const SampleArgs &a, const RowAt
             if ((first || before < hi) && upto >= hi) s_b.p_end = bin;
             rw += vw[j];
         }
+        __syncthreads();
     }
-    __syncthreads();
     return s_b;
 }
 
 __global__ void __launch_bounds__(SA_WG) k_sample_border(SampleArgs a)
 {
     __shared__ u64 s_sum[SA_WG / 64];
-    __shared__ uint32_t s_cnt[SA_WG / 64];
-    const int c = blockIdx.x, r = blockIdx.y, c0 = c * a.ch, c1 = min(a.n, c0 + a.ch);
+    __shared__ uint32_t s_cnt[SA_WG / 64], s_n;
+    const int r = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const RowAt w = row_at(a, r);
     if (w.kmax == 0 || w.greedy) return;
     const Border bd = find_border<SA_WG>(a, w, r);
-    u64 sum = 0;
-    uint32_t cnt = 0;
-    for (int i = c0 + threadIdx.x; i < c1; i += SA_WG) {
-        int bin;
-        const float x = w.x[i];
-        const u64 v = word_weight(w, x, &bin);
-        if (v == 0) continue;
-        if (bin < bd.sure) {
-            if (min_p_stays(w, v, word_key(x, i))) {
-                sum += v;
+    my_blocks(a, [&](int b) {
+        float v[SA_PER];
+        load_block(a, w.x, b, v);
+        if (threadIdx.x == 0) s_n = 0;
+        __syncthreads();
+        u64 sum = 0;
+        uint32_t cnt = 0;
+#pragma unroll
+        for (int j = 0; j < SA_PER; j++) {
+            const uint32_t at = j * SA_WG + threadIdx.x;
+            int bin;
+            const u64 m = word_weight(w, v[j], &bin);
+            const bool border = m && bin >= bd.sure && (bin <= bd.p_end || bin == bd.k_bin);
+            if (m && bin < bd.sure && min_p_stays(w, m, v[j], b * SA_BLOCK + at)) {
+                sum += m;
                 cnt++;
             }
-        } else if (bin <= bd.p_end || bin == bd.k_bin) {
-            a.list[(int64_t)r * a.n + atomicAdd(&a.nlist[r], 1u)] = i;
+            if (const u64 listed = __ballot(border)) {
+                uint32_t base = 0;
+                if (lane == __builtin_ctzll(listed)) base = atomicAdd(&s_n, (uint32_t)__popcll(listed));
+                base = of_lane(base, __builtin_ctzll(listed));
+                if (border)
+                    a.list[((int64_t)r * a.blocks + b) * SA_BLOCK + base + __popcll(listed & ((1ull << lane) - 1))] = at;
+            }
         }
-    }
-    sum = wave_add64(sum);
-    cnt = (uint32_t)wave_add64(cnt);
-    if ((threadIdx.x & 63) == 0) {
-        s_sum[threadIdx.x >> 6] = sum;
-        s_cnt[threadIdx.x >> 6] = cnt;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int q = 1; q < SA_WG / 64; q++) {
-            sum += s_sum[q];
-            cnt += s_cnt[q];
+        sum = wave_total(sum);
+        cnt = wave_total(cnt);
+        if (lane == 0) {
+            s_sum[wave] = sum;
+            s_cnt[wave] = cnt;
         }
-        a.csum[(int64_t)r * a.G + c] = sum;
-        a.ccnt[(int64_t)r * a.G + c] = cnt;
-    }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int q = 1; q < SA_WG / 64; q++) {
+                sum += s_sum[q];
+                cnt += s_cnt[q];
+            }
+            const int64_t o = (int64_t)r * a.blocks + b;
+            a.sum[o] = sum;
+            a.cnt[o] = cnt;
+            a.lcnt[o] = s_n;
+        }
+        __syncthreads();
+    });
 }
 
 // -------------------------------------------------------------- 4: finish --
-// The last key that stays of the list's words in bins [b0, b1], of which
-// those below `floor` do not count: the first `need` of them (BY_WEIGHT: the
-// shortest run, the first word at least, before whose end less than `need`
-// lies); *weight their weight.  Words are told apart by a radix selection of
-// 8 bits a pass until at most FI_WG are left, which are then ranked each
-// against all.
+// The border words of a row: key, and weight with the bin above 48 bits, in
+// LDS where there are at most FI_LIST (in no order), else formed from the
+// lists whenever they are looked at.
+struct Words {
+    const SampleArgs &a;
+    const RowAt &w;
+    int r, m;
+    const uint32_t *s_cnt;  // [blocks]
+    u64 *s_key, *s_val;     // [FI_LIST]
+    __device__ __forceinline__ void word(int b, uint32_t at, u64 &k, u64 &v) const
+    {
+        const uint32_t i = b * SA_BLOCK + at;
+        const float x = w.x[i];
+        int bin;
+        v = word_weight(w, x, &bin) | (u64)bin << 48;
+        k = word_key(x, i);
+    }
+    // f(key, weight and bin) for all words, over the workgroup's threads
+    template <typename F> __device__ __forceinline__ void each(bool from_lists, F f) const
+    {
+        if (!from_lists) {
+            for (int j = threadIdx.x; j < m; j += FI_WG) f(s_key[j], s_val[j]);
+            return;
+        }
+        for (int b = threadIdx.x >> 6; b < a.blocks; b += FI_WAVES) {
+            const uint16_t *list = a.list + ((int64_t)r * a.blocks + b) * SA_BLOCK;
+            for (uint32_t j = threadIdx.x & 63; j < s_cnt[b]; j += 64) {
+                u64 k, v;
+                word(b, list[j], k, v);
+                f(k, v);
+            }
+        }
+    }
+};
+constexpr u64 WEIGHT = (1ull << 48) - 1;
+
+// The last key that stays of the words in bins [b0, b1], of which those below
+// `floor` do not count: the first `need_n` of them (BY_WEIGHT: the shortest
+// run, the first word of the row at least, before whose end less than need_w
+// lies; `base` lies before them all); *weight: all weight up to it.  A radix
+// selection of 8 bits a pass, from the highest bit in which the words that
+// are left differ, until at most FI_PAIRS are; these are ranked each against
+// all.
 struct Chosen {
     u64 key, weight;
 };
 template <bool BY_WEIGHT>
-__device__ Chosen choose(const SampleArgs &a, const RowAt &w, const uint32_t *list, uint32_t m, int b0, int b1,
-                         u64 floor, uint32_t need_n, u64 base, double need_w, u64 *s_key, u64 *s_val)
+__device__ Chosen choose(const Words &ws, int b0, int b1, u64 floor, uint32_t need_n, u64 base, double need_w)
 {
-    __shared__ u64 bw[256];
-    __shared__ uint32_t bc[256], s_left, s_digit, s_n;
-    __shared__ u64 s_w, s_out_key, s_out_w;
-    const int tid = threadIdx.x;
+    __shared__ u64 bw[256], p_key[FI_PAIRS], p_val[FI_PAIRS], s_lo, s_hi, s_w, s_key, s_weight;
+    __shared__ uint32_t bc[256], s_n, s_left, s_digit;
+    const int tid = threadIdx.x, lane = tid & 63;
     u64 prefix = 0, mask = 0, before_w = base;
     uint32_t before_n = 0;
-    auto word = [&](uint32_t j, u64 *v) -> u64 {
-        int bin;
-        const uint32_t i = list[j];
-        const float x = w.x[i];
-        *v = word_weight(w, x, &bin);
-        const u64 k = word_key(x, i);
-        return bin >= b0 && bin <= b1 && k >= floor && (k & mask) == prefix ? k : 0;
+    const bool lists = ws.m > FI_LIST;
+    auto in = [&](u64 k, u64 v) {
+        const int bin = (int)(v >> 48);
+        return bin >= b0 && bin <= b1 && k >= floor && (k & mask) == prefix;
     };
-    int shift = 56;
-    for (;; shift -= 8) {
-        if (tid < 256) bw[tid] = bc[tid] = 0;
-        if (tid == 0) s_left = 0;
-        __syncthreads();
-        uint32_t mine = 0;
-        for (uint32_t j = tid; j < m; j += FI_WG) {
-            u64 v;
-            const u64 k = word(j, &v);
-            if (!k) continue;
-            mine++;
-            if (shift >= 0) {
-                atomicAdd(&bw[(k >> shift) & 255], v);
-                atomicAdd(&bc[(k >> shift) & 255], 1u);
-            }
-        }
-        mine = (uint32_t)wave_add64(mine);
-        if ((tid & 63) == 0 && mine) atomicAdd(&s_left, mine);
-        __syncthreads();
-        if (s_left <= FI_WG || shift < 0) break;
+    for (;;) {
         if (tid == 0) {
-            uint32_t n = before_n;
-            u64 s = before_w;
-            for (int d = 255; d >= 0; d--) {
-                if (!bc[d]) continue;
-                s_digit = d;
-                s_n = n;
-                s_w = s;
-                n += bc[d];
-                s += bw[d];
-                if (BY_WEIGHT ? (double)s >= need_w : n >= need_n) break;
+            s_left = s_n = 0;
+            s_lo = ~0ull;
+            s_hi = 0;
+        }
+        if (tid < 256) bw[tid] = bc[tid] = 0;
+        __syncthreads();
+        u64 lo = ~0ull, hi = 0;
+        uint32_t mine = 0;
+        ws.each(lists, [&](u64 k, u64 v) {
+            if (!in(k, v)) return;
+            mine++;
+            lo = k < lo ? k : lo;
+            hi = k > hi ? k : hi;
+        });
+        mine = wave_total(mine);
+        lo = ~wave_most(~lo);
+        hi = wave_most(hi);
+        if (lane == 0 && mine) {
+            atomicAdd(&s_left, mine);
+            atomicMin(&s_lo, lo);
+            atomicMax(&s_hi, hi);
+        }
+        __syncthreads();
+        if (s_left <= FI_PAIRS) break;
+        const int top = 63 - __builtin_clzll(s_lo ^ s_hi), shift = top > 7 ? top - 7 : 0;
+        ws.each(lists, [&](u64 k, u64 v) {
+            if (!in(k, v)) return;
+            atomicAdd(&bw[(k >> shift) & 255], v & WEIGHT);
+            atomicAdd(&bc[(k >> shift) & 255], 1u);
+        });
+        __syncthreads();
+        if (tid < 64) {
+            // lane i: digits 255 - 4 i downwards
+            u64 w4[4], sw = 0;
+            uint32_t c4[4], sc = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                w4[j] = bw[255 - 4 * lane - j];
+                c4[j] = bc[255 - 4 * lane - j];
+                sw += w4[j];
+                sc += c4[j];
+            }
+            u64 aw = before_w + wave_upto(sw) - sw;
+            uint32_t an = before_n + wave_upto(sc) - sc;
+            // the first digit whose words reach what is needed; should
+            // rounding leave none, the last that has words
+            int at = -1, any = -1;
+            u64 at_w = 0, any_w = 0;
+            uint32_t at_n = 0, any_n = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const bool reach = c4[j] && (BY_WEIGHT ? (double)(aw + w4[j]) >= need_w : an + c4[j] >= need_n);
+                if (reach && at < 0) at = 255 - 4 * lane - j, at_w = aw, at_n = an;
+                if (c4[j]) any = 255 - 4 * lane - j, any_w = aw, any_n = an;
+                aw += w4[j];
+                an += c4[j];
+            }
+            const u64 hit = __ballot(at >= 0), has = __ballot(any >= 0);
+            const int l = hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(has);
+            if (lane == l) {
+                s_digit = hit ? at : any;
+                s_w = hit ? at_w : any_w;
+                s_n = hit ? at_n : any_n;
             }
         }
         __syncthreads();
-        prefix |= (u64)s_digit << shift;
-        mask |= 255ull << shift;
-        before_n = s_n;
+        // all bits from the digit's lowest up are settled
+        mask = ~0ull << shift;
+        prefix = (s_hi & ~(255ull << shift) & mask) | (u64)s_digit << shift;
         before_w = s_w;
+        before_n = s_n;
         __syncthreads();
     }
-    // at most FI_WG words: each against all
     const uint32_t left = s_left;
-    __syncthreads();
-    if (tid == 0) s_n = 0;
-    __syncthreads();
-    for (uint32_t j = tid; j < m; j += FI_WG) {
-        u64 v;
-        const u64 k = word(j, &v);
-        if (!k) continue;
+    ws.each(lists, [&](u64 k, u64 v) {
+        if (!in(k, v)) return;
         const uint32_t p = atomicAdd(&s_n, 1u);
-        s_key[p] = k;
-        s_val[p] = v;
-    }
+        p_key[p] = k;
+        p_val[p] = v & WEIGHT;
+    });
     if (tid == 0) {
-        s_out_key = ~0ull;
-        s_out_w = before_w;
+        s_key = ~0ull;
+        s_weight = before_w;
     }
     __syncthreads();
     if (tid < (int)left) {
-        const u64 k = s_key[tid];
+        const u64 k = p_key[tid];
         uint32_t rank = before_n;
         u64 sum = before_w;
-        for (uint32_t j = 0; j < left; j++)
-            if (s_key[j] > k) {
-                rank++;
-                sum += s_val[j];
-            }
-        const bool in = BY_WEIGHT ? (double)sum < need_w || k == w.kmax : rank < need_n;
-        if (in) {
+        for (uint32_t j = 0; j < left; j++) {
+            const bool first = p_key[j] > k;
+            rank += first;
+            sum += first ? p_val[j] : 0;
+        }
+        if (BY_WEIGHT ? (double)sum < need_w || k == ws.w.kmax : rank < need_n) {
             // the last that stays has the smallest key and the largest sum
-            atomicMin(&s_out_key, k);
-            atomicMax(&s_out_w, sum + s_val[tid]);
+            atomicMin(&s_key, k);
+            atomicMax(&s_weight, sum + p_val[tid]);
         }
     }
     __syncthreads();
-    return {s_out_key, s_out_w};
+    return {s_key, s_weight};
 }
 
 __global__ void __launch_bounds__(FI_WG) k_sample_finish(SampleArgs a)
 {
-    __shared__ u64 s_key[FI_WG], s_val[FI_WG], s_sum[256], s_wave[FI_WAVES], s_total, s_target;
-    __shared__ uint32_t s_cnt, s_chunk;
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ u64 s_key[FI_LIST], s_val[FI_LIST], s_sum[FI_BLOCKS], s_wave[FI_WAVES], s_total, s_target;
+    __shared__ uint32_t s_lcnt[FI_BLOCKS], s_cnt, s_m, s_block;
+    static_assert(FI_BLOCKS == 256, "four blocks a lane");
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t o = (int64_t)r * a.blocks;
     const RowAt w = row_at(a, r);
     if (w.kmax == 0 || w.greedy) {
         if (tid == 0) {
@@ -428,48 +511,55 @@ __global__ void __launch_bounds__(FI_WG) k_sample_finish(SampleArgs a)
         }
         return;
     }
-    const Border bd = find_border<FI_WG>(a, w, r);
-    const uint32_t *list = a.list + (int64_t)r * a.n;
-    const uint32_t m = w.top_p || w.k ? a.nlist[r] : 0;
-    // keys at or above `stay` are left of the border
-    u64 stay = 0;
-    if (bd.k_bin >= 0) {
-        const Chosen ck = choose<false>(a, w, list, m, bd.k_bin, bd.k_bin, 1, w.k - bd.k_count, bd.k_weight, 0.0,
-                                        s_key, s_val);
-        stay = ck.key;
-        if (w.top_p) {
-            __syncthreads();
-            stay = choose<true>(a, w, list, m, bd.sure, bd.p_end, stay, 0, bd.p_weight,
-                                (double)w.p.top_p * (double)ck.weight, s_key, s_val)
-                       .key;
+    uint32_t cnt = 0;
+    if (tid < FI_BLOCKS) {
+        const bool there = tid < a.blocks;
+        s_sum[tid] = there ? a.sum[o + tid] : 0;
+        s_lcnt[tid] = there ? a.lcnt[o + tid] : 0;
+        cnt = there ? a.cnt[o + tid] : 0;
+    }
+    if (tid == 0) s_cnt = s_m = 0;
+    u64 stay = 0;  // keys at or above it are left of the border
+    if (w.top_p || w.k) {
+        const Border bd = find_border<FI_WG>(a, w, r);
+        // the border words into LDS, in whatever order the waves come
+        Words ws{a, w, r, 0, s_lcnt, s_key, s_val};
+        if (tid < FI_BLOCKS) {
+            const uint32_t all = wave_total(s_lcnt[tid]);
+            if (lane == 0 && all) atomicAdd(&s_m, all);
         }
-    } else if (w.top_p) {
-        // (no word is cut off by top-k: S is the weight of all bins)
-        u64 total = 0;
-        for (int i = lane; i < SAMPLE_BINS; i += 64) total += a.hw[(int64_t)r * SAMPLE_BINS + i];
-        total = wave_add64(total);
-        stay = choose<true>(a, w, list, m, bd.sure, bd.p_end, 1, 0, bd.p_weight,
-                            (double)w.p.top_p * (double)total, s_key, s_val)
-                   .key;
+        __syncthreads();
+        ws.m = (int)s_m;
+        __syncthreads();
+        if (tid == 0) s_m = 0;
+        __syncthreads();
+        if (ws.m <= FI_LIST)
+            ws.each(true, [&](u64 k, u64 v) {
+                const uint32_t p = atomicAdd(&s_m, 1u);
+                s_key[p] = k;
+                s_val[p] = v;
+            });
+        __syncthreads();
+        if (bd.k_bin >= 0) {
+            const Chosen ck = choose<false>(ws, bd.k_bin, bd.k_bin, 1, w.k - bd.k_count, bd.k_weight, 0.0);
+            stay = ck.key;
+            if (w.top_p)
+                stay = choose<true>(ws, bd.sure, bd.p_end, stay, 0, bd.p_weight, w.p * (double)ck.weight).key;
+        } else if (w.top_p) {
+            // (no word is cut off by top-k: S is the weight of all bins)
+            stay = choose<true>(ws, bd.sure, bd.p_end, 1, 0, bd.p_weight, w.p * (double)bd.total).key;
+        }
+        // block sums: what surely stays, and the border words that do
+        ws.each(ws.m > FI_LIST, [&](u64 k, u64 v) {
+            const uint32_t i = key_index(k);
+            if (k < stay || (w.min_p && !((double)(v & WEIGHT) >= w.min_w || k == w.kmax))) return;
+            atomicAdd(&s_sum[i / SA_BLOCK], v & WEIGHT);
+            cnt++;
+        });
     }
     __syncthreads();
-    // chunk sums: what surely stays, and the border words that do
-    if (tid < 256) s_sum[tid] = tid < a.G ? a.csum[(int64_t)r * a.G + tid] : 0;
-    if (tid == 0) s_cnt = 0;
-    __syncthreads();
-    uint32_t cnt = tid < a.G ? a.ccnt[(int64_t)r * a.G + tid] : 0;
-    for (uint32_t j = tid; j < m; j += FI_WG) {
-        int bin;
-        const uint32_t i = list[j];
-        const float x = w.x[i];
-        const u64 k = word_key(x, i), v = word_weight(w, x, &bin);
-        if (k < stay || !min_p_stays(w, v, k)) continue;
-        atomicAdd(&s_sum[i / a.ch], v);
-        cnt++;
-    }
-    cnt = (uint32_t)wave_add64(cnt);
+    cnt = wave_total(cnt);
     if (lane == 0 && cnt) atomicAdd(&s_cnt, cnt);
-    __syncthreads();
     if (wave == 0) {
         u64 v[4], run = 0;
 #pragma unroll
@@ -477,8 +567,7 @@ __global__ void __launch_bounds__(FI_WG) k_sample_finish(SampleArgs a)
             v[j] = s_sum[4 * lane + j];
             run += v[j];
         }
-        const u64 incl = wave_scan64(run);
-        const u64 total = __shfl(incl, 63);
+        const u64 incl = wave_upto(run), total = of_lane(incl, 63);
         const double f = (double)a.u[r] * (double)total;
         u64 t = f > 0.0 ? (u64)fmin(f, 9.2e18) : 0;
         if (t >= total) t = total - 1;
@@ -486,7 +575,7 @@ __global__ void __launch_bounds__(FI_WG) k_sample_finish(SampleArgs a)
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             if (at <= t && t < at + v[j]) {
-                s_chunk = 4 * lane + j;
+                s_block = 4 * lane + j;
                 s_target = t - at;
             }
             at += v[j];
@@ -494,67 +583,60 @@ __global__ void __launch_bounds__(FI_WG) k_sample_finish(SampleArgs a)
         if (lane == 0) s_total = total;
     }
     __syncthreads();
-    // the token in its chunk: a contiguous part per wave, then 64 at a time
-    const int c0 = s_chunk * a.ch, c1 = min(a.n, c0 + a.ch), per = (c1 - c0 + FI_WAVES - 1) / FI_WAVES;
-    auto kept = [&](int i) -> u64 {
+    // the token in its block: 128 words of each wave, in two rows of 64
+    constexpr int ROWS = SA_BLOCK / FI_WG;
+    const int i0 = s_block * SA_BLOCK + wave * ROWS * 64 + lane;
+    u64 v[ROWS], upto[ROWS], part = 0;
+#pragma unroll
+    for (int j = 0; j < ROWS; j++) {
+        const int i = i0 + 64 * j;
         int bin;
-        const float x = w.x[i];
-        const u64 v = word_weight(w, x, &bin), k = word_key(x, i);
-        if (v == 0 || !min_p_stays(w, v, k)) return 0;
-        return k >= stay ? v : 0;
-    };
-    const int i0 = c0 + wave * per, i1 = min(c1, i0 + per);
-    u64 part = 0;
-    for (int i = i0 + lane; i < i1; i += 64) part += kept(i);
-    part = wave_add64(part);
+        const float x = i < a.n ? w.x[i] : -INFINITY;
+        v[j] = word_weight(w, x, &bin);
+        if (word_key(x, i) < stay || !min_p_stays(w, v[j], x, i)) v[j] = 0;
+        upto[j] = part + wave_upto(v[j]);
+        part = of_lane(upto[j], 63);
+    }
     if (lane == 0) s_wave[wave] = part;
     __syncthreads();
     u64 at = 0;
     for (int q = 0; q < wave; q++) at += s_wave[q];
     const u64 t = s_target;
-    if (at <= t && t < at + part) {
-        for (int i = i0; i < i1; i += 64) {
-            const u64 v = i + lane < i1 ? kept(i + lane) : 0, incl = at + wave_scan64(v);
-            const unsigned long long hit = __ballot(v && incl > t);
-            if (hit) {
-                if (lane == __builtin_ctzll(hit)) {
-                    a.token[r] = i + lane;
-                    if (a.logprob) a.logprob[r] = (float)log((double)v / (double)s_total);
-                    if (a.n_kept) a.n_kept[r] = s_cnt;
-                }
-                break;
-            }
-            at = __shfl(incl, 63);
+#pragma unroll
+    for (int j = 0; j < ROWS; j++)
+        if (v[j] && t < at + upto[j] && t >= at + upto[j] - v[j]) {
+            a.token[r] = i0 + 64 * j;
+            if (a.logprob) a.logprob[r] = (float)log((double)v[j] / (double)s_total);
+            if (a.n_kept) a.n_kept[r] = s_cnt;
         }
-    }
 }
 
 SampleWs sample_ws(int rows, int n)
 {
     SampleWs s{};
-    // about four workgroups per CU over all rows; at most 256 chunks
-    const int most = std::min(256, (n + SA_MIN - 1) / SA_MIN);
-    s.G = std::max(1, std::min(most, 1024 / rows));
-    s.ch = ((n + s.G - 1) / s.G + SA_WG - 1) / SA_WG * SA_WG;
-    s.G = (n + s.ch - 1) / s.ch;
-    const int64_t per = (int64_t)s.G * 20 + SAMPLE_BINS * 12 + 8 + 4 * (int64_t)n + 8;
-    s.bytes = rows * per;
+    s.blocks = (n + SA_BLOCK - 1) / SA_BLOCK;
+    // about four workgroups per CU over all rows
+    s.per = (int)std::max<int64_t>(1, (int64_t)s.blocks * rows / 1024);
+    s.G = (s.blocks + s.per - 1) / s.per;
+    const int64_t per_row = (int64_t)s.G * 8 + (int64_t)s.blocks * (16 + 2 * SA_BLOCK) + SAMPLE_BINS * 12;
+    s.bytes = rows * per_row;
     return s;
 }
 
 hipError_t launch_sample(hipStream_t st, SampleArgs a, void *ws)
 {
     const SampleWs s = sample_ws(a.rows, a.n);
+    a.blocks = s.blocks;
+    a.per = s.per;
     a.G = s.G;
-    a.ch = s.ch;
     const int64_t rows = a.rows;
-    a.cmax = (u64 *)ws;
-    a.csum = a.cmax + rows * a.G;
-    a.hw = a.csum + rows * a.G;
+    a.top = (u64 *)ws;
+    a.sum = a.top + rows * a.G;
+    a.hw = a.sum + rows * a.blocks;
     a.hc = (uint32_t *)(a.hw + rows * SAMPLE_BINS);
-    a.ccnt = a.hc + rows * SAMPLE_BINS;
-    a.nlist = a.ccnt + rows * a.G;
-    a.list = a.nlist + rows;
+    a.cnt = a.hc + rows * SAMPLE_BINS;
+    a.lcnt = a.cnt + rows * a.blocks;
+    a.list = (uint16_t *)(a.lcnt + rows * a.blocks);
     const dim3 grid(a.G, a.rows);
     hipLaunchKernelGGL(k_sample_max, grid, dim3(SA_WG), 0, st, a);
     hipLaunchKernelGGL(k_sample_bins, grid, dim3(SA_WG), 0, st, a);
