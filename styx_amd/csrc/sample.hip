@@ -13,7 +13,7 @@
 //
 // Nothing is sorted.  Four launches over blocks of 2048 words:
 //   1 the rows' largest logits
-//   2 weight and number of the words in bins of 1/64 of (max - x) / T
+//   2 weight and number of the words in bins of (ln 2) / 32 of (max - x) / T
 //   3 from these, the bins in which the k-th word and the end of the top-p
 //     run lie: the words of those bins are listed, the weight that surely
 //     stays is summed per block
@@ -86,16 +86,37 @@ __device__ __forceinline__ RowAt row_at(const SampleArgs &a, int r)
     return w;
 }
 
-// Weight of a candidate, and its bin.
-__device__ __forceinline__ u64 word_weight(const RowAt &w, float x, int *bin)
+// Weight of a candidate, and its bin: with k = rint(64 d / ln 2) the weight is
+// 2^(44 - k/64) e^(k ln2/64 - d), the power from a table of 64 in LDS, the
+// rest, of at most ln2/128, by its series to the fifth power (3e-17).  The
+// product k ln2/64 is off by 2^-60 k, which reaches a thousandth of a unit
+// nowhere.  14 operations in f64, where a library exponential takes three
+// times as many.  Every launch must come to the same weights and bins:
+// contraction is off.
+__device__ __forceinline__ void fill_powers(double *pow)  // 64, by the first wave
 {
+    if (threadIdx.x < 64) pow[threadIdx.x] = exp2((double)threadIdx.x * (-1.0 / 64.0));
+}
+__device__ __forceinline__ u64 word_weight(const RowAt &w, const double *pow, float x, int *bin)
+{
+#pragma clang fp contract(off)
+    constexpr double ROUND = 6755399441055744.0;  // 1.5 2^52: a sum with it is a whole number
     *bin = 0;
     if (x == w.mx) return (u64)SA_ONE;
-    if (!(x > -INFINITY) || w.mx == INFINITY) return 0;
     const double d = ((double)w.mx - (double)x) * w.inv_t;
-    if (!(d < 31.5)) return 0;
-    *bin = (int)(d * 64.0);
-    return (u64)rint(exp(-d) * SA_ONE);
+    if (!(x > -INFINITY) || !(d < 31.5)) return 0;
+    const double t = d * 92.33248261893498 + ROUND;  // 64 / ln 2
+    const int k = (int)(uint32_t)__builtin_bit_cast(u64, t);
+    const double s = __builtin_fma(t - ROUND, 0.010830424696249145, -d);  // ln 2 / 64
+    double p = __builtin_fma(s, 1.0 / 120.0, 1.0 / 24.0);
+    p = __builtin_fma(s, p, 1.0 / 6.0);
+    p = __builtin_fma(s, p, 0.5);
+    p = __builtin_fma(s, p, 1.0);
+    p = __builtin_fma(s, p, 1.0);
+    const u64 v = __builtin_bit_cast(u64, pow[k & 63] * p) + ((u64)(44 - (k >> 6)) << 52);
+    *bin = k >> 1;
+    // rounded to a whole number by a sum with 2^52
+    return __builtin_bit_cast(u64, __builtin_bit_cast(double, v) + 4503599627370496.0) - 0x4330000000000000ull;
 }
 __device__ __forceinline__ bool min_p_stays(const RowAt &w, u64 weight, float x, uint32_t i)
 {
@@ -152,12 +173,15 @@ __global__ void __launch_bounds__(SA_WG) k_sample_max(SampleArgs a)
 // ---------------------------------------------------------------- 2: bins --
 __global__ void __launch_bounds__(SA_WG) k_sample_bins(SampleArgs a)
 {
-    __shared__ u64 hw[SAMPLE_BINS];
-    __shared__ uint32_t hc[SAMPLE_BINS];
+    // two copies by lane: logits in steps crowd into few bins
+    __shared__ u64 hw[2 * SAMPLE_BINS];
+    __shared__ uint32_t hc[2 * SAMPLE_BINS];
+    __shared__ double pow[64];
     const int r = blockIdx.y;
     const RowAt w = row_at(a, r);
     if (w.kmax == 0 || w.greedy || !(w.top_p || w.k)) return;
-    for (int i = threadIdx.x; i < SAMPLE_BINS; i += SA_WG) hw[i] = hc[i] = 0;
+    for (int i = threadIdx.x; i < 2 * SAMPLE_BINS; i += SA_WG) hw[i] = hc[i] = 0;
+    fill_powers(pow);
     __syncthreads();
     my_blocks(a, [&](int b) {
         float v[SA_PER];
@@ -165,18 +189,20 @@ __global__ void __launch_bounds__(SA_WG) k_sample_bins(SampleArgs a)
 #pragma unroll
         for (int j = 0; j < SA_PER; j++) {
             int bin;
-            const u64 m = word_weight(w, v[j], &bin);
+            const u64 m = word_weight(w, pow, v[j], &bin);
             if (m == 0) continue;
-            atomicAdd(&hw[bin], m);
+            bin += (threadIdx.x & 1) * SAMPLE_BINS;
+            if (w.top_p) atomicAdd(&hw[bin], m);
             if (w.k) atomicAdd(&hc[bin], 1u);
         }
     });
     __syncthreads();
-    for (int i = threadIdx.x; i < SAMPLE_BINS; i += SA_WG)
-        if (hw[i]) {
-            atomicAdd(&a.hw[(int64_t)r * SAMPLE_BINS + i], hw[i]);
-            if (w.k) atomicAdd(&a.hc[(int64_t)r * SAMPLE_BINS + i], hc[i]);
-        }
+    for (int i = threadIdx.x; i < SAMPLE_BINS; i += SA_WG) {
+        const u64 m = hw[i] + hw[SAMPLE_BINS + i];
+        const uint32_t c = hc[i] + hc[SAMPLE_BINS + i];
+        if (m) atomicAdd(&a.hw[(int64_t)r * SAMPLE_BINS + i], m);
+        if (c) atomicAdd(&a.hc[(int64_t)r * SAMPLE_BINS + i], c);
+    }
 }
 
 // -------------------------------------------------------------- 3: border --
@@ -279,9 +305,11 @@ __global__ void __launch_bounds__(SA_WG) k_sample_border(SampleArgs a)
 {
     __shared__ u64 s_sum[SA_WG / 64];
     __shared__ uint32_t s_cnt[SA_WG / 64], s_n;
+    __shared__ double pow[64];
     const int r = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const RowAt w = row_at(a, r);
     if (w.kmax == 0 || w.greedy) return;
+    fill_powers(pow);
     const Border bd = find_border<SA_WG>(a, w, r);
     my_blocks(a, [&](int b) {
         float v[SA_PER];
@@ -294,7 +322,7 @@ __global__ void __launch_bounds__(SA_WG) k_sample_border(SampleArgs a)
         for (int j = 0; j < SA_PER; j++) {
             const uint32_t at = j * SA_WG + threadIdx.x;
             int bin;
-            const u64 m = word_weight(w, v[j], &bin);
+            const u64 m = word_weight(w, pow, v[j], &bin);
             const bool border = m && bin >= bd.sure && (bin <= bd.p_end || bin == bd.k_bin);
             if (m && bin < bd.sure && min_p_stays(w, m, v[j], b * SA_BLOCK + at)) {
                 sum += m;
@@ -338,13 +366,14 @@ struct Words {
     const RowAt &w;
     int r, m;
     const uint32_t *s_cnt;  // [blocks]
+    const double *pow;
     u64 *s_key, *s_val;     // [FI_LIST]
     __device__ __forceinline__ void word(int b, uint32_t at, u64 &k, u64 &v) const
     {
         const uint32_t i = b * SA_BLOCK + at;
         const float x = w.x[i];
         int bin;
-        v = word_weight(w, x, &bin) | (u64)bin << 48;
+        v = word_weight(w, pow, x, &bin) | (u64)bin << 48;
         k = word_key(x, i);
     }
     // f(key, weight and bin) for all words, over the workgroup's threads
@@ -389,7 +418,9 @@ __device__ Chosen choose(const Words &ws, int b0, int b1, u64 floor, uint32_t ne
         const int bin = (int)(v >> 48);
         return bin >= b0 && bin <= b1 && k >= floor && (k & mask) == prefix;
     };
-    for (;;) {
+    // few words altogether: ranked where they lie
+    const bool few = ws.m <= FI_PAIRS;
+    while (!few) {
         if (tid == 0) {
             s_left = s_n = 0;
             s_lo = ~0ull;
@@ -464,31 +495,34 @@ __device__ Chosen choose(const Words &ws, int b0, int b1, u64 floor, uint32_t ne
         before_n = s_n;
         __syncthreads();
     }
-    const uint32_t left = s_left;
-    ws.each(lists, [&](u64 k, u64 v) {
-        if (!in(k, v)) return;
-        const uint32_t p = atomicAdd(&s_n, 1u);
-        p_key[p] = k;
-        p_val[p] = v & WEIGHT;
-    });
+    if (!few)
+        ws.each(lists, [&](u64 k, u64 v) {
+            if (!in(k, v)) return;
+            const uint32_t p = atomicAdd(&s_n, 1u);
+            p_key[p] = k;
+            p_val[p] = v;
+        });
+    const u64 *key = few ? ws.s_key : p_key, *val = few ? ws.s_val : p_val;
     if (tid == 0) {
         s_key = ~0ull;
         s_weight = before_w;
     }
     __syncthreads();
-    if (tid < (int)left) {
-        const u64 k = p_key[tid];
+    const int left = few ? ws.m : (int)s_left;
+    if (tid < left && in(key[tid], val[tid])) {
+        const u64 k = key[tid];
         uint32_t rank = before_n;
         u64 sum = before_w;
-        for (uint32_t j = 0; j < left; j++) {
-            const bool first = p_key[j] > k;
+        for (int j = 0; j < left; j++) {
+            const u64 v = val[j];
+            const bool first = key[j] > k && in(key[j], v);
             rank += first;
-            sum += first ? p_val[j] : 0;
+            sum += first ? v & WEIGHT : 0;
         }
         if (BY_WEIGHT ? (double)sum < need_w || k == ws.w.kmax : rank < need_n) {
             // the last that stays has the smallest key and the largest sum
             atomicMin(&s_key, k);
-            atomicMax(&s_weight, sum + p_val[tid]);
+            atomicMax(&s_weight, sum + (val[tid] & WEIGHT));
         }
     }
     __syncthreads();
@@ -499,6 +533,7 @@ __global__ void __launch_bounds__(FI_WG) k_sample_finish(SampleArgs a)
 {
     __shared__ u64 s_key[FI_LIST], s_val[FI_LIST], s_sum[FI_BLOCKS], s_wave[FI_WAVES], s_total, s_target;
     __shared__ uint32_t s_lcnt[FI_BLOCKS], s_cnt, s_m, s_block;
+    __shared__ double pow[64];
     static_assert(FI_BLOCKS == 256, "four blocks a lane");
     const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t o = (int64_t)r * a.blocks;
@@ -511,6 +546,7 @@ __global__ void __launch_bounds__(FI_WG) k_sample_finish(SampleArgs a)
         }
         return;
     }
+    fill_powers(pow);
     uint32_t cnt = 0;
     if (tid < FI_BLOCKS) {
         const bool there = tid < a.blocks;
@@ -523,7 +559,7 @@ __global__ void __launch_bounds__(FI_WG) k_sample_finish(SampleArgs a)
     if (w.top_p || w.k) {
         const Border bd = find_border<FI_WG>(a, w, r);
         // the border words into LDS, in whatever order the waves come
-        Words ws{a, w, r, 0, s_lcnt, s_key, s_val};
+        Words ws{a, w, r, 0, s_lcnt, pow, s_key, s_val};
         if (tid < FI_BLOCKS) {
             const uint32_t all = wave_total(s_lcnt[tid]);
             if (lane == 0 && all) atomicAdd(&s_m, all);
@@ -592,7 +628,7 @@ __global__ void __launch_bounds__(FI_WG) k_sample_finish(SampleArgs a)
         const int i = i0 + 64 * j;
         int bin;
         const float x = i < a.n ? w.x[i] : -INFINITY;
-        v[j] = word_weight(w, x, &bin);
+        v[j] = word_weight(w, pow, x, &bin);
         if (word_key(x, i) < stay || !min_p_stays(w, v[j], x, i)) v[j] = 0;
         upto[j] = part + wave_upto(v[j]);
         part = of_lane(upto[j], 63);
