@@ -19,10 +19,10 @@ struct SampleArgs {
     uint32_t *token;
     float *logprob;   // or null
     uint32_t *n_kept; // or null
-    // workspace (filled by the launch), per row: the workgroups' largest keys;
-    // per block of words the sum and number of those that surely stay and the
-    // number of border words; weights and numbers of the bins; border words,
-    // each block's at its own place
+    // workspace (filled by the launch), per row: per block of words the first
+    // one's key, sum and number of those that surely stay, number of border
+    // words; weights and numbers of the bins; border words, each block's at
+    // its own place
     unsigned long long *top, *sum, *hw;
     uint32_t *cnt, *lcnt, *hc;
     uint16_t *list;

@@ -13,7 +13,7 @@
 //
 // Nothing is sorted.  Four launches over blocks of 2048 words:
 //   1 the rows' largest logits
-//   2 weight and number of the words in bins of (ln 2) / 32 of (max - x) / T
+//   2 weight and number of the words in bins of about 1/64 of (max - x) / T
 //   3 from these, the bins in which the k-th word and the end of the top-p
 //     run lie: the words of those bins are listed, the weight that surely
 //     stays is summed per block
@@ -34,7 +34,7 @@ constexpr int SA_WG = 256, FI_WG = 1024, FI_WAVES = FI_WG / 64;
 constexpr int SA_BLOCK = 2048, SA_PER = SA_BLOCK / SA_WG;  // words of a block, of a thread
 constexpr int FI_BLOCKS = (SAMPLE_MAX_N + SA_BLOCK - 1) / SA_BLOCK;
 constexpr int FI_LIST = 2048;       // border words that are kept in LDS
-constexpr int FI_PAIRS = 256;       // words that are ranked each against all
+constexpr int FI_PAIRS = FI_WG / 8;  // words that are ranked each against all, by 8 threads each
 constexpr double SA_ONE = 17592186044416.0;  // 2^44
 typedef unsigned long long u64;
 
@@ -57,21 +57,27 @@ struct RowAt {
     const float *x;
     u64 kmax;       // the first word
     float mx;
+    float x_min;    // no word below it is one of the first k
     double inv_t, p, min_w;
     bool greedy, top_p, min_p;
     int k;          // 0: all
 };
 
-// The row's settings and, from the workgroups, its first word; every wave by
-// itself.
+// The row's settings and, from the blocks' first words, its own; every wave
+// by itself.  (The k-th largest of the blocks' first words has k words at or
+// above it: none below it is one of the row's first k.  Looked for in its
+// upper 16 bits, so a little lower.)
 __device__ __forceinline__ RowAt row_at(const SampleArgs &a, int r)
 {
     RowAt w;
     const styx_sample_params p = a.params[a.one_params ? 0 : r];
-    u64 k = 0;
-    for (int c = threadIdx.x & 63; c < a.G; c += 64) {
-        const u64 o = a.top[(int64_t)r * a.G + c];
-        k = o > k ? o : k;
+    const int lane = threadIdx.x & 63;
+    u64 top[FI_BLOCKS / 64], k = 0;
+#pragma unroll
+    for (int j = 0; j < FI_BLOCKS / 64; j++) {
+        const int c = lane + 64 * j;
+        top[j] = c < a.blocks ? a.top[(int64_t)r * a.blocks + c] : 0;
+        k = top[j] > k ? top[j] : k;
     }
     w.x = a.logits + r * a.ld;
     w.kmax = wave_most(k);
@@ -83,6 +89,18 @@ __device__ __forceinline__ RowAt row_at(const SampleArgs &a, int r)
     w.min_p = p.min_p > 0.0f;
     w.min_w = (double)p.min_p * SA_ONE;
     w.k = p.top_k > 0 && p.top_k < a.n ? p.top_k : 0;
+    w.x_min = -INFINITY;
+    if (w.k && w.k <= a.blocks) {
+        uint32_t least = 0;
+        for (uint32_t bit = 0x8000; bit; bit >>= 1) {
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < FI_BLOCKS / 64; j++) n += __popcll(__ballot((uint32_t)(top[j] >> 48) >= (least | bit)));
+            if (n >= w.k) least |= bit;
+        }
+        // (below every candidate's key, or a NaN's: fewer than k blocks have one)
+        if (least > 0x007Fu) w.x_min = key_value((u64)least << 48);
+    }
     return w;
 }
 
@@ -114,7 +132,7 @@ __device__ __forceinline__ u64 word_weight(const RowAt &w, const double *pow, fl
     p = __builtin_fma(s, p, 1.0);
     p = __builtin_fma(s, p, 1.0);
     const u64 v = __builtin_bit_cast(u64, pow[k & 63] * p) + ((u64)(44 - (k >> 6)) << 52);
-    *bin = k >> 1;
+    *bin = k * 11 >> 4;  // k is at most 2909
     // rounded to a whole number by a sum with 2^52
     return __builtin_bit_cast(u64, __builtin_bit_cast(double, v) + 4503599627370496.0) - 0x4330000000000000ull;
 }
@@ -144,30 +162,31 @@ __device__ __forceinline__ void load_block(const SampleArgs &a, const float *x, 
 // ------------------------------------------------------------- 1: largest --
 __global__ void __launch_bounds__(SA_WG) k_sample_max(SampleArgs a)
 {
-    __shared__ u64 s[SA_WG / 64];
+    __shared__ u64 s[2][SA_WG / 64];
     const int r = blockIdx.y;
-    u64 k = 0;
-    my_blocks(a, [&](int b) {
-        float v[SA_PER];
-        load_block(a, a.logits + r * a.ld, b, v);
-#pragma unroll
-        for (int j = 0; j < SA_PER; j++) {
-            const u64 o = word_key(v[j], b * SA_BLOCK + j * SA_WG + threadIdx.x);
-            k = o > k ? o : k;
-        }
-    });
-    k = wave_most(k);
-    if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = k;
     // the row's bins, emptied by its workgroups together
     for (int i = blockIdx.x * SA_WG + threadIdx.x; i < SAMPLE_BINS; i += a.G * SA_WG) {
         a.hw[(int64_t)r * SAMPLE_BINS + i] = 0;
         a.hc[(int64_t)r * SAMPLE_BINS + i] = 0;
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < SA_WG / 64; w++) k = s[w] > k ? s[w] : k;
-        a.top[(int64_t)r * a.G + blockIdx.x] = k;
-    }
+    my_blocks(a, [&](int b) {
+        float v[SA_PER];
+        load_block(a, a.logits + r * a.ld, b, v);
+        u64 k = 0;
+#pragma unroll
+        for (int j = 0; j < SA_PER; j++) {
+            const u64 o = word_key(v[j], b * SA_BLOCK + j * SA_WG + threadIdx.x);
+            k = o > k ? o : k;
+        }
+        k = wave_most(k);
+        u64 *t = s[b & 1];  // (a block later than one whose reader may be behind)
+        if ((threadIdx.x & 63) == 0) t[threadIdx.x >> 6] = k;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int w = 1; w < SA_WG / 64; w++) k = t[w] > k ? t[w] : k;
+            a.top[(int64_t)r * a.blocks + b] = k;
+        }
+    });
 }
 
 // ---------------------------------------------------------------- 2: bins --
@@ -188,6 +207,7 @@ __global__ void __launch_bounds__(SA_WG) k_sample_bins(SampleArgs a)
         load_block(a, w.x, b, v);
 #pragma unroll
         for (int j = 0; j < SA_PER; j++) {
+            if (!(v[j] >= w.x_min)) continue;
             int bin;
             const u64 m = word_weight(w, pow, v[j], &bin);
             if (m == 0) continue;
@@ -311,6 +331,12 @@ __global__ void __launch_bounds__(SA_WG) k_sample_border(SampleArgs a)
     if (w.kmax == 0 || w.greedy) return;
     fill_powers(pow);
     const Border bd = find_border<SA_WG>(a, w, r);
+    // words below x_lim lie past the last bin that matters: k rounds to one
+    // of that bin's only up to (bin + 1) 16/11 + 1/2
+    const int past = max(max(bd.p_end, bd.k_bin), bd.sure - 1) + 1;
+    float x_lim = (float)((double)w.mx - (past * (16.0 / 11.0) + 2.0) / 92.33248261893498 / w.inv_t);
+    x_lim = past >= SAMPLE_BINS || !(x_lim > -INFINITY) || w.mx == INFINITY ? -INFINITY : x_lim - fabsf(x_lim) * 1e-6f;
+    x_lim = fmaxf(x_lim, w.x_min);
     my_blocks(a, [&](int b) {
         float v[SA_PER];
         load_block(a, w.x, b, v);
@@ -321,8 +347,9 @@ __global__ void __launch_bounds__(SA_WG) k_sample_border(SampleArgs a)
 #pragma unroll
         for (int j = 0; j < SA_PER; j++) {
             const uint32_t at = j * SA_WG + threadIdx.x;
+            if (!__any(v[j] >= x_lim)) continue;
             int bin;
-            const u64 m = word_weight(w, pow, v[j], &bin);
+            const u64 m = v[j] >= x_lim ? word_weight(w, pow, v[j], &bin) : 0;
             const bool border = m && bin >= bd.sure && (bin <= bd.p_end || bin == bd.k_bin);
             if (m && bin < bd.sure && min_p_stays(w, m, v[j], b * SA_BLOCK + at)) {
                 sum += m;
@@ -359,7 +386,7 @@ __global__ void __launch_bounds__(SA_WG) k_sample_border(SampleArgs a)
 
 // -------------------------------------------------------------- 4: finish --
 // The border words of a row: key, and weight with the bin above 48 bits, in
-// LDS where there are at most FI_LIST (in no order), else formed from the
+// LDS where there are at most FI_LIST, else formed from the
 // lists whenever they are looked at.
 struct Words {
     const SampleArgs &a;
@@ -405,6 +432,14 @@ constexpr u64 WEIGHT = (1ull << 48) - 1;
 struct Chosen {
     u64 key, weight;
 };
+// Sum over eight lanes.
+template <typename T> __device__ __forceinline__ T eight_total(T v)
+{
+    v += by_words(v, [](uint32_t x) { return dpp_u<0xB1>(x); });
+    v += by_words(v, [](uint32_t x) { return dpp_u<0x4E>(x); });
+    v += by_words(v, [](uint32_t x) { return dpp_u<0x141>(x); });
+    return v;
+}
 template <bool BY_WEIGHT>
 __device__ Chosen choose(const Words &ws, int b0, int b1, u64 floor, uint32_t need_n, u64 base, double need_w)
 {
@@ -508,21 +543,23 @@ __device__ Chosen choose(const Words &ws, int b0, int b1, u64 floor, uint32_t ne
         s_weight = before_w;
     }
     __syncthreads();
-    const int left = few ? ws.m : (int)s_left;
-    if (tid < left && in(key[tid], val[tid])) {
-        const u64 k = key[tid];
-        uint32_t rank = before_n;
-        u64 sum = before_w;
-        for (int j = 0; j < left; j++) {
+    const int left = few ? ws.m : (int)s_left, item = tid / 8;
+    if (item < left) {
+        const u64 k = key[item], mine = val[item];
+        uint32_t rank = 0;
+        u64 sum = 0;
+        for (int j = tid % 8; j < left; j += 8) {
             const u64 v = val[j];
             const bool first = key[j] > k && in(key[j], v);
             rank += first;
             sum += first ? v & WEIGHT : 0;
         }
-        if (BY_WEIGHT ? (double)sum < need_w || k == ws.w.kmax : rank < need_n) {
+        rank = before_n + eight_total(rank);
+        sum = before_w + eight_total(sum);
+        if (tid % 8 == 0 && in(k, mine) && (BY_WEIGHT ? (double)sum < need_w || k == ws.w.kmax : rank < need_n)) {
             // the last that stays has the smallest key and the largest sum
             atomicMin(&s_key, k);
-            atomicMax(&s_weight, sum + (val[tid] & WEIGHT));
+            atomicMax(&s_weight, sum + (mine & WEIGHT));
         }
     }
     __syncthreads();
@@ -532,7 +569,8 @@ __device__ Chosen choose(const Words &ws, int b0, int b1, u64 floor, uint32_t ne
 __global__ void __launch_bounds__(FI_WG) k_sample_finish(SampleArgs a)
 {
     __shared__ u64 s_key[FI_LIST], s_val[FI_LIST], s_sum[FI_BLOCKS], s_wave[FI_WAVES], s_total, s_target;
-    __shared__ uint32_t s_lcnt[FI_BLOCKS], s_cnt, s_m, s_block;
+    __shared__ uint32_t s_lcnt[FI_BLOCKS], s_cnt, s_block;
+    __shared__ int s_begin[FI_BLOCKS], s_m;
     __shared__ double pow[64];
     static_assert(FI_BLOCKS == 256, "four blocks a lane");
     const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -554,27 +592,38 @@ __global__ void __launch_bounds__(FI_WG) k_sample_finish(SampleArgs a)
         s_lcnt[tid] = there ? a.lcnt[o + tid] : 0;
         cnt = there ? a.cnt[o + tid] : 0;
     }
-    if (tid == 0) s_cnt = s_m = 0;
+    if (tid == 0) s_cnt = 0;
     u64 stay = 0;  // keys at or above it are left of the border
     if (w.top_p || w.k) {
         const Border bd = find_border<FI_WG>(a, w, r);
-        // the border words into LDS, in whatever order the waves come
+        // the border words into LDS, if they fit
         Words ws{a, w, r, 0, s_lcnt, pow, s_key, s_val};
-        if (tid < FI_BLOCKS) {
-            const uint32_t all = wave_total(s_lcnt[tid]);
-            if (lane == 0 && all) atomicAdd(&s_m, all);
+        if (wave == 0) {
+            int c[4], all = 0;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                c[j] = s_lcnt[4 * lane + j];
+                all += c[j];
+            }
+            int at = wave_upto(all) - all;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                s_begin[4 * lane + j] = at;
+                at += c[j];
+            }
+            if (lane == 63) s_m = at;
         }
         __syncthreads();
-        ws.m = (int)s_m;
-        __syncthreads();
-        if (tid == 0) s_m = 0;
-        __syncthreads();
+        ws.m = s_m;
         if (ws.m <= FI_LIST)
-            ws.each(true, [&](u64 k, u64 v) {
-                const uint32_t p = atomicAdd(&s_m, 1u);
-                s_key[p] = k;
-                s_val[p] = v;
-            });
+            for (int j = tid; j < ws.m; j += FI_WG) {
+                // the last block that begins at or before j
+                int b = 0;
+#pragma unroll
+                for (int d = FI_BLOCKS / 2; d; d /= 2)
+                    if (s_begin[b + d] <= j) b += d;
+                ws.word(b, a.list[(o + b) * SA_BLOCK + j - s_begin[b]], s_key[j], s_val[j]);
+            }
         __syncthreads();
         if (bd.k_bin >= 0) {
             const Chosen ck = choose<false>(ws, bd.k_bin, bd.k_bin, 1, w.k - bd.k_count, bd.k_weight, 0.0);
@@ -654,7 +703,7 @@ SampleWs sample_ws(int rows, int n)
     // about four workgroups per CU over all rows
     s.per = (int)std::max<int64_t>(1, (int64_t)s.blocks * rows / 1024);
     s.G = (s.blocks + s.per - 1) / s.per;
-    const int64_t per_row = (int64_t)s.G * 8 + (int64_t)s.blocks * (16 + 2 * SA_BLOCK) + SAMPLE_BINS * 12;
+    const int64_t per_row = (int64_t)s.blocks * (24 + 2 * SA_BLOCK) + SAMPLE_BINS * 12;
     s.bytes = rows * per_row;
     return s;
 }
@@ -667,7 +716,7 @@ hipError_t launch_sample(hipStream_t st, SampleArgs a, void *ws)
     a.G = s.G;
     const int64_t rows = a.rows;
     a.top = (u64 *)ws;
-    a.sum = a.top + rows * a.G;
+    a.sum = a.top + rows * a.blocks;
     a.hw = a.sum + rows * a.blocks;
     a.hc = (uint32_t *)(a.hw + rows * SAMPLE_BINS);
     a.cnt = a.hc + rows * SAMPLE_BINS;
