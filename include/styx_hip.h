@@ -558,6 +558,21 @@ int styx_moe_generate(styx_moe *m, const uint32_t *prompt, int n_prompt, int n_p
  * each on the previous argmax token (generate_moe.rs:58-67 loop body);
  * out[i] = the token produced by step i. */
 int styx_moe_decode(styx_moe *m, int n_steps, uint32_t *out);
+/* A token from the logits of the last token forwarded, by styx_op_sample's
+ * rules with one set of settings and one random number u (no counterpart in
+ * the reference); logprob may be NULL.  The model's state is unchanged:
+ * forward the token to go on.  STYX_E_STATE before the first token (also
+ * after styx_moe_reset or styx_moe_fill_kv) and when no logit is above
+ * -infinity. */
+int styx_moe_sample(styx_moe *m, const styx_sample_params *params, float u, uint32_t *token,
+                    float *logprob);
+/* styx_moe_generate with sampled tokens: token i of out_tokens by u[i] of the
+ * n_predict random numbers; logprobs [n_predict] or NULL.  Each token is
+ * waited for before the next is forwarded. */
+int styx_moe_generate_sampled(styx_moe *m, const uint32_t *prompt, int n_prompt, int n_predict,
+                              const styx_sample_params *params, const float *u,
+                              uint32_t *out_tokens, float *logprobs, double *prefill_s,
+                              double *decode_s);
 /* The fused launches' wait bound (styx_moe_opts.max_polls) for the tokens
  * that follow (test helper, no reference counterpart). */
 int styx_moe_set_wait_limit(styx_moe *m, int max_polls);

@@ -193,6 +193,8 @@ _SIGS = {
     "styx_moe_forward_token": (i32, [vp, u32, vp]),
     "styx_moe_generate": (i32, [vp, vp, i32, i32, vp, vp, vp]),
     "styx_moe_decode": (i32, [vp, i32, vp]),
+    "styx_moe_sample": (i32, [vp, vp, C.c_float, C.POINTER(u32), C.POINTER(C.c_float)]),
+    "styx_moe_generate_sampled": (i32, [vp, vp, i32, i32, vp, vp, vp, vp, vp, vp]),
     "styx_moe_set_timing": (i32, [vp, i32]),
     "styx_moe_moe_block_trace": (i32, [vp, vp, i64, C.POINTER(i32), C.POINTER(C.c_double)]),
     "styx_moe_set_wait_limit": (i32, [vp, i32]),

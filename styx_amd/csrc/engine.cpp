@@ -30,6 +30,7 @@
 #include "gguf.h"
 #include "kernels.h"
 #include "runtime.h"
+#include "sample.h"
 
 namespace styx {
 }  // namespace styx
@@ -186,6 +187,16 @@ struct styx_moe {
     hipStream_t st_copy = nullptr;
     hipEvent_t ev_fork = nullptr, ev_join = nullptr;
     int n_past = 0;
+    bool has_logits = false;  // `logits` are those of the token before n_past
+    // Sampling: workspace, the call's settings and random number on the
+    // device; {token, log probability} in pinned memory, before them the
+    // inputs on their way.  Allocated at the first sample.
+    void *smp_ws = nullptr;
+    struct SampleIn {
+        styx_sample_params p;
+        float u;
+    } *smp_in = nullptr, *h_smp_in = nullptr;
+    uint32_t *h_smp = nullptr, *h_smp_dev = nullptr;
     // Prompt batches (prompt.hip): workspace of one batch of up to pb_t
     // tokens, allocated at the first prompt long enough and kept with the
     // model; pb_t < 0: it did not fit, prompts then run token by token.
@@ -233,6 +244,7 @@ struct styx_moe {
     int run_token(bool gen);
     int prompt_workspace();
     int prompt_batch(const uint32_t *tok, int n);
+    int sample(const styx_sample_params &p, float u);
     bool attn_merge_in_kernel(int n_t) const;
     int attn_mode(int n_t) const;
     int ensure_pages(int upto_pos);
@@ -1261,9 +1273,47 @@ int styx_moe::prompt_batch(const uint32_t *tok, int n)
             }));
         }
         n_past += T;
+        has_logits = false;
         tok += T;
         n -= T;
     }
+    return STYX_OK;
+}
+
+// A token from the logits of the last one, waited for: h_smp[0], its log
+// probability as bits in h_smp[1].
+int styx_moe::sample(const styx_sample_params &p, float u)
+{
+    if (!h_smp) {
+        if (V > SAMPLE_MAX_N) return fail(STYX_E_UNSUPPORTED, "sampling: vocabulary of 2^19 words or more");
+        void *ws = nullptr, *in = nullptr, *host = nullptr;
+        if (int r = alloc(&ws, sample_ws(1, V).bytes)) return r;
+        if (int r = alloc(&in, sizeof(SampleIn))) return r;
+        if (int r = alloc_host(&host, 64)) return r;
+        void *dev = nullptr;
+        STYX_HIP(hipHostGetDevicePointer(&dev, host, 0));
+        smp_ws = ws;
+        smp_in = (SampleIn *)in;
+        h_smp_in = (SampleIn *)((char *)host + 16);
+        h_smp_dev = (uint32_t *)dev;
+        h_smp = (uint32_t *)host;
+    }
+    hipStream_t st = gpu->stream;
+    *h_smp_in = {p, u};
+    CK(hipMemcpyAsync(smp_in, h_smp_in, sizeof(SampleIn), hipMemcpyHostToDevice, st));
+    SampleArgs a{};
+    a.logits = logits;
+    a.ld = V;
+    a.rows = 1;
+    a.n = V;
+    a.params = &smp_in->p;
+    a.one_params = 1;
+    a.u = &smp_in->u;
+    a.token = h_smp_dev;
+    a.logprob = (float *)(h_smp_dev + 1);
+    CK(launch_sample(st, a, smp_ws));
+    STYX_HIP(hipStreamSynchronize(st));
+    if (h_smp[0] == SKIP) return fail(STYX_E_STATE, "sampling: no logit is above -infinity");
     return STYX_OK;
 }
 
@@ -2073,6 +2123,7 @@ int styx_moe_forward_token(styx_moe *m, uint32_t token, float *logits_out)
     STYX_HIP(launch_set_token(m->gpu->stream, m->d_tok, m->d_pos, token, m->n_past));
     if (int r = m->run_token(false)) return r;
     m->n_past++;
+    m->has_logits = true;
     if (logits_out)
         STYX_HIP(hipMemcpyAsync(logits_out, m->logits, sizeof(float) * m->V, hipMemcpyDeviceToHost,
                                 m->gpu->stream));
@@ -2125,6 +2176,7 @@ int styx_moe_decode(styx_moe *m, int n_steps, uint32_t *out)
         again = false;
         if (int r = m->run_token(true)) return r;
         m->n_past++;
+        m->has_logits = true;
         if (host_work && !m->opts.no_fuse) {
             STYX_HIP(hipStreamSynchronize(m->gpu->stream));
             if (m->check_abort()) {
@@ -2154,19 +2206,12 @@ int styx_moe_decode(styx_moe *m, int n_steps, uint32_t *out)
     return m->collect_stats();
 }
 
-int styx_moe_generate(styx_moe *m, const uint32_t *prompt, int n_prompt, int n_predict,
-                      uint32_t *out, double *prefill_s, double *decode_s)
+// The prompt's tokens: all but the last in batches, unless the host works
+// between tokens (repinning counts each token's experts, timing each launch),
+// the rows do not fit a pack workgroup's LDS, or a token is out of range:
+// forward_token reports that one, after the tokens before it as ever.
+static int prefill(styx_moe *m, const uint32_t *prompt, int n_prompt)
 {
-    if (!m || !prompt || n_prompt < 1 || n_predict < 1 || !out)
-        return fail(STYX_E_INVALID, "styx_moe_generate: bad argument");
-    if (m->n_past + n_prompt + n_predict - 1 > m->n_ctx)
-        return fail(STYX_E_STATE, "prompt + generation exceeds n_ctx");
-    using clk = std::chrono::steady_clock;
-    const auto t0 = clk::now();
-    // every token but the last in batches, unless the host works between
-    // tokens (repinning counts each token's experts, timing each launch),
-    // the rows do not fit a pack workgroup's LDS, or a token is out of range:
-    // forward_token reports that one, after the tokens before it as ever
     int i = 0;
     const int widest = std::max(std::max(m->H, m->nh * m->hd), std::max(m->F, m->Fsh));
     if (n_prompt > PROMPT_MIN_T && widest <= PROMPT_MAX_N && m->broken.empty() && !m->opts.time_kernels &&
@@ -2182,11 +2227,59 @@ int styx_moe_generate(styx_moe *m, const uint32_t *prompt, int n_prompt, int n_p
     }
     for (; i < n_prompt; i++)
         if (int r = styx_moe_forward_token(m, prompt[i], nullptr)) return r;
+    return STYX_OK;
+}
+
+int styx_moe_generate(styx_moe *m, const uint32_t *prompt, int n_prompt, int n_predict,
+                      uint32_t *out, double *prefill_s, double *decode_s)
+{
+    if (!m || !prompt || n_prompt < 1 || n_predict < 1 || !out)
+        return fail(STYX_E_INVALID, "styx_moe_generate: bad argument");
+    if (m->n_past + n_prompt + n_predict - 1 > m->n_ctx)
+        return fail(STYX_E_STATE, "prompt + generation exceeds n_ctx");
+    using clk = std::chrono::steady_clock;
+    const auto t0 = clk::now();
+    if (int r = prefill(m, prompt, n_prompt)) return r;
     const auto t1 = clk::now();
     // the first generated token is the prefill's argmax, left in the stage by
     // its read-out
     out[0] = m->h_stage[5];
     if (int r = styx_moe_decode(m, n_predict - 1, out + 1)) return r;
+    const auto t2 = clk::now();
+    if (prefill_s) *prefill_s = std::chrono::duration<double>(t1 - t0).count();
+    if (decode_s) *decode_s = std::chrono::duration<double>(t2 - t1).count();
+    return STYX_OK;
+}
+
+int styx_moe_sample(styx_moe *m, const styx_sample_params *params, float u, uint32_t *token, float *logprob)
+{
+    if (!m || !params || !token) return fail(STYX_E_INVALID, "styx_moe_sample: NULL argument");
+    if (!m->has_logits) return fail(STYX_E_STATE, "styx_moe_sample: no token forwarded yet");
+    if (!m->broken.empty()) return fail(STYX_E_STATE, m->broken);
+    STYX_HIP(hipSetDevice(m->gpu->device));
+    if (int r = m->sample(*params, u)) return r;
+    *token = m->h_smp[0];
+    if (logprob) std::memcpy(logprob, &m->h_smp[1], 4);
+    return STYX_OK;
+}
+
+int styx_moe_generate_sampled(styx_moe *m, const uint32_t *prompt, int n_prompt, int n_predict,
+                              const styx_sample_params *params, const float *u, uint32_t *out, float *logprobs,
+                              double *prefill_s, double *decode_s)
+{
+    if (!m || !prompt || n_prompt < 1 || n_predict < 1 || !params || !u || !out)
+        return fail(STYX_E_INVALID, "styx_moe_generate_sampled: bad argument");
+    if (m->n_past + n_prompt + n_predict - 1 > m->n_ctx)
+        return fail(STYX_E_STATE, "prompt + generation exceeds n_ctx");
+    using clk = std::chrono::steady_clock;
+    const auto t0 = clk::now();
+    if (int r = prefill(m, prompt, n_prompt)) return r;
+    const auto t1 = clk::now();
+    for (int i = 0; i < n_predict; i++) {
+        if (i > 0)
+            if (int r = styx_moe_forward_token(m, out[i - 1], nullptr)) return r;
+        if (int r = styx_moe_sample(m, params, u[i], &out[i], logprobs ? &logprobs[i] : nullptr)) return r;
+    }
     const auto t2 = clk::now();
     if (prefill_s) *prefill_s = std::chrono::duration<double>(t1 - t0).count();
     if (decode_s) *decode_s = std::chrono::duration<double>(t2 - t1).count();
@@ -2370,6 +2463,7 @@ int styx_moe_reset(styx_moe *m)
 {
     if (!m) return fail(STYX_E_INVALID, "styx_moe_reset: NULL model");
     m->n_past = 0;
+    m->has_logits = false;
     return STYX_OK;
 }
 
@@ -2392,6 +2486,7 @@ int styx_moe_fill_kv(styx_moe *m, int n_t, uint64_t seed, float sigma)
         }
     STYX_HIP(hipStreamSynchronize(m->gpu->stream));
     m->n_past = n_t;
+    m->has_logits = false;
     return STYX_OK;
 }
 

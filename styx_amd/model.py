@@ -125,6 +125,29 @@ class MoeModel:
         L.check(self.lib.styx_moe_decode(self.h, n_steps, out.ctypes.data))
         return out[:n_steps]
 
+    def sample(self, u: float, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+               min_p: float = 0.0) -> tuple[int, float]:
+        """(token, log probability) from the last token's logits by one random
+        number u of [0, 1); the state is unchanged."""
+        p = L.SampleParams(temperature, top_k, top_p, min_p)
+        tok, lp = C.c_uint32(), C.c_float()
+        L.check(self.lib.styx_moe_sample(self.h, C.byref(p), u, C.byref(tok), C.byref(lp)))
+        return tok.value, lp.value
+
+    def generate_sampled(self, prompt, u, temperature: float = 1.0, top_k: int = 0,
+                         top_p: float = 1.0, min_p: float = 0.0):
+        """generate with a token sampled by each random number of u:
+        (tokens, log probabilities, prefill_s, decode_s)."""
+        p = np.ascontiguousarray(np.asarray(prompt, np.uint32))
+        u = np.ascontiguousarray(np.asarray(u, np.float32))
+        out, lp = np.empty(len(u), np.uint32), np.empty(len(u), np.float32)
+        par = L.SampleParams(temperature, top_k, top_p, min_p)
+        ps, ds = C.c_double(), C.c_double()
+        L.check(self.lib.styx_moe_generate_sampled(self.h, p.ctypes.data, len(p), len(u), C.byref(par),
+                                                   u.ctypes.data, out.ctypes.data, lp.ctypes.data,
+                                                   C.byref(ps), C.byref(ds)))
+        return out, lp, ps.value, ds.value
+
     def set_timing(self, on: bool) -> None:
         L.check(self.lib.styx_moe_set_timing(self.h, int(on)))
 

@@ -211,3 +211,88 @@ def from_split(gpu: Gpu, type_: int, split: Buffer, rows: int, cols: int, nmat: 
     L.check(gpu.lib.styx_op_from_split(gpu.h, type_, split.ptr, out.ptr,
                                        split_nblocks(type_, rows, cols), nmat))
     return out
+
+
+class KvBatch:
+    """The paged KV cache of a batch of sequences (styx_kv_cache) with what its
+    operators keep beside it: page table, lengths and positions, and with
+    `scored` every row's accumulated attention weight and position.  attend()
+    and evict() run on the gpu's stream; lengths and positions stay on the
+    device and are the caller's to advance (set)."""
+
+    def __init__(self, gpu: Gpu, n_seq: int, nkv: int, hd: int, page_tokens: int, n_pages: int,
+                 table_len: int, type_: int = L.F32, scored: bool = True):
+        self.gpu, self.lib, self.scored = gpu, gpu.lib, scored
+        self.n_seq, self.nkv, self.hd, self.cap = n_seq, nkv, hd, table_len * page_tokens
+        nbytes = n_pages * page_tokens * nkv * hd * (2 if type_ == L.F16 else 4)
+        self.kpool, self.vpool = gpu.buffer(nbytes), gpu.buffer(nbytes)
+        self.table = gpu.from_numpy(np.full((n_seq, table_len), -1, np.int32))
+        self.len = gpu.from_numpy(np.full(n_seq, -1, np.int32))
+        self.pos = gpu.from_numpy(np.zeros(n_seq, np.int32))
+        self.acc = gpu.zeros(4 * n_seq * nkv * self.cap) if scored else None
+        self.slot_pos = gpu.zeros(4 * n_seq * nkv * self.cap) if scored else None
+        self.c = L.KvCache(type_, n_seq, nkv, hd, page_tokens, n_pages, table_len, self.kpool.ptr,
+                           self.vpool.ptr, self.table.ptr)
+        self._ws = None
+
+    def set(self, len=None, pos=None, table=None) -> None:
+        """Upload lengths, positions or the page table (-1: no page)."""
+        for buf, a in ((self.len, len), (self.pos, pos), (self.table, table)):
+            if a is not None:
+                buf.upload(np.asarray(a, np.int32))
+
+    def lengths(self) -> np.ndarray:
+        return self.len.download(np.int32, self.n_seq)
+
+    def _workspace(self, nbytes: int) -> "Buffer":
+        if self._ws is None or self._ws.nbytes < nbytes:
+            if self._ws is not None:
+                self._ws.free()
+            self._ws = self.gpu.buffer(max(nbytes, 16))
+        return self._ws
+
+    def attend(self, nh: int, q: Buffer, k: Buffer, v: Buffer, out: Buffer, rope: Buffer, n_rope: int,
+               scale: float, q_norm: Buffer | None = None, k_norm: Buffer | None = None,
+               eps: float = 1e-6, decay: float = 1.0) -> None:
+        """styx_op_attn_decode_batch; the weights are added in place."""
+        ws = self._workspace(self.lib.styx_op_attn_batch_ws_bytes(C.byref(self.c), nh, int(self.scored)))
+        ptr = lambda b: b.ptr if b is not None else None  # noqa: E731
+        L.check(self.lib.styx_op_attn_decode_batch(
+            self.gpu.h, C.byref(self.c), self.len.ptr, self.pos.ptr, nh, q.ptr, k.ptr, v.ptr, ptr(q_norm),
+            ptr(k_norm), eps, rope.ptr, n_rope, scale, decay, ptr(self.acc), ptr(self.acc),
+            ptr(self.slot_pos), out.ptr, ws.ptr, ws.nbytes))
+
+    def evict(self, trigger: int, keep: int, recent: int = 0, sinks: int = 0) -> None:
+        """styx_op_kv_evict in place, the lengths too."""
+        if not self.scored:
+            raise ValueError("a cache without scores has nothing to evict by")
+        ws = self._workspace(self.lib.styx_op_kv_evict_ws_bytes(C.byref(self.c), keep))
+        L.check(self.lib.styx_op_kv_evict(
+            self.gpu.h, C.byref(self.c), self.len.ptr, self.pos.ptr, trigger, keep, recent, sinks,
+            self.acc.ptr, self.acc.ptr, self.slot_pos.ptr, self.slot_pos.ptr, self.len.ptr, ws.ptr,
+            ws.nbytes))
+
+    def free(self) -> None:
+        for b in (self.kpool, self.vpool, self.table, self.len, self.pos, self.acc, self.slot_pos, self._ws):
+            if b is not None:
+                b.free()
+
+
+def sample(gpu: Gpu, logits: Buffer, n: int, params, u, ld: int | None = None):
+    """styx_op_sample of a token for every random number of u: (tokens, log
+    probabilities, words left).  params: one (temperature, top_k, top_p,
+    min_p), or one for every row."""
+    u = np.ascontiguousarray(np.asarray(u, np.float32))
+    params = [params] if np.ndim(params) == 1 else list(params)
+    arr = (L.SampleParams * len(params))(*[L.SampleParams(float(t), int(k), float(p), float(m))
+                                           for t, k, p, m in params])
+    rows = len(u)
+    par, uu = gpu.from_numpy(np.frombuffer(arr, np.uint8)), gpu.from_numpy(u)
+    out = [gpu.buffer(max(4 * rows, 16)) for _ in range(3)]
+    ws = gpu.buffer(max(int(gpu.lib.styx_op_sample_ws_bytes(rows, n)), 16))
+    L.check(gpu.lib.styx_op_sample(gpu.h, logits.ptr, ld or n, rows, n, par.ptr, len(params), uu.ptr, out[0].ptr,
+                                   out[1].ptr, out[2].ptr, ws.ptr, ws.nbytes))
+    got = (out[0].download(np.uint32, rows), out[1].download(np.float32, rows), out[2].download(np.uint32, rows))
+    for b in (par, uu, ws, *out):
+        b.free()
+    return got
