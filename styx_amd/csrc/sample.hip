@@ -172,13 +172,17 @@ __global__ void __launch_bounds__(SA_WG) k_sample_max(SampleArgs a)
     my_blocks(a, [&](int b) {
         float v[SA_PER];
         load_block(a, a.logits + r * a.ld, b, v);
-        u64 k = 0;
+        // a thread's first of its largest words (NaN and -inf are above
+        // nothing); a third of the instructions of comparing keys
+        float best = -INFINITY;
+        int at = 0;
 #pragma unroll
         for (int j = 0; j < SA_PER; j++) {
-            const u64 o = word_key(v[j], b * SA_BLOCK + j * SA_WG + threadIdx.x);
-            k = o > k ? o : k;
+            const bool more = v[j] > best;
+            best = more ? v[j] : best;
+            at = more ? j * SA_WG : at;
         }
-        k = wave_most(k);
+        u64 k = wave_most(word_key(best, b * SA_BLOCK + at + threadIdx.x));
         u64 *t = s[b & 1];  // (a block later than one whose reader may be behind)
         if ((threadIdx.x & 63) == 0) t[threadIdx.x >> 6] = k;
         __syncthreads();
