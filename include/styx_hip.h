@@ -320,7 +320,9 @@ typedef struct styx_kv_cache {
 /* Slot t of a sequence is row t % page_tokens of its page t / page_tokens;
  * cap = table_len * page_tokens slots.  Rows in pages that are not one of the
  * pool's (an entry outside [0, n_pages)) are neither read nor written and not
- * attended to; no page may hold two pages' slots that are in use.
+ * attended to.  Sequences may share pages that no call writes to (a common
+ * prefix): the page of a new row, and for styx_op_kv_evict every page of a
+ * sequence that loses rows, must be in one place of the table alone.
  *
  * Sequence b has rows in slots [0, len[b]); its new token is at position
  * pos[b] (its rope angle, rope [n_rope][hd/2][2] from styx_rope_table) and

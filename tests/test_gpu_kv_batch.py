@@ -206,6 +206,52 @@ def test_attn_many_ragged_sequences(gpu, f16):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n_seq,nkv,hd,longest", [(100, 2, 64, 2000), (40, 8, 256, 150), (130, 8, 64, 90),
+                                                  (300, 4, 64, 3), (3, 600, 64, 40), (2, 5, 128, 5000)])
+def test_attn_shares_of_the_workgroups(gpu, n_seq, nkv, hd, longest):
+    """More rows or heads than the workgroups that run at once, so that shares
+    end inside a head and begin others; head counts that do not divide them."""
+    rng = np.random.default_rng(n_seq)
+    c = Case(rng, True, [int(x) for x in rng.integers(0, longest, n_seq)], nkv, 1, hd, 64)
+    check_attn(c, run_attn(gpu, c))
+
+
+@pytest.mark.gpu
+def test_attn_pages_shared_by_sequences(gpu):
+    """A common prefix in the same pages of three sequences, their own rows
+    and the new ones in pages of their own."""
+    rng = np.random.default_rng(21)
+    c = Case(rng, False, [100, 75, 64], 2, 4, 64, 16)
+    c.table[1, :4] = c.table[2, :4] = c.table[0, :4]
+    check_attn(c, run_attn(gpu, c))
+
+
+@pytest.mark.gpu
+def test_attn_two_calls_on_one_stream_share_a_workspace_in_turn(gpu):
+    """What a call leaves in the workspace does not reach the next one."""
+    rng = np.random.default_rng(22)
+    lib = gpu.lib
+    cases = [Case(rng, False, [300, 20], 2, 8, 128, 64), Case(rng, True, [7], 1, 3, 64, 16),
+             Case(rng, False, [5, 900, 31], 1, 16, 64, 32)]
+    kvs = [c.kv(gpu) for c in cases]
+    need = [lib.styx_op_attn_batch_ws_bytes(C.byref(kv), c.nh, 1) for kv, c in zip(kvs, cases)]
+    ws = gpu.buffer(max(need))
+    held = []
+    for kv, c in zip(kvs, cases):
+        b = [gpu.from_numpy(x) for x in (c.lens, c.pos, c.q, c.kn, c.vn, c.qw, c.kw, c.rope, c.acc, c.where)]
+        out, acc_out = gpu.buffer(c.q.nbytes), gpu.from_numpy(np.full(c.acc.shape, -3.0, np.float32))
+        held.append((b, out, acc_out))
+        L.check(lib.styx_op_attn_decode_batch(
+            gpu.h, C.byref(kv), b[0].ptr, b[1].ptr, c.nh, b[2].ptr, b[3].ptr, b[4].ptr, b[5].ptr, b[6].ptr, EPS,
+            b[7].ptr, c.n_rope, c.scale, c.decay, b[8].ptr, acc_out.ptr, b[9].ptr, out.ptr, ws.ptr, ws.nbytes))
+    gpu.sync()
+    for c, (b, out, acc_out) in zip(cases, held):
+        check_attn(c, (out.download(np.float32).reshape(c.q.shape), acc_out.download(np.float32).reshape(c.acc.shape),
+                       b[9].download(np.int32).reshape(c.where.shape), c.bufs[0].download(c.dt).reshape(c.k.shape),
+                       c.bufs[1].download(c.dt).reshape(c.v.shape)))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("f16", [False, True])
 def test_attn_long_context_split(gpu, f16):
     rng = np.random.default_rng(6)

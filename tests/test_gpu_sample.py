@@ -206,6 +206,37 @@ def test_strides_offsets_and_outputs_left_out(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mean", [-1e30, -300.0, 0.0, 1e6, 1e30])
+def test_logits_far_from_zero(gpu, mean):
+    """Only the differences to the largest logit count: rows whose logits are
+    large against the temperature, of both signs."""
+    rng = np.random.default_rng(10)
+    x = (mean + 2 * max(1.0, abs(mean) * 2.0 ** -22) * rng.standard_normal((len(SETTINGS), 9000))).astype(np.float32)
+    check(gpu, x, params(SETTINGS), rng.random(len(SETTINGS)).astype(np.float32))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [1, 2, 3, 4, 5, 7, 8, 9, 40])
+def test_top_k_about_the_number_of_blocks(gpu, k):
+    """Rows of a few blocks of words whose best words lie together, apart, at
+    the ends, or number fewer than k."""
+    rng = np.random.default_rng(k)
+    n = 8 * 2048 - 5
+    x = rng.standard_normal((6, n)).astype(np.float32)
+    x[0, :50] += 20
+    x[1, ::2048] += 20
+    x[2, -9:] += 20
+    x[3, [0, n - 1]] = 30
+    x[4, :] = -np.inf
+    x[4, [5, 3000, 9000]] = [1.0, 1.0, 0.5]
+    x[5, 2000:2100] = 8.0
+    u = rng.random(6).astype(np.float32)
+    check(gpu, x, params([(1.0, k, 1.0, 0.0)]), u)
+    check(gpu, x, params([(0.7, k, 0.8, 0.05)]), u)
+    check(gpu, x, params([(0.01, k, 0.999, 0.0)]), u)
+
+
+@pytest.mark.gpu
 def test_the_longest_rows(gpu):
     """2^19 - 1 words, all of one logit among them: sums just below 2^63, and
     a border list that is the whole row."""
