@@ -39,9 +39,9 @@ constexpr int AB_WG = 256, AB_WAVES = AB_WG / 64;
 __host__ __device__ constexpr int ab_slots(int hd) { return hd == 64 ? 768 : hd == 128 ? 512 : 256; }
 // Rows of a unit: a 16-row tile (f32), or half of a 32-row one, per wave.
 constexpr int AB_UNIT = 64;
-// Slots of a step of the joining launch's weights: 8 of a thread's in flight
-// with up to 4 query heads per kv head, 2 with more.
-__host__ __device__ constexpr int ab_wper(int gqa) { return gqa <= 4 ? 8 : 2; }
+// Slots of a thread in a step of the joining launch's weights: with its query
+// heads (4, 8 or 16 per kv head) 32 scores in flight.
+__host__ __device__ constexpr int ab_wper(int gqa) { return gqa <= 4 ? 8 : gqa <= 8 ? 4 : 2; }
 // Pieces whose partials a thread of the joining launch has in flight.
 constexpr int AB_BATCH = 8;
 
@@ -871,6 +871,8 @@ template <int DIMS> static void launch_join(hipStream_t st, const AttnBatchArgs 
 {
     if (a.gqa <= 4)
         hipLaunchKernelGGL((k_attn_batch_join<DIMS, 4>), dim3((unsigned)grid), dim3(AB_WG), 0, st, a);
+    else if (a.gqa <= 8)
+        hipLaunchKernelGGL((k_attn_batch_join<DIMS, 8>), dim3((unsigned)grid), dim3(AB_WG), 0, st, a);
     else
         hipLaunchKernelGGL((k_attn_batch_join<DIMS, 16>), dim3((unsigned)grid), dim3(AB_WG), 0, st, a);
 }
