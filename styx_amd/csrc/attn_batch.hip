@@ -218,15 +218,24 @@ template <int HD> struct HeadRow {
     }
 };
 
+// A row's piece; ONCE: one that nothing will find in a cache again.
+template <bool ONCE, typename V> __device__ __forceinline__ V row_piece(const void *p)
+{
+    if constexpr (ONCE)
+        return __builtin_nontemporal_load((const V *)p);
+    else
+        return *(const V *)p;
+}
+
 // Lane (n = lane & 15, g = lane >> 4) holds query row n.  Scores are formed
 // transposed, keys x queries, so a lane has its own query's scores of keys
 // 4 g + i of a 16-key tile: the softmax factors are lane-local, and the
 // scores already are the operand of the value product.
-template <typename T, int HD, bool WIDE> struct Tile;
+template <typename T, int HD, bool WIDE, bool ONCE> struct Tile;
 
 // f32 rows: v_mfma_f32_16x16x4_f32, 16 keys a step.  The head's dimensions
 // are permuted alike on both sides of each product, for 16-byte loads.
-template <int HD, bool WIDE> struct Tile<float, HD, WIDE> {
+template <int HD, bool WIDE, bool ONCE> struct Tile<float, HD, WIDE, ONCE> {
     static constexpr int KEYS = 16, NS = 4, NQ = HD / 16, NV = HD / 64, QROWS = 16;
     int lane;
     f4 q[NQ], kf[NQ], vf[4][NV], o[NV][4];
@@ -247,7 +256,7 @@ template <int HD, bool WIDE> struct Tile<float, HD, WIDE> {
     {
         const float *p = pool + max(row[0], 0) * stride + 4 * (lane >> 4);
 #pragma unroll
-        for (int i = 0; i < NQ; i++) kf[i] = *(const f4 *)(p + 16 * i);
+        for (int i = 0; i < NQ; i++) kf[i] = row_piece<ONCE, f4>(p + 16 * i);
     }
     __device__ __forceinline__ void load_v(const float *pool, const int *row, int64_t stride)
     {
@@ -255,7 +264,7 @@ template <int HD, bool WIDE> struct Tile<float, HD, WIDE> {
         for (int i = 0; i < 4; i++) {
             const float *p = pool + max(__shfl(row[0], key_of(i)), 0) * stride + 4 * (lane & 15);
 #pragma unroll
-            for (int j = 0; j < NV; j++) vf[i][j] = *(const f4 *)(p + 64 * j);
+            for (int j = 0; j < NV; j++) vf[i][j] = row_piece<ONCE, f4>(p + 64 * j);
         }
     }
     // the new row, at key `at` of the tile, from LDS; values of keys that
@@ -323,7 +332,7 @@ template <int HD, bool WIDE> struct Tile<float, HD, WIDE> {
 // Lane group g's keys are 4 g + i and 16 + 4 g + i on both sides of the value
 // product; its V operand, 8 keys of one dimension, is made of 16-byte pieces
 // of 8 rows by lane-local byte permutes.
-template <int HD, bool WIDE> struct Tile<_Float16, HD, WIDE> {
+template <int HD, bool WIDE, bool ONCE> struct Tile<_Float16, HD, WIDE, ONCE> {
     static constexpr int KEYS = 32, NS = 8, NQ = HD / 32, DPL = HD / 16, QROWS = WIDE ? 16 : 8;
     static constexpr int NB = DPL > 8 ? DPL / 8 : 1, ND = DPL > 8 ? 4 : DPL / 2;  // 16-byte blocks, dwords of each
     static constexpr int EB = 2 * ND;  // dims of a lane in a block
@@ -367,20 +376,20 @@ template <int HD, bool WIDE> struct Tile<_Float16, HD, WIDE> {
         for (int t = 0; t < 2; t++) {
             const _Float16 *p = pool + max(row[t], 0) * stride + 8 * (lane >> 4);
 #pragma unroll
-            for (int i = 0; i < NQ; i++) kf[t][i] = *(const h8 *)(p + 32 * i);
+            for (int i = 0; i < NQ; i++) kf[t][i] = row_piece<ONCE, h8>(p + 32 * i);
         }
     }
-    __device__ __forceinline__ void load_v_row(int i, const _Float16 *p)
+    template <bool NT> __device__ __forceinline__ void load_v_row(int i, const _Float16 *p)
     {
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             const uint32_t *s = (const uint32_t *)(p + 128 * b + EB * (lane & 15));
             if constexpr (ND == 4) {
-                const styx_u4 v = *(const styx_u4 *)s;
+                const styx_u4 v = row_piece<NT, styx_u4>(s);
 #pragma unroll
                 for (int d = 0; d < 4; d++) vf[i][b][d] = v[d];
             } else {
-                const styx_u2 v = *(const styx_u2 *)s;
+                const styx_u2 v = row_piece<NT, styx_u2>(s);
                 vf[i][b][0] = v[0];
                 vf[i][b][1] = v[1];
             }
@@ -390,7 +399,7 @@ template <int HD, bool WIDE> struct Tile<_Float16, HD, WIDE> {
     {
 #pragma unroll
         for (int i = 0; i < 8; i++)
-            load_v_row(i, pool + max(__shfl(row[i >> 2], key_of(i & 3)), 0) * stride);
+            load_v_row<ONCE>(i, pool + max(__shfl(row[i >> 2], key_of(i & 3)), 0) * stride);
     }
     __device__ __forceinline__ void patch_k(const _Float16 *knew, int at)
     {
@@ -406,7 +415,7 @@ template <int HD, bool WIDE> struct Tile<_Float16, HD, WIDE> {
     {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            if (key_of(i) == at) load_v_row(i, vnew);
+            if (key_of(i) == at) load_v_row<false>(i, vnew);
             if (!((seen >> key_of(i)) & 1u)) {
 #pragma unroll
                 for (int b = 0; b < NB; b++)
@@ -482,10 +491,10 @@ template <int HD, bool WIDE> struct Tile<_Float16, HD, WIDE> {
     }
 };
 
-template <typename T, int HD, bool WIDE, bool SCORED>
+template <typename T, int HD, bool WIDE, bool SCORED, bool ONCE>
 __global__ void __launch_bounds__(AB_WG, ab_slots(HD) / 256) k_attn_batch(AttnBatchArgs a)
 {
-    using Tl = Tile<T, HD, WIDE>;
+    using Tl = Tile<T, HD, WIDE, ONCE>;
     constexpr int KEYS = Tl::KEYS, NS = Tl::NS, QROWS = Tl::QROWS, NR = KEYS / 16;
     __shared__ __align__(16) float s_q[QROWS][HD + 4];
     __shared__ float s_qmax[QROWS];
@@ -851,10 +860,24 @@ AttnBatchWs attn_batch_ws(int n_seq, int nkv, int hd, int cap, int gqa, bool sco
 template <typename T, int HD, bool WIDE>
 static void launch_ab(hipStream_t st, const AttnBatchArgs &a, int64_t grid)
 {
-    if (a.acc_out)
-        hipLaunchKernelGGL((k_attn_batch<T, HD, WIDE, true>), dim3((unsigned)grid), dim3(AB_WG), 0, st, a);
-    else
-        hipLaunchKernelGGL((k_attn_batch<T, HD, WIDE, false>), dim3((unsigned)grid), dim3(AB_WG), 0, st, a);
+    const dim3 g((unsigned)grid), wg(AB_WG);
+    // Pools larger than the Infinity Cache: their rows come from HBM, and
+    // loads that leave nothing behind stream them 5-9% faster (40 f16
+    // sequences of 8 heads, 327 MB: 83 -> 76 us); smaller ones may be found
+    // there (24 conversations, 102 MB: 27 us against 32 with such loads).
+    const KvView &kv = a.kv;
+    const bool once = 2.0 * sizeof(T) * kv.n_pages * kv.page_tokens * kv.nkv * kv.hd > 256.0 * (1 << 20);
+    if (a.acc_out) {
+        if (once)
+            hipLaunchKernelGGL((k_attn_batch<T, HD, WIDE, true, true>), g, wg, 0, st, a);
+        else
+            hipLaunchKernelGGL((k_attn_batch<T, HD, WIDE, true, false>), g, wg, 0, st, a);
+    } else {
+        if (once)
+            hipLaunchKernelGGL((k_attn_batch<T, HD, WIDE, false, true>), g, wg, 0, st, a);
+        else
+            hipLaunchKernelGGL((k_attn_batch<T, HD, WIDE, false, false>), g, wg, 0, st, a);
+    }
 }
 
 template <int HD> static void launch_ab_hd(hipStream_t st, const AttnBatchArgs &a, int64_t grid)

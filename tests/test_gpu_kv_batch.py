@@ -322,19 +322,21 @@ def test_attn_f16_queries_of_any_size(gpu, size):
 
 
 @pytest.mark.gpu
-def test_attn_pools_past_32_bit_offsets(gpu):
+@pytest.mark.parametrize("f16,hd", [(True, 256), (True, 64), (False, 128)])
+def test_attn_pools_past_32_bit_offsets(gpu, f16, hd):
     """Rows more than 2^32 bytes (2^31 elements) into the pools."""
     rng = np.random.default_rng(12)
-    c = Case(rng, True, [70], 8, 2, 256, 32)
+    c = Case(rng, f16, [70], 8, 2, hd, 32)
     far = 2 ** 31 // (c.nkv * c.hd * c.page) + 1  # pages before the used ones
     n_pages = far + c.n_pages
-    nb = n_pages * c.page * c.nkv * c.hd * 2
+    size = np.dtype(c.dt).itemsize
+    nb = n_pages * c.page * c.nkv * c.hd * size
     pools = [gpu.buffer(nb), gpu.buffer(nb)]
-    off = far * c.page * c.nkv * c.hd * 2
+    off = far * c.page * c.nkv * c.hd * size
     for p, x in zip(pools, (c.k, c.v)):
         p.upload(x, off)
     table = gpu.from_numpy(np.where(c.table >= 0, c.table + far, c.table).astype(np.int32))
-    kv = L.KvCache(L.F16, 1, c.nkv, c.hd, c.page, n_pages, c.table_len, pools[0].ptr, pools[1].ptr, table.ptr)
+    kv = L.KvCache(L.F16 if f16 else L.F32, 1, c.nkv, c.hd, c.page, n_pages, c.table_len, pools[0].ptr, pools[1].ptr, table.ptr)
     b = [gpu.from_numpy(x) for x in (c.lens, c.pos, c.q, c.kn, c.vn, c.qw, c.kw, c.rope, c.acc, c.where)]
     out = gpu.buffer(c.q.nbytes)
     acc_out = gpu.from_numpy(np.full(c.acc.shape, -3.0, np.float32))
