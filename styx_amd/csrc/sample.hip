@@ -22,6 +22,15 @@
 // Bound: latency for a few rows (each launch waits for all of the one
 // before); for many, the f64 exponentials of launches 2 and 3 and one read of
 // the logits from HBM (the other two hit the Infinity Cache).
+//
+// Measured: one row of 151936 words with top-k and top-p 2.6 + 5.2 + 6.2 + 8.7
+// us, of 4096 with a temperature alone 13 us in all; 64 rows of 151936 with
+// settings of their own 8 + 19 + 23 + 16 us (logits read three times, 1.8
+// TB/s; the launches 2 and 3 run 4 and 6 million VALU instructions, most for
+// the rows that neither top-k nor top-p cuts); 17 flat rows of 50257, a
+// nucleus of most words, 30 us.  (A wave per block of 512 words without
+// barriers, the border found by a launch of its own, and words weighed four
+// side by side were tried: each no faster over these.)
 #include "../../include/styx_hip.h"
 #include "lanes.h"
 #include "sample.h"
