@@ -356,7 +356,8 @@ uint64_t styx_op_attn_batch_ws_bytes(const styx_kv_cache *kv, int nh, int scored
  * rows (trigger >= keep), by itself for each kv head: the `keep` rows of the
  * largest acc_in stay, before all others the rows whose position slot_pos is
  * one of the `recent` last up to pos[b] (> pos[b] - recent) or below `sinks`;
- * NaN counts least, ties go to the lower slot; recent + sinks <= keep.  Rows
+ * NaN counts least, ties go to the lower slot; recent + sinks <= keep, cap up
+ * to 2^26.  Rows
  * that stay in slots below keep lie still; the slots below keep that lose
  * their row, ascending, take the rows that stay in slots at or past keep,
  * ascending: K and V, weight and position (attention does not depend on the

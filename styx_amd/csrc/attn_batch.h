@@ -71,6 +71,10 @@ struct AttnBatchWs {
 AttnBatchWs attn_batch_ws(int n_seq, int nkv, int hd, int cap, int gqa, bool scored);
 hipError_t launch_attn_batch(hipStream_t st, AttnBatchArgs a, float *ws);
 
+// Most slots of a sequence that rows are evicted from: its parts all read each
+// other's bins, which takes the square of their number (4096 at most).
+constexpr int EVICT_MAX_CAP = 1 << 26;
+
 struct KvEvictArgs {
     KvView kv;
     const int32_t *len, *pos;

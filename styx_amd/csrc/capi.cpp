@@ -583,7 +583,9 @@ int styx_op_attn_decode_batch(styx_gpu *g, const styx_kv_cache *kv, const int32_
 
 uint64_t styx_op_kv_evict_ws_bytes(const styx_kv_cache *kv, int keep)
 {
-    if (!kv_shape_ok(kv) || keep < 1 || keep > kv->table_len * kv->page_tokens) return 0;
+    if (!kv_shape_ok(kv) || (int64_t)kv->table_len * kv->page_tokens > EVICT_MAX_CAP || keep < 1 ||
+        keep > kv->table_len * kv->page_tokens)
+        return 0;
     return kv_evict_ws_bytes(kv->n_seq, kv->nkv, kv->table_len * kv->page_tokens, keep);
 }
 
@@ -603,6 +605,7 @@ int styx_op_kv_evict(styx_gpu *g, const styx_kv_cache *kv, const int32_t *len, c
     if (!len || !pos || !acc_in || !acc_out || !slot_pos_in || !slot_pos_out || !len_out)
         return fail(STYX_E_INVALID, std::string(who) + ": NULL pointer");
     const uint64_t need = styx_op_kv_evict_ws_bytes(kv, keep);
+    if (!need) return fail(STYX_E_INVALID, std::string(who) + ": more than 2^26 slots per sequence");
     if (int r = ws_ok(ws, ws_bytes, need, who)) return r;
     a.len = len;
     a.pos = pos;

@@ -237,9 +237,13 @@ class KvBatch:
 
     def set(self, len=None, pos=None, table=None) -> None:
         """Upload lengths, positions or the page table (-1: no page)."""
-        for buf, a in ((self.len, len), (self.pos, pos), (self.table, table)):
+        for buf, a, n in ((self.len, len, self.n_seq), (self.pos, pos, self.n_seq),
+                          (self.table, table, self.n_seq * self.c.table_len)):
             if a is not None:
-                buf.upload(np.asarray(a, np.int32))
+                a = np.asarray(a, np.int32)
+                if a.size != n:
+                    raise ValueError(f"{a.size} values, {n} expected")
+                buf.upload(a)
 
     def lengths(self) -> np.ndarray:
         return self.len.download(np.int32, self.n_seq)
@@ -255,6 +259,11 @@ class KvBatch:
                scale: float, q_norm: Buffer | None = None, k_norm: Buffer | None = None,
                eps: float = 1e-6, decay: float = 1.0) -> None:
         """styx_op_attn_decode_batch; the weights are added in place."""
+        for name, b, n in (("q", q, self.n_seq * nh), ("out", out, self.n_seq * nh),
+                           ("k", k, self.n_seq * self.nkv), ("v", v, self.n_seq * self.nkv),
+                           ("q_norm", q_norm, 1), ("k_norm", k_norm, 1), ("rope", rope, 2 * n_rope)):
+            if b is not None and b.nbytes < 4 * n * self.hd:
+                raise ValueError(f"{name}: {b.nbytes} bytes, {4 * n * self.hd} needed")
         ws = self._workspace(self.lib.styx_op_attn_batch_ws_bytes(C.byref(self.c), nh, int(self.scored)))
         ptr = lambda b: b.ptr if b is not None else None  # noqa: E731
         L.check(self.lib.styx_op_attn_decode_batch(
@@ -287,6 +296,10 @@ def sample(gpu: Gpu, logits: Buffer, n: int, params, u, ld: int | None = None):
     arr = (L.SampleParams * len(params))(*[L.SampleParams(float(t), int(k), float(p), float(m))
                                            for t, k, p, m in params])
     rows = len(u)
+    if len(params) not in (1, rows):
+        raise ValueError(f"{len(params)} settings for {rows} rows")
+    if rows and logits.nbytes < 4 * ((rows - 1) * (ld or n) + n):
+        raise ValueError(f"logits: {logits.nbytes} bytes hold fewer than {rows} rows of {n}")
     par, uu = gpu.from_numpy(np.frombuffer(arr, np.uint8)), gpu.from_numpy(u)
     out = [gpu.buffer(max(4 * rows, 16)) for _ in range(3)]
     ws = gpu.buffer(max(int(gpu.lib.styx_op_sample_ws_bytes(rows, n)), 16))

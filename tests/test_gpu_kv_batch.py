@@ -269,6 +269,38 @@ def test_attn_accumulator_forms(gpu, in_place, with_acc_in):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scored", [True, False])
+def test_attn_positions_with_and_without_weights(gpu, scored):
+    """slot_pos left out of a call with weights; given to one without."""
+    rng = np.random.default_rng(23)
+    c = Case(rng, False, [40, 0, 77], 2, 4, 64, 32)
+    kv = c.kv(gpu)
+    b = [gpu.from_numpy(x) for x in (c.lens, c.pos, c.q, c.kn, c.vn, c.qw, c.kw, c.rope, c.where)]
+    out, acc_out = gpu.buffer(c.q.nbytes), gpu.from_numpy(np.full(c.acc.shape, -3.0, np.float32))
+    acc = gpu.from_numpy(c.acc)
+    nbytes = gpu.lib.styx_op_attn_batch_ws_bytes(C.byref(kv), c.nh, int(scored))
+    ws = gpu.buffer(nbytes)
+    L.check(gpu.lib.styx_op_attn_decode_batch(
+        gpu.h, C.byref(kv), b[0].ptr, b[1].ptr, c.nh, b[2].ptr, b[3].ptr, b[4].ptr, b[5].ptr, b[6].ptr, EPS, b[7].ptr,
+        c.n_rope, c.scale, c.decay, acc.ptr if scored else None, acc_out.ptr if scored else None,
+        None if scored else b[8].ptr, out.ptr, ws.ptr, nbytes))
+    gpu.sync()
+    where = b[8].download(np.int32).reshape(c.where.shape)
+    if scored:
+        assert np.array_equal(where, c.where)
+        for i in range(c.B):
+            where[i, :, c.lens[i]] = c.pos[i]  # (what check_attn looks for)
+    else:
+        want = c.where.copy()
+        for i in range(c.B):
+            want[i, :, c.lens[i]] = c.pos[i]
+        assert np.array_equal(where, want)
+    check_attn(c, (out.download(np.float32).reshape(c.q.shape), acc_out.download(np.float32).reshape(c.acc.shape), where,
+                   c.bufs[0].download(c.dt).reshape(c.k.shape), c.bufs[1].download(c.dt).reshape(c.v.shape)),
+               scored=scored)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("f16", [False, True])
 def test_attn_rows_in_pages_outside_the_pool_are_not_seen(gpu, f16):
     """Entries below 0 and past the pool: in the middle, at the new row, and
@@ -529,6 +561,8 @@ def cache(**kw):
 BAD_SHAPES = [dict(type=L.Q8_0), dict(type=30), dict(n_seq=0), dict(nkv=0), dict(hd=96), dict(hd=0),
               dict(page_tokens=0), dict(n_pages=0), dict(table_len=0), dict(table_len=2 ** 28, page_tokens=2 ** 28),
               dict(n_pages=2 ** 30, page_tokens=4), dict(n_seq=2 ** 24), dict(n_seq=-1)]
+# what only the eviction refuses: more than 2^26 slots
+LONG = dict(table_len=2 ** 23, page_tokens=16)
 
 
 @pytest.mark.parametrize("kw", BAD_SHAPES)
@@ -550,6 +584,13 @@ def test_workspace_sizes():
     # scores: a float per slot (in multiples of 64) and query head
     assert lib.styx_op_attn_batch_ws_bytes(C.byref(cache()), 16, 1) == plain + 2 * 16 * 64 * 4
     assert lib.styx_op_kv_evict_ws_bytes(C.byref(cache()), 32) >= 2 * 2 * 32 * 4
+
+
+def test_eviction_is_refused_past_its_longest_cache():
+    lib = L.load()
+    assert lib.styx_op_kv_evict_ws_bytes(C.byref(cache(**LONG)), 8) == 0
+    assert lib.styx_op_attn_batch_ws_bytes(C.byref(cache(**LONG)), 16, 0) > 0
+    assert lib.styx_op_kv_evict_ws_bytes(C.byref(cache(table_len=2 ** 22, page_tokens=16)), 8) > 0
 
 
 def test_no_gpu_is_refused():
@@ -612,5 +653,7 @@ def test_evict_refusals(gpu):
     for kw in (dict(keep=0), dict(keep=33, trigger=33), dict(trigger=7), dict(recent=-1), dict(sinks=-1),
                dict(recent=7, sinks=2), dict(recent=2 ** 31 - 1, sinks=2 ** 31 - 1)):
         assert call(**kw)[0] == -1, kw
+    rc, msg = call(kv=cache(kpool=p, vpool=p, page_table=p, **LONG))
+    assert rc == -1 and "2^26" in msg
     assert call(ws_bytes=8)[0] == -1 and call(ws=None)[0] == -1 and call(ws=p + 8)[0] == -1
     gpu.sync()

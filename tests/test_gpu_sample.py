@@ -237,6 +237,17 @@ def test_top_k_about_the_number_of_blocks(gpu, k):
 
 
 @pytest.mark.gpu
+def test_the_most_rows(gpu):
+    rng = np.random.default_rng(11)
+    x = (2 * rng.standard_normal((65535, 7))).astype(np.float32)
+    par, u = params([(0.8, 5, 0.9, 0.02)]), rng.random(65535).astype(np.float32)
+    tok, lp, left = run(gpu, x, par, u)
+    for r in [0, 1, 65534, *rng.integers(0, 65535, 2000).tolist()]:
+        want = define(x[r], par[0], u[r])
+        assert (tok[r], left[r]) == (want[0], want[2]), r
+
+
+@pytest.mark.gpu
 def test_the_longest_rows(gpu):
     """2^19 - 1 words, all of one logit among them: sums just below 2^63, and
     a border list that is the whole row."""

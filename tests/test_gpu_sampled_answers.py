@@ -95,6 +95,36 @@ def test_answers_within_a_budget(gpu, f16, hd, page):
     kv.free()
 
 
+def test_the_package_checks_what_it_is_given(gpu):
+    from styx_amd import KvBatch, StyxError, sample
+    kv = KvBatch(gpu, 2, 1, 64, 16, 4, 2, scored=False)
+    with pytest.raises(ValueError):
+        kv.set(len=[1, 2, 3])
+    with pytest.raises(ValueError):
+        kv.set(table=np.zeros((2, 3)))
+    with pytest.raises(ValueError):
+        kv.evict(8, 8)
+    z = gpu.zeros(2 * 4 * 64 * 4)
+    small = gpu.zeros(64)
+    kv.set(len=[0, -1], pos=[0, 0], table=[[0, 1], [2, 3]])
+    for bad in range(5):
+        a = [z] * 5
+        a[bad] = small
+        with pytest.raises(ValueError):
+            kv.attend(4, *a, 2, 0.125)
+    with pytest.raises(StyxError):
+        kv.attend(17, gpu.zeros(1 << 14), z, z, gpu.zeros(1 << 14), z, 1, 0.125)
+    kv.attend(4, z, z, z, z, z, 1, 0.125)
+    gpu.sync()
+    with pytest.raises(ValueError):
+        sample(gpu, z, 300, (1.0, 0, 1.0, 0.0), [0.5, 0.5])
+    with pytest.raises(ValueError):
+        sample(gpu, z, 30, [(1.0, 0, 1.0, 0.0)] * 3, [0.5, 0.5])
+    with pytest.raises(StyxError):
+        sample(gpu, z, 30, (1.0, 0, 1.0, 0.0), [0.5], ld=20)
+    kv.free()
+
+
 # ------------------------------------------------------------- engine ------
 def model(gpu, **kw):
     from styx_amd import MoeModel, SynthConfig
