@@ -94,17 +94,18 @@ template <int KPT> struct EvKeys {
         per = (t1 - t0 + EV_WG - 1) / EV_WG;
         first = t0 + wave * per * 64;
         end = t1;
+        // all loads on every path, rows past the wave's at its last slot: with
+        // a branch for each row they were waited for one by one
         float w[KPT];
         int32_t p[KPT];
 #pragma unroll
         for (int j = 0; j < KPT; j++) {
-            if (j >= per) break;
-            const int t = min(first + 64 * j + lane, t1 - 1);
+            const int t = min(first + 64 * min(j, per - 1) + lane, t1 - 1);
             w[j] = a.acc_in[base + t];
             p[j] = a.pos_in[base + t];
         }
 #pragma unroll
-        for (int j = 0; j < KPT; j++) key[j] = j < per ? evict_key(a, w[j], p[j], newest) : 0;
+        for (int j = 0; j < KPT; j++) key[j] = evict_key(a, w[j], p[j], newest);
     }
     // f(row, key, whether there is one), the wave's lanes together
     template <typename F> __device__ __forceinline__ void each(F f) const
