@@ -798,14 +798,17 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch_join(AttnBatchArgs a)
     if (tile * STEP >= at.rows) return;
     const int64_t base = (int64_t)b * kv.nkv + kvh;
     const float *sc = a.score + base * a.gqa * a.stride;
+    // (every load on every path: heads past the last read it again, and without
+    // weights to add to, those that are to be written are read and dropped)
+    const float *acc = (a.acc_in ? a.acc_in : a.acc_out) + base * kv.cap;
     float s[PER][HM], old[PER];
     auto load = [&](int t0) {
 #pragma unroll
         for (int j = 0; j < PER; j++) {
             const int t = min(t0 + tid + AB_WG * j, at.rows - 1);
 #pragma unroll
-            for (int h = 0; h < HM; h++) s[j][h] = h < a.gqa ? sc[(int64_t)h * a.stride + t] : -INFINITY;
-            old[j] = a.acc_in && t < at.rows - 1 ? a.acc_in[base * kv.cap + t] : 0.0f;
+            for (int h = 0; h < HM; h++) s[j][h] = sc[(int64_t)min(h, a.gqa - 1) * a.stride + t];
+            old[j] = acc[t];
         }
     };
     load(tile * STEP);
@@ -829,7 +832,7 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch_join(AttnBatchArgs a)
 #pragma unroll
             for (int h = 0; h < HM; h++)
                 if (h < a.gqa) sum += exp2_(s[j][h] - s_M[h]) * s_R[h];
-            if (t < at.rows) a.acc_out[base * kv.cap + t] = a.decay * old[j] + sum;
+            if (t < at.rows) a.acc_out[base * kv.cap + t] = (a.acc_in && t < at.rows - 1 ? a.decay * old[j] : 0.0f) + sum;
         }
         t0 += a.tiles * STEP;
         if (t0 >= at.rows) break;
