@@ -330,10 +330,11 @@ typedef struct styx_kv_cache {
  * pos[b] outside [0, n_rope) is skipped: nothing of it is read or written
  * (padding).  The lengths are the caller's to advance.
  * q [n_seq][nh*hd], k and v [n_seq][nkv*hd] f32 raw projections, q_norm and
- * k_norm [hd] or NULL, out [n_seq][nh*hd]; nh / nkv from 1 to 16.  An f16
- * cache holds k and v rounded once; scores, sums and outputs are f32 (a V
- * value that is not finite makes its dimension of the outputs infinite, or,
- * in an f16 cache, infinite or NaN).  No row seen: out is 0.
+ * k_norm [hd] or NULL, out [n_seq][nh*hd]; nh / nkv from 1 to 16.  k is
+ * normalised and turned in f64 and rounded to f32, and k and v to f16 for an
+ * f16 cache; scores, sums and outputs are f32 (a V value that is not finite
+ * makes its dimension of the outputs infinite, or, in an f16 cache, infinite
+ * or NaN).  No row seen: out is 0.
  * acc_in / acc_out [n_seq][nkv][cap] f32: for the rows t <= len[b]
  *   acc_out[t] = decay * acc_in[t] + sum over the kv head's query heads of
  *                the softmax weight of row t

@@ -222,8 +222,13 @@ template <int HD> struct HeadRow {
             if (HALF < 64 && lane >= HALF) continue;
             const int i = lane + 64 * j;
             const double a = norm ? x0[j] * f * w.x0[j] : x0[j], b = norm ? x1[j] * f * w.x1[j] : x1[j];
-            emit(i, (float)(a * cs[j].x - b * cs[j].y));
-            emit(i + HALF, (float)(a * cs[j].y + b * cs[j].x));
+            // (kept apart from a conversion to f16 that may follow: contracted
+            // with it, the f64 value would be rounded to f16 directly, which
+            // differs for one value of some 15000 and takes a dozen instructions)
+            float lo = (float)(a * cs[j].x - b * cs[j].y), hi = (float)(a * cs[j].y + b * cs[j].x);
+            asm volatile("" : "+v"(lo), "+v"(hi));
+            emit(i, lo);
+            emit(i + HALF, hi);
         }
     }
 };

@@ -354,6 +354,31 @@ def test_attn_f16_queries_of_any_size(gpu, size):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("norms", [False, True])
+def test_attn_appended_f16_rows_are_rounded_by_way_of_f32(gpu, norms, hd):
+    """Bit for bit: of 2^18 values some ten lie so near the middle of two f16
+    values that rounding the f64 row directly gives the other one.  The two f64
+    rows differ by less than 2^-44 of their head's largest value (64 roundings
+    of 2^-53 and the order of the sums), so values that near to the middle of
+    two f32 values may go either way."""
+    rng = np.random.default_rng(14)
+    c = Case(rng, True, list(range(1, 65)) * 2, 2 ** 11 // hd, 1, hd, 16, norms=norms)
+    kp = run_attn(gpu, c, scored=False)[3]
+    direct = 0
+    for b in range(c.B):
+        row, p = c.rows(b, c.lens[b] + 1)[-1], int(c.pos[b])
+        for j in range(c.nkv):
+            k64 = c.head(c.kn[b, j], c.kw, p)
+            near = 2.0 ** -44 * np.abs(k64).max()
+            k32 = k64.astype(np.float32)
+            sure = (k64 - near).astype(np.float32) == (k64 + near).astype(np.float32)
+            assert np.array_equal(kp[row, j][sure], k32.astype(np.float16)[sure])
+            direct += int(np.sum(sure & (k64.astype(np.float16) != k32.astype(np.float16))))
+    assert direct > 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("f16,hd", [(True, 256), (True, 64), (False, 128)])
 def test_attn_pools_past_32_bit_offsets(gpu, f16, hd):
     """Rows more than 2^32 bytes (2^31 elements) into the pools."""
