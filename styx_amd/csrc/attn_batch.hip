@@ -28,11 +28,11 @@
 // in the first launch and 1 to 4 us slower in the second.)
 //
 // Measured, both launches: one context of 32767 f32 rows, 16 query heads for
-// each of 4 kv heads, 33 + 7.5 us (135 MB, 3.3 TB/s); six of up to 20011 f32
+// each of 4 kv heads, 34 + 7 us (135 MB, 3.3 TB/s); six of up to 20011 f32
 // rows, head_dim 256, without weights 62 + 5 us (302 MB, 4.5 TB/s); 24
-// conversations of up to 4096 f16 rows 27 + 6.5 us (102 MB, 3.1 TB/s); 40 of
-// up to 8192, head_dim 64, 76 + 8.5 us (327 MB, 3.9 TB/s); one of 37 rows 8 +
-// 4 us, the chain lengths, page table, rows, and the second launch.
+// conversations of up to 4096 f16 rows 29 + 6.5 us (102 MB, 2.9 TB/s); 40 of
+// up to 8192, head_dim 64, 76 + 8 us (327 MB, 3.9 TB/s); one of 37 rows 8 +
+// 3.5 us, the chain lengths, page table, rows, and the second launch.
 #include <algorithm>
 #include <type_traits>
 

@@ -18,9 +18,9 @@
 // holes and movers, and which slots stay; a moving launch does the rest.
 //
 // Measured: one conversation of 1088 rows cut to 1024, 4 kv heads, 6.9 + 4 us;
-// 32 of up to 9001 f16 rows cut to 4096, 20 + 25 us, of which the moves run
-// at 3.7 TB/s; two of 65536 f32 rows, 8 kv heads, cut to 16384, 41 us in four
-// launches, then 88 us of moves (4.6 TB/s, a large copy's rate).
+// 32 of up to 9001 f16 rows cut to 4096, 14.5 + 24.5 us, of which the moves
+// run at 3.8 TB/s; two of 65536 f32 rows, 8 kv heads, cut to 16384, 41 us in
+// four launches, then 88 us of moves (4.6 TB/s, a large copy's rate).
 #include <algorithm>
 #include <type_traits>
 
