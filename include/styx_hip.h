@@ -334,7 +334,9 @@ typedef struct styx_kv_cache {
  * normalised and turned in f64 and rounded to f32, and k and v to f16 for an
  * f16 cache; scores, sums and outputs are f32 (a V value that is not finite
  * makes its dimension of the outputs infinite, or, in an f16 cache, infinite
- * or NaN).  No row seen: out is 0.
+ * or NaN; a K value that is not finite makes those of its heads NaN, or its
+ * row one without weight where the score is -infinity).  No row seen: out is
+ * 0.
  * acc_in / acc_out [n_seq][nkv][cap] f32: for the rows t <= len[b]
  *   acc_out[t] = decay * acc_in[t] + sum over the kv head's query heads of
  *                the softmax weight of row t
@@ -566,8 +568,8 @@ int styx_moe_decode(styx_moe *m, int n_steps, uint32_t *out);
  * rules with one set of settings and one random number u (no counterpart in
  * the reference); logprob may be NULL.  The model's state is unchanged:
  * forward the token to go on.  STYX_E_STATE before the first token (also
- * after styx_moe_reset or styx_moe_fill_kv) and when no logit is above
- * -infinity. */
+ * after styx_moe_reset, styx_moe_fill_kv or styx_moe_time_stage, and after a
+ * token that failed) and when no logit is above -infinity. */
 int styx_moe_sample(styx_moe *m, const styx_sample_params *params, float u, uint32_t *token,
                     float *logprob);
 /* styx_moe_generate with sampled tokens: token i of out_tokens by u[i] of the

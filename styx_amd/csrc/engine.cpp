@@ -2121,9 +2121,9 @@ int styx_moe_forward_token(styx_moe *m, uint32_t token, float *logits_out)
         if (int r = m->maybe_repin()) return r;
     if (int r = m->ensure_pages(m->n_past)) return r;
     STYX_HIP(launch_set_token(m->gpu->stream, m->d_tok, m->d_pos, token, m->n_past));
+    m->has_logits = false;
     if (int r = m->run_token(false)) return r;
     m->n_past++;
-    m->has_logits = true;
     if (logits_out)
         STYX_HIP(hipMemcpyAsync(logits_out, m->logits, sizeof(float) * m->V, hipMemcpyDeviceToHost,
                                 m->gpu->stream));
@@ -2141,6 +2141,7 @@ int styx_moe_forward_token(styx_moe *m, uint32_t token, float *logits_out)
                                     hipMemcpyDeviceToHost, m->gpu->stream));
         STYX_HIP(hipStreamSynchronize(m->gpu->stream));
     }
+    m->has_logits = true;
     return m->collect_stats();
 }
 
@@ -2174,9 +2175,9 @@ int styx_moe_decode(styx_moe *m, int n_steps, uint32_t *out)
             if (int r = m->collect_stats()) return r;
         }
         again = false;
+        m->has_logits = false;
         if (int r = m->run_token(true)) return r;
         m->n_past++;
-        m->has_logits = true;
         if (host_work && !m->opts.no_fuse) {
             STYX_HIP(hipStreamSynchronize(m->gpu->stream));
             if (m->check_abort()) {
@@ -2203,6 +2204,7 @@ int styx_moe_decode(styx_moe *m, int n_steps, uint32_t *out)
         STYX_HIP(hipMemcpyAsync(m->d_tok, m->tok_save, 4, hipMemcpyDeviceToDevice, m->gpu->stream));
         return styx_moe_decode(m, n_steps, out);
     }
+    if (n_steps > 0) m->has_logits = true;
     return m->collect_stats();
 }
 
@@ -2291,7 +2293,7 @@ int styx_moe_generate_sampled(styx_moe *m, const uint32_t *prompt, int n_prompt,
 // back to back between two HIP events.  Each layer's launch reads its own
 // weights, so the replays stream as much memory as a token does for that
 // stage.  The replays overwrite per-token scratch (ids rows, partials, the
-// residual and the KV row at the pending position), all of which the next
+// residual, the logits and the KV row at the pending position), all of which the next
 // token rewrites before reading; argmax, which advances the decode state, is
 // not a stage here.
 int styx_moe_time_stage(styx_moe *m, const char *stage, int reps, double *us_per_replay,
@@ -2308,6 +2310,7 @@ int styx_moe_time_stage(styx_moe *m, const char *stage, int reps, double *us_per
     if (m->n_past < 1) return fail(STYX_E_STATE, "styx_moe_time_stage: run a token first");
     STYX_HIP(hipSetDevice(m->gpu->device));
     if (int r = m->collect_stats()) return r;
+    m->has_logits = false;
     hipStream_t st = m->gpu->stream;
     const int saved = m->opts.time_kernels;
     m->opts.time_kernels = 0;

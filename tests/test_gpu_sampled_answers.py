@@ -219,3 +219,20 @@ def test_sampling_refusals(gpu):
     assert gpu.lib.styx_moe_sample(m.h, None, 0.5, None, None) == -1
     assert gpu.lib.styx_moe_sample(None, C.byref(p), 0.5, None, None) == -1
     m.close()
+
+
+def test_sampling_after_stage_timing_is_refused(gpu):
+    """Its replays of the head overwrite the logits with those of another
+    state; the next token brings them back."""
+    from styx_amd import StyxError
+    m = model(gpu)
+    m.generate(PROMPT, 1)
+    m.forward_token(5)
+    m.time_stage("lm_head", 1)
+    with pytest.raises(StyxError, match="no token forwarded"):
+        m.sample(0.5)
+    lg = m.forward_token(6)
+    assert m.sample(0.5, temperature=0.0)[0] == int(np.argmax(lg))
+    m.decode(2)
+    m.sample(0.5)
+    m.close()
