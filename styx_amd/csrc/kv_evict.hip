@@ -363,7 +363,9 @@ template <int STAGE, int KPT> __global__ void __launch_bounds__(EV_WG) k_evict_p
 // The moves of a list: weight and position by one lane, the rows of K and V
 // by ROW16 lanes, MV_DEEP moves in flight for each; workgroups past
 // move_tiles per head: weights and positions of the rows that lie still,
-// where these go to other buffers.
+// where these go to other buffers.  (Rows stored with non-temporal stores: 22
+// us instead of 25 where the call runs alone, but 57 instead of 49 behind an
+// attention call that has read the rows, as in use.)
 template <int ROW16>  // 16-byte pieces of a row
 __global__ void __launch_bounds__(MV_WG) k_evict_move(KvEvictArgs a)
 {
@@ -455,8 +457,10 @@ static void evict_tiles(KvEvictArgs &a)
     const KvView &kv = a.kv;
     const int heads = kv.n_seq * kv.nkv, most = std::min(a.keep, kv.cap - a.keep);
     const int step = MV_WG / (kv.hd * (kv.f16 ? 2 : 4) / 16) * MV_DEEP;
-    // sixteen workgroups per CU, or one for every step of the longest list
-    a.move_tiles = std::max(1, std::min((most + step - 1) / step, 4096 / heads));
+    // 32 workgroups per CU, of which 8 run at once, or one for every step of
+    // the longest list: 25 us for 32 conversations and 88 for two of 64K rows,
+    // where 16 take 26 and 90.5 and more gain nothing
+    a.move_tiles = std::max(1, std::min((most + step - 1) / step, 8192 / heads));
     // rows that lie still are copied only into other buffers
     const bool apart = a.acc_out != a.acc_in || a.pos_out != a.pos_in;
     a.copy_tiles = apart ? (std::min(a.trigger, kv.cap) + CP_SLOTS - 1) / CP_SLOTS : 0;
