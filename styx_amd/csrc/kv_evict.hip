@@ -18,7 +18,7 @@
 // holes and movers, and which slots stay; a moving launch does the rest.
 //
 // Measured: one conversation of 1088 rows cut to 1024, 4 kv heads, 6.9 + 4 us;
-// 32 of up to 9001 f16 rows cut to 4096, 14.5 + 24.5 us, of which the moves
+// 32 of up to 9001 f16 rows cut to 4096, 14.5 + 25 us, of which the moves
 // run at 3.8 TB/s; two of 65536 f32 rows, 8 kv heads, cut to 16384, 41 us in
 // four launches, then 88 us of moves (4.6 TB/s, a large copy's rate).
 #include <algorithm>
@@ -458,8 +458,8 @@ static void evict_tiles(KvEvictArgs &a)
     const int heads = kv.n_seq * kv.nkv, most = std::min(a.keep, kv.cap - a.keep);
     const int step = MV_WG / (kv.hd * (kv.f16 ? 2 : 4) / 16) * MV_DEEP;
     // 32 workgroups per CU, of which 8 run at once, or one for every step of
-    // the longest list: 25 us for 32 conversations and 88 for two of 64K rows,
-    // where 16 take 26 and 90.5 and more gain nothing
+    // the longest list: 39.2 us in all for 32 conversations, where 16 take
+    // 39.9; two of 64K rows take the same with either, and more gain nothing
     a.move_tiles = std::max(1, std::min((most + step - 1) / step, 8192 / heads));
     // rows that lie still are copied only into other buffers
     const bool apart = a.acc_out != a.acc_in || a.pos_out != a.pos_in;
