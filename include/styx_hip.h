@@ -332,11 +332,13 @@ typedef struct styx_kv_cache {
  * q [n_seq][nh*hd], k and v [n_seq][nkv*hd] f32 raw projections, q_norm and
  * k_norm [hd] or NULL, out [n_seq][nh*hd]; nh / nkv from 1 to 16.  k is
  * normalised and turned in f64 and rounded to f32, and k and v to f16 for an
- * f16 cache; scores, sums and outputs are f32 (a V value that is not finite
- * makes its dimension of the outputs infinite, or, in an f16 cache, infinite
- * or NaN; a K value that is not finite makes those of its heads NaN, or its
- * row one without weight where the score is -infinity).  No row seen: out is
- * 0.
+ * f16 cache; scores, sums and outputs are f32.  A score that is NaN or +infinity
+ * (of a K or q value that is not finite) makes all outputs and weights of its
+ * head NaN; one of -infinity makes its row one without weight (in an f16
+ * cache, whose products take q in two pieces, such a score may be NaN).  A V
+ * value that is not finite makes its dimension of the outputs infinite or NaN
+ * (infinite in an f32 cache, if it is the only one there, infinite itself, and
+ * its row's weight is above 2^-126).  Else, with no row of any weight: 0.
  * acc_in / acc_out [n_seq][nkv][cap] f32: for the rows t <= len[b]
  *   acc_out[t] = decay * acc_in[t] + sum over the kv head's query heads of
  *                the softmax weight of row t

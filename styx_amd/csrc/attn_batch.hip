@@ -59,6 +59,13 @@ constexpr int AB_BATCH = 8;
 // v_exp_f32 is then the exponential, good to a unit in the last place.
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// What a part (M, L, o) of a softmax is multiplied by where the maximum of all
+// parts is `all`.  No part is left out of a sum for a factor of 0, or for a
+// maximum of -infinity: that is where nothing was seen (L and o are 0), but
+// also where every score was NaN (a maximum takes no NaN; L is one then), and
+// a value that is not finite has to be so in the sum.
+__device__ __forceinline__ float part_factor(float m, float all) { return m == -INFINITY ? 0.0f : exp2_(m - all); }
+
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 // Rows that the new token of sequence b sees, itself among them; 0: skipped.
@@ -687,9 +694,9 @@ __global__ void __launch_bounds__(AB_WG, ab_slots(HD) / 256) k_attn_batch(AttnBa
             float L = 0.0f, O = 0.0f;
 #pragma unroll
             for (int w = 0; w < AB_WAVES; w++) {
-                const float f = s_m[w][h] == -INFINITY ? 0.0f : exp2_(s_m[w][h] - M);
+                const float f = part_factor(s_m[w][h], M);
                 L += s_l[w][h] * f;
-                O += f == 0.0f ? 0.0f : s_o[w][h][d] * f;
+                O += s_o[w][h][d] * f;
             }
             a.part_o[(pc + h) * HD + d0 + d] = O;
             if (d0 == 0 && d == 0) {
@@ -736,17 +743,18 @@ __device__ __forceinline__ void merge_pieces(const AttnBatchArgs &a, const Piece
         float mn = m;
 #pragma unroll
         for (int i = 0; i < AB_BATCH; i++) {
-            if (c + STEP * i >= at.count) ml[i].x = -INFINITY;
+            if (c + STEP * i >= at.count) {
+                ml[i] = float2{-INFINITY, 0.0f};
+                oc[i] = 0.0f;
+            }
             mn = fmaxf(mn, ml[i].x);
         }
-        if (mn == -INFINITY) continue;  // nothing seen in these
-        const float fa = exp2_(m - mn);
+        const float fa = part_factor(m, mn);
         l *= fa;
         o *= fa;
 #pragma unroll
         for (int i = 0; i < AB_BATCH; i++) {
-            if (ml[i].x == -INFINITY) continue;
-            const float f = exp2_(ml[i].x - mn);
+            const float f = part_factor(ml[i].x, mn);
             l += ml[i].y * f;
             if (O) o += oc[i] * f;
         }
@@ -787,12 +795,12 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch_join(AttnBatchArgs a)
             for (int w = 0; w < PARTS; w++) M = fmaxf(M, s_m[w]);
 #pragma unroll
             for (int w = 0; w < PARTS; w++) {
-                const float f = s_m[w] == -INFINITY ? 0.0f : exp2_(s_m[w] - M);
+                const float f = part_factor(s_m[w], M);
                 L += s_l[w] * f;
                 O += s_o[w][tid] * f;
             }
-            // no row seen (M = -inf): 0
-            a.out[((int64_t)b * a.nh + h) * kv.hd + d0 + tid] = M == -INFINITY ? 0.0f : O / L;
+            // no row with a weight (M = -inf): 0, or NaN
+            a.out[((int64_t)b * a.nh + h) * kv.hd + d0 + tid] = M == -INFINITY ? O + L : O / L;
         }
         return;
     }
@@ -822,10 +830,10 @@ __global__ void __launch_bounds__(AB_WG) k_attn_batch_join(AttnBatchArgs a)
         float m = -INFINITY, l = 0.0f, o;
         if (h < a.gqa) merge_pieces<16, false>(a, pieces_of(a, sp, at, kvh), tid & 15, h, 0, m, l, o);
         const float M = bfly<16>(m, [](float x, float y) { return fmaxf(x, y); });
-        const float L = bfly_sum<16>(m == -INFINITY ? 0.0f : l * exp2_(m - M));
+        const float L = bfly_sum<16>(l * part_factor(m, M));
         if ((tid & 15) == 0) {
             s_M[h] = M == -INFINITY ? 0.0f : M;
-            s_R[h] = M == -INFINITY ? 0.0f : 1.0f / L;
+            s_R[h] = M == -INFINITY ? L : 1.0f / L;
         }
     }
     __syncthreads();
