@@ -126,11 +126,16 @@ __device__ __forceinline__ RowSplit split_rows(const AttnBatchArgs &a)
     if (heads < slots) {
         // at most all / share and one for every head
         const uint32_t most = (all + slots - heads - 1) / (slots - heads);
+        const uint32_t worth = least + (a.kv.f16 ? AB_MORE_F16 : AB_MORE_F32);
         uint32_t at = most;
+        // (looked for only as far as it is worth taking: with nearly as many
+        // heads as slots `most` is hundreds of steps away, each a division and
+        // a sum over the wave; 59 sequences of 13 heads, one of 64K rows and
+        // the others of one, took 328 us so, and 95 now)
         if (a.kv.n_seq <= 64)
-            for (at = sp.share; at < most && wave_total((u + at - 1) / at) * nkv > slots; at++)
+            for (at = sp.share; at < most && at <= worth && wave_total((u + at - 1) / at) * nkv > slots; at++)
                 ;
-        if (at <= least + (a.kv.f16 ? AB_MORE_F16 : AB_MORE_F32)) {
+        if (at <= worth) {
             sp.padded = 1;
             sp.share = at;
         }
