@@ -127,7 +127,7 @@ __device__ __forceinline__ RowSplit split_rows(const AttnBatchArgs &a)
         // at most all / share and one for every head
         const uint32_t most = (all + slots - heads - 1) / (slots - heads);
         const uint32_t worth = least + (a.kv.f16 ? AB_MORE_F16 : AB_MORE_F32);
-        uint32_t at = most;
+        uint32_t at = max(most, 1u);  // (1: no rows at all)
         // (looked for only as far as it is worth taking: with nearly as many
         // heads as slots `most` is hundreds of steps away, each a division and
         // a sum over the wave; 59 sequences of 13 heads, one of 64K rows and
