@@ -60,6 +60,7 @@ struct AttnBatchArgs {
     uint32_t *plan;
     int stride;  // slots of a score row (a multiple of 64)
     int n_merge, tiles;  // the joining launch's workgroups (filled by the launch)
+    uint32_t once_units; // units of rows that the Infinity Cache holds (filled by the launch)
 };
 
 // Sizes of the workspace's pieces in floats for a cache of this shape.

@@ -518,11 +518,12 @@ template <int HD, bool WIDE, bool ONCE> struct Tile<_Float16, HD, WIDE, ONCE> {
     }
 };
 
-template <typename T, int HD, bool WIDE, bool SCORED, bool ONCE>
+// LARGE: pools larger than the Infinity Cache (launch_ab).
+template <typename T, int HD, bool WIDE, bool SCORED, bool LARGE>
 __global__ void __launch_bounds__(AB_WG, ab_slots(HD) / 256) k_attn_batch(AttnBatchArgs a)
 {
-    using Tl = Tile<T, HD, WIDE, ONCE>;
-    constexpr int KEYS = Tl::KEYS, NS = Tl::NS, QROWS = Tl::QROWS, NR = KEYS / 16;
+    using Any = Tile<T, HD, WIDE, false>;
+    constexpr int KEYS = Any::KEYS, NS = Any::NS, QROWS = Any::QROWS, NR = KEYS / 16;
     __shared__ __align__(16) float s_q[QROWS][HD + 4];
     __shared__ float s_qmax[QROWS];
     __shared__ __align__(16) T s_k[HD], s_v[HD];
@@ -534,6 +535,8 @@ __global__ void __launch_bounds__(AB_WG, ab_slots(HD) / 256) k_attn_batch(AttnBa
     const RowSplit sp = split_rows(a);
     if (blockIdx.x == 0 && wave == 0) split_store(a, sp);
     const uint32_t end = min(sp.units, (blockIdx.x + 1) * sp.share);
+    auto pieces = [&](auto once) __attribute__((always_inline)) {
+    using Tl = Tile<T, HD, WIDE, decltype(once)::value>;
     for (uint32_t u = blockIdx.x * sp.share; u < end;) {
     // (a lane number that the compiler takes for a new one in every trip:
     // what is computed from it would else be kept in registers over the
@@ -711,6 +714,14 @@ __global__ void __launch_bounds__(AB_WG, ab_slots(HD) / 256) k_attn_batch(AttnBa
         }
     }
     }
+    };
+    if constexpr (LARGE) {
+        if (__builtin_amdgcn_readfirstlane(sp.units) > a.once_units) {
+            pieces(std::true_type{});
+            return;
+        }
+    }
+    pieces(std::false_type{});
 }
 
 // The pieces of one kv head: their partials lie one after another (piece i of
@@ -889,22 +900,29 @@ AttnBatchWs attn_batch_ws(int n_seq, int nkv, int hd, int cap, int gqa, bool sco
 }
 
 template <typename T, int HD, bool WIDE>
-static void launch_ab(hipStream_t st, const AttnBatchArgs &a, int64_t grid)
+static void launch_ab(hipStream_t st, AttnBatchArgs a, int64_t grid)
 {
     const dim3 g((unsigned)grid), wg(AB_WG);
-    // Pools larger than the Infinity Cache: their rows come from HBM, and
-    // loads that leave nothing behind stream them 5-9% faster (40 f16
-    // sequences of 8 heads, 327 MB: 83 -> 76 us); smaller ones may be found
-    // there (24 conversations, 102 MB: 27 us against 32 with such loads).
+    // Rows past the Infinity Cache come from HBM, and loads that leave nothing
+    // behind stream them 5-9% faster (40 f16 sequences of 8 heads, 327 MB: 83
+    // -> 76 us); fewer may be found there by the next call, which such loads
+    // would spoil (24 conversations, 102 MB, call after call: 32 us against
+    // 38).  What counts are the rows that the call reads, which the device
+    // knows (those of shared pages count for each sequence), and no more than
+    // there are: a kernel that looks carries both loops, of which a call of few
+    // rows notices the length (eight conversations: 21.0 us without, 21.7
+    // with), and is taken only where the pools are larger.
     const KvView &kv = a.kv;
-    const bool once = 2.0 * sizeof(T) * kv.n_pages * kv.page_tokens * kv.nkv * kv.hd > 256.0 * (1 << 20);
+    constexpr double ROW = 2.0 * sizeof(T) * HD, CACHE = 256.0 * (1 << 20);
+    const bool large = ROW * kv.nkv * kv.n_pages * kv.page_tokens > CACHE;
+    a.once_units = (uint32_t)(CACHE / (ROW * AB_UNIT));
     if (a.acc_out) {
-        if (once)
+        if (large)
             hipLaunchKernelGGL((k_attn_batch<T, HD, WIDE, true, true>), g, wg, 0, st, a);
         else
             hipLaunchKernelGGL((k_attn_batch<T, HD, WIDE, true, false>), g, wg, 0, st, a);
     } else {
-        if (once)
+        if (large)
             hipLaunchKernelGGL((k_attn_batch<T, HD, WIDE, false, true>), g, wg, 0, st, a);
         else
             hipLaunchKernelGGL((k_attn_batch<T, HD, WIDE, false, false>), g, wg, 0, st, a);

@@ -1,4 +1,5 @@
-"""What the choice of a batch's split costs styx_op_attn_decode_batch."""
+"""What styx_op_attn_decode_batch's choices cost: of a batch's split, and of how
+its rows are read."""
 from __future__ import annotations
 
 import ctypes as C
@@ -20,16 +21,17 @@ def gpu():
     g.close()
 
 
-def time_call(gpu, lens, nkv, hd, f16, n_seq):
-    """Microseconds of a call among others, the best of five runs: the
-    sequences of `lens` and, up to n_seq, ones that are skipped."""
+def time_call(gpu, lens, nkv, hd, f16, n_seq, spare=0):
+    """Microseconds of a call among others, the best of six runs: the
+    sequences of `lens` and, up to n_seq, ones that are skipped; pages that no
+    sequence has behind each of theirs."""
     page, es = 512, 2 if f16 else 4
     used = [-(-(n + 1) // page) for n in lens]
-    n_pages, table_len = sum(used), max(used)
+    n_pages, table_len = sum(used) * (1 + spare), max(used)
     table = np.full((n_seq, table_len), -1, np.int32)
     at = 0
     for b, m in enumerate(used):
-        table[b, :m] = np.arange(at, at + m)
+        table[b, :m] = np.arange(at, at + m) * (1 + spare)
         at += m
     ln = np.full(n_seq, -1, np.int32)
     ln[:len(lens)] = lens
@@ -68,3 +70,13 @@ def test_a_split_that_is_not_taken_is_not_searched_for(gpu, longs, n_long, short
     alone, beside = (time_call(gpu, lens, nkv, hd, f16, n) for n in (n_seq, 65))
     print(f"{alone:.1f} us, {beside:.1f} us with skipped sequences")
     assert alone <= 1.3 * beside + 10.0
+
+
+@pytest.mark.parametrize("times", [5, 8])
+def test_rows_that_the_caches_hold_are_read_from_them_in_a_pool_of_any_size(gpu, times):
+    """Calls in turn on the same rows, which the Infinity Cache holds: as fast
+    in a pool several times its size as in one of their own."""
+    lens = [4096, 700, 2000, 3500] * times
+    own, large = (time_call(gpu, lens, 4, 128, True, len(lens), spare) for spare in (0, 4))
+    print(f"{own:.1f} us, {large:.1f} us in a large pool")
+    assert large <= 1.08 * own
