@@ -328,7 +328,8 @@ typedef struct styx_kv_cache {
  * pos[b] (its rope angle, rope [n_rope][hd/2][2] from styx_rope_table) and
  * its row goes to slot len[b].  A sequence with len[b] outside [0, cap) or
  * pos[b] outside [0, n_rope) is skipped: nothing of it is read or written
- * (padding).  The lengths are the caller's to advance.
+ * (padding, and a full one).  The lengths are the caller's to advance, for the
+ * sequences that were not skipped.
  * q [n_seq][nh*hd], k and v [n_seq][nkv*hd] f32 raw projections, q_norm and
  * k_norm [hd] or NULL, out [n_seq][nh*hd]; nh / nkv from 1 to 16.  k is
  * normalised and turned in f64 and rounded to f32, and k and v to f16 for an

@@ -218,7 +218,8 @@ class KvBatch:
     operators keep beside it: page table, lengths and positions, and with
     `scored` every row's accumulated attention weight and position.  attend()
     and evict() run on the gpu's stream; lengths and positions stay on the
-    device and are the caller's to advance (set)."""
+    device and are the caller's to advance (set): of the sequences that attend()
+    took, those with a length in [0, cap) and a position in the rope table."""
 
     def __init__(self, gpu: Gpu, n_seq: int, nkv: int, hd: int, page_tokens: int, n_pages: int,
                  table_len: int, type_: int = L.F32, scored: bool = True):
