@@ -28,7 +28,7 @@
 // in the first launch and 1 to 4 us slower in the second.)
 //
 // Measured, both launches: one context of 32767 f32 rows, 16 query heads for
-// each of 4 kv heads, 34 + 7 us (135 MB, 3.3 TB/s); six of up to 20011 f32
+// each of 4 kv heads, 34 + 6 us (135 MB, 3.4 TB/s); six of up to 20011 f32
 // rows, head_dim 256, without weights 62 + 5 us (302 MB, 4.5 TB/s); 24
 // conversations of up to 4096 f16 rows 29 + 6.5 us (102 MB, 2.9 TB/s); 40 of
 // up to 8192, head_dim 64, 76 + 8 us (327 MB, 3.9 TB/s); one of 37 rows 8 +
@@ -84,7 +84,7 @@ __device__ __forceinline__ int rows_of(const AttnBatchArgs &a, int b)
 // 10 instead of 9: 62 against 68).  It does not pay where the heads are too
 // many for the workgroups (40 sequences of 8 heads, 45 units instead of 27:
 // 105 us against 81).  AB_MORE: units of a share that cost about as much as
-// a second start.
+// a second start, from these three batches (no others were measured).
 // `mine`, `upto`: rows of sequence `lane` and units of the sequences up to it.
 constexpr int AB_MORE_F16 = 3, AB_MORE_F32 = 1;
 struct RowSplit {

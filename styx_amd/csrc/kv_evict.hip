@@ -19,7 +19,8 @@
 //
 // Measured: one conversation of 1088 rows cut to 1024, 4 kv heads, 6.9 + 4 us;
 // 32 of up to 9001 f16 rows cut to 4096, 14.5 + 25 us, of which the moves
-// run at 3.8 TB/s; two of 65536 f32 rows, 8 kv heads, cut to 16384, 41 us in
+// run at 3.8 TB/s where the call runs alone (behind an attention call that has
+// read such a batch's rows, as in use, the moves take 47); two of 65536 f32 rows, 8 kv heads, cut to 16384, 41 us in
 // four launches, then 88 us of moves (4.6 TB/s, a large copy's rate).
 #include <algorithm>
 #include <type_traits>
@@ -364,8 +365,9 @@ template <int STAGE, int KPT> __global__ void __launch_bounds__(EV_WG) k_evict_p
 // by ROW16 lanes, MV_DEEP moves in flight for each; workgroups past
 // move_tiles per head: weights and positions of the rows that lie still,
 // where these go to other buffers.  (Rows stored with non-temporal stores: 22
-// us instead of 25 where the call runs alone, but 57 instead of 49 behind an
-// attention call that has read the rows, as in use.)
+// us instead of 25 where the call runs alone, but 57 behind an attention call
+// that has read the rows, as in use, where plain stores took 49 and, since
+// there are 32 workgroups per CU, take 47.)
 template <int ROW16>  // 16-byte pieces of a row
 __global__ void __launch_bounds__(MV_WG) k_evict_move(KvEvictArgs a)
 {

@@ -19,16 +19,22 @@
 //     stays is summed per block
 //   4 one workgroup per row: the border words in their order, which of them
 //     stay, and the token in its block
-// Bound: latency for a few rows (each launch waits for all of the one
-// before); for many, the f64 exponentials of launches 2 and 3 and one read of
-// the logits from HBM (the other two hit the Infinity Cache).
+// Bound: latency, for a few rows (each launch waits for all of the one before)
+// and in each workgroup of many.
 //
 // Measured: one row of 151936 words with top-k and top-p 2.6 + 5.2 + 6.2 + 8.7
 // us, of 4096 with a temperature alone 13 us in all; 64 rows of 151936 with
 // settings of their own 8 + 19 + 23 + 16 us (logits read three times, 1.8
-// TB/s; the launches 2 and 3 run 4 and 6 million VALU instructions, most for
-// the rows that neither top-k nor top-p cuts); 17 flat rows of 50257, a
-// nucleus of most words, 30 us.  (A wave per block of 512 words without
+// TB/s); 17 flat rows of 50257, a nucleus of most words, 30 us.  Of the 64
+// rows, those that are greedy or that nothing cuts take no part in launch 2,
+// and those with a top-p but no small top-k are weighed in both 2 and 3.
+// Neither launch is bound by its VALU work: it takes 35 and 43% of the cycles
+// (4 and 6 million instructions), and half of the waves' time is waiting.
+// Launch 2's bins (48.5 KB of LDS) let three workgroups run on a CU where
+// sample_ws plans about four, so they come in uneven rounds, 6.6 waves per CU
+// on average (launch 3: 8.5), and every workgroup forms its row's settings
+// from the blocks' first words, in launch 3 also the border from the bins,
+// before it asks for its words.  (A wave per block of 512 words without
 // barriers, the border found by a launch of its own, and words weighed four
 // side by side were tried: each no faster over these.)
 #include "../../include/styx_hip.h"

@@ -1,4 +1,4 @@
-"""The step of a batch's loop that INTEGRATION.md shows, run on the CPU against
+"""The step of a batch's loop that the integration guide shows, run on the CPU against
 the operators' rules for lengths.  No GPU needed."""
 from __future__ import annotations
 
