@@ -672,8 +672,9 @@ __global__ void __launch_bounds__(FI_WG) k_sample_finish(SampleArgs a)
             run += v[j];
         }
         const u64 incl = wave_upto(run), total = of_lane(incl, 63);
+        // (the largest total is 2^63 - 2^44: what is below it can be converted)
         const double f = (double)a.u[r] * (double)total;
-        u64 t = f > 0.0 ? (u64)fmin(f, 9.2e18) : 0;
+        u64 t = f > 0.0 ? f < (double)total ? (u64)f : total - 1 : 0;
         if (t >= total) t = total - 1;
         u64 at = incl - run;
 #pragma unroll
