@@ -380,10 +380,136 @@ int styx_op_kv_evict(styx_gpu *gpu, const styx_kv_cache *kv, const int32_t *len,
                      const float *acc_in, float *acc_out, const int32_t *slot_pos_in,
                      int32_t *slot_pos_out, int32_t *len_out, void *ws, uint64_t ws_bytes);
 uint64_t styx_op_kv_evict_ws_bytes(const styx_kv_cache *kv, int keep);
+/* New tokens of a batch -- prompts, parts of prompts and single tokens
+ * together -- into the same cache (no counterpart in the reference, which
+ * feeds one sequence token by token).  A step: styx_op_kv_plan gives the
+ * sequences their pages and says where the step's rows belong,
+ * styx_op_kv_append writes K and V and turns q, styx_op_attn_chunk attends,
+ * styx_op_kv_weigh adds the last tokens' attention weights to what
+ * styx_op_kv_evict goes by.  Token i of sequence b, i < count[b], is row
+ * first[b] + i of q, k, v and out, and slot len[b] + i of its sequence.  All of
+ * it is read on the device.  A sequence without new tokens (count[b] <= 0),
+ * with len[b] < 0, slots past cap or rows outside [0, n_rows) is skipped:
+ * nothing of it is read or written; rows of no sequence stay as they are.
+ * Rows of two sequences may not overlap. */
+typedef struct styx_kv_chunk {
+    int n_rows;                          /* rows of q, k, v and out */
+    const int32_t *first, *count, *len;  /* [n_seq] */
+} styx_kv_chunk;
+/* Who has which page.  free_pages is a stack: its n_free[0] first entries, the
+ * last one on top. */
+typedef struct styx_kv_pages {
+    int32_t *page_table; /* [n_seq][table_len] */
+    int32_t *held;       /* [n_seq] entries of it that are the sequence's */
+    int32_t *free_pages; /* [n_pages] */
+    int32_t *n_free;     /* [1] */
+} styx_kv_pages;
+/* Page tables and row maps of a step.  Sequence b has len[b] rows (-1: it has
+ * ended, or waits) and asks for n_new[b] more (a negative number is 0) from
+ * position pos[b] on.  first[b] is the sum of n_new before b.  In this order:
+ *   pages past those that the rows fill, new ones included, and past the
+ *   first shared[b] (pages of another's; NULL: none) go to the stack, sequence
+ *   by sequence, in the order of the table; their entries become -1.  Entries
+ *   outside the pool are dropped.
+ *   the pages that are missing come from the top of the stack, sequence by
+ *   sequence; stack entries taken become -1.  The first sequence for which there
+ *   are not enough, and every later one that asks for any, gets none.
+ * count[b] = n_new[b] where the sequence got its pages, its slots are below
+ * cap and its rows below n_rows, else 0 (it keeps what its len[b] rows fill,
+ * all it holds if len[b] > cap).  held counts the entries; held and n_free are
+ * taken as their nearest possible value.  row_seq, row_pos and row_at
+ * [n_rows], each or NULL: sequence, position and row of the pools (page *
+ * page_tokens + row of the page; -1 for an entry outside the pool) of every
+ * row, -1 for rows of no sequence and of those with count 0.  kv gives n_seq,
+ * page_tokens, n_pages and table_len, its pointers are not read.  out's four
+ * arrays are in's (in place), or others that overlap none of them; entries
+ * past those named stay as they are.  Advance len by count for the next step. */
+int styx_op_kv_plan(styx_gpu *gpu, const styx_kv_cache *kv, const styx_kv_pages *in,
+                    const styx_kv_pages *out, const int32_t *shared, const int32_t *len,
+                    const int32_t *n_new, const int32_t *pos, int n_rows, int32_t *first,
+                    int32_t *count, int32_t *row_seq, int32_t *row_pos, int32_t *row_at);
+/* Rotary positions: dims below n_rot (even) of a head in pairs, (i, i +
+ * n_rot/2), or (2i, 2i+1) where interleaved; table [n_pos][n_rot/2][2] = (cos,
+ * sin) from styx_rope_table_scaled, 16-byte aligned. */
+typedef struct styx_rope {
+    const double *table;
+    int n_pos, n_rot, interleaved;
+} styx_rope;
+/* Per-head RMSNorm and rotation of q and k, and k and v into the cache.  q
+ * [n_rows][nh*hd] and k, v [n_rows][nkv*hd] of type_in (STYX_F32 or
+ * STYX_F16), rows ldq, ldk and ldv values apart (one product's output may
+ * hold all three); q_norm, k_norm [hd] or NULL; rope NULL: no rotation.
+ * q_out [n_rows][nh*hd] of type_q, rows ldo apart; it may be q itself.  k and
+ * v NULL: q alone; q and q_out NULL: k and v alone.  A row whose row_pos is
+ * outside the rope table is skipped; one whose row_at is outside the pools
+ * has its q turned and no K and V.  Normalised and turned in f64, rounded to
+ * f32 and from there to the type.  Two rows may not have one row_at.  Rows must
+ * be 16-byte aligned.  The cache's page table is not read.  Allocates nothing. */
+int styx_op_kv_append(styx_gpu *gpu, const styx_kv_cache *kv, int n_rows, const int32_t *row_pos,
+                      const int32_t *row_at, int nh, int type_in, const void *q, int64_t ldq,
+                      const void *k, int64_t ldk, const void *v, int64_t ldv, const float *q_norm,
+                      const float *k_norm, float eps, const styx_rope *rope, int type_q,
+                      void *q_out, int64_t ldo);
+/* Causal attention of the new tokens over their sequence's slots: token i sees
+ * slots t <= len[b] + i, with window > 0 those of t > len[b] + i - window
+ * alone, as far as their pages are in the pool.  q (turned) and out
+ * [n_rows][nh*hd] of type_q: STYX_F32, or STYX_F16 for an f16 cache; rows ldq
+ * and ldo values apart, 16-byte aligned; nh / nkv from 1 to 16.
+ *   s_t = scale q . K[t], out = sum e^(s_t - M) V[t] / sum e^(s_t - M)
+ * lse [n_rows][nh] f32 or NULL: ln of the sum of e^s_t.  A token that sees
+ * nothing: out 0, lse -infinity.  Scores, sums and lse are f32; with f16 q the
+ * factors are rounded to f16 on their way to V, with f32 q they are not.  A
+ * score that is NaN or +infinity makes the outputs of its token and head NaN
+ * (with f32 q on an f16 cache one of -infinity, too); a V value that is not
+ * finite makes its dimension infinite or NaN where the token sees the row.
+ * What a token does not see, slots behind the last row and rows of missing
+ * pages among it, has no influence, whatever it holds.  out may not overlap
+ * q.  ws: styx_op_attn_chunk_ws_bytes() bytes, 16-byte aligned, which no other
+ * call uses meanwhile (its contents need not be kept).  Allocates nothing. */
+int styx_op_attn_chunk(styx_gpu *gpu, const styx_kv_cache *kv, const styx_kv_chunk *chunk, int nh,
+                       int type_q, const void *q, int64_t ldq, float scale, int window, void *out,
+                       int64_t ldo, float *lse, void *ws, uint64_t ws_bytes);
+/* 0: a shape that the call refuses. */
+uint64_t styx_op_attn_chunk_ws_bytes(const styx_kv_cache *kv, int n_rows, int nh);
+/* The attention weights of the last tokens of each sequence's chunk, by the
+ * same q, scale and window and the lse that styx_op_attn_chunk gave:
+ *   acc_out[t] = decay * acc_in[t] + sum over the last min(last, count[b])
+ *                tokens that see slot t and the kv head's query heads of
+ *                e^(s_t - lse)
+ * for t < len[b] + count[b], with 0 in place of acc_in for the new rows (acc
+ * [n_seq][nkv][cap], acc_in NULL: zeros; it may be acc_out); slots past them
+ * stay as they are.  A token with lse -infinity adds nothing, one with a NaN
+ * makes what it sees NaN.  slot_pos [n_seq][nkv][cap] or NULL: the new slots
+ * get pos[b] + i.  With one token per sequence and last 1 this is what
+ * styx_op_attn_decode_batch adds.  Allocates nothing. */
+int styx_op_kv_weigh(styx_gpu *gpu, const styx_kv_cache *kv, const styx_kv_chunk *chunk,
+                     const int32_t *pos, int nh, int type_q, const void *q, int64_t ldq,
+                     float scale, int window, const float *lse, int last, float decay,
+                     const float *acc_in, float *acc_out, int32_t *slot_pos);
 /* Host-side NEOX rope table: out[p][i] = (cos, sin)(p * base^(-2i/hd)) in
  * f64 for p < n_pos, i < hd/2 (crates/vk-backend/tests/ops2.rs:426-442).
  * out holds n_pos * hd doubles.  Needs no GPU. */
 void styx_rope_table(float base, int hd, int n_pos, double *out);
+/* The same for the first n_rot dims of a head, scaled for contexts longer than
+ * a model was trained on.  With f_i = base^(-2i/n_rot):
+ *   PLAIN   f_i (and styx_rope_table's values, with gain 0 or 1)
+ *   LINEAR  f_i / factor
+ *   BASE    base * factor^(n_rot/(n_rot-2)) in place of base
+ *   PARTS   pairs that make more than `fast` turns in n_orig positions keep
+ *           f_i, those of fewer than `slow` get f_i / factor, between the pairs'
+ *           whole-numbered indices a ramp; the table is times gain
+ *   BANDS   the same with a ramp in the number of turns itself
+ * fast, slow 0: 32 and 1 (PARTS), 4 and 1 (BANDS).  gain multiplies the table;
+ * 0: 0.1 ln factor + 1 for PARTS with factor > 1, else 1.  s NULL: PLAIN.  out
+ * holds n_pos * n_rot doubles.  Needs no GPU. */
+enum { STYX_ROPE_PLAIN = 0, STYX_ROPE_LINEAR, STYX_ROPE_BASE, STYX_ROPE_PARTS, STYX_ROPE_BANDS };
+typedef struct styx_rope_scaling {
+    int kind;
+    float factor;
+    int n_orig;
+    float fast, slow, gain;
+} styx_rope_scaling;
+int styx_rope_table_scaled(float base, int n_rot, int n_pos, const styx_rope_scaling *s, double *out);
 /* gather_slabs_f32 (shaders/gather_slabs_f32.comp:40-86): for slot s < k
  * with expert ids[s] != SKIP copy that expert's slab of each of the three
  * tensors into arena slot layer*k+s.  Slab sizes multiples of 16. */

@@ -14,6 +14,7 @@ LIB_PATH = Path(__file__).resolve().parent / "libstyx_hip.so"
 STYX_OK = 0
 F32, F16, Q8_0, Q4_K, Q5_K, Q6_K = 0, 1, 8, 12, 13, 14
 SKIP = 0xFFFFFFFF
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_PARTS, ROPE_BANDS = range(5)
 BUF_DEVICE, BUF_HOST_PINNED = 0, 1
 
 BLOCK = {F32: (1, 4), F16: (1, 2), Q8_0: (32, 34), Q4_K: (256, 144), Q5_K: (256, 176), Q6_K: (256, 210)}
@@ -84,6 +85,23 @@ class KvCache(C.Structure):
 class SampleParams(C.Structure):
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_int32), ("top_p", C.c_float),
                 ("min_p", C.c_float)]
+
+
+class KvChunk(C.Structure):
+    _fields_ = [("n_rows", C.c_int), ("first", C.c_void_p), ("count", C.c_void_p), ("len", C.c_void_p)]
+
+
+class KvPages(C.Structure):
+    _fields_ = [("page_table", C.c_void_p), ("held", C.c_void_p), ("free_pages", C.c_void_p), ("n_free", C.c_void_p)]
+
+
+class Rope(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("n_pos", C.c_int), ("n_rot", C.c_int), ("interleaved", C.c_int)]
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [("kind", C.c_int), ("factor", C.c_float), ("n_orig", C.c_int), ("fast", C.c_float),
+                ("slow", C.c_float), ("gain", C.c_float)]
 
 
 class KernelStat(C.Structure):
@@ -171,8 +189,15 @@ _SIGS = {
     "styx_op_attn_batch_ws_bytes": (u64, [vp, i32, i32]),
     "styx_op_kv_evict": (i32, [vp, vp, vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, u64]),
     "styx_op_kv_evict_ws_bytes": (u64, [vp, i32]),
+    "styx_op_kv_plan": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, vp, vp, vp, vp, vp]),
+    "styx_op_kv_append": (i32, [vp, vp, i32, vp, vp, i32, i32, vp, i64, vp, i64, vp, i64, vp, vp, C.c_float, vp,
+                                i32, vp, i64]),
+    "styx_op_attn_chunk": (i32, [vp, vp, vp, i32, i32, vp, i64, C.c_float, i32, vp, i64, vp, vp, u64]),
+    "styx_op_attn_chunk_ws_bytes": (u64, [vp, i32, i32]),
+    "styx_op_kv_weigh": (i32, [vp, vp, vp, vp, i32, i32, vp, i64, C.c_float, i32, vp, i32, C.c_float, vp, vp, vp]),
     "styx_op_sample": (i32, [vp, vp, i64, i32, i32, vp, i32, vp, vp, vp, vp, vp, u64]),
     "styx_op_sample_ws_bytes": (u64, [i32, i32]),
+    "styx_rope_table_scaled": (i32, [C.c_float, i32, i32, vp, vp]),
     "styx_rope_table": (None, [C.c_float, i32, i32, vp]),
     "styx_op_read_probe": (i32, [vp, vp, i64, vp, i32]),
     "styx_residency_plan": (i32, [C.c_char_p, i32, i32, vp, i64, vp, vp]),

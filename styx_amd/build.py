@@ -27,10 +27,15 @@ SOURCES = [
     "attn.hip",
     "attn_batch.hip",
     "kv_evict.hip",
+    "kv_plan.hip",
+    "kv_append.hip",
+    "attn_chunk.hip",
+    "kv_weigh.hip",
     "sample.hip",
     "moe_block.hip",
     "prompt.hip",
     "capi.cpp",
+    "capi_chunk.cpp",
     "dispatch.cpp",
     "dispatch_fused.cpp",
     "engine.cpp",

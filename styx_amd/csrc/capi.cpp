@@ -6,9 +6,8 @@
 #include <vector>
 #include <string>
 
-#include "attn_batch.h"
+#include "capi.h"
 #include "kernels.h"
-#include "runtime.h"
 #include "sample.h"
 
 namespace styx {
@@ -233,18 +232,6 @@ int styx_copy_region(styx_gpu *g, const styx_buf *src, uint64_t soff, styx_buf *
 }
 
 // ---------------------------------------------------------------- ops ----
-#define OP_GPU(g)                                                         \
-    do {                                                                  \
-        if (!(g)) return fail(STYX_E_INVALID, "NULL gpu");                \
-    } while (0)
-#define OP_RUN(expr, what)                                                \
-    do {                                                                  \
-        hipError_t _e = (expr);                                           \
-        if (_e == hipErrorInvalidValue)                                   \
-            return fail(STYX_E_INVALID, std::string(what) + ": unsupported shape or type"); \
-        if (_e != hipSuccess) return hip_fail(_e, what);                  \
-    } while (0)
-
 int styx_op_to_split(styx_gpu *g, int type, const void *src, void *dst, int64_t nblocks,
                      int64_t nmat)
 {
@@ -481,53 +468,6 @@ int styx_op_argmax(styx_gpu *g, const float *v, int n, uint32_t *out, float *sv,
 {
     OP_GPU(g);
     OP_RUN(launch_argmax(g->stream, v, n, out, sv, si, nullptr, 0, nullptr), "styx_op_argmax");
-    return STYX_OK;
-}
-
-// The gpu's device current for a call, whatever device the caller has current.
-struct DeviceScope {
-    int before = -1, now;
-    explicit DeviceScope(int device) : now(device)
-    {
-        if (hipGetDevice(&before) == hipSuccess && before != now) hipSetDevice(now);
-    }
-    ~DeviceScope()
-    {
-        if (before >= 0 && before != now) hipSetDevice(before);
-    }
-};
-
-// A launch's workgroups times its threads stay below 2^32.
-static constexpr int64_t MAX_WG_256 = (1 << 24) - 1;
-
-static bool kv_shape_ok(const styx_kv_cache *kv)
-{
-    return kv && (kv->type == STYX_F32 || kv->type == STYX_F16) && kv->n_seq >= 1 && kv->nkv >= 1 &&
-           (kv->hd == 64 || kv->hd == 128 || kv->hd == 256) && kv->page_tokens >= 1 && kv->n_pages >= 1 &&
-           kv->table_len >= 1 && (int64_t)kv->table_len * kv->page_tokens <= (1 << 30) &&
-           (int64_t)kv->n_pages * kv->page_tokens <= INT32_MAX && (int64_t)kv->n_seq * kv->nkv <= MAX_WG_256 / 4;
-}
-
-static int kv_view(const styx_kv_cache *kv, KvView *v, const char *who)
-{
-    if (!kv_shape_ok(kv))
-        return fail(STYX_E_INVALID, std::string(who) + ": unsupported cache type or shape");
-    if (!kv->kpool || !kv->vpool || !kv->page_table)
-        return fail(STYX_E_INVALID, std::string(who) + ": NULL pointer in the cache");
-    if (((uintptr_t)kv->kpool | (uintptr_t)kv->vpool) & 15)
-        return fail(STYX_E_INVALID, std::string(who) + ": pools must be 16-byte aligned");
-    *v = KvView{kv->kpool, kv->vpool, kv->page_table, kv->type == STYX_F16, kv->n_seq, kv->nkv, kv->hd,
-                kv->page_tokens, kv->n_pages, kv->table_len, kv->table_len * kv->page_tokens,
-                page_div((uint32_t)kv->page_tokens)};
-    return STYX_OK;
-}
-
-static int ws_ok(const void *ws, uint64_t have, uint64_t need, const char *who)
-{
-    if (!ws || have < need)
-        return fail(STYX_E_INVALID, std::string(who) + ": workspace of " + std::to_string(have) + " bytes, " +
-                                        std::to_string(need) + " needed");
-    if ((uintptr_t)ws & 15) return fail(STYX_E_INVALID, std::string(who) + ": workspace must be 16-byte aligned");
     return STYX_OK;
 }
 

@@ -235,6 +235,7 @@ class KvBatch:
         self.c = L.KvCache(type_, n_seq, nkv, hd, page_tokens, n_pages, table_len, self.kpool.ptr,
                            self.vpool.ptr, self.table.ptr)
         self._ws = None
+        self.held = self.free_pages = self.n_free = None
 
     def set(self, len=None, pos=None, table=None) -> None:
         """Upload lengths, positions or the page table (-1: no page)."""
@@ -282,10 +283,131 @@ class KvBatch:
             self.acc.ptr, self.acc.ptr, self.slot_pos.ptr, self.slot_pos.ptr, self.len.ptr, ws.ptr,
             ws.nbytes))
 
-    def free(self) -> None:
-        for b in (self.kpool, self.vpool, self.table, self.len, self.pos, self.acc, self.slot_pos, self._ws):
+    def manage(self) -> None:
+        """Hand all pages to plan(): no sequence has any."""
+        n = self.c.n_pages
+        self.set(table=np.full(self.n_seq * self.c.table_len, -1), len=np.full(self.n_seq, -1))
+        self.held = self.held or self.gpu.buffer(4 * self.n_seq)
+        self.free_pages = self.free_pages or self.gpu.buffer(4 * n)
+        self.n_free = self.n_free or self.gpu.buffer(16)
+        self.held.upload(np.zeros(self.n_seq, np.int32))
+        self.free_pages.upload(np.arange(n, dtype=np.int32)[::-1])
+        self.n_free.upload(np.array([n], np.int32))
+
+    def plan(self, n_new, shared=None) -> "Chunk":
+        """styx_op_kv_plan in place: pages for n_new[b] tokens of each sequence
+        from position pos[b] on, and the chunk that they make.  Advance the
+        lengths by chunk.counts() before the next plan()."""
+        if self.held is None:
+            raise ValueError("the pages are the caller's: manage() first")
+        n_new = np.asarray(n_new, np.int32).ravel()
+        shared = None if shared is None else np.asarray(shared, np.int32).ravel()
+        for a in (n_new, shared):
+            if a is not None and a.size != self.n_seq:
+                raise ValueError(f"{a.size} values, {self.n_seq} expected")
+        ch = Chunk(self, int(np.maximum(n_new, 0).astype(np.int64).sum()))
+        asked, owned = self.gpu.from_numpy(n_new), None if shared is None else self.gpu.from_numpy(shared)
+        pages = L.KvPages(self.table.ptr, self.held.ptr, self.free_pages.ptr, self.n_free.ptr)
+        L.check(self.lib.styx_op_kv_plan(
+            self.gpu.h, C.byref(self.c), C.byref(pages), C.byref(pages), owned.ptr if owned else None, self.len.ptr,
+            asked.ptr, self.pos.ptr, ch.n_rows, ch.first.ptr, ch.count.ptr, ch.row_seq.ptr, ch.row_pos.ptr,
+            ch.row_at.ptr))
+        self.gpu.sync()
+        for b in (asked, owned):
             if b is not None:
                 b.free()
+        return ch
+
+    def _rows(self, name: str, b, type_: int, n_rows: int, heads: int, ld) -> int:
+        """Values from one row to the next, after a check of the buffer's size."""
+        ld, es = ld or heads * self.hd, 2 if type_ == L.F16 else 4
+        buf, off = b if isinstance(b, tuple) else (b, 0)
+        if off < 0 or n_rows and buf.nbytes < off + es * ((n_rows - 1) * ld + heads * self.hd):
+            raise ValueError(f"{name}: {buf.nbytes} bytes hold fewer than {n_rows} rows of {heads} heads")
+        return ld
+
+    def append(self, ch: "Chunk", nh: int, q, k, v, q_out, rope: Buffer | None, n_pos: int = 0, n_rot: int | None = None,
+               interleaved: bool = False, q_norm: Buffer | None = None, k_norm: Buffer | None = None, eps: float = 1e-6,
+               type_in: int = L.F32, type_q: int = L.F32, ldq=None, ldk=None, ldv=None, ldo=None) -> None:
+        """styx_op_kv_append of the chunk's rows; q, k, v and q_out are buffers
+        or (buffer, byte offset), ld* the values from one row to the next."""
+        n_rot = self.hd if n_rot is None else n_rot
+        if rope is not None and rope.nbytes < 8 * n_pos * n_rot:
+            raise ValueError(f"rope: {rope.nbytes} bytes, {8 * n_pos * n_rot} needed")
+        for name, b in (("q_norm", q_norm), ("k_norm", k_norm)):
+            if b is not None and b.nbytes < 4 * self.hd:
+                raise ValueError(f"{name}: {b.nbytes} bytes, {4 * self.hd} needed")
+        at = lambda b: None if b is None else b[0].ptr + b[1] if isinstance(b, tuple) else b.ptr  # noqa: E731
+        lds = [self._rows(name, b, t, ch.n_rows, heads, ld) if b is not None else 0
+               for name, b, t, heads, ld in (("q", q, type_in, nh, ldq), ("k", k, type_in, self.nkv, ldk),
+                                             ("v", v, type_in, self.nkv, ldv), ("q_out", q_out, type_q, nh, ldo))]
+        r = L.Rope(rope.ptr, n_pos, n_rot, int(interleaved)) if rope is not None else None
+        L.check(self.lib.styx_op_kv_append(
+            self.gpu.h, C.byref(self.c), ch.n_rows, ch.row_pos.ptr, ch.row_at.ptr, nh, type_in, at(q), lds[0], at(k),
+            lds[1], at(v), lds[2], at(q_norm), at(k_norm), eps, C.byref(r) if r else None, type_q, at(q_out), lds[3]))
+
+    def attend_chunk(self, ch: "Chunk", nh: int, q, out, scale: float, window: int = 0, lse: Buffer | None = None,
+                     type_q: int = L.F32, ldq=None, ldo=None) -> None:
+        """styx_op_attn_chunk of the chunk's rows; q and out are buffers or
+        (buffer, byte offset)."""
+        at = lambda b: b[0].ptr + b[1] if isinstance(b, tuple) else b.ptr  # noqa: E731
+        ldq, ldo = (self._rows(name, b, type_q, ch.n_rows, nh, ld) for name, b, ld in (("q", q, ldq), ("out", out, ldo)))
+        if lse is not None and lse.nbytes < 4 * ch.n_rows * nh:
+            raise ValueError(f"lse: {lse.nbytes} bytes, {4 * ch.n_rows * nh} needed")
+        ws = self._workspace(self.lib.styx_op_attn_chunk_ws_bytes(C.byref(self.c), ch.n_rows, nh))
+        L.check(self.lib.styx_op_attn_chunk(
+            self.gpu.h, C.byref(self.c), C.byref(ch.c), nh, type_q, at(q), ldq, scale, window, at(out), ldo,
+            lse.ptr if lse is not None else None, ws.ptr, ws.nbytes))
+
+    def weigh(self, ch: "Chunk", nh: int, q, lse: Buffer, scale: float, last: int, decay: float = 1.0, window: int = 0,
+              type_q: int = L.F32, ldq=None) -> None:
+        """styx_op_kv_weigh in place: the weights of each sequence's last new
+        tokens, and the new rows' positions."""
+        if not self.scored:
+            raise ValueError("a cache without scores has nothing to add to")
+        ldq = self._rows("q", q, type_q, ch.n_rows, nh, ldq)
+        if lse.nbytes < 4 * ch.n_rows * nh:
+            raise ValueError(f"lse: {lse.nbytes} bytes, {4 * ch.n_rows * nh} needed")
+        L.check(self.lib.styx_op_kv_weigh(
+            self.gpu.h, C.byref(self.c), C.byref(ch.c), self.pos.ptr, nh, type_q,
+            q[0].ptr + q[1] if isinstance(q, tuple) else q.ptr, ldq, scale, window, lse.ptr, last, decay,
+            self.acc.ptr, self.acc.ptr, self.slot_pos.ptr))
+
+    def free(self) -> None:
+        for b in (self.kpool, self.vpool, self.table, self.len, self.pos, self.acc, self.slot_pos, self._ws,
+                  self.held, self.free_pages, self.n_free):
+            if b is not None:
+                b.free()
+
+
+class Chunk:
+    """New tokens of a KvBatch (styx_kv_chunk) as plan() lays them out: rows
+    [first[b], first[b] + count[b]) are sequence b's; row_seq, row_pos and row_at
+    say the same by row.  Lengths are the cache's: append, attend_chunk and weigh
+    come before they are advanced."""
+
+    def __init__(self, kv: KvBatch, n_rows: int):
+        self.n_rows, self.n_seq = n_rows, kv.n_seq
+        self.first, self.count = (kv.gpu.buffer(max(4 * kv.n_seq, 16)) for _ in range(2))
+        self.row_seq, self.row_pos, self.row_at = (kv.gpu.buffer(max(4 * n_rows, 16)) for _ in range(3))
+        self.c = L.KvChunk(n_rows, self.first.ptr, self.count.ptr, kv.len.ptr)
+
+    def counts(self) -> np.ndarray:
+        """New tokens of each sequence that got its pages."""
+        return self.count.download(np.int32, self.n_seq)
+
+    def free(self) -> None:
+        for b in (self.first, self.count, self.row_seq, self.row_pos, self.row_at):
+            b.free()
+
+
+def rope_table(n_rot: int, n_pos: int, base: float = 1e6, kind: int = L.ROPE_PLAIN, factor: float = 1.0, n_orig: int = 0,
+               fast: float = 0.0, slow: float = 0.0, gain: float = 0.0) -> np.ndarray:
+    """styx_rope_table_scaled: [n_pos][n_rot/2][2] (cos, sin) in f64."""
+    out = np.empty((max(n_pos, 0), max(n_rot, 0) // 2, 2), np.float64)
+    s = L.RopeScaling(kind, factor, n_orig, fast, slow, gain)
+    L.check(L.load().styx_rope_table_scaled(base, n_rot, n_pos, C.byref(s), out.ctypes.data if out.size else None))
+    return out
 
 
 def sample(gpu: Gpu, logits: Buffer, n: int, params, u, ld: int | None = None):

@@ -1,0 +1,218 @@
+"""styx_op_attn_chunk (no counterpart in the reference) against its definition
+in 64 bits, through the C ABI.  Tolerances: chunk_cases.Chunked.attend."""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from chunk_cases import Chunked, check_chunk, run_chunk
+from styx_amd import _lib as L
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": (False, False), "f16": (True, True), "mixed": (True, False)}  # cache, q in 16 bits
+
+
+@pytest.fixture(scope="module")
+def gpu():
+    from styx_amd import Gpu
+    g = Gpu(0)
+    yield g
+    g.close()
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("gqa", [1, 3, 8, 16])
+def test_ragged_batch(gpu, types, hd, gqa):
+    """Sequences of no rows and of many, one token and many, waiting ones between them."""
+    rng = np.random.default_rng(hd + gqa)
+    c = Chunked(rng, *TYPES[types], [0, 0, 5, -1, 130, 63, 1, 300], [1, 37, 1, 4, 66, 2, 0, 17], 2, gqa, hd, 16)
+    check_chunk(c, *run_chunk(gpu, c))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("page", [1, 7, 100, 512])
+def test_pages_that_end_inside_a_tile(gpu, types, page):
+    c = Chunked(np.random.default_rng(page), *TYPES[types], [211, 64], [45, 64], 1, 4, 128, page)
+    check_chunk(c, *run_chunk(gpu, c))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("window", [1, 2, 31, 64, 200, 1 << 30])
+def test_window(gpu, types, window):
+    c = Chunked(np.random.default_rng(window % 97), *TYPES[types], [0, 150, 400], [140, 33, 1], 2, 2, 64, 32, window=window)
+    check_chunk(c, *run_chunk(gpu, c))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("lens,counts", [([2000], [1]), ([5000, 3], [2, 1]), ([0], [600]), ([1500, 900, 0, 40], [16, 128, 1, 300])])
+def test_long_contexts(gpu, types, lens, counts):
+    """Few tokens over many rows (split over workgroups), and prompts of several tiles."""
+    c = Chunked(np.random.default_rng(len(lens)), *TYPES[types], lens, counts, 2, 8, 128, 64)
+    check_chunk(c, *run_chunk(gpu, c), tokens=lambda n: range(n) if n < 20 else sorted({0, 1, n // 3, n // 2, n - 2, n - 1}))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_many_sequences_of_one_token(gpu, types):
+    lens = [(37 * b) % 500 for b in range(150)]
+    c = Chunked(np.random.default_rng(3), *TYPES[types], lens, [1] * 150, 1, 4, 64, 16)
+    check_chunk(c, *run_chunk(gpu, c))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_rows_in_any_order_with_gaps_and_strides(gpu, types):
+    """Sequences' rows in no order with rows of none between them, rows farther apart than they are long, no lse."""
+    c = Chunked(np.random.default_rng(5), *TYPES[types], [9, 70, 0], [5, 20, 3], 2, 4, 64, 16, first=[30, 7, 1], n_rows=40,
+                ld=2 * 4 * 64 + 72)
+    out, lse = run_chunk(gpu, c, lse=False, ldo=2 * 4 * 64 + 24)
+    check_chunk(c, out)
+    assert (lse == 7.5).all()
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_skipped_sequences(gpu, types):
+    """Lengths, counts and rows outside their ranges: nothing of the sequence is read or written."""
+    big = 2 ** 31 - 1
+    lens, counts = [10, -1, 40, 10, 10, big, 5, 10, 5], [4, 4, 30, 4, -3, 4, big, 4, 0]
+    first = [0, 4, 8, -1, 12, 16, 20, 61, 24]
+    c = Chunked(np.random.default_rng(6), *TYPES[types], [10] * 9, [4] * 9, 1, 2, 64, 8, first=first, n_rows=64, table_len=8)
+    c.lens, c.counts = np.array(lens, np.int32), np.array(counts, np.int32)
+    assert [c.taken(b) for b in range(9)] == [True] + [False] * 8
+    check_chunk(c, *run_chunk(gpu, c))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_full_cache(gpu, types):
+    c = Chunked(np.random.default_rng(8), *TYPES[types], [50, 0], [14, 64], 1, 4, 128, 16, table_len=4, spare=0)
+    assert c.cap == 64
+    check_chunk(c, *run_chunk(gpu, c))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("hd", [64, 128])
+def test_missing_pages(gpu, types, hd):
+    """Entries outside the pool: their rows are not seen; a token that sees nothing gets 0 and -infinity."""
+    c = Chunked(np.random.default_rng(9), *TYPES[types], [90, 0, 200], [20, 40, 3], 1, 4, hd, 16)
+    c.table[0, [0, 3]] = -1
+    c.table[0, 6] = c.n_pages
+    c.table[1, :2] = -7
+    c.table[2, 1:] = 2 ** 31 - 1
+    out, lse = run_chunk(gpu, c)
+    check_chunk(c, out, lse)
+    f = int(c.first[1])
+    assert (out[f:f + 32] == 0).all() and np.isneginf(lse[f:f + 32]).all() and np.isfinite(lse[f + 32]).all()
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_what_is_not_seen_has_no_influence(gpu, types, bad, hd):
+    """Values that are not finite behind the last row, in pages of others, outside the window, and in new rows that
+    only later tokens see: the others' outputs are those of the definition."""
+    c = Chunked(np.random.default_rng(10), *TYPES[types], [70, 20], [50, 9], 1, 4, hd, 16, window=60)
+    rows = [c.rows(b) for b in range(2)]
+    own = np.concatenate(rows)
+    for p in (c.k, c.v):
+        rest = np.ones(len(p), bool)
+        rest[own] = False
+        p[rest] = bad
+        p[rows[0][:5]] = bad       # outside every token's window
+        p[rows[0][70 + 41]] = bad  # seen by the tokens from 41 on
+    out, lse = run_chunk(gpu, c)
+    later = np.zeros(c.n_rows, bool)
+    later[41:50] = True
+    assert np.isfinite(out[~later]).all() and np.isfinite(lse[~later]).all()
+    check_chunk(c, out, lse, tokens=lambda n: range(min(n, 41)))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("count", [1, 50])
+def test_values_that_are_not_finite_reach_the_outputs(gpu, types, count):
+    c = Chunked(np.random.default_rng(11), *TYPES[types], [300], [count], 1, 2, 128, 16)
+    rows = c.rows(0)
+    c.v[rows[17], 0, 5] = np.nan
+    c.v[rows[200], 0, 9] = np.inf
+    c.v[rows[300], 0, 70] = np.inf  # the first new row
+    out, lse = run_chunk(gpu, c)
+    out = out.reshape(count, 2, 128)
+    assert not np.isfinite(out[:, :, [5, 9, 70]]).any() and np.isfinite(lse).all()
+    assert np.isfinite(np.delete(out, [5, 9, 70], 2)).all()
+    c.k[rows[40], 0, 3] = np.nan
+    out, lse = run_chunk(gpu, c)
+    assert np.isnan(out).all() and np.isnan(lse).all()
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_large_and_equal_scores(gpu, types):
+    """Scores of hundreds, whose exponentials underflow or are all 1."""
+    c = Chunked(np.random.default_rng(12), *TYPES[types], [100, 80], [30, 3], 1, 4, 64, 16)
+    c.q = (c.q * 40).astype(c.qt)
+    c.q[30:] = 0
+    check_chunk(c, *run_chunk(gpu, c))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_results_repeat(gpu, types):
+    """No result depends on an order of execution or on what the workspace held."""
+    c = Chunked(np.random.default_rng(13), *TYPES[types], [3000, 40, 900], [7, 100, 1], 2, 8, 128, 64)
+    a, b = run_chunk(gpu, c), run_chunk(gpu, c)
+    assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
+
+
+def test_offsets_past_32_bits(gpu):
+    """Pools of more than 2^32 bytes and 2^31 values: rows at their ends."""
+    c = Chunked(np.random.default_rng(14), True, True, [40], [9], 8, 2, 128, 64)
+    n_pages = (2 ** 31 + 2 ** 20) // (64 * 8 * 128)
+    kv, ch, q = c.buffers(gpu)
+    table = np.array([[n_pages - 1]], np.int32)
+    big = [gpu.buffer(2 * n_pages * 64 * 8 * 128) for _ in range(2)]
+    at = 2 * (n_pages - 1) * 64 * 8 * 128
+    page = c.table[0, 0]
+    for buf, x in zip(big, (c.k, c.v)):
+        buf.upload(x[page * 64:(page + 1) * 64], at)
+    tab = gpu.from_numpy(table)
+    kv.n_pages, kv.kpool, kv.vpool, kv.page_table = n_pages, big[0].ptr, big[1].ptr, tab.ptr
+    out = gpu.zeros(2 * c.n_rows * c.nh * c.hd)
+    need = gpu.lib.styx_op_attn_chunk_ws_bytes(C.byref(kv), c.n_rows, c.nh)
+    ws = gpu.buffer(need)
+    L.check(gpu.lib.styx_op_attn_chunk(gpu.h, C.byref(kv), C.byref(ch), c.nh, L.F16, q.ptr, c.ld, c.scale, 0, out.ptr,
+                                       c.ld, None, ws.ptr, need))
+    gpu.sync()
+    check_chunk(c, out.download(np.float16).reshape(c.n_rows, -1))
+    for b in big:
+        b.free()
+
+
+def test_refusals(gpu):
+    c = Chunked(np.random.default_rng(15), True, True, [9], [3], 2, 4, 64, 16)
+    kv, ch, q = c.buffers(gpu)
+    need = gpu.lib.styx_op_attn_chunk_ws_bytes(C.byref(kv), 3, 8)
+    ws, out = gpu.buffer(need + 16), gpu.zeros(4 * 3 * 8 * 64)
+
+    def call(kv=kv, ch=ch, nh=8, tq=L.F16, q=q.ptr, ldq=512, window=0, out=out.ptr, ldo=512, ws=ws.ptr, n=need):
+        return gpu.lib.styx_op_attn_chunk(gpu.h, C.byref(kv) if kv else None, C.byref(ch) if ch else None, nh, tq, q, ldq,
+                                          0.1, window, out, ldo, None, ws, n)
+
+    def other(**f):
+        k = L.KvCache(*(getattr(kv, n) for n, _ in kv._fields_))
+        for n, v in f.items():
+            setattr(k, n, v)
+        return k
+
+    assert call() == 0
+    bad = [dict(kv=None), dict(ch=None), dict(nh=7), dict(nh=0), dict(nh=34), dict(tq=L.Q8_0), dict(q=None), dict(out=None),
+           dict(ldq=511), dict(ldq=516), dict(ldo=504), dict(ldo=2 ** 31), dict(q=q.ptr + 2), dict(out=out.ptr + 8), dict(window=-1),
+           dict(ws=None), dict(n=need - 1), dict(ws=ws.ptr + 4), dict(kv=other(hd=96)), dict(kv=other(kpool=None)),
+           dict(kv=other(kpool=kv.kpool + 8)), dict(kv=other(type=L.F32)), dict(kv=other(page_tokens=0)),
+           dict(kv=other(table_len=0)), dict(ch=L.KvChunk(-1, ch.first, ch.count, ch.len)),
+           dict(ch=L.KvChunk(3, None, ch.count, ch.len)), dict(ch=L.KvChunk(3, ch.first, None, ch.len)),
+           dict(ch=L.KvChunk(3, ch.first, ch.count, None)), dict(ch=L.KvChunk(2 ** 31 - 1, ch.first, ch.count, ch.len))]
+    for b in bad:
+        assert call(**b) == -1, b
+    assert call(ch=L.KvChunk(0, ch.first, ch.count, ch.len)) == 0  # no rows: nothing to do
+    assert gpu.lib.styx_op_attn_chunk(None, C.byref(kv), C.byref(ch), 8, L.F16, q.ptr, 512, 0.1, 0, out.ptr, 512, None,
+                                      ws.ptr, need) == -1
+    gpu.sync()

@@ -1,0 +1,122 @@
+"""The C layouts of the structs of the operators on new tokens (printed by a gcc
+build of the header) against their ctypes and Rust mirrors, the rope tables
+against their formulas, and the sizes of workspaces.  No GPU needed."""
+from __future__ import annotations
+
+import ctypes as C
+import json
+import math
+import shutil
+import subprocess
+
+import numpy as np
+import pytest
+
+from styx_amd import _lib as L, rope_table
+from test_abi_drift import HDR, rust_layout, rust_structs
+
+STRUCTS = {"styx_kv_chunk": "KvChunk", "styx_kv_pages": "KvPages", "styx_rope": "Rope", "styx_rope_scaling": "RopeScaling"}
+
+
+@pytest.mark.parametrize("name", sorted(STRUCTS))
+def test_mirrors_have_the_header_layout(name, tmp_path):
+    gcc = shutil.which("gcc")
+    if not gcc:
+        pytest.skip("gcc not available")
+    cls = getattr(L, STRUCTS[name])
+    fields = [f for f, _ in cls._fields_]
+    src = "\n".join(["#include <stdio.h>", "#include <stddef.h>", f'#include "{HDR}"', "int main(void) {",
+                     f'printf("[%zu", sizeof({name}));',
+                     *[f'printf(", %zu", offsetof({name}, {f}));' for f in fields], 'printf("]"); return 0; }'])
+    (tmp_path / "lay.c").write_text(src)
+    subprocess.run([gcc, "-std=c11", "-o", str(tmp_path / "lay"), str(tmp_path / "lay.c")], check=True)
+    size, *offs = json.loads(subprocess.run([str(tmp_path / "lay")], capture_output=True, text=True, check=True).stdout)
+    assert C.sizeof(cls) == size and [getattr(cls, f).offset for f in fields] == offs
+    rust = rust_structs()[name]
+    assert [f for f, _ in rust] == fields
+    assert rust_layout(rust, {}) == (offs, size)
+
+
+
+def near(got, freq, gain=1.0, n_pos=200):
+    """(cos, sin)(p f) gain; an angle p f is off by at most 2^-50 of itself."""
+    th = np.arange(n_pos)[:, None] * np.asarray(freq)
+    want = gain * np.stack([np.cos(th), np.sin(th)], -1)
+    assert np.abs(got - want).max() <= 1e-15 * 8 * n_pos * max(gain, 1)
+
+
+def plain(n_rot, base):
+    return np.array([base ** (-2 * i / n_rot) for i in range(n_rot // 2)])
+
+
+@pytest.mark.parametrize("n_rot", [2, 64, 98, 128, 256])
+def test_plain_table_is_styx_rope_table(n_rot):
+    want = np.empty((200, n_rot // 2, 2))
+    L.load().styx_rope_table(1e6, n_rot, 200, want.ctypes.data)
+    assert np.array_equal(rope_table(n_rot, 200, 1e6), want)
+    near(want, plain(n_rot, 1e6))
+
+
+def test_linear_and_stretched_base():
+    near(rope_table(64, 200, 1e4, L.ROPE_LINEAR, 4.0), plain(64, 1e4) / 4)
+    near(rope_table(64, 200, 1e4, L.ROPE_LINEAR, 4.0, gain=1.5), plain(64, 1e4) / 4, 1.5)
+    near(rope_table(64, 200, 1e4, L.ROPE_BASE, 8.0), plain(64, 1e4 * 8 ** (64 / 62)))
+
+
+@pytest.mark.parametrize("fast,slow,n_orig", [(32, 1, 4096), (8, 2, 8192), (32, 1, 4)])
+def test_by_parts(fast, slow, n_orig):
+    n_rot, base, s = 128, 1e6, 8.0
+    f = plain(n_rot, base)
+    pair = lambda turns: n_rot * math.log(n_orig / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+    low, high = max(0.0, math.floor(pair(fast))), min(n_rot - 1.0, math.ceil(pair(slow)))
+    if high <= low:
+        high = low + 0.001
+    r = np.clip((np.arange(n_rot // 2) - low) / (high - low), 0, 1)
+    want = f * (1 - r) + f / np.float32(s) * r
+    gain = 0.1 * math.log(s) + 1
+    near(rope_table(n_rot, 200, base, L.ROPE_PARTS, s, n_orig, fast, slow), want, gain)
+    near(rope_table(n_rot, 200, base, L.ROPE_PARTS, s, n_orig, fast, slow, gain=1.0), want)
+    if n_orig > 1000:  # fast pairs are kept, slow ones interpolated
+        turns = n_orig * f / (2 * math.pi)
+        assert np.array_equal(want[turns > 2 * fast], f[turns > 2 * fast])
+        assert np.allclose(want[turns < slow / 2], f[turns < slow / 2] / s, rtol=1e-12)
+
+
+def test_bands():
+    f = plain(128, 5e5)
+    turns = 8192 * f / (2 * math.pi)
+    r = np.clip((turns - 1) / 3, 0, 1)
+    want = f / 8 * (1 - r) + f * r
+    near(rope_table(128, 200, 5e5, L.ROPE_BANDS, 8.0, 8192), want)
+    assert (want[turns > 4] == f[turns > 4]).all() and np.allclose(want[turns < 1] * 8, f[turns < 1])
+
+
+def test_rope_refusals():
+    ok = dict(n_rot=64, n_pos=4, base=1e4)
+    rope_table(**ok)
+    for bad in [dict(n_rot=0), dict(n_rot=63), dict(n_rot=-2), dict(n_pos=0), dict(base=0.0), dict(base=-1.0), dict(base=math.nan),
+                dict(base=math.inf), dict(kind=5), dict(kind=-1), dict(kind=L.ROPE_LINEAR, factor=0.0),
+                dict(kind=L.ROPE_LINEAR, factor=math.inf), dict(kind=L.ROPE_BASE, factor=2.0, n_rot=2),
+                dict(kind=L.ROPE_PARTS, factor=2.0), dict(kind=L.ROPE_PARTS, factor=2.0, n_orig=8, fast=1.0, slow=2.0),
+                dict(kind=L.ROPE_PARTS, factor=2.0, n_orig=8, base=1.0), dict(kind=L.ROPE_BANDS, factor=2.0),
+                dict(kind=L.ROPE_BANDS, factor=2.0, n_orig=8, slow=-1.0), dict(gain=math.nan)]:
+        with pytest.raises(L.StyxError):
+            rope_table(**{**ok, **bad})
+
+
+def test_workspace_sizes():
+    lib = L.load()
+    kv = lambda **f: C.byref(L.KvCache(*{**dict(type=L.F16, n_seq=4, nkv=2, hd=128, page=16, n_pages=100, table_len=20, k=None,  # noqa: E731
+                                                v=None, t=None), **f}.values()))
+    assert lib.styx_op_attn_chunk_ws_bytes(kv(), 50, 8) > 0 and lib.styx_op_attn_chunk_ws_bytes(kv(), 0, 8) > 0
+    for args in [(None, 50, 8), (kv(), -1, 8), (kv(), 50, 7), (kv(), 50, 0), (kv(), 50, 34), (kv(hd=80), 50, 8), (kv(type=8), 50, 8),
+                 (kv(n_seq=0), 50, 8), (kv(page=1 << 20, table_len=1 << 20), 50, 8), (kv(), 2 ** 31 - 1, 32)]:
+        assert lib.styx_op_attn_chunk_ws_bytes(*args) == 0, args[1:]
+
+
+def test_entry_points_refuse_a_null_gpu():
+    lib = L.load()
+    assert lib.styx_op_kv_plan(*[None] * 8, 0, *[None] * 5) == -1
+    assert lib.styx_op_kv_append(None, None, 0, None, None, 0, 0, None, 0, None, 0, None, 0, None, None, 0.0, None, 0, None, 0) == -1
+    assert lib.styx_op_attn_chunk(None, None, None, 0, 0, None, 0, 0.0, 0, None, 0, None, None, 0) == -1
+    assert lib.styx_op_kv_weigh(None, None, None, None, 0, 0, None, 0, 0.0, 0, None, 0, 0.0, None, None, None) == -1
