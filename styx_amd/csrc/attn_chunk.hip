@@ -86,8 +86,8 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD> {
     using TC = _Float16;
     using La = Lay<TC, HD>;
     static constexpr int NP = sizeof(TQ) == 4 ? 2 : 1;  // pieces
-    static constexpr int QT = HD == 256 ? 1 : 2, KT = 64, NK = HD / 16, ND = HD / 32;
-    static constexpr int PER_CU = HD == 64 ? 2 : 1;
+    static constexpr int QT = 1, KT = 64, NK = HD / 16, ND = HD / 32;
+    static constexpr int PER_CU = HD == 256 ? 1 : 2;
     h8 q[QT][NP][NK], p[QT][NP][KT / 16];
     f16v s[KT / 32][QT], o[QT][ND];
     float mul[QT];
@@ -351,6 +351,7 @@ __global__ void __launch_bounds__(AC_WG, (Wave<TQ, TC, HD>::PER_CU)) k_attn_chun
     int64_t orow[QT];          // row of q and out
     int head[QT];
     float m[QT], l[QT];
+    uint32_t nan_at[QT][HD / 64];  // dims that are NaN whatever the sums are
     const int wrow0 = 32 * QT * wave;
     const bool works = row0 + wrow0 < rows;
 #pragma unroll
@@ -362,6 +363,8 @@ __global__ void __launch_bounds__(AC_WG, (Wave<TQ, TC, HD>::PER_CU)) k_attn_chun
         at[qt] = r < rows ? s.len + tok : -1;
         m[qt] = -INFINITY;
         l[qt] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < HD / 64; w++) nan_at[qt][w] = 0;
         x.init(qt, (const TQ *)a.q + orow[qt] * a.ldq + (int64_t)head[qt] * HD, a.scale);
 #pragma unroll
         for (int d = 0; d < ND; d++) x.o[qt][d] = f16v{};
@@ -426,7 +429,7 @@ __global__ void __launch_bounds__(AC_WG, (Wave<TQ, TC, HD>::PER_CU)) k_attn_chun
                 }
             // A value that is not finite must not reach those that do not see
             // it, whose factor is 0: where there is one, the dims of those that
-            // do see it become NaN, and the value 0.
+            // do see it are noted to be NaN, and the value becomes 0.
             char *mine = s_v[buf] + threadIdx.x * (BLOCK / AC_WG);
             bool odd = false;
 #pragma unroll
@@ -436,20 +439,26 @@ __global__ void __launch_bounds__(AC_WG, (Wave<TQ, TC, HD>::PER_CU)) k_attn_chun
                 for (int e = 0; e < 4; e++) odd |= not_finite<TC>(v[e]) != 0;
             }
             if (__syncthreads_or(odd)) {
-                for (int t = 0; t < KT; t++)
+#pragma unroll 1
+                for (int t = 0; t < KT; t++) {
+                    uint32_t see[QT];
 #pragma unroll
-                    for (int d = 0; d < ND; d++)
+                    for (int qt = 0; qt < QT; qt++) see[qt] = 0u - (vis[qt][KT == 64 ? t >> 5 : 0] >> (t & 31) & 1);
+                    // bits 4 j + e: dims 8 j + 4 h + e
+#pragma unroll 1
+                    for (int j = 0; j < HD / 8; j++) {
+                        const TC *v = (const TC *)(vb + La::at(t, 8 * j + 4 * h));
+                        uint32_t bad = 0;
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            const TC *v = (const TC *)(vb + La::at(t, 32 * d + 2 * i + 4 * h));
+                        for (int e = 0; e < 4; e++) bad |= (uint32_t) !(fabsf((float)v[e]) < INFINITY) << e;
+                        if (bad)
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const bool bad = !(fabsf((float)v[e]) < INFINITY);
+                            for (int w = 0; w < HD / 64; w++)
 #pragma unroll
                                 for (int qt = 0; qt < QT; qt++)
-                                    if (bad & (vis[qt][t / 32] >> (t & 31) & 1)) x.o[qt][d][i + e] = NAN;
-                            }
-                        }
+                                    nan_at[qt][w] |= w == j >> 3 ? (bad & see[qt]) << (4 * (j & 7)) : 0;
+                    }
+                }
                 __syncthreads();
                 for (int i = 0; i < BLOCK / AC_WG; i += 4) {
                     uint32_t *v = (uint32_t *)(mine + i);
@@ -506,6 +515,11 @@ __global__ void __launch_bounds__(AC_WG, (Wave<TQ, TC, HD>::PER_CU)) k_attn_chun
     for (int qt = 0; qt < QT; qt++) {
         if (at[qt] < 0) continue;
         l[qt] += other_half(l[qt]);
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (nan_at[qt][d / 2] >> (16 * (d & 1) + i) & 1) x.o[qt][d][i] = NAN;
         if (sp.share) {
             // a partial result: M, L and the sums
             const int64_t p = ((it.first + it.piece) * kv.nkv + kvh) * part_rows + wrow0 + 32 * qt + n;
