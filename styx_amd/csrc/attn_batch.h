@@ -14,6 +14,7 @@ namespace styx {
 struct PageDiv {
     uint32_t mul;
     int sh;
+    __device__ __forceinline__ int of(int t) const { return (int)(__umulhi(2u * (uint32_t)t, mul) >> sh); }
 };
 inline PageDiv page_div(uint32_t d)
 {

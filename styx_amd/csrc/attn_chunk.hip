@@ -7,11 +7,11 @@
 //
 // A workgroup takes a tile of query rows -- a row is a token and one of a kv
 // head's gqa heads, token by token -- and goes once over the slots that they see,
-// in blocks that lie in LDS for its four waves, the next block under way
-// meanwhile.  Scores are formed transposed, slots x queries: lane (n = lane & 31,
-// h = lane >> 5) then has its own query's scores of slots 8 (i / 4) + 4 h + i % 4
-// of each 32, the softmax factors are lane-local, and they are the operand of
-// the value product as they stand.
+// in blocks that lie in LDS for its waves, the next block under way meanwhile.
+// Scores are formed transposed, slots x queries: lane (n = lane & 31, h = lane >>
+// 5) then has its own query's scores of slots 8 (i / 4) + 4 h + i % 4 of each 32,
+// the softmax factors are lane-local, and they are the operand of the value
+// product as they stand.
 #include <algorithm>
 #include <type_traits>
 
@@ -20,7 +20,6 @@
 
 namespace styx {
 
-constexpr int AC_WG = 256, AC_WAVES = AC_WG / 64;
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
@@ -33,6 +32,11 @@ __device__ __forceinline__ float other_half(float v)
     const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return __uint_as_float((threadIdx.x & 32) ? x[0] : x[1]);
 }
+// A value that all lanes have, for the scalar unit.
+template <typename T> __device__ __forceinline__ T uniform(T v)
+{
+    return by_words(v, [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); });
+}
 
 // 16 bytes a lane from memory to LDS at off + 16 lane (off uniform), in the
 // background: the caller waits (landed) before it reads them.  Not the builtin:
@@ -40,6 +44,10 @@ __device__ __forceinline__ float other_half(float v)
 __device__ __forceinline__ void to_lds(const void *from, uint32_t off)
 {
     asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(off), "v"(from) : "memory");
+}
+__device__ __forceinline__ void to_lds(const void *base, uint32_t at, uint32_t off)
+{
+    asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(off), "v"(at), "s"(base) : "memory");
 }
 __device__ __forceinline__ void landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ uint32_t lds_at(const char *p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char *)p; }
@@ -75,6 +83,11 @@ template <typename TC> __device__ __forceinline__ uint32_t not_finite(uint32_t v
     return (((v & 0x7FFF7FFFu) + 0x04000400u) >> 15 & 0x00010001u) * 0xFFFFu;
 }
 
+// Nothing is moved across: the products below are written in the order in which
+// they are to be issued, operand reads some matrix instructions ahead of their
+// use, the factors' arithmetic between matrix instructions.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
 template <typename TQ, typename TC, int HD> struct Wave;
 
 // f16 caches: v_mfma_f32_32x32x16_f16.  f32 queries and their factors are two
@@ -86,28 +99,38 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD> {
     using TC = _Float16;
     using La = Lay<TC, HD>;
     static constexpr int NP = sizeof(TQ) == 4 ? 2 : 1;  // pieces
-    static constexpr int QT = 1, KT = 64, NK = HD / 16, ND = HD / 32;
-    static constexpr int PER_CU = HD == 256 ? 1 : 2;
-    h8 q[QT][NP][NK], p[QT][NP][KT / 16];
-    f16v s[KT / 32][QT], o[QT][ND];
-    float mul[QT];
+    // waves that share a query's dims, dims of a wave
+    static constexpr int DS = HD == 256 && NP == 2 ? 2 : 1, HW = HD / DS, NK = HW / 16, ND = HW / 32;
+    static constexpr int KT = HD == 256 ? 32 : 64;
+    static constexpr int NW = DS == 2 ? 8 : 4, PER_CU = 8 / NW, BM = 32 * NW / DS;
+    h8 q[NP][NK];
+    f16v s[KT / 32], o[ND];
+    float mul;
+    int lane;
 
-    __device__ __forceinline__ void init(int qt, const TQ *row, float scale)
+    // row: this wave's dims of the query, the first of which is d0
+    __device__ __forceinline__ void init(const TQ *row, int d0, float scale)
     {
-        const int h = (threadIdx.x & 63) >> 5;
+        const int h = lane >> 5;
         // (a scale of 0 goes into q: -infinity times it would be NaN)
         const float a = scale == 0.0f ? 1.0f : fabsf(scale), sign = scale < 0.0f ? -1.0f : scale == 0.0f ? 0.0f : 1.0f;
         if constexpr (NP == 1) {
-            mul[qt] = a;
+            mul = a;
 #pragma unroll
-            for (int i = 0; i < NK; i++) {
-                const h8 v = *(const h8 *)(row + 16 * i + 8 * h);
-#pragma unroll
-                for (int e = 0; e < 8; e++) q[qt][0][i][e] = v[e] * (_Float16)sign;
-            }
+            for (int i = 0; i < NK; i++) q[0][i] = *(const h8 *)(row + 16 * i + 8 * h) * (_Float16)sign;
         } else {
             styx_f4 v[NK][2];
             float m = 0.0f;
+            if constexpr (DS == 2) {  // the dims of the other wave
+#pragma unroll
+                for (int i = 0; i < NK; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const styx_f4 y = *(const styx_f4 *)(row + (HW - 2 * d0) + 16 * i + 8 * h + 4 * j);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) m = fmaxf(m, fabsf(y[e]));
+                    }
+            }
 #pragma unroll
             for (int i = 0; i < NK; i++)
 #pragma unroll
@@ -120,52 +143,49 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD> {
             const int e = m > 0.0f && m < INFINITY ? (int)((__float_as_uint(m) >> 23) & 255) - 127 : 9;
             // 2^(9 - e), in range for every exponent: 9 - e within [-118, 136]
             const float up = e < -100 ? ldexpf(1.0f, 109) : ldexpf(1.0f, 9 - e);
-            mul[qt] = a / up;
+            mul = a / up;
 #pragma unroll
             for (int i = 0; i < NK; i++)
 #pragma unroll
                 for (int x = 0; x < 8; x++) {
                     const float y = v[i][x >> 2][x & 3] * (up * sign);
                     const _Float16 hi = (_Float16)y;
-                    q[qt][0][i][x] = hi;
-                    q[qt][NP - 1][i][x] = (_Float16)(y - (float)hi);
+                    q[0][i][x] = hi;
+                    q[NP - 1][i][x] = (_Float16)(y - (float)hi);
                 }
         }
     }
     __device__ __forceinline__ void scores(const char *kb)
     {
-        const int lane = threadIdx.x & 63, m = lane & 31, h = lane >> 5;
+        constexpr int N = NK * KT / 32, AHEAD = 4;
+        const int m = lane & 31, h = lane >> 5;
         const f16v zero = {};
         const int at = m * La::ROW + ((h ^ La::perm(m)) << 4);
+        // (piece 2 i + h: its bits above 256 bytes are not permuted)
+        auto read = [&](int j) {
+            const int i = j / (KT / 32), kt = j % (KT / 32);
+            return *(const h8 *)(kb + (at ^ ((32 * i) & 255)) + ((32 * i) & ~255) + kt * 32 * La::ROW);
+        };
+        h8 k[AHEAD];
 #pragma unroll
-        for (int i = 0; i < NK; i++)
+        for (int j = 0; j < AHEAD; j++) k[j] = read(j);
+        in_order();
 #pragma unroll
-            for (int kt = 0; kt < KT / 32; kt++) {
-                // (piece 2 i + h: its bits above 256 bytes are not permuted)
-                const h8 k = *(const h8 *)(kb + (at ^ ((32 * i) & 255)) + ((32 * i) & ~255) + kt * 32 * La::ROW);
+        for (int j = 0; j < N; j++) {
+            const int i = j / (KT / 32), kt = j % (KT / 32);
 #pragma unroll
-                for (int x = 0; x < NP; x++)
-#pragma unroll
-                    for (int qt = 0; qt < QT; qt++)
-                        s[kt][qt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q[qt][x][i], i + x == 0 ? zero : s[kt][qt], 0, 0, 0);
-            }
+            for (int x = 0; x < NP; x++)
+                s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[j % AHEAD], q[x][i], i + x == 0 ? zero : s[kt], 0, 0, 0);
+            if (j + AHEAD < N) k[j % AHEAD] = read(j + AHEAD);
+            in_order();
+        }
     }
-    // factors from s, which holds them unrounded
-    __device__ __forceinline__ void factors(int qt)
+    // o += factors times V; returns their sum
+    __device__ __forceinline__ float values(const char *vb, float ref)
     {
-#pragma unroll
-        for (int k = 0; k < KT / 16; k++)
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const float v = s[k / 2][qt][8 * (k & 1) + i];
-                const _Float16 hi = (_Float16)v;
-                p[qt][0][k][i] = hi;
-                if constexpr (NP == 2) p[qt][1][k][i] = (_Float16)(v - (float)hi);
-            }
-    }
-    __device__ __forceinline__ void values(const char *vb)
-    {
-        const int lane = threadIdx.x & 63, h = lane >> 5, u = (lane >> 4) & 1, kk = (lane & 15) >> 2;
+        constexpr int N = ND * KT / 16, AHEAD = 4, PER = 8 / ND;
+        static_assert(8 % ND == 0, "factors of a step");
+        const int h = lane >> 5, u = (lane >> 4) & 1, kk = (lane & 15) >> 2;
         // piece of dims 16 u + 4 (lane & 3) .. of the first 32, row kk + 4 (h + 2 r)
         auto at = [&](int r) {
             const int t = kk + 4 * h + 8 * r;
@@ -173,23 +193,45 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD> {
         };
         const int at0 = at(0), at1 = at(1);
         typedef __attribute__((address_space(3))) s4 *lds4;
+        union Part {
+            s4 part[2];
+            h8 v;
+        };
+        auto read = [&](int j) {
+            const int d = j % ND, k = j / ND;
+            const int flip = (64 * d) & (La::ROW < 256 ? La::ROW - 1 : 255), far = ((64 * d) & ~255) + k * 16 * La::ROW;
+            Part x;
+            x.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vb + (at0 ^ flip) + far));
+            x.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vb + (at1 ^ flip) + far));
+            return x.v;
+        };
+        float sum[2] = {};
+        h8 p[2][NP];  // of the step under way and the next
+        auto factor = [&](int k, int i) {
+            const float f = exp2_(fmaf(s[k / 2][8 * (k & 1) + i], mul, ref));
+            sum[i & 1] += f;
+            const _Float16 hi = (_Float16)f;
+            p[k & 1][0][i] = hi;
+            if constexpr (NP == 2) p[k & 1][1][i] = (_Float16)(f - (float)hi);
+        };
+        h8 v[AHEAD];
 #pragma unroll
-        for (int d = 0; d < ND; d++)
+        for (int j = 0; j < AHEAD; j++) v[j] = read(j);
 #pragma unroll
-            for (int k = 0; k < KT / 16; k++) {
-                const int flip = (64 * d) & (La::ROW < 256 ? La::ROW - 1 : 255), far = ((64 * d) & ~255) + k * 16 * La::ROW;
-                union {
-                    s4 part[2];
-                    h8 v;
-                } x;
-                x.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vb + (at0 ^ flip) + far));
-                x.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vb + (at1 ^ flip) + far));
+        for (int i = 0; i < 8; i++) factor(0, i);
+        in_order();
 #pragma unroll
-                for (int y = 0; y < NP; y++)
+        for (int j = 0; j < N; j++) {
+            const int d = j % ND, k = j / ND;
 #pragma unroll
-                    for (int qt = 0; qt < QT; qt++)
-                        o[qt][d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x.v, p[qt][y][k], o[qt][d], 0, 0, 0);
-            }
+            for (int y = 0; y < NP; y++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[j % AHEAD], p[k & 1][y], o[d], 0, 0, 0);
+            if (j + AHEAD < N) v[j % AHEAD] = read(j + AHEAD);
+            if (k + 1 < KT / 16)
+#pragma unroll
+                for (int i = 0; i < PER; i++) factor(k + 1, PER * d + i);
+            in_order();
+        }
+        return sum[0] + sum[1];
     }
 };
 
@@ -198,179 +240,249 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD> {
 template <int HD> struct Wave<float, float, HD> {
     using TC = float;
     using La = Lay<TC, HD>;
-    static constexpr int QT = 1, KT = 32, NK = HD / 8, ND = HD / 32;
-    static constexpr int PER_CU = HD == 256 ? 1 : 2;
+    static constexpr int DS = HD == 256 ? 2 : 1, HW = HD / DS, NK = HW / 8, ND = HW / 32;
+    static constexpr int KT = 32;
+    static constexpr int NW = HD == 256 ? 8 : 4, PER_CU = 8 / NW, BM = 32 * NW / DS;
     styx_f4 q[NK];
-    f16v s[1][1], o[1][ND];
-    float mul[1];
+    f16v s[1], o[ND];
+    float mul;
+    int lane;
 
-    __device__ __forceinline__ void init(int, const float *row, float scale)
+    __device__ __forceinline__ void init(const float *row, int, float scale)
     {
-        const int h = (threadIdx.x & 63) >> 5;
-        mul[0] = scale == 0.0f ? 1.0f : fabsf(scale);
+        const int h = lane >> 5;
+        mul = scale == 0.0f ? 1.0f : fabsf(scale);
         const float sign = scale < 0.0f ? -1.0f : scale == 0.0f ? 0.0f : 1.0f;
 #pragma unroll
         for (int i = 0; i < NK; i++) q[i] = *(const styx_f4 *)(row + 8 * i + 4 * h) * sign;
     }
     __device__ __forceinline__ void scores(const char *kb)
     {
-        const int lane = threadIdx.x & 63, m = lane & 31, h = lane >> 5;
+        const int m = lane & 31, h = lane >> 5;
         const f16v zero = {};
         const int at = m * La::ROW + ((h ^ La::perm(m)) << 4);
         f16v c[2];  // two chains: a product follows the one before on its sum at once otherwise
+        constexpr int AHEAD = 2;
+        auto read = [&](int i) { return *(const styx_f4 *)(kb + (at ^ ((32 * i) & 255)) + ((32 * i) & ~255)); };
+        styx_f4 k[AHEAD];
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) k[i] = read(i);
+        in_order();
 #pragma unroll
         for (int i = 0; i < NK; i++) {
-            const styx_f4 k = *(const styx_f4 *)(kb + (at ^ ((32 * i) & 255)) + ((32 * i) & ~255));
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                c[e & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[i][e], i == 0 && e < 2 ? zero : c[e & 1], 0, 0, 0);
+                c[e & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[i % AHEAD][e], q[i][e], i == 0 && e < 2 ? zero : c[e & 1], 0, 0, 0);
+            if (i + AHEAD < NK) k[i % AHEAD] = read(i + AHEAD);
+            in_order();
         }
-        s[0][0] = c[0] + c[1];
+        s[0] = c[0] + c[1];
     }
-    __device__ __forceinline__ void factors(int) {}
-    __device__ __forceinline__ void values(const char *vb)
+    __device__ __forceinline__ float values(const char *vb, float ref)
     {
-        const int lane = threadIdx.x & 63, m = lane & 31, h = lane >> 5;
-#pragma unroll
-        for (int i = 0; i < 16; i++) {
-            const int t = 8 * (i >> 2) + 4 * h + (i & 3);
+        constexpr int N = 16 * ND, AHEAD = 8;
+        const int m = lane & 31, h = lane >> 5;
+        auto read = [&](int j) {
+            const int d = j % ND, i = j / ND, t = 8 * (i >> 2) + 4 * h + (i & 3);
             const int at = t * La::ROW + (((m >> 2) ^ La::perm(t)) << 4) + 4 * (m & 3);
+            return *(const float *)(vb + (at ^ ((128 * d) & 255)) + ((128 * d) & ~255));
+        };
+        float sum[2] = {}, p[2];
+        auto factor = [&](int i) {
+            p[i & 1] = exp2_(fmaf(s[0][i], mul, ref));
+            sum[i & 1] += p[i & 1];
+        };
+        float v[AHEAD];
 #pragma unroll
-            for (int d = 0; d < ND; d++) {
-                const float v = *(const float *)(vb + (at ^ ((128 * d) & 255)) + ((128 * d) & ~255));
-                o[0][d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[0][0][i], o[0][d], 0, 0, 0);
-            }
+        for (int j = 0; j < AHEAD; j++) v[j] = read(j);
+        factor(0);
+        in_order();
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const int d = j % ND, i = j / ND;
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[j % AHEAD], p[i & 1], o[d], 0, 0, 0);
+            if (j + AHEAD < N) v[j % AHEAD] = read(j + AHEAD);
+            if (d == 0 && i + 1 < 16) factor(i + 1);
+            in_order();
         }
+        return sum[0] + sum[1];
     }
 };
 
 // ------------------------------------------------------------- the split ---
-// Tiles of query rows in the order sequence, last tokens first; the slots of a
-// tile are cut into pieces of `share` blocks where the tiles alone are fewer
-// than the workgroups that run at once.
-struct Cut {
-    int share;      // blocks of a piece; 0: tiles are not cut
-    int64_t items;  // of all sequences, kv heads aside
-};
-struct SeqWork {
-    int tiles, pieces;
-};
-constexpr int AC_SLOTS_CU = 256;  // CUs
-constexpr int AC_LEAST = 4;       // blocks of a piece at least
+// The work of a kv head is a line: sequences one after another, of each its
+// tiles of query rows, of each tile its blocks.  Either a workgroup takes a
+// tile, the longest of a sequence first, or every workgroup takes an equal
+// share of the line, as many as run at once: a share ends inside a tile, whose
+// pieces are joined afterwards.  Both are known from the lengths alone, to every
+// workgroup by itself.
+constexpr int AC_CUS = 256;
+constexpr int AC_LEAST = 4;   // blocks of a share at least
+constexpr int AC_START = 16;  // what a share's starts, partial results and joining cost, in blocks
 
-template <int BM, int KT> __device__ __forceinline__ SeqWork seq_work(const AttnChunkArgs &a, const ChunkSeq &s, int share)
+// A sequence's part of the line: tile t is first + t step long, in slots times
+// rows of a token.
+struct SeqLine {
+    int tiles;
+    int64_t first, step;
+    __device__ __forceinline__ int64_t upto(int64_t t) const { return t * first + step * (t * (t - 1) / 2); }
+};
+template <int BM> __device__ __forceinline__ SeqLine seq_line(const AttnChunkArgs &a, const ChunkSeq &s)
 {
-    if (s.count == 0) return {0, 0};
-    const int64_t rows = (int64_t)s.count * a.gqa;
-    const int tiles = (int)((rows + BM - 1) / BM);
-    int blocks = (s.len + s.count + KT - 1) / KT;
-    if (a.window) blocks = min(blocks, (int)min((int64_t)1 << 30, ((int64_t)a.window + BM / a.gqa + 1) / KT + 2));
-    return {tiles, share ? (blocks + share - 1) / share : blocks};
+    if (s.count == 0) return {0, 0, 0};
+    const int tiles = (s.count * a.gqa + BM - 1) / BM;
+    const int64_t most = (int64_t)a.window * a.gqa + BM;
+    if (a.window && most < ((int64_t)s.len + s.count) * a.gqa) return {tiles, most, 0};
+    return {tiles, (int64_t)s.len * a.gqa + BM, BM};
 }
-
-template <int BM, int KT> __device__ __forceinline__ Cut cut_chunk(const AttnChunkArgs &a, int slots)
+struct Line {
+    int64_t share, total;  // share 0: by tiles
+};
+template <int BM, int KT> __device__ __forceinline__ Line line_of(const AttnChunkArgs &a, int slots)
 {
     const int lane = threadIdx.x & 63;
-    int64_t tiles = 0, work = 0;
+    int64_t tiles = 0, total = 0, longest = 0;
     for (int b0 = 0; b0 < a.kv.n_seq; b0 += 64) {
-        const SeqWork w = seq_work<BM, KT>(a, chunk_seq(a.chunk, a.kv, b0 + lane), 0);
+        const SeqLine w = seq_line<BM>(a, chunk_seq(a.chunk, a.kv, b0 + lane));
         tiles += w.tiles;
-        work += (int64_t)w.tiles * w.pieces;
+        total += w.upto(w.tiles);
+        longest = max(longest, w.tiles ? w.upto(w.tiles) - w.upto(w.tiles - 1) : (int64_t)0);
     }
-    tiles = wave_total(tiles) * a.kv.nkv;
-    work = wave_total(work) * a.kv.nkv;
-    if (4 * tiles > 3 * slots) return {0, tiles};
-    const int64_t room = slots - tiles;
-    return {(int)min((int64_t)1 << 30, max((int64_t)AC_LEAST, (work + room - 1) / room)), tiles};
+    tiles = uniform(wave_total(tiles));
+    total = uniform(wave_total(total));
+    longest = uniform(wave_most(longest));
+    if (tiles == 0) return {0, 0};
+    // What either costs: tiles that all run at once take as long as the longest,
+    // more of them leave half a tile's time unused at the end.
+    const int64_t unit = (int64_t)KT * a.gqa, even = total * a.kv.nkv / slots;
+    const int64_t by_tiles = tiles * a.kv.nkv <= slots ? longest : even + total / tiles / 2;
+    if (by_tiles <= even + even / 10 + AC_START * unit + BM) return {0, tiles};
+    const int64_t shares = max(slots / a.kv.nkv, 1);
+    return {max((total + shares - 1) / shares, AC_LEAST * unit), total};
 }
 
-// Item `item` of the batch (kv heads aside): sequence, tile, piece; b < 0: past
-// the last.
-struct Item {
-    int b, tile, tiles, piece, pieces;
-    int64_t first;  // pieces of the batch before this tile's
+// A tile and what of its length lies before `at`.  TILES: `at` counts tiles, the
+// last of each sequence first.  b < 0: past the end.
+struct Place {
+    int b, tile;
+    int64_t in, length, before;  // at - before = in, of length
     ChunkSeq s;
 };
-template <int BM, int KT> __device__ __forceinline__ Item find_item(const AttnChunkArgs &a, int share, int64_t item)
+template <int BM, bool TILES> __device__ __forceinline__ Place find_place(const AttnChunkArgs &a, int64_t at)
 {
     const int lane = threadIdx.x & 63;
     int64_t base = 0;
     for (int b0 = 0; b0 < a.kv.n_seq; b0 += 64) {
         const ChunkSeq s = chunk_seq(a.chunk, a.kv, b0 + lane);
-        SeqWork w = seq_work<BM, KT>(a, s, share);
-        if (!share) w.pieces = 1;
-        const int64_t mine = (int64_t)w.tiles * w.pieces, upto = base + wave_upto(mine);
-        if (const unsigned long long hit = __ballot(upto > item)) {
+        const SeqLine w = seq_line<BM>(a, s);
+        const int64_t mine = TILES ? w.tiles : w.upto(w.tiles), upto = base + wave_upto(mine);
+        if (const unsigned long long hit = __ballot(upto > at)) {
             const int l = __builtin_ctzll(hit);
-            const int tiles = __builtin_amdgcn_readlane(w.tiles, l), pieces = __builtin_amdgcn_readlane(w.pieces, l);
-            const int64_t before = of_lane(upto, l) - of_lane(mine, l);
-            const int in = (int)(item - before), tile = in / pieces;
-            return {b0 + l, tiles - 1 - tile, tiles, in - tile * pieces, pieces, before + (int64_t)tile * pieces,
+            const SeqLine o{(int)__builtin_amdgcn_readlane(w.tiles, l), of_lane(w.first, l), of_lane(w.step, l)};
+            const int64_t start = of_lane(upto, l) - of_lane(mine, l), in = at - start;
+            int tile = 0;
+            if (TILES)
+                tile = o.tiles - 1 - (int)in;
+            else
+                for (int n = o.tiles; n > 1;) {  // the last tile that begins at or before it
+                    const int half = n >> 1;
+                    const bool on = o.upto(tile + half) <= in;
+                    tile += on ? half : 0;
+                    n = on ? n - half : half;
+                }
+            const int64_t before = o.upto(tile);
+            return {b0 + l, tile, TILES ? 0 : in - before, o.upto(tile + 1) - before, start + before,
                     {(int)__builtin_amdgcn_readlane(s.first, l), (int)__builtin_amdgcn_readlane(s.count, l),
                      (int)__builtin_amdgcn_readlane(s.len, l)}};
         }
         base = of_lane(upto, 63);
     }
-    return {-1, 0, 0, 0, 0, 0, {0, 0, 0}};
+    return {-1, 0, 0, 0, 0, {0, 0, 0}};
 }
 
-// -------------------------------------------------------------- a piece ----
+// ------------------------------------------------------------- the tiles ---
+// Partial results, of a share's first piece and of its last: sums o, and m and l.
+struct Parts {
+    float *o;
+    float2 *ml;
+    int rows;  // of a piece
+};
+
 template <typename TQ, typename TC, int HD>
-__global__ void __launch_bounds__(AC_WG, (Wave<TQ, TC, HD>::PER_CU)) k_attn_chunk(AttnChunkArgs a, float *part_ml, float *part_o, int part_rows)
+__global__ void __launch_bounds__((64 * Wave<TQ, TC, HD>::NW), 2) k_attn_chunk(AttnChunkArgs a, Parts parts)
 {
     using W = Wave<TQ, TC, HD>;
     using La = Lay<TC, HD>;
-    constexpr int QT = W::QT, KT = W::KT, BM = 32 * QT * AC_WAVES, ND = W::ND;
-    constexpr int BLOCK = KT * La::ROW, PER_WAVE = KT / AC_WAVES, NI = PER_WAVE / La::RPI;
+    constexpr int KT = W::KT, DS = W::DS, HW = W::HW, BM = W::BM, ND = W::ND;
+    constexpr int NW = W::NW, WG = 64 * NW, BLOCK = KT * La::ROW, PER_WAVE = KT / NW, NI = PER_WAVE / La::RPI;
+    static_assert(PER_WAVE % La::RPI == 0, "whole loads");
     __shared__ __align__(1024) char s_k[2][BLOCK];
     __shared__ __align__(1024) char s_v[2][BLOCK];
+    // scores of half the dims; in the block of K where there is no other place
+    constexpr int PIECES = KT / 32 * 4;
+    constexpr bool APART = 4 * BLOCK + NW * PIECES * 1024 < 150000;
+    __shared__ styx_f4 s_half[DS == 2 && APART ? NW * PIECES : 1][64];
     const KvView &kv = a.kv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
-    const Cut sp = cut_chunk<BM, KT>(a, AC_SLOTS_CU * W::PER_CU);
-    const int kvh = blockIdx.x % kv.nkv;
-    const Item it = find_item<BM, KT>(a, sp.share, blockIdx.x / kv.nkv);
-    if (it.b < 0) return;
-    const ChunkSeq &s = it.s;
-    const int64_t rows = (int64_t)s.count * a.gqa, row0 = (int64_t)it.tile * BM;
-    // tokens of the tile, the slots that any of them sees, the piece's blocks
-    const int tok0 = (int)(row0 / a.gqa), tok1 = (int)(min(row0 + BM, rows) - 1) / a.gqa;
-    const int t1 = s.len + tok1 + 1, t0 = a.window && s.len + tok0 >= a.window ? s.len + tok0 - a.window + 1 : 0;
-    int b0 = t0 / KT, b1 = (t1 + KT - 1) / KT;
-    if (sp.share) {
-        b0 += min((int64_t)it.piece * sp.share, (int64_t)(b1 - b0));
-        b1 = (int)min((int64_t)b1, (int64_t)b0 + sp.share);
-    }
-    const int32_t *tab = kv.table + (int64_t)it.b * kv.table_len;
+    const int dw = wave % DS * HW;  // the wave's first dim
+    const Line line = line_of<BM, KT>(a, AC_CUS * W::PER_CU);
+    const int kvh = blockIdx.x % kv.nkv, nth = blockIdx.x / kv.nkv;
+    int64_t u = nth * line.share;
+    const int64_t end = min(u + line.share, line.total);
     const int64_t stride = (int64_t)kv.nkv * La::ROW;
     const char *kp = (const char *)kv.kpool + kvh * La::ROW, *vp = (const char *)kv.vpool + kvh * La::ROW;
-
-    // this lane's queries
-    W x;
-    int at[QT];                // last slot seen, -1: no such row
-    int64_t orow[QT];          // row of q and out
-    int head[QT];
-    float m[QT], l[QT];
-    uint32_t nan_at[QT][HD / 64];  // dims that are NaN whatever the sums are
-    const int wrow0 = 32 * QT * wave;
-    const bool works = row0 + wrow0 < rows;
-#pragma unroll
-    for (int qt = 0; qt < QT; qt++) {
-        const int64_t r = row0 + wrow0 + 32 * qt + n, rr = min(r, rows - 1);
-        const int tok = (int)(rr / a.gqa);
-        head[qt] = kvh * a.gqa + (int)(rr - (int64_t)tok * a.gqa);
-        orow[qt] = s.first + tok;
-        at[qt] = r < rows ? s.len + tok : -1;
-        m[qt] = -INFINITY;
-        l[qt] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < HD / 64; w++) nan_at[qt][w] = 0;
-        x.init(qt, (const TQ *)a.q + orow[qt] * a.ldq + (int64_t)head[qt] * HD, a.scale);
-#pragma unroll
-        for (int d = 0; d < ND; d++) x.o[qt][d] = f16v{};
+    const uint32_t lk = lds_at(&s_k[0][0]), lv = lds_at(&s_v[0][0]);
+    for (bool more = true; more;) {
+    // (a lane number that the compiler takes for a new one in every trip: what
+    // is computed from it would else be kept in registers over the trips)
+    int lane = threadIdx.x & 63;
+    asm volatile("" : "+v"(lane));
+    const int n = lane & 31, h = lane >> 5;
+    const Place it = line.share ? find_place<BM, false>(a, u) : find_place<BM, true>(a, nth);
+    if (it.b < 0 || (line.share && u >= end)) return;
+    const ChunkSeq &s = it.s;
+    const int rows = s.count * a.gqa, row0 = it.tile * BM;
+    // tokens of the tile, the slots that any of them sees, the piece's blocks
+    const int tok0 = a.by_gqa.of(row0), tok1 = a.by_gqa.of(min(row0 + BM, rows) - 1);
+    const int t1 = s.len + tok1 + 1, t0 = a.window && s.len + tok0 >= a.window ? s.len + tok0 - a.window + 1 : 0;
+    int b0 = t0 / KT, b1 = (t1 + KT - 1) / KT;
+    bool whole = true;
+    // a piece that is not whole is its share's first, or its last, which goes on
+    // in the next share's first
+    const int64_t part = (2 * (int64_t)nth + (it.in == 0 && u > nth * line.share)) * kv.nkv + kvh;
+    more = false;
+    if (line.share) {
+        const int64_t to = min(it.in + (end - u), it.length);
+        whole = it.in == 0 && to == it.length;
+        if (!whole) {
+            const int64_t nb = b1 - b0;
+            b1 = b0 + (int)((uint64_t)(to * nb) / (uint64_t)it.length);
+            b0 += (int)((uint64_t)(it.in * nb) / (uint64_t)it.length);
+        }
+        u += to - it.in;
+        more = u < end;
     }
+    b0 = uniform(b0);
+    b1 = uniform(b1);
+    const int32_t *tab = kv.table + (int64_t)it.b * kv.table_len;
+
+    // this lane's query
+    W x;
+    x.lane = lane;
+    const int wrow0 = row0 + 32 * (wave / DS);
+    const bool works = wrow0 < rows;
+    const int r = min(wrow0 + n, rows - 1), tok = a.by_gqa.of(r), head = kvh * a.gqa + (r - tok * a.gqa);
+    const int at = wrow0 + n < rows ? s.len + tok : -1;  // last slot seen, -1: no such row
+    const int64_t orow = s.first + tok;                  // row of q and out
+    float m = -INFINITY, l = 0.0f;
+    uint32_t nan_at[HW / 64];  // dims that are NaN whatever the sums are
+#pragma unroll
+    for (int w = 0; w < HW / 64; w++) nan_at[w] = 0;
+    x.init((const TQ *)a.q + orow * a.ldq + (int64_t)head * HD + dw, dw, a.scale);
+#pragma unroll
+    for (int d = 0; d < ND; d++) x.o[d] = f16v{};
     // slots that all of the wave's queries see, and those that none sees
-    const int wtok0 = (int)(min(row0 + wrow0, rows - 1) / a.gqa), wtok1 = (int)(min(row0 + wrow0 + 32 * QT, rows) - 1) / a.gqa;
+    const int wtok0 = a.by_gqa.of(min(wrow0, rows - 1)), wtok1 = a.by_gqa.of(min(wrow0 + 32, rows) - 1);
     const int all_hi = s.len + wtok0, any_hi = s.len + wtok1;
     const int all_lo = a.window ? s.len + wtok1 - a.window + 1 : 0, any_lo = a.window ? s.len + wtok0 - a.window + 1 : 0;
 
@@ -378,16 +490,34 @@ __global__ void __launch_bounds__(AC_WG, (Wave<TQ, TC, HD>::PER_CU)) k_attn_chun
     const int my = lane & (KT - 1);
     auto entry_of = [&](int blk) { return kv.entry(tab, min(blk * KT + my, t1 - 1)); };
     auto row_of = [&](int e, int blk) { return blk * KT + my < t1 ? kv.row_of(e, min(blk * KT + my, t1 - 1)) : -1; };
-    const uint32_t lk = lds_at(&s_k[0][0]), lv = lds_at(&s_v[0][0]);
-    auto fetch = [&](int buf, int row) {
+    // where a lane's 16 bytes of a load come from, of the first of the wave's rows
+    uint32_t from[NI];
 #pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const int t = wave * PER_WAVE + i * La::RPI + lane / La::LPR;
-            const int64_t r = max(__shfl(row, t), 0);
-            const int c = (lane & (La::LPR - 1)) ^ La::perm(t);
-            const int to = (wave * PER_WAVE + i * La::RPI) * La::ROW;
-            to_lds(kp + r * stride + 16 * c, __builtin_amdgcn_readfirstlane(lk + buf * BLOCK + to));
-            to_lds(vp + r * stride + 16 * c, __builtin_amdgcn_readfirstlane(lv + buf * BLOCK + to));
+    for (int i = 0; i < NI; i++) {
+        const int t = i * La::RPI + lane / La::LPR;
+        from[i] = t * (uint32_t)stride + 16 * ((lane & (La::LPR - 1)) ^ La::perm(wave * PER_WAVE + t));
+    }
+    auto fetch = [&](int buf, int row) {
+        const uint32_t to = buf * BLOCK + wave * PER_WAVE * La::ROW;
+        if (a.runs) {  // a wave's rows lie one after another
+            const int64_t off = (int64_t)max((int)__builtin_amdgcn_readlane(row, wave * PER_WAVE), 0) * stride;
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                to_lds(kp + off, from[i], lk + to + i * 1024);
+                to_lds(vp + off, from[i], lv + to + i * 1024);
+            }
+        } else {
+            int64_t off[NI];
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                const int t = wave * PER_WAVE + i * La::RPI + lane / La::LPR;
+                off[i] = max(__shfl(row, t), 0) * stride + 16 * ((lane & (La::LPR - 1)) ^ La::perm(t));
+            }
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                to_lds(kp + off[i], lk + to + i * 1024);
+                to_lds(vp + off[i], lv + to + i * 1024);
+            }
         }
     };
     unsigned long long there = 0;  // slots of the block under way whose page is there
@@ -412,28 +542,25 @@ __global__ void __launch_bounds__(AC_WG, (Wave<TQ, TC, HD>::PER_CU)) k_attn_chun
         }
         const int tb = blk * KT;
         const char *kb = s_k[buf], *vb = s_v[buf];
+        // the slots of the block that this lane's query sees
+        uint32_t vis[KT / 32];
         // (uniform over the workgroup: whether every query of the tile sees the block)
-        const bool plain = seen == full && tb + KT - 1 <= s.len + tok0 && (!a.window || tb > s.len + tok1 - a.window);
-        // the slots of the block that each query sees
-        uint32_t vis[QT][KT / 32];
-        if (!plain) {
+        if (seen != full || tb + KT - 1 > s.len + tok0 || (a.window && tb <= s.len + tok1 - a.window)) {
 #pragma unroll
-            for (int kt = 0; kt < KT / 32; kt++)
-#pragma unroll
-                for (int qt = 0; qt < QT; qt++) {
-                    const int last = at[qt] - (tb + 32 * kt), before = a.window ? last - a.window : -1;
-                    uint32_t v = (uint32_t)(seen >> (32 * kt));
-                    v &= last < 0 ? 0u : last > 30 ? ~0u : (2u << last) - 1u;
-                    v &= before < 0 ? ~0u : before > 30 ? 0u : ~0u << (before + 1);
-                    vis[qt][kt] = v;
-                }
+            for (int kt = 0; kt < KT / 32; kt++) {
+                const int last = at - (tb + 32 * kt), before = a.window ? last - a.window : -1;
+                uint32_t v = (uint32_t)(seen >> (32 * kt));
+                v &= last < 0 ? 0u : last > 30 ? ~0u : (2u << last) - 1u;
+                v &= before < 0 ? ~0u : before > 30 ? 0u : ~0u << (before + 1);
+                vis[kt] = v;
+            }
             // A value that is not finite must not reach those that do not see
             // it, whose factor is 0: where there is one, the dims of those that
             // do see it are noted to be NaN, and the value becomes 0.
-            char *mine = s_v[buf] + threadIdx.x * (BLOCK / AC_WG);
+            char *mine = s_v[buf] + (64 * wave + lane) * (BLOCK / WG);
             bool odd = false;
 #pragma unroll
-            for (int i = 0; i < BLOCK / AC_WG; i += 16) {
+            for (int i = 0; i < BLOCK / WG; i += 16) {
                 const styx_u4 v = *(const styx_u4 *)(mine + i);
 #pragma unroll
                 for (int e = 0; e < 4; e++) odd |= not_finite<TC>(v[e]) != 0;
@@ -441,213 +568,234 @@ __global__ void __launch_bounds__(AC_WG, (Wave<TQ, TC, HD>::PER_CU)) k_attn_chun
             if (__syncthreads_or(odd)) {
 #pragma unroll 1
                 for (int t = 0; t < KT; t++) {
-                    uint32_t see[QT];
-#pragma unroll
-                    for (int qt = 0; qt < QT; qt++) see[qt] = 0u - (vis[qt][KT == 64 ? t >> 5 : 0] >> (t & 31) & 1);
+                    const uint32_t see = 0u - (vis[KT == 64 ? t >> 5 : 0] >> (t & 31) & 1);
                     // bits 4 j + e: dims 8 j + 4 h + e
 #pragma unroll 1
-                    for (int j = 0; j < HD / 8; j++) {
-                        const TC *v = (const TC *)(vb + La::at(t, 8 * j + 4 * h));
+                    for (int j = 0; j < HW / 8; j++) {
+                        const TC *v = (const TC *)(vb + La::at(t, dw + 8 * j + 4 * h));
                         uint32_t bad = 0;
 #pragma unroll
                         for (int e = 0; e < 4; e++) bad |= (uint32_t) !(fabsf((float)v[e]) < INFINITY) << e;
                         if (bad)
 #pragma unroll
-                            for (int w = 0; w < HD / 64; w++)
-#pragma unroll
-                                for (int qt = 0; qt < QT; qt++)
-                                    nan_at[qt][w] |= w == j >> 3 ? (bad & see[qt]) << (4 * (j & 7)) : 0;
+                            for (int w = 0; w < HW / 64; w++) nan_at[w] |= w == j >> 3 ? (bad & see) << (4 * (j & 7)) : 0;
                     }
                 }
                 __syncthreads();
-                for (int i = 0; i < BLOCK / AC_WG; i += 4) {
+                for (int i = 0; i < BLOCK / WG; i += 4) {
                     uint32_t *v = (uint32_t *)(mine + i);
                     *v &= ~not_finite<TC>(*v);
                 }
                 __syncthreads();
             }
         }
-        if (!works || tb > any_hi || tb + KT <= any_lo) continue;
-        x.scores(kb);
+        const bool idle = !works || tb > any_hi || tb + KT <= any_lo;
+        if constexpr (DS == 1) {
+            if (idle) continue;
+            x.scores(kb);
+        } else {
+            // each wave of a pair has half the dims: both add the halves up
+            styx_f4 (*half)[64] = APART ? s_half : (styx_f4(*)[64])s_k[buf];
+            if (!idle) x.scores(kb + dw * (int)sizeof(TC));
+            if constexpr (!APART) {
+                static_assert(NW * PIECES * 1024 <= BLOCK, "scores in the place of K");
+                __syncthreads();
+            }
+            if (!idle)
+#pragma unroll
+                for (int i = 0; i < PIECES; i++) {
+                    const f16v &y = x.s[i / 4];
+                    half[wave * PIECES + i][lane] = styx_f4{y[4 * (i & 3)], y[4 * (i & 3) + 1], y[4 * (i & 3) + 2], y[4 * (i & 3) + 3]};
+                }
+            __syncthreads();
+            if (idle) continue;
+#pragma unroll
+            for (int i = 0; i < PIECES; i++) {
+                const styx_f4 y = half[(wave ^ 1) * PIECES + i][lane];
+#pragma unroll
+                for (int e = 0; e < 4; e++) x.s[i / 4][4 * (i & 3) + e] += y[e];
+            }
+        }
         if (seen != full || tb + KT - 1 > all_hi || tb < all_lo) {
 #pragma unroll
-            for (int kt = 0; kt < KT / 32; kt++)
+            for (int kt = 0; kt < KT / 32; kt++) {
+                const uint32_t mine = vis[kt] >> (4 * h);
 #pragma unroll
-                for (int qt = 0; qt < QT; qt++) {
-                    const uint32_t mine = vis[qt][kt] >> (4 * h);
-#pragma unroll
-                    for (int i = 0; i < 16; i++)
-                        if (!(mine >> (8 * (i >> 2) + (i & 3)) & 1)) x.s[kt][qt][i] = -INFINITY;
-                }
-        }
-#pragma unroll
-        for (int qt = 0; qt < QT; qt++) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int kt = 0; kt < KT / 32; kt++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) mx = fmaxf(mx, x.s[kt][qt][i]);
-            mx = fmaxf(mx, other_half(mx)) * x.mul[qt];
-            if (__ballot(mx > m[qt] + AC_LAG)) {
-                const float mn = fmaxf(m[qt], mx), corr = mn == -INFINITY ? 1.0f : exp2_(m[qt] - mn);
-                m[qt] = mn;
-                l[qt] *= corr;
-#pragma unroll
-                for (int d = 0; d < ND; d++) x.o[qt][d] *= corr;
+                for (int i = 0; i < 16; i++)
+                    if (!(mine >> (8 * (i >> 2) + (i & 3)) & 1)) x.s[kt][i] = -INFINITY;
             }
-            const float ref = (m[qt] == -INFINITY ? 0.0f : m[qt]) - AC_OFF;
-            float sum[4] = {};
-#pragma unroll
-            for (int kt = 0; kt < KT / 32; kt++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float v = exp2_(fmaf(x.s[kt][qt][i], x.mul[qt], -ref));
-                    x.s[kt][qt][i] = v;
-                    sum[i & 3] += v;
-                }
-            l[qt] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            x.factors(qt);
         }
-        x.values(vb);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < KT / 32; kt++)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(mx, x.s[kt][i]), x.s[kt][i + 1]);
+        mx = fmaxf(mx, other_half(mx)) * x.mul;
+        if (__ballot(mx > m + AC_LAG)) {
+            const float mn = fmaxf(m, mx), corr = mn == -INFINITY ? 1.0f : exp2_(m - mn);
+            m = mn;
+            l *= corr;
+#pragma unroll
+            for (int d = 0; d < ND; d++) x.o[d] *= corr;
+        }
+        const float ref = AC_OFF - (m == -INFINITY ? 0.0f : m);
+        l += x.values(vb + dw * (int)sizeof(TC), ref);
     }
-    if (!works) return;
+    if (more) __syncthreads();  // (the next piece's blocks take the place of this one's)
+    if (at < 0) continue;
+    l += other_half(l);
 #pragma unroll
-    for (int qt = 0; qt < QT; qt++) {
-        if (at[qt] < 0) continue;
-        l[qt] += other_half(l[qt]);
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (nan_at[d / 2] >> (16 * (d & 1) + i) & 1) x.o[d][i] = NAN;
+    if (!whole) {
+        const int64_t p = part * parts.rows + (wrow0 - row0) + n;
+        if (h == 0 && dw == 0) parts.ml[p] = float2{m, l};
 #pragma unroll
         for (int d = 0; d < ND; d++)
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (nan_at[qt][d / 2] >> (16 * (d & 1) + i) & 1) x.o[qt][d][i] = NAN;
-        if (sp.share) {
-            // a partial result: M, L and the sums
-            const int64_t p = ((it.first + it.piece) * kv.nkv + kvh) * part_rows + wrow0 + 32 * qt + n;
-            if (h == 0) {
-                part_ml[2 * p] = m[qt];
-                part_ml[2 * p + 1] = l[qt];
+            for (int i = 0; i < 16; i += 4)
+                *(styx_f4 *)(parts.o + p * HD + dw + 32 * d + 2 * i + 4 * h) =
+                    styx_f4{x.o[d][i], x.o[d][i + 1], x.o[d][i + 2], x.o[d][i + 3]};
+        continue;
+    }
+    // no slot with a weight (m = -inf): 0, or NaN
+    const bool none = m == -INFINITY;
+    const float f = none ? 1.0f : 1.0f / l, add = none ? l : 0.0f;
+    TQ *out = (TQ *)a.out + orow * a.ldo + (int64_t)head * HD + dw;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            TQ *dst = out + 32 * d + 2 * i + 4 * h;
+            if constexpr (sizeof(TQ) == 2) {
+                h4 v;
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = (_Float16)(x.o[d][i + e] * f + add);
+                *(h4 *)dst = v;
+            } else {
+                styx_f4 v;
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = x.o[d][i + e] * f + add;
+                *(styx_f4 *)dst = v;
             }
-#pragma unroll
-            for (int d = 0; d < ND; d++)
-#pragma unroll
-                for (int i = 0; i < 16; i += 4)
-                    *(styx_f4 *)(part_o + p * HD + 32 * d + 2 * i + 4 * h) =
-                        styx_f4{x.o[qt][d][i], x.o[qt][d][i + 1], x.o[qt][d][i + 2], x.o[qt][d][i + 3]};
-            continue;
         }
-        // no slot with a weight (m = -inf): 0, or NaN
-        const bool none = m[qt] == -INFINITY;
-        const float r = none ? 1.0f : 1.0f / l[qt], add = none ? l[qt] : 0.0f;
-        TQ *out = (TQ *)a.out + orow[qt] * a.ldo + (int64_t)head[qt] * HD;
-#pragma unroll
-        for (int d = 0; d < ND; d++)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                TQ *dst = out + 32 * d + 2 * i + 4 * h;
-                if constexpr (sizeof(TQ) == 2) {
-                    h4 v;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = (_Float16)(x.o[qt][d][i + e] * r + add);
-                    *(h4 *)dst = v;
-                } else {
-                    styx_f4 v;
-#pragma unroll
-                    for (int e = 0; e < 4; e++) v[e] = x.o[qt][d][i + e] * r + add;
-                    *(styx_f4 *)dst = v;
-                }
-            }
-        if (a.lse && h == 0)
-            a.lse[orow[qt] * a.nh + head[qt]] =
-                none ? (l[qt] == 0.0f ? -INFINITY : l[qt]) : (m[qt] - AC_OFF + __builtin_amdgcn_logf(l[qt])) * 0.69314718056f;
+    if (a.lse && h == 0 && dw == 0)
+        a.lse[orow * a.nh + head] = none ? (l == 0.0f ? -INFINITY : l) : (m - AC_OFF + __builtin_amdgcn_logf(l)) * 0.69314718056f;
     }
 }
 
-// The pieces of a tile joined: a workgroup for 16 of its rows, where the split
-// cut tiles at all; a wave goes through 4 rows, its lanes through the dims.
-template <typename TQ, typename TC, int HD>
-__global__ void __launch_bounds__(AC_WG) k_attn_chunk_join(AttnChunkArgs a, const float *part_ml, const float *part_o, int part_rows)
+// The pieces of a tile that lies across an end of a share joined, by those of
+// the first such end: ROWS rows a workgroup, four dims a thread, threads beyond
+// the rows taking every other piece.
+constexpr int AC_JOIN = 256;
+template <typename TQ, typename TC, int HD, int ROWS>
+__global__ void __launch_bounds__(AC_JOIN) k_attn_chunk_join(AttnChunkArgs a, Parts parts)
 {
     using W = Wave<TQ, TC, HD>;
-    constexpr int KT = W::KT, BM = 32 * W::QT * AC_WAVES, DPL = HD / 64, PARTS = BM / 16, AHEAD = 4;
+    constexpr int KT = W::KT, BM = W::BM, PER_ROW = HD / 4, GROUPS = AC_JOIN / PER_ROW / ROWS, AHEAD = 4;
+    static_assert(GROUPS >= 1, "threads for the rows");
+    __shared__ styx_f4 s_o[AC_JOIN];
+    __shared__ float2 s_ml[AC_JOIN];
     const KvView &kv = a.kv;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const Cut sp = cut_chunk<BM, KT>(a, AC_SLOTS_CU * W::PER_CU);
-    if (!sp.share) return;
-    const int kvh = blockIdx.x / PARTS % kv.nkv, part = blockIdx.x % PARTS;
-    const int64_t nth = blockIdx.x / PARTS / kv.nkv;  // tile of the batch
-    if (nth * kv.nkv >= sp.items) return;
-    // the tile: found among tiles of one piece, then counted in pieces
-    Item it = find_item<BM, KT>(a, 0, nth);
-    if (it.b < 0) return;
-    const SeqWork w = seq_work<BM, KT>(a, it.s, sp.share);
-    int64_t before = 0;
-    for (int b0 = 0; b0 <= it.b; b0 += 64) {
-        const SeqWork y = seq_work<BM, KT>(a, chunk_seq(a.chunk, kv, b0 + lane), sp.share);
-        before += wave_total(b0 + lane < it.b ? (int64_t)y.tiles * y.pieces : (int64_t)0);
-    }
-    const int64_t first = before + (int64_t)(w.tiles - 1 - it.tile) * w.pieces;
-    const int64_t rows = (int64_t)it.s.count * a.gqa;
-    for (int i = 0; i < 4; i++) {
-        const int in = 16 * part + 4 * wave + i;
-        const int64_t r = (int64_t)it.tile * BM + in;
-        if (r >= rows) return;
-        float m = -INFINITY, l = 0.0f, o[DPL] = {};
-        for (int c0 = 0; c0 < w.pieces; c0 += AHEAD) {
-            float pm[AHEAD], pl[AHEAD], po[AHEAD][DPL], mn = m;
+    const Line line = line_of<BM, KT>(a, AC_CUS * W::PER_CU);
+    const int w0 = blockIdx.z, kvh = blockIdx.y;
+    const int64_t u = (w0 + 1) * line.share;
+    if (!line.share || u >= line.total) return;
+    const Place it = find_place<BM, false>(a, u);
+    if (it.b < 0 || it.in == 0 || it.before < w0 * line.share) return;
+    const int pieces = (int)((it.before + it.length - 1) / line.share - w0) + 1;
+    // the first piece is its share's last unless the share begins with it
+    const int64_t part0 = 2 * (int64_t)w0 + (it.before > w0 * line.share);
+    const int tid = threadIdx.x, d = tid % PER_ROW * 4, in = blockIdx.x * ROWS + tid / PER_ROW % ROWS, group = tid / PER_ROW / ROWS;
+    const int r = it.tile * BM + in;
+    const bool is = in < parts.rows && r < it.s.count * a.gqa;
+    if (blockIdx.x * ROWS >= parts.rows || it.tile * BM + (int)blockIdx.x * ROWS >= it.s.count * a.gqa) return;
+    float m = -INFINITY, l = 0.0f;
+    styx_f4 o = {};
+    for (int c0 = group; c0 < pieces; c0 += GROUPS * AHEAD) {
+        float2 ml[AHEAD];
+        styx_f4 po[AHEAD];
+        float mn = m;
 #pragma unroll
-            for (int c = 0; c < AHEAD; c++) {
-                const int64_t p = ((first + min(c0 + c, w.pieces - 1)) * kv.nkv + kvh) * part_rows + in;
-                pm[c] = part_ml[2 * p];
-                pl[c] = part_ml[2 * p + 1];
-#pragma unroll
-                for (int d = 0; d < DPL; d++) po[c][d] = part_o[p * HD + lane + 64 * d];
-            }
-#pragma unroll
-            for (int c = 0; c < AHEAD; c++) {
-                if (c0 + c >= w.pieces) pm[c] = -INFINITY, pl[c] = 0.0f;
-                mn = fmaxf(mn, pm[c]);
-            }
-            const float f = m == -INFINITY ? 0.0f : exp2_(m - mn);
-            l *= f;
-#pragma unroll
-            for (int d = 0; d < DPL; d++) o[d] *= f;
-#pragma unroll
-            for (int c = 0; c < AHEAD; c++) {
-                // a piece without a slot that counts has sums of 0, or of NaN
-                const float g = pm[c] == -INFINITY ? (pl[c] == 0.0f ? 0.0f : 1.0f) : exp2_(pm[c] - mn);
-                l += pl[c] * g;
-                if (c0 + c < w.pieces) {
-#pragma unroll
-                    for (int d = 0; d < DPL; d++) o[d] += po[c][d] * g;
-                }
-            }
-            m = mn;
+        for (int c = 0; c < AHEAD; c++) {
+            const int cc = min(c0 + c * GROUPS, pieces - 1);
+            const int64_t p = ((cc ? 2 * (int64_t)(w0 + cc) : part0) * kv.nkv + kvh) * parts.rows + (is ? in : 0);
+            ml[c] = parts.ml[p];
+            po[c] = *(const styx_f4 *)(parts.o + p * HD + d);
         }
-        const int tok = (int)(r / a.gqa), head = kvh * a.gqa + (int)(r - (int64_t)tok * a.gqa);
-        const int64_t row = it.s.first + tok;
-        const bool none = m == -INFINITY;
 #pragma unroll
-        for (int d = 0; d < DPL; d++)
-            ((TQ *)a.out)[row * a.ldo + (int64_t)head * HD + lane + 64 * d] = (TQ)(none ? o[d] + l : o[d] / l);
-        if (a.lse && lane == 0)
-            a.lse[row * a.nh + head] =
-                none ? (l == 0.0f ? -INFINITY : l) : (m - AC_OFF + __builtin_amdgcn_logf(l)) * 0.69314718056f;
+        for (int c = 0; c < AHEAD; c++) {
+            if (c0 + c * GROUPS >= pieces) {
+                ml[c] = float2{-INFINITY, 0.0f};
+                po[c] = styx_f4{};
+            }
+            mn = fmaxf(mn, ml[c].x);
+        }
+        const float f = m == -INFINITY ? 1.0f : exp2_(m - mn);
+        l *= f;
+        o *= f;
+#pragma unroll
+        for (int c = 0; c < AHEAD; c++) {
+            // a piece without a slot that counts has sums of 0, or of NaN
+            const float g = ml[c].x == -INFINITY ? 1.0f : exp2_(ml[c].x - mn);
+            l += ml[c].y * g;
+            o += po[c] * g;
+        }
+        m = mn;
     }
+    if constexpr (GROUPS > 1) {
+        s_o[tid] = o;
+        s_ml[tid] = float2{m, l};
+        __syncthreads();
+        if (group) return;
+        float mn = m;
+#pragma unroll
+        for (int c = 1; c < GROUPS; c++) mn = fmaxf(mn, s_ml[tid + c * ROWS * PER_ROW].x);
+        const float f = m == -INFINITY ? 1.0f : exp2_(m - mn);
+        l *= f;
+        o *= f;
+#pragma unroll
+        for (int c = 1; c < GROUPS; c++) {
+            const float2 y = s_ml[tid + c * ROWS * PER_ROW];
+            const float g = y.x == -INFINITY ? 1.0f : exp2_(y.x - mn);
+            l += y.y * g;
+            o += s_o[tid + c * ROWS * PER_ROW] * g;
+        }
+        m = mn;
+    }
+    if (!is) return;
+    const int tok = a.by_gqa.of(r), head = kvh * a.gqa + (r - tok * a.gqa);
+    const int64_t row = it.s.first + tok;
+    const bool none = m == -INFINITY;
+    const float f = none ? 1.0f : 1.0f / l, add = none ? l : 0.0f;
+    TQ *dst = (TQ *)a.out + row * a.ldo + (int64_t)head * HD + d;
+    if constexpr (sizeof(TQ) == 2) {
+        h4 v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = (_Float16)(o[e] * f + add);
+        *(h4 *)dst = v;
+    } else {
+        *(styx_f4 *)dst = o * f + add;
+    }
+    if (a.lse && d == 0) a.lse[row * a.nh + head] = none ? (l == 0.0f ? -INFINITY : l) : (m - AC_OFF + __builtin_amdgcn_logf(l)) * 0.69314718056f;
 }
 
 // ----------------------------------------------------------------- launch ---
 struct ChunkShape {
-    int bm, slots;
-    int64_t tiles, items;  // at most
+    int64_t tiles;  // at most
+    int shares;     // of a kv head, at most
+    int rows;       // of a piece's partial results
+    int64_t parts(int nkv) const { return 2 * (int64_t)shares * nkv * rows; }
 };
 static ChunkShape shape_of(int bm, int per_cu, int n_seq, int nkv, int gqa, int n_rows)
 {
-    ChunkShape s{bm, AC_SLOTS_CU * per_cu, 0, 0};
+    ChunkShape s{};
     // (a sequence has at least a row, and its last tile may be partly filled)
-    const int64_t seqs = std::min(n_seq, n_rows);
-    s.tiles = (((int64_t)n_rows * gqa + bm - 1) / bm + seqs) * nkv;
-    // tiles that are cut are at most 3/4 of the slots, and make at most `slots` pieces
-    s.items = std::max(s.tiles, (int64_t)s.slots);
+    s.tiles = (((int64_t)n_rows * gqa + bm - 1) / bm + std::min(n_seq, n_rows)) * nkv;
+    s.shares = std::max(AC_CUS * per_cu / nkv, 1);
+    s.rows = (int)std::min<int64_t>(bm, (int64_t)n_rows * gqa);
     return s;
 }
 template <typename F> static auto with_kernel(bool f16, bool q16, int hd, F f)
@@ -662,15 +810,11 @@ template <typename F> static auto with_kernel(bool f16, bool q16, int hd, F f)
     if (!f16) return by_hd(float{}, float{});
     return q16 ? by_hd(_Float16{}, _Float16{}) : by_hd(float{}, _Float16{});
 }
+// (times 8, so that rows times gqa stay below 2^28)
 int64_t attn_chunk_grid(int n_seq, int nkv, int gqa, int n_rows)
 {
-    return shape_of(128, 2, n_seq, nkv, gqa, n_rows).items;
-}
-// Rows of a piece's partial results, and floats of all pieces'.
-static int part_rows(const ChunkShape &s, int gqa, int n_rows) { return (int)std::min<int64_t>(s.bm, (int64_t)n_rows * gqa); }
-static int64_t part_floats(const ChunkShape &s, int gqa, int n_rows, int hd)
-{
-    return (int64_t)s.slots * part_rows(s, gqa, n_rows) * (hd + 2);
+    const ChunkShape s = shape_of(128, 2, n_seq, nkv, gqa, n_rows);
+    return std::max<int64_t>(s.tiles, (int64_t)s.shares * nkv) * 8;
 }
 uint64_t attn_chunk_ws_bytes(int n_seq, int nkv, int hd, int gqa, int n_rows)
 {
@@ -679,8 +823,8 @@ uint64_t attn_chunk_ws_bytes(int n_seq, int nkv, int hd, int gqa, int n_rows)
     for (int t = 0; t < 3; t++)
         with_kernel(t > 0, t > 1, hd, [&](auto tq, auto tc, auto n) {
             using W = Wave<decltype(tq), decltype(tc), decltype(n)::value>;
-            const ChunkShape s = shape_of(32 * W::QT * AC_WAVES, W::PER_CU, n_seq, nkv, gqa, n_rows);
-            floats = std::max(floats, part_floats(s, gqa, n_rows, hd));
+            static_assert(W::BM >= 128 && W::PER_CU <= 2, "attn_chunk_grid");
+            floats = std::max(floats, shape_of(W::BM, W::PER_CU, n_seq, nkv, gqa, n_rows).parts(nkv) * (hd + 2));
             return 0;
         });
     return 4ull * floats;
@@ -689,17 +833,29 @@ uint64_t attn_chunk_ws_bytes(int n_seq, int nkv, int hd, int gqa, int n_rows)
 hipError_t launch_attn_chunk(hipStream_t st, AttnChunkArgs a, void *ws)
 {
     a.scale = (float)((double)a.scale * 1.4426950408889634);  // log2 e
+    a.by_gqa = page_div((uint32_t)a.gqa);
     with_kernel(a.kv.f16, a.q_f16, a.kv.hd, [&](auto tq, auto tc, auto hd) {
         using TQ = decltype(tq);
         using TC = decltype(tc);
         constexpr int HD = decltype(hd)::value;
         using W = Wave<TQ, TC, HD>;
-        const ChunkShape s = shape_of(32 * W::QT * AC_WAVES, W::PER_CU, a.kv.n_seq, a.kv.nkv, a.gqa, a.chunk.n_rows);
-        const int pr = part_rows(s, a.gqa, a.chunk.n_rows);
-        float *o = (float *)ws, *ml = o + (int64_t)s.slots * pr * HD;
-        hipLaunchKernelGGL((k_attn_chunk<TQ, TC, HD>), dim3((unsigned)s.items), dim3(AC_WG), 0, st, a, ml, o, pr);
-        const int64_t joins = std::min(s.tiles, (int64_t)s.slots) * (s.bm / 16);
-        hipLaunchKernelGGL((k_attn_chunk_join<TQ, TC, HD>), dim3((unsigned)joins), dim3(AC_WG), 0, st, a, ml, o, pr);
+        const ChunkShape s = shape_of(W::BM, W::PER_CU, a.kv.n_seq, a.kv.nkv, a.gqa, a.chunk.n_rows);
+        const Parts parts{(float *)ws, (float2 *)((float *)ws + s.parts(a.kv.nkv) * HD), s.rows};
+        // rows of a wave in pages one after another, within 32 bits
+        constexpr int PER_WAVE = W::KT / W::NW;
+        a.runs = a.kv.page_tokens % PER_WAVE == 0 && (int64_t)a.kv.nkv * HD * (int)sizeof(TC) < (1 << 26);
+        const int64_t grid = std::max<int64_t>(s.tiles, (int64_t)s.shares * a.kv.nkv);
+        hipLaunchKernelGGL((k_attn_chunk<TQ, TC, HD>), dim3((unsigned)grid), dim3(64 * W::NW), 0, st, a, parts);
+        // (tiles of at most AC_START blocks are never cut: line_of)
+        if (s.shares > 1 && a.kv.cap > AC_START * W::KT) {
+            constexpr int MANY = AC_JOIN / (HD / 4), FEW = MANY > 4 ? 4 : MANY;
+            if (s.rows > 64)
+                hipLaunchKernelGGL((k_attn_chunk_join<TQ, TC, HD, MANY>), dim3((s.rows + MANY - 1) / MANY, a.kv.nkv, s.shares - 1),
+                                   dim3(AC_JOIN), 0, st, a, parts);
+            else
+                hipLaunchKernelGGL((k_attn_chunk_join<TQ, TC, HD, FEW>), dim3((s.rows + FEW - 1) / FEW, a.kv.nkv, s.shares - 1),
+                                   dim3(AC_JOIN), 0, st, a, parts);
+        }
         return 0;
     });
     return hipGetLastError();

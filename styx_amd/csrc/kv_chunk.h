@@ -63,6 +63,8 @@ struct AttnChunkArgs {
     float scale;
     void *out;
     float *lse;
+    PageDiv by_gqa;  // (filled by the launch, as is runs)
+    int runs;        // a wave's rows of a block lie in one page
 };
 // Workgroups of the largest launch; bytes of the workspace.
 int64_t attn_chunk_grid(int n_seq, int nkv, int gqa, int n_rows);
