@@ -103,9 +103,9 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD> {
     static constexpr int DS = HD == 256 && NP == 2 ? 2 : 1, HW = HD / DS, NK = HW / 16, ND = HW / 32;
     static constexpr int KT = HD == 256 ? 32 : 64;
     static constexpr int NW = DS == 2 ? 8 : 4, PER_CU = 8 / NW, BM = 32 * NW / DS;
-    h8 q[NP][NK];
+    h8 q[NP][NK], p[KT / 32][NP][2];
     f16v s[KT / 32], o[ND];
-    float mul;
+    float mul, ref, sum[2];  // score to factor: 2^(s mul + ref); the factors' sum
     int lane;
 
     // row: this wave's dims of the query, the first of which is d0
@@ -155,36 +155,44 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD> {
                 }
         }
     }
-    __device__ __forceinline__ void scores(const char *kb)
+    // The scores of 32 slots, with fill(j, N) done behind the j-th of N operands.
+    template <typename F> __device__ __forceinline__ void scores(int kt, const char *kb, F fill)
     {
-        constexpr int N = NK * KT / 32, AHEAD = 4;
+        constexpr int AHEAD = 4;
         const int m = lane & 31, h = lane >> 5;
         const f16v zero = {};
         const int at = m * La::ROW + ((h ^ La::perm(m)) << 4);
         // (piece 2 i + h: its bits above 256 bytes are not permuted)
-        auto read = [&](int j) {
-            const int i = j / (KT / 32), kt = j % (KT / 32);
-            return *(const h8 *)(kb + (at ^ ((32 * i) & 255)) + ((32 * i) & ~255) + kt * 32 * La::ROW);
-        };
+        auto read = [&](int i) { return *(const h8 *)(kb + (at ^ ((32 * i) & 255)) + ((32 * i) & ~255) + kt * 32 * La::ROW); };
         h8 k[AHEAD];
 #pragma unroll
-        for (int j = 0; j < AHEAD; j++) k[j] = read(j);
+        for (int i = 0; i < AHEAD; i++) k[i] = read(i);
         in_order();
 #pragma unroll
-        for (int j = 0; j < N; j++) {
-            const int i = j / (KT / 32), kt = j % (KT / 32);
+        for (int i = 0; i < NK; i++) {
 #pragma unroll
             for (int x = 0; x < NP; x++)
-                s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[j % AHEAD], q[x][i], i + x == 0 ? zero : s[kt], 0, 0, 0);
-            if (j + AHEAD < N) k[j % AHEAD] = read(j + AHEAD);
+                s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[i % AHEAD], q[x][i], i + x == 0 ? zero : s[kt], 0, 0, 0);
+            if (i + AHEAD < NK) k[i % AHEAD] = read(i + AHEAD);
+            fill(i, NK);
             in_order();
         }
     }
-    // o += factors times V; returns their sum
-    __device__ __forceinline__ float values(const char *vb, float ref)
+    // The factor of score i of 32 slots.
+    __device__ __forceinline__ void factor(int kt, int i)
     {
-        constexpr int N = ND * KT / 16, AHEAD = 4, PER = 8 / ND;
-        static_assert(8 % ND == 0, "factors of a step");
+        const float f = exp2_(fmaf(s[kt][i], mul, ref));
+        sum[i & 1] += f;
+        asm volatile("" : "+v"(sum[i & 1]));  // (here, not behind the products)
+        const _Float16 hi = (_Float16)f;
+        p[kt][0][i >> 3][i & 7] = hi;
+        if constexpr (NP == 2) p[kt][1][i >> 3][i & 7] = (_Float16)(f - (float)hi);
+    }
+    // o += factors of 32 slots times V, with fill(j, N) done behind the j-th of N
+    // operands; the factors of a step of 16 slots are needed at its first.
+    template <typename F> __device__ __forceinline__ void values(int kt, const char *vb, F fill)
+    {
+        constexpr int N = 2 * ND, AHEAD = 4;
         const int h = lane >> 5, u = (lane >> 4) & 1, kk = (lane & 15) >> 2;
         // piece of dims 16 u + 4 (lane & 3) .. of the first 32, row kk + 4 (h + 2 r)
         auto at = [&](int r) {
@@ -198,40 +206,40 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD> {
             h8 v;
         };
         auto read = [&](int j) {
-            const int d = j % ND, k = j / ND;
+            const int d = j % ND, k = 2 * kt + j / ND;
             const int flip = (64 * d) & (La::ROW < 256 ? La::ROW - 1 : 255), far = ((64 * d) & ~255) + k * 16 * La::ROW;
             Part x;
             x.part[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vb + (at0 ^ flip) + far));
             x.part[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(vb + (at1 ^ flip) + far));
             return x.v;
         };
-        float sum[2] = {};
-        h8 p[2][NP];  // of the step under way and the next
-        auto factor = [&](int k, int i) {
-            const float f = exp2_(fmaf(s[k / 2][8 * (k & 1) + i], mul, ref));
-            sum[i & 1] += f;
-            const _Float16 hi = (_Float16)f;
-            p[k & 1][0][i] = hi;
-            if constexpr (NP == 2) p[k & 1][1][i] = (_Float16)(f - (float)hi);
-        };
         h8 v[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; j++) v[j] = read(j);
-#pragma unroll
-        for (int i = 0; i < 8; i++) factor(0, i);
         in_order();
 #pragma unroll
         for (int j = 0; j < N; j++) {
-            const int d = j % ND, k = j / ND;
 #pragma unroll
-            for (int y = 0; y < NP; y++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[j % AHEAD], p[k & 1][y], o[d], 0, 0, 0);
+            for (int y = 0; y < NP; y++)
+                o[j % ND] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[j % AHEAD], p[kt][y][j / ND], o[j % ND], 0, 0, 0);
             if (j + AHEAD < N) v[j % AHEAD] = read(j + AHEAD);
-            if (k + 1 < KT / 16)
-#pragma unroll
-                for (int i = 0; i < PER; i++) factor(k + 1, PER * d + i);
+            fill(j, N);
             in_order();
         }
-        return sum[0] + sum[1];
+    }
+    // All but the scores times c, a power of two; `pending`: factors of the first
+    // 32 slots that have not met V.
+    __device__ __forceinline__ void rescale(float c, bool pending)
+    {
+        sum[0] *= c;
+        sum[1] *= c;
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[d] *= c;
+        if (pending)
+#pragma unroll
+            for (int y = 0; y < NP; y++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) p[0][y][k] *= (_Float16)c;
     }
 };
 
@@ -245,7 +253,7 @@ template <int HD> struct Wave<float, float, HD> {
     static constexpr int NW = HD == 256 ? 8 : 4, PER_CU = 8 / NW, BM = 32 * NW / DS;
     styx_f4 q[NK];
     f16v s[1], o[ND];
-    float mul;
+    float mul, ref, sum[2], p[2];
     int lane;
 
     __device__ __forceinline__ void init(const float *row, int, float scale)
@@ -256,7 +264,7 @@ template <int HD> struct Wave<float, float, HD> {
 #pragma unroll
         for (int i = 0; i < NK; i++) q[i] = *(const styx_f4 *)(row + 8 * i + 4 * h) * sign;
     }
-    __device__ __forceinline__ void scores(const char *kb)
+    template <typename F> __device__ __forceinline__ void scores(int, const char *kb, F)
     {
         const int m = lane & 31, h = lane >> 5;
         const f16v zero = {};
@@ -278,7 +286,12 @@ template <int HD> struct Wave<float, float, HD> {
         }
         s[0] = c[0] + c[1];
     }
-    __device__ __forceinline__ float values(const char *vb, float ref)
+    __device__ __forceinline__ void factor(int, int i)
+    {
+        p[i & 1] = exp2_(fmaf(s[0][i], mul, ref));
+        sum[i & 1] += p[i & 1];
+    }
+    template <typename F> __device__ __forceinline__ void values(int, const char *vb, F fill)
     {
         constexpr int N = 16 * ND, AHEAD = 8;
         const int m = lane & 31, h = lane >> 5;
@@ -287,25 +300,24 @@ template <int HD> struct Wave<float, float, HD> {
             const int at = t * La::ROW + (((m >> 2) ^ La::perm(t)) << 4) + 4 * (m & 3);
             return *(const float *)(vb + (at ^ ((128 * d) & 255)) + ((128 * d) & ~255));
         };
-        float sum[2] = {}, p[2];
-        auto factor = [&](int i) {
-            p[i & 1] = exp2_(fmaf(s[0][i], mul, ref));
-            sum[i & 1] += p[i & 1];
-        };
         float v[AHEAD];
 #pragma unroll
         for (int j = 0; j < AHEAD; j++) v[j] = read(j);
-        factor(0);
         in_order();
 #pragma unroll
         for (int j = 0; j < N; j++) {
-            const int d = j % ND, i = j / ND;
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[j % AHEAD], p[i & 1], o[d], 0, 0, 0);
+            o[j % ND] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[j % AHEAD], p[j / ND & 1], o[j % ND], 0, 0, 0);
             if (j + AHEAD < N) v[j % AHEAD] = read(j + AHEAD);
-            if (d == 0 && i + 1 < 16) factor(i + 1);
+            fill(j, N);
             in_order();
         }
-        return sum[0] + sum[1];
+    }
+    __device__ __forceinline__ void rescale(float c, bool)
+    {
+        sum[0] *= c;
+        sum[1] *= c;
+#pragma unroll
+        for (int d = 0; d < ND; d++) o[d] *= c;
     }
 };
 
@@ -419,7 +431,7 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD>::NW), 2) k_attn_chunk(A
     __shared__ __align__(1024) char s_k[2][BLOCK];
     __shared__ __align__(1024) char s_v[2][BLOCK];
     // scores of half the dims; in the block of K where there is no other place
-    constexpr int PIECES = KT / 32 * 4;
+    constexpr int PIECES = 4;
     constexpr bool APART = 4 * BLOCK + NW * PIECES * 1024 < 150000;
     __shared__ styx_f4 s_half[DS == 2 && APART ? NW * PIECES : 1][64];
     const KvView &kv = a.kv;
@@ -474,7 +486,9 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD>::NW), 2) k_attn_chunk(A
     const int r = min(wrow0 + n, rows - 1), tok = a.by_gqa.of(r), head = kvh * a.gqa + (r - tok * a.gqa);
     const int at = wrow0 + n < rows ? s.len + tok : -1;  // last slot seen, -1: no such row
     const int64_t orow = s.first + tok;                  // row of q and out
-    float m = -INFINITY, l = 0.0f;
+    float m = -INFINITY;  // the reference, a whole number
+    x.ref = AC_OFF;
+    x.sum[0] = x.sum[1] = 0.0f;
     uint32_t nan_at[HW / 64];  // dims that are NaN whatever the sums are
 #pragma unroll
     for (int w = 0; w < HW / 64; w++) nan_at[w] = 0;
@@ -590,59 +604,89 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD>::NW), 2) k_attn_chunk(A
             }
         }
         const bool idle = !works || tb > any_hi || tb + KT <= any_lo;
-        if constexpr (DS == 1) {
-            if (idle) continue;
-            x.scores(kb);
-        } else {
-            // each wave of a pair has half the dims: both add the halves up
-            styx_f4 (*half)[64] = APART ? s_half : (styx_f4(*)[64])s_k[buf];
-            if (!idle) x.scores(kb + dw * (int)sizeof(TC));
-            if constexpr (!APART) {
-                static_assert(NW * PIECES * 1024 <= BLOCK, "scores in the place of K");
-                __syncthreads();
-            }
-            if (!idle)
+        const bool masked = seen != full || tb + KT - 1 > all_hi || tb < all_lo;
+        auto mask = [&](int kt) {
+            const uint32_t mine = vis[kt] >> (4 * h);
 #pragma unroll
-                for (int i = 0; i < PIECES; i++) {
-                    const f16v &y = x.s[i / 4];
-                    half[wave * PIECES + i][lane] = styx_f4{y[4 * (i & 3)], y[4 * (i & 3) + 1], y[4 * (i & 3) + 2], y[4 * (i & 3) + 3]};
-                }
-            __syncthreads();
-            if (idle) continue;
-#pragma unroll
-            for (int i = 0; i < PIECES; i++) {
-                const styx_f4 y = half[(wave ^ 1) * PIECES + i][lane];
-#pragma unroll
-                for (int e = 0; e < 4; e++) x.s[i / 4][4 * (i & 3) + e] += y[e];
-            }
-        }
-        if (seen != full || tb + KT - 1 > all_hi || tb < all_lo) {
-#pragma unroll
-            for (int kt = 0; kt < KT / 32; kt++) {
-                const uint32_t mine = vis[kt] >> (4 * h);
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    if (!(mine >> (8 * (i >> 2) + (i & 3)) & 1)) x.s[kt][i] = -INFINITY;
-            }
-        }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int kt = 0; kt < KT / 32; kt++)
+            for (int i = 0; i < 16; i++)
+                if (!(mine >> (8 * (i >> 2) + (i & 3)) & 1)) x.s[kt][i] = -INFINITY;
+        };
+        auto follow = [&](int kt) {
+            float mx = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(mx, x.s[kt][i]), x.s[kt][i + 1]);
-        mx = fmaxf(mx, other_half(mx)) * x.mul;
-        if (__ballot(mx > m + AC_LAG)) {
-            const float mn = fmaxf(m, mx), corr = mn == -INFINITY ? 1.0f : exp2_(m - mn);
-            m = mn;
-            l *= corr;
+            mx = fmaxf(mx, other_half(mx)) * x.mul;
+            if (__ballot(mx > m + AC_LAG)) {
+                const float mn = fmaxf(m, ceilf(mx));
+                if (mn != -INFINITY) {
+                    x.rescale(exp2_(m - mn), kt > 0);
+                    x.ref = AC_OFF - mn;
+                }
+                m = mn;
+            }
+        };
+        auto nothing = [](int, int) {};
+        if constexpr (KT == 64) {
+            // the products of one half of the block while the other's factors are formed
+            if (idle) continue;
+            auto factors = [&](int kt, int j, int steps) {
 #pragma unroll
-            for (int d = 0; d < ND; d++) x.o[d] *= corr;
+                for (int i = 0; i < 16; i++)
+                    if (i / (16 / steps) == j) x.factor(kt, i);
+            };
+            x.scores(0, kb, nothing);
+            if (masked) mask(0);
+            follow(0);
+            x.scores(1, kb, [&](int j, int steps) { factors(0, j, steps); });
+            if (masked) mask(1);
+            follow(1);
+            x.values(0, vb, [&](int j, int steps) { factors(1, j, steps); });
+            x.values(1, vb, nothing);
+        } else {
+            if constexpr (DS == 1) {
+                if (idle) continue;
+                x.scores(0, kb, nothing);
+            } else {
+                // each wave of a pair has half the dims: both add the halves up
+                styx_f4 (*half)[64] = APART ? s_half : (styx_f4(*)[64])s_k[buf];
+                if (!idle) x.scores(0, kb + dw * (int)sizeof(TC), nothing);
+                if constexpr (!APART) {
+                    static_assert(NW * PIECES * 1024 <= BLOCK, "scores in the place of K");
+                    __syncthreads();
+                }
+                if (!idle)
+#pragma unroll
+                    for (int i = 0; i < PIECES; i++)
+                        half[wave * PIECES + i][lane] = styx_f4{x.s[0][4 * i], x.s[0][4 * i + 1], x.s[0][4 * i + 2], x.s[0][4 * i + 3]};
+                __syncthreads();
+                if (idle) continue;
+#pragma unroll
+                for (int i = 0; i < PIECES; i++) {
+                    const styx_f4 y = half[(wave ^ 1) * PIECES + i][lane];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x.s[0][4 * i + e] += y[e];
+                }
+            }
+            if (masked) mask(0);
+            follow(0);
+            // factors a step ahead of their product: 8 of f16 caches, one of f32
+            constexpr int LEAD = sizeof(TC) == 2 ? 8 : 1;
+#pragma unroll
+            for (int i = 0; i < LEAD; i++) x.factor(0, i);
+            x.values(0, vb + dw * (int)sizeof(TC), [&](int j, int steps) {
+                if constexpr (sizeof(TC) == 4) {
+                    if (j % (steps / 16) == 0 && j < steps - steps / 16) x.factor(0, j / (steps / 16) + 1);
+                } else {
+#pragma unroll
+                    for (int i = LEAD; i < 16; i++)
+                        if ((i - LEAD) * steps / 16 == j) x.factor(0, i);
+                }
+            });
         }
-        const float ref = AC_OFF - (m == -INFINITY ? 0.0f : m);
-        l += x.values(vb + dw * (int)sizeof(TC), ref);
     }
     if (more) __syncthreads();  // (the next piece's blocks take the place of this one's)
     if (at < 0) continue;
+    float l = x.sum[0] + x.sum[1];
     l += other_half(l);
 #pragma unroll
     for (int d = 0; d < ND; d++)
