@@ -260,7 +260,7 @@ int styx_op_kv_weigh(styx_gpu *g, const styx_kv_cache *kv, const styx_kv_chunk *
     a.acc_in = acc_in;
     a.acc_out = acc_out;
     a.slot_pos = slot_pos;
-    if (kv_weigh_grid(a) > MAX_WG_256) return fail(STYX_E_INVALID, std::string(who) + ": too many sequences, heads or slots");
+    if ((int64_t)chunk->n_rows * a.gqa > (1 << 28) || kv_weigh_grid(a) > MAX_WG_256) return fail(STYX_E_INVALID, std::string(who) + ": too many sequences, heads, rows or slots");
     if (chunk->n_rows == 0) return STYX_OK;
     const DeviceScope on(g->device);
     OP_RUN(launch_kv_weigh(g->stream, a), who);

@@ -82,6 +82,7 @@ struct KvWeighArgs {
     const float *lse, *acc_in;
     float *acc_out;
     int32_t *slot_pos;
+    PageDiv by_gqa;  // (filled by the launch)
 };
 int64_t kv_weigh_grid(const KvWeighArgs &a);
 hipError_t launch_kv_weigh(hipStream_t st, KvWeighArgs a);

@@ -5,69 +5,210 @@
 //                 + sum over the last tokens i that see t and the heads h of j
 //                   of e^(scale q_ih . K[t] - lse_ih),  t < len + count
 //
-// The plain kernel: a wave for 64 slots of a kv head, a slot a lane, the tokens
-// and heads one after another.
+// A wave holds 32 slots of a kv head in registers and goes over the query rows
+// (tokens times heads) in tiles of 32 that its workgroup keeps in LDS, the next
+// tile on its way meanwhile: K is read once, and no sum crosses waves.  Scores
+// are formed queries x slots, so a lane has its own slot's of 16 rows of a tile
+// (its other half, lane ^ 32, the other 16): weights are summed lane by lane.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_chunk.h"
 #include "lanes.h"
 
 namespace styx {
 
-constexpr int KW_WG = 256, KW_WAVES = KW_WG / 64;
+constexpr int KW_WG = 256, KW_WAVES = KW_WG / 64, KW_KEYS = 32 * KW_WAVES, KW_ROWS = 32;
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+
+// A tile of query rows in LDS, of type T: 16-byte pieces permuted within 256
+// bytes, so that 16 rows' reads of a piece lie in banks of their own.
+template <typename T, int HD> struct RowLay {
+    static constexpr int ROW = HD * (int)sizeof(T);
+    static __device__ __forceinline__ int at(int r, int byte)
+    {
+        const int p = ROW == 128 ? (r >> 1) & 7 : r & 15;
+        return r * ROW + (byte ^ (p << 4));
+    }
+};
 
 template <typename TQ, typename TC, int HD>
-__global__ void __launch_bounds__(KW_WG) k_kv_weigh(KvWeighArgs a, int tiles)
+__global__ void __launch_bounds__(KW_WG, HD == 256 && sizeof(TQ) == 4 ? 2 : 3) k_kv_weigh(KvWeighArgs a)
 {
+    // f32 queries on f16 rows are two f16 pieces, brought to [2^9, 2^10) by a
+    // power of two per row, as in the attention
+    constexpr int NP = sizeof(TQ) == 4 && sizeof(TC) == 2 ? 2 : 1;
+    using La = RowLay<TC, HD>;
+    constexpr int NK = sizeof(TC) == 2 ? HD / 16 : HD / 8;  // operands of a row
+    constexpr int PER = KW_ROWS * HD / KW_WG;               // values of a thread in a tile
+    constexpr int TPR = HD / PER;                           // threads of a row: 8
+    typedef typename std::conditional<sizeof(TC) == 2, h8, styx_f4>::type Op;
+    __shared__ __align__(16) char s_q[2][NP][KW_ROWS * La::ROW];
+    __shared__ __align__(16) float s_lse[2][KW_ROWS], s_mul[2][KW_ROWS];
+    __shared__ __align__(16) int s_at[2][KW_ROWS];
     const KvView &kv = a.kv;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int bk = blockIdx.x / tiles, b = bk / kv.nkv, kvh = bk % kv.nkv;
-    const ChunkSeq s = chunk_seq(a.chunk, kv, b);
-    if (s.count == 0) return;
-    const int rows = s.len + s.count;
-    const int32_t *tab = kv.table + (int64_t)b * kv.table_len;
-    const int64_t stride = (int64_t)kv.nkv * HD, base = (int64_t)bk * kv.cap;
-    for (int64_t t64 = ((int64_t)(blockIdx.x % tiles) * KW_WAVES + wave) * 64; t64 < rows; t64 += (int64_t)tiles * KW_WG) {
-        const int t = (int)t64 + lane, r = t < rows ? kv.row(tab, t) : -1;
-        const TC *k = (const TC *)kv.kpool + max(r, 0) * stride + kvh * HD;
-        float sum = 0.0f;
-        for (int i = max(0, s.count - a.last); i < s.count; i++) {
-            const int at = s.len + i;
-            if (t > at || (a.window && t <= at - a.window) || r < 0) continue;
-            for (int g = 0; g < a.gqa; g++) {
-                const int h = kvh * a.gqa + g, row = s.first + i;
-                const TQ *q = (const TQ *)a.q + row * a.ldq + (int64_t)h * HD;
-                float x = 0.0f;
-                for (int d = 0; d < HD; d++) x += (float)q[d] * (float)k[d];
-                const float lse = a.lse[(int64_t)row * a.nh + h];
-                if (lse != -INFINITY) sum += __expf(x * a.scale - lse);
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t stride = (int64_t)kv.nkv * HD;
+    for (int64_t item = blockIdx.x;; item += gridDim.x) {
+        // the sequence and its 128 slots
+        const int kvh = (int)(item % kv.nkv);
+        int64_t nth = item / kv.nkv;
+        int b = -1;
+        ChunkSeq s{};
+        for (int b0 = 0; b0 < kv.n_seq && b < 0; b0 += 64) {
+            const ChunkSeq mine = chunk_seq(a.chunk, kv, b0 + lane);
+            const int64_t tiles = mine.count ? ((int64_t)mine.len + mine.count + KW_KEYS - 1) / KW_KEYS : 0, upto = wave_upto(tiles);
+            if (const unsigned long long hit = __ballot(upto > nth)) {
+                const int l = __builtin_ctzll(hit);
+                b = b0 + l;
+                s = {(int)__builtin_amdgcn_readlane(mine.first, l), (int)__builtin_amdgcn_readlane(mine.count, l),
+                     (int)__builtin_amdgcn_readlane(mine.len, l)};
+                nth -= of_lane(upto, l) - of_lane(tiles, l);
+            } else {
+                nth -= of_lane(upto, 63);
             }
         }
-        if (t >= rows) continue;
-        a.acc_out[base + t] = (a.acc_in && t < s.len ? a.decay * a.acc_in[base + t] : 0.0f) + sum;
-        if (a.slot_pos && t >= s.len) a.slot_pos[base + t] = a.pos[b] + (t - s.len);
+        if (b < 0) return;
+        const int k0 = (int)nth * KW_KEYS, slots = s.len + s.count;
+        const int t = k0 + 32 * wave + n;  // this lane's slot
+        const int row = t < slots ? kv.row(kv.table + (int64_t)b * kv.table_len, t) : -1;
+        Op k[NK];
+        const TC *kp = (const TC *)kv.kpool + max(row, 0) * stride + kvh * HD + (sizeof(TC) == 2 ? 8 : 4) * h;
+#pragma unroll
+        for (int i = 0; i < NK; i++) k[i] = *(const Op *)(kp + (sizeof(TC) == 2 ? 16 : 8) * i);
+        // tokens that count and see any of the 128 slots, and their rows
+        const int i0 = max(max(s.count - min(a.last, s.count), k0 - s.len), 0);
+        const int i1 = a.window ? (int)max((int64_t)i0, min((int64_t)s.count, (int64_t)k0 + KW_KEYS - 1 + a.window - s.len)) : s.count;
+        const int r0 = i0 * a.gqa, r1 = max(i0, i1) * a.gqa;
+        // a thread's part of a row of the next tile
+        __align__(16) TQ in[PER];
+        float in_lse = 0.0f;
+        const int mr = tid / TPR, md = tid % TPR * PER;
+        auto ask = [&](int base) {
+            const int r = min(base + mr, r1 - 1), tok = a.by_gqa.of(r), head = kvh * a.gqa + (r - tok * a.gqa);
+            const TQ *p = (const TQ *)a.q + (int64_t)(s.first + tok) * a.ldq + (int64_t)head * HD + md;
+            constexpr int M = 16 / sizeof(TQ);
+            typedef typename std::conditional<sizeof(TQ) == 2, h8, styx_f4>::type V;
+#pragma unroll
+            for (int i = 0; i < PER; i += M) *(V *)(in + i) = *(const V *)(p + i);
+            in_lse = a.lse[(int64_t)(s.first + tok) * a.nh + head];
+        };
+        auto put = [&](int buf, int base) {
+            float mul = a.scale;
+            if constexpr (NP == 2) {
+                float m = 0.0f;
+#pragma unroll
+                for (int i = 0; i < PER; i++) m = fmaxf(m, fabsf((float)in[i]));
+#pragma unroll
+                for (int d = 1; d < TPR; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+                const int e = m > 0.0f && m < INFINITY ? (int)((__float_as_uint(m) >> 23) & 255) - 127 : 9;
+                const float up = e < -100 ? ldexpf(1.0f, 109) : ldexpf(1.0f, 9 - e);
+                mul /= up;
+#pragma unroll
+                for (int i = 0; i < PER; i += 8) {
+                    h8 hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float y = (float)in[i + e] * up;
+                        hi[e] = (_Float16)y;
+                        lo[e] = (_Float16)(y - (float)hi[e]);
+                    }
+                    *(h8 *)(s_q[buf][0] + La::at(mr, 2 * (md + i))) = hi;
+                    *(h8 *)(s_q[buf][NP - 1] + La::at(mr, 2 * (md + i))) = lo;
+                }
+            } else {
+                constexpr int M = 16 / sizeof(TC);
+#pragma unroll
+                for (int i = 0; i < PER; i += M) *(Op *)(s_q[buf][0] + La::at(mr, (int)sizeof(TC) * (md + i))) = *(const Op *)(in + i);
+            }
+            if (tid % TPR == 0) {
+                const int r = base + mr;
+                // a token that sees nothing has no weights
+                s_lse[buf][mr] = r < r1 && in_lse != -INFINITY ? in_lse * 1.44269504f : INFINITY;
+                s_mul[buf][mr] = mul;
+                s_at[buf][mr] = r < r1 ? s.len + a.by_gqa.of(r) : -1;
+            }
+        };
+        float sum[2] = {};
+        __syncthreads();  // (the last item's tiles are read no more)
+        if (r0 < r1) {
+            ask(r0);
+            put(0, r0);
+            if (r0 + KW_ROWS < r1) ask(r0 + KW_ROWS);
+        }
+        for (int base = r0, buf = 0; base < r1; base += KW_ROWS, buf ^= 1) {
+            __syncthreads();
+            f16v x = {};
+#pragma unroll
+            for (int i = 0; i < NK; i++) {
+                const int at = La::at(n, 32 * i + 16 * h);
+                if constexpr (sizeof(TC) == 2) {
+#pragma unroll
+                    for (int y = 0; y < NP; y++) x = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const h8 *)(s_q[buf][y] + at), k[i], x, 0, 0, 0);
+                } else {
+                    const styx_f4 q = *(const styx_f4 *)(s_q[buf][0] + at);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x = __builtin_amdgcn_mfma_f32_32x32x2f32(q[e], k[i][e], x, 0, 0, 0);
+                }
+            }
+            if (base + KW_ROWS < r1) {
+                put(buf ^ 1, base + KW_ROWS);
+                if (base + 2 * KW_ROWS < r1) ask(base + 2 * KW_ROWS);
+            }
+            // whether every row of the tile sees all of the wave's slots
+            const int w0 = k0 + 32 * wave;
+            const bool whole = base + KW_ROWS <= r1 && w0 + 31 <= s.len + a.by_gqa.of(base) &&
+                               (!a.window || w0 > s.len + a.by_gqa.of(base + KW_ROWS - 1) - a.window);
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int r = 2 * i + 4 * h;
+                const styx_f4 lse = *(const styx_f4 *)&s_lse[buf][r], mul = *(const styx_f4 *)&s_mul[buf][r];
+                float w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_exp2f(fmaf(x[i + e], mul[e], -lse[e]));
+                if (!whole) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int at = s_at[buf][r + e];
+                        if (t > at || (a.window && t <= at - a.window)) w[e] = 0.0f;
+                    }
+                }
+                sum[0] += w[0] + w[1];
+                sum[1] += w[2] + w[3];
+            }
+        }
+        float all = sum[0] + sum[1];
+        const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(all), __float_as_uint(all), false, false);
+        all = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+        if (h == 0 && t < slots) {
+            const int64_t at = ((int64_t)b * kv.nkv + kvh) * kv.cap + t;
+            a.acc_out[at] = (a.acc_in && t < s.len ? a.decay * a.acc_in[at] : 0.0f) + (row >= 0 ? all : 0.0f);
+            if (a.slot_pos && t >= s.len) a.slot_pos[at] = a.pos[b] + (t - s.len);
+        }
     }
 }
 
-static int64_t weigh_tiles(const KvWeighArgs &a)
+int64_t kv_weigh_grid(const KvWeighArgs &a)
 {
-    return std::min<int64_t>(((int64_t)a.kv.cap + KW_WG - 1) / KW_WG,
-                             std::max<int64_t>(1, 4096 / ((int64_t)a.kv.n_seq * a.kv.nkv)));
+    const int64_t tiles = ((int64_t)a.kv.cap + KW_KEYS - 1) / KW_KEYS;
+    return std::min<int64_t>(tiles * a.kv.n_seq * a.kv.nkv, 4096);
 }
-int64_t kv_weigh_grid(const KvWeighArgs &a) { return weigh_tiles(a) * a.kv.n_seq * a.kv.nkv; }
 
 template <typename TQ, typename TC> static void launch_hd(hipStream_t st, const KvWeighArgs &a)
 {
     const dim3 g((unsigned)kv_weigh_grid(a)), wg(KW_WG);
-    const int tiles = (int)weigh_tiles(a);
     switch (a.kv.hd) {
-    case 64: hipLaunchKernelGGL((k_kv_weigh<TQ, TC, 64>), g, wg, 0, st, a, tiles); break;
-    case 128: hipLaunchKernelGGL((k_kv_weigh<TQ, TC, 128>), g, wg, 0, st, a, tiles); break;
-    default: hipLaunchKernelGGL((k_kv_weigh<TQ, TC, 256>), g, wg, 0, st, a, tiles); break;
+    case 64: hipLaunchKernelGGL((k_kv_weigh<TQ, TC, 64>), g, wg, 0, st, a); break;
+    case 128: hipLaunchKernelGGL((k_kv_weigh<TQ, TC, 128>), g, wg, 0, st, a); break;
+    default: hipLaunchKernelGGL((k_kv_weigh<TQ, TC, 256>), g, wg, 0, st, a); break;
     }
 }
 hipError_t launch_kv_weigh(hipStream_t st, KvWeighArgs a)
 {
+    a.scale = (float)((double)a.scale * 1.4426950408889634);  // log2 e
+    a.by_gqa = page_div((uint32_t)a.gqa);
     if (!a.kv.f16)
         launch_hd<float, float>(st, a);
     else if (a.q_f16)
