@@ -18,7 +18,13 @@
 
 namespace styx {
 
-constexpr int KW_WG = 256, KW_WAVES = KW_WG / 64, KW_KEYS = 32 * KW_WAVES, KW_ROWS = 32;
+constexpr int KW_ROWS = 32;
+// Waves of a workgroup, all of which read its tiles: f16 products are so fast
+// that fetching the tiles counts (64 tokens over 32768 slots: 8 waves 31 us, 4
+// waves 35, 2 waves 36), f32 ones are not, and smaller workgroups fill the chip
+// more evenly (16 conversations: 4 waves 63 us, 2 waves 69, 1 wave 77).
+// (Heads of 64 have no 16 bytes of a tile for more than 4 waves' threads.)
+__host__ __device__ constexpr int kw_waves(bool f16, int hd) { return f16 && hd > 64 ? 8 : 4; }
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 
@@ -34,15 +40,17 @@ template <typename T, int HD> struct RowLay {
 };
 
 template <typename TQ, typename TC, int HD>
-__global__ void __launch_bounds__(KW_WG, HD == 256 && sizeof(TQ) == 4 ? 2 : 3) k_kv_weigh(KvWeighArgs a)
+__global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), HD == 256 && sizeof(TQ) == 4 ? 2 : 3) k_kv_weigh(KvWeighArgs a)
 {
     // f32 queries on f16 rows are two f16 pieces, brought to [2^9, 2^10) by a
     // power of two per row, as in the attention
     constexpr int NP = sizeof(TQ) == 4 && sizeof(TC) == 2 ? 2 : 1;
     using La = RowLay<TC, HD>;
+    constexpr int KW_WG = 64 * kw_waves(sizeof(TC) == 2, HD), KW_KEYS = KW_WG / 2;
     constexpr int NK = sizeof(TC) == 2 ? HD / 16 : HD / 8;  // operands of a row
     constexpr int PER = KW_ROWS * HD / KW_WG;               // values of a thread in a tile
-    constexpr int TPR = HD / PER;                           // threads of a row: 8
+    constexpr int TPR = HD / PER;                           // threads of a row
+    static_assert(PER % 8 == 0 || (sizeof(TQ) == 4 && NP == 1 && PER % 4 == 0), "whole pieces");
     typedef typename std::conditional<sizeof(TC) == 2, h8, styx_f4>::type Op;
     __shared__ __align__(16) char s_q[2][NP][KW_ROWS * La::ROW];
     __shared__ __align__(16) float s_lse[2][KW_ROWS], s_mul[2][KW_ROWS];
@@ -136,6 +144,9 @@ __global__ void __launch_bounds__(KW_WG, HD == 256 && sizeof(TQ) == 4 ? 2 : 3) k
         if (r0 < r1) {
             ask(r0);
             put(0, r0);
+            // (here, so that no trip waits for them, and with them for the next tile)
+#pragma unroll
+            for (int i = 0; i < NK; i++) asm volatile("" : "+v"(k[i]));
             if (r0 + KW_ROWS < r1) ask(r0 + KW_ROWS);
         }
         for (int base = r0, buf = 0; base < r1; base += KW_ROWS, buf ^= 1) {
@@ -161,22 +172,26 @@ __global__ void __launch_bounds__(KW_WG, HD == 256 && sizeof(TQ) == 4 ? 2 : 3) k
             const int w0 = k0 + 32 * wave;
             const bool whole = base + KW_ROWS <= r1 && w0 + 31 <= s.len + a.by_gqa.of(base) &&
                                (!a.window || w0 > s.len + a.by_gqa.of(base + KW_ROWS - 1) - a.window);
+            float w[16];
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const int r = 2 * i + 4 * h;
                 const styx_f4 lse = *(const styx_f4 *)&s_lse[buf][r], mul = *(const styx_f4 *)&s_mul[buf][r];
-                float w[4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_exp2f(fmaf(x[i + e], mul[e], -lse[e]));
-                if (!whole) {
+                for (int e = 0; e < 4; e++) w[i + e] = __builtin_amdgcn_exp2f(fmaf(x[i + e], mul[e], -lse[e]));
+            }
+            if (!whole) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int at = s_at[buf][r + e];
-                        if (t > at || (a.window && t <= at - a.window)) w[e] = 0.0f;
-                    }
+                for (int i = 0; i < 16; i++) {
+                    const int at = s_at[buf][8 * (i >> 2) + 4 * h + (i & 3)];
+                    const bool see = (t <= at) & ((a.window == 0) | (t > at - a.window));
+                    w[i] = see ? w[i] : 0.0f;
                 }
-                sum[0] += w[0] + w[1];
-                sum[1] += w[2] + w[3];
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                sum[0] += w[i];
+                sum[1] += w[i + 1];
             }
         }
         float all = sum[0] + sum[1];
@@ -192,13 +207,14 @@ __global__ void __launch_bounds__(KW_WG, HD == 256 && sizeof(TQ) == 4 ? 2 : 3) k
 
 int64_t kv_weigh_grid(const KvWeighArgs &a)
 {
+    const int KW_KEYS = 32 * kw_waves(a.kv.f16, a.kv.hd);
     const int64_t tiles = ((int64_t)a.kv.cap + KW_KEYS - 1) / KW_KEYS;
     return std::min<int64_t>(tiles * a.kv.n_seq * a.kv.nkv, 4096);
 }
 
 template <typename TQ, typename TC> static void launch_hd(hipStream_t st, const KvWeighArgs &a)
 {
-    const dim3 g((unsigned)kv_weigh_grid(a)), wg(KW_WG);
+    const dim3 g((unsigned)kv_weigh_grid(a)), wg(64 * kw_waves(a.kv.f16, a.kv.hd));
     switch (a.kv.hd) {
     case 64: hipLaunchKernelGGL((k_kv_weigh<TQ, TC, 64>), g, wg, 0, st, a); break;
     case 128: hipLaunchKernelGGL((k_kv_weigh<TQ, TC, 128>), g, wg, 0, st, a); break;
