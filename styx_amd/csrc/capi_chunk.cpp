@@ -112,6 +112,8 @@ int styx_op_kv_plan(styx_gpu *g, const styx_kv_cache *kv, const styx_kv_pages *i
         return fail(STYX_E_INVALID, std::string(who) + ": all arrays of the pages in place, or none");
     if (!len || !n_new || !first || !count || (row_pos && !pos)) return fail(STYX_E_INVALID, std::string(who) + ": NULL pointer");
     if (n_rows < 0) return fail(STYX_E_INVALID, std::string(who) + ": n_rows must not be negative");
+    if ((int64_t)kv->n_seq * kv->table_len > INT32_MAX)
+        return fail(STYX_E_INVALID, std::string(who) + ": more than 2^31 page-table entries");
     KvPlanArgs a{};
     a.kv = KvView{nullptr, nullptr, nullptr, 0, kv->n_seq, kv->nkv, kv->hd, kv->page_tokens, kv->n_pages,
                   kv->table_len, kv->table_len * kv->page_tokens, page_div((uint32_t)kv->page_tokens)};

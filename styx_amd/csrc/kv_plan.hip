@@ -11,47 +11,44 @@
 // not depend on an order of execution.
 //
 // Two launches: the sequences by one workgroup (1024 at a time; entries that
-// come back and pages that go out are dealt to its threads one by one,
+// come back and pages that go out are dealt to its threads, four at a time,
 // whatever sequence they belong to), then the rows, and where the result goes
-// to arrays of its own the entries and pages that stay, by many.
+// to arrays of its own the entries and pages that stay, by many.  Bound: the
+// latency of the first launch, whose few reads wait for each other: lengths,
+// entries, stack.
 #include "kv_chunk.h"
 #include "lanes.h"
 
 namespace styx {
 
-constexpr int KP_WG = 1024, KP_ROWS = 256;
+constexpr int KP_WG = 1024, KP_WAVES = KP_WG / 64, KP_ROWS = 256, KP_PER = 4;
 
-// Inclusive sums over the workgroup's threads, and their total.
-__device__ __forceinline__ int64_t group_upto(int64_t v, int64_t *s_wave, int64_t &total)
+// Inclusive sums of N numbers over the workgroup's threads, and their totals.
+template <typename T, int N> __device__ __forceinline__ void group_upto(T (&v)[N], T (&total)[N], T (*s_wave)[KP_WAVES])
 {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    v = wave_upto(v);
-    __syncthreads();
-    if (lane == 63) s_wave[wave] = v;
-    __syncthreads();
-    int64_t before = 0;
-    total = 0;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-    for (int w = 0; w < KP_WG / 64; w++) {
-        before += w < wave ? s_wave[w] : 0;
-        total += s_wave[w];
+    for (int i = 0; i < N; i++) v[i] = wave_upto(v[i]);
+    __syncthreads();
+    if (lane == 63)
+#pragma unroll
+        for (int i = 0; i < N; i++) s_wave[i][wave] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const T all = wave_upto(lane < KP_WAVES ? s_wave[i][lane] : T(0));
+        v[i] += wave ? of_lane(all, wave - 1) : T(0);
+        total[i] = of_lane(all, KP_WAVES - 1);
     }
-    return before + v;
 }
 
-// The first of n ascending sums that exceeds k (it is there).
-__device__ __forceinline__ int first_above(const int64_t *upto, int n, int64_t k)
+// The first of KP_WG ascending sums that exceeds k (it is there).
+__device__ __forceinline__ int first_above(const uint32_t *upto, uint32_t k)
 {
     int lo = 0;
-    for (int half = n; half > 0;) {
-        const int step = half >> 1;
-        if (upto[lo + step] <= k) {
-            lo += step + 1;
-            half -= step + 1;
-        } else {
-            half = step;
-        }
-    }
+#pragma unroll
+    for (int step = KP_WG / 2; step > 0; step >>= 1)
+        if (upto[lo + step - 1] <= k) lo += step;
     return lo;
 }
 
@@ -59,99 +56,152 @@ struct SeqPlan {
     int n, held, stays, asks;
     int64_t first;
 };
-__device__ __forceinline__ SeqPlan plan_seq(const KvPlanArgs &a, int b, int64_t first)
+// Of the sequence of this thread, by all threads; rows: those of the sequences
+// before the workgroup's, which it adds to.
+__device__ __forceinline__ SeqPlan plan_seq(const KvPlanArgs &a, int b, int64_t &rows, int64_t (*s_wave)[KP_WAVES])
 {
     const KvView &kv = a.kv;
-    const int n = max(a.n_new[b], 0), len = a.len[b];
-    SeqPlan s;
-    s.first = first;
-    s.held = min(max(a.in.held[b], 0), kv.table_len);
-    const bool ok = len >= 0 && n <= kv.cap && len <= kv.cap - n && first <= (int64_t)a.n_rows - n;
+    const bool is = b < kv.n_seq;
+    const int at = is ? b : 0;
+    // (all asked for before any is waited for)
+    int n = a.n_new[at], len = a.len[at], held = a.in.held[at], shared = a.shared ? a.shared[at] : 0;
+    asm volatile("" : "+v"(n), "+v"(len), "+v"(held), "+v"(shared));
+    n = is ? max(n, 0) : 0;
+    int64_t upto[1] = {n}, total[1];
+    group_upto(upto, total, s_wave);
+    SeqPlan s{};
+    s.first = rows + upto[0] - n;
+    rows += total[0];
+    if (!is) return s;
+    s.held = min(max(held, 0), kv.table_len);
+    const bool ok = len >= 0 && n <= kv.cap && len <= kv.cap - n && s.first <= (int64_t)a.n_rows - n;
     s.n = ok ? n : 0;
     int need = 0;
     if (len > kv.cap)
         need = s.held;
     else if (len + s.n > 0)
         need = kv.page_of(len + s.n - 1) + 1;
-    s.stays = min(s.held, max(need, a.shared ? a.shared[b] : 0));
+    s.stays = min(s.held, max(need, shared));
     s.asks = s.n > 0 ? max(0, need - s.held) : 0;
     return s;
 }
 
+// Places in the table of KP_PER entries from the k-th of the workgroup's
+// sequences' on, -1 past the last: entry k is (its sequence's sum - k) before its
+// sequence's end.
+__device__ __forceinline__ void deal(int64_t (&e)[KP_PER], const uint32_t *s_upto, const int *s_end, int table_len, int c0, uint32_t k,
+                                     uint32_t items)
+{
+#pragma unroll
+    for (int j = 0; j < KP_PER; j++) e[j] = -1;
+    if (k >= items) return;
+    int i = first_above(s_upto, k);
+    uint32_t upto = s_upto[i];
+#pragma unroll
+    for (int j = 0; j < KP_PER; j++)
+        if (k + j < items) {
+            if (upto <= k + j) {
+                i = first_above(s_upto, k + j);
+                upto = s_upto[i];
+            }
+            e[j] = (int64_t)(c0 + i) * table_len + s_end[i] - (int)(upto - (k + j));
+        }
+}
+
 __global__ void __launch_bounds__(KP_WG) k_kv_plan(KvPlanArgs a)
 {
-    __shared__ int64_t s_wave[KP_WG / 64], s_upto[KP_WG];
-    __shared__ int s_from[KP_WG];
+    __shared__ int64_t s_rows[1][KP_WAVES];
+    __shared__ uint32_t s_wave[2][KP_WAVES], s_upto[KP_WG];
+    __shared__ int s_end[KP_WG];
     const KvView &kv = a.kv;
     const int tid = threadIdx.x;
-    const int had = min(max(a.in.n_free[0], 0), kv.n_pages);
+    const int top = a.in.n_free[0];
+    const bool one = kv.n_seq <= KP_WG;  // one round: what the first pass finds, the second has
     // entries that come back, in order
     int64_t rows = 0, back = 0;
+    SeqPlan s{};
+    uint32_t upto[2], total[2];
     for (int c0 = 0; c0 < kv.n_seq; c0 += KP_WG) {
-        const int b = c0 + tid;
-        const bool is = b < kv.n_seq;
-        const int64_t n = is ? max(a.n_new[b], 0) : 0;
-        int64_t total, items;
-        const int64_t upto = group_upto(n, s_wave, total);
-        SeqPlan s{};
-        if (is) s = plan_seq(a, b, rows + upto - n);
-        rows += total;
-        const int64_t mine = group_upto(s.held - s.stays, s_wave, items);
-        if (items == 0) continue;
-        s_upto[tid] = mine;
-        s_from[tid] = s.held;
+        s = plan_seq(a, c0 + tid, rows, s_rows);
+        upto[0] = s.held - s.stays;
+        upto[1] = s.asks;
+        group_upto(upto, total, s_wave);
+        if (total[0] == 0) continue;
+        const int had = min(max(top, 0), kv.n_pages);
+        s_upto[tid] = upto[0];
+        s_end[tid] = s.held;
         __syncthreads();
-        for (int64_t k0 = 0; k0 < items; k0 += KP_WG) {
-            const int64_t k = k0 + tid;
-            int page = -1;
-            if (k < items) {
-                // counted from the end of the sequence's entries
-                const int i = first_above(s_upto, KP_WG, k);
-                const int64_t e = (int64_t)(c0 + i) * kv.table_len + s_from[i] - (s_upto[i] - k);
-                page = a.in.table[e];
-                a.out.table[e] = -1;
+        for (uint32_t k0 = 0; k0 < total[0]; k0 += KP_WG * KP_PER) {
+            int64_t e[KP_PER];
+            deal(e, s_upto, s_end, kv.table_len, c0, k0 + tid * KP_PER, total[0]);
+            int page[KP_PER];
+#pragma unroll
+            for (int j = 0; j < KP_PER; j++) page[j] = e[j] >= 0 ? a.in.table[e[j]] : -1;
+            uint32_t good[1] = {0}, found[1];
+#pragma unroll
+            for (int j = 0; j < KP_PER; j++) {
+                if (e[j] >= 0) a.out.table[e[j]] = -1;
+                good[0] += (uint32_t)page[j] < (uint32_t)kv.n_pages;
             }
-            const bool good = (uint32_t)page < (uint32_t)kv.n_pages;
-            int64_t found;
-            const int64_t at = had + back + group_upto(good, s_wave, found) - 1;
-            if (good && at < kv.n_pages) a.out.free_pages[at] = page;
-            back += found;
+            const uint32_t mine = good[0];
+            group_upto(good, found, s_wave);
+            int64_t to = had + back + good[0] - mine;
+#pragma unroll
+            for (int j = 0; j < KP_PER; j++)
+                if ((uint32_t)page[j] < (uint32_t)kv.n_pages) {
+                    if (to < kv.n_pages) a.out.free_pages[to] = page[j];
+                    to++;
+                }
+            back += found[0];
         }
     }
-    const int high = (int)min((int64_t)kv.n_pages, had + back);
+    const int had = min(max(top, 0), kv.n_pages), high = (int)min((int64_t)kv.n_pages, had + back);
     // pages that go out
     rows = 0;
     int64_t asked = 0, taken = 0;
     for (int c0 = 0; c0 < kv.n_seq; c0 += KP_WG) {
         const int b = c0 + tid;
-        const bool is = b < kv.n_seq;
-        const int64_t n = is ? max(a.n_new[b], 0) : 0;
-        int64_t total;
-        const int64_t upto = group_upto(n, s_wave, total);
-        SeqPlan s{};
-        if (is) s = plan_seq(a, b, rows + upto - n);
-        rows += total;
-        const int64_t sum = asked + group_upto(s.asks, s_wave, total);
-        asked += total;
-        const bool given = s.asks == 0 || sum <= high;
-        if (is) {
+        if (!one) {
+            s = plan_seq(a, b, rows, s_rows);
+            upto[1] = s.asks;
+            group_upto(upto, total, s_wave);
+        }
+        const bool given = s.asks == 0 || asked + upto[1] <= high;
+        if (b < kv.n_seq) {
             a.first[b] = (int)min(s.first, (int64_t)INT32_MAX);
             a.count[b] = given ? s.n : 0;
             a.out.held[b] = s.stays + (given ? s.asks : 0);
         }
-        const int64_t mine = group_upto(given ? s.asks : 0, s_wave, total);
-        if (total == 0) continue;
-        s_upto[tid] = mine;
-        s_from[tid] = s.held + s.asks;
+        const int64_t room = high - asked;  // (those who are served come first)
+        asked += total[1];
+        if (total[1] == 0 || room <= 0) continue;
         __syncthreads();
-        for (int64_t k = tid; k < total; k += KP_WG) {
-            const int i = first_above(s_upto, KP_WG, k);
-            const int at = high - 1 - (int)(taken + k);
-            a.out.table[(int64_t)(c0 + i) * kv.table_len + s_from[i] - (s_upto[i] - k)] =
-                at < had ? a.in.free_pages[at] : a.out.free_pages[at];
-            a.out.free_pages[at] = -1;
+        s_upto[tid] = upto[1];
+        s_end[tid] = s.held + s.asks;
+        __syncthreads();
+        uint32_t items = total[1];
+        if (items > room) {  // up to the last that is served
+            const int i = first_above(s_upto, (uint32_t)room);
+            items = i ? s_upto[i - 1] : 0;
         }
-        taken += total;
+        for (uint32_t k0 = 0; k0 < items; k0 += KP_WG * KP_PER) {
+            const uint32_t k = k0 + tid * KP_PER;
+            int64_t e[KP_PER];
+            deal(e, s_upto, s_end, kv.table_len, c0, k, items);
+            int page[KP_PER];
+#pragma unroll
+            for (int j = 0; j < KP_PER; j++) {
+                const int at = high - 1 - (int)(taken + k + j);
+                page[j] = e[j] < 0 ? 0 : at < had ? a.in.free_pages[at] : a.out.free_pages[at];
+            }
+#pragma unroll
+            for (int j = 0; j < KP_PER; j++)
+                if (e[j] >= 0) {
+                    a.out.table[e[j]] = page[j];
+                    a.out.free_pages[high - 1 - (int)(taken + k + j)] = -1;
+                }
+        }
+        taken += items;
     }
     if (tid == 0) a.out.n_free[0] = high - (int)taken;
 }
