@@ -7,9 +7,13 @@
 // in f64 to the end and rounded to f32 and then to the type, so that a cache
 // holds the same bits whatever the order of a sum.
 //
-// Bound: HBM, each value read once and written once.  A head is VEC values a
-// lane; the partner of a dim, which for a part of a head may lie anywhere, is
-// read back from LDS.
+// Bound: HBM, each value read once and written once.  A head is 16 bytes a lane;
+// a wave takes heads of one row, the next under way while one is turned, and
+// keeps the row's sines and cosines.  The partner of a dim is in the same lane
+// where pairs are neighbours, else it is read back from LDS (for a part of a
+// head it may lie anywhere).
+#include <algorithm>
+
 #include "kv_chunk.h"
 #include "lanes.h"
 
@@ -49,17 +53,39 @@ template <typename T, int N> __device__ __forceinline__ void store_row(T *p, con
 template <typename TI, typename TQ, typename TC, int HD>
 __global__ void __launch_bounds__(KA_WG) k_kv_append(KvAppendArgs a)
 {
-    constexpr int VEC = sizeof(TI) == 2 ? 8 : 4, LPH = HD / VEC, HEADS = KA_WG / LPH;
-    __shared__ float s_x[HEADS][HD + 4];
+    constexpr int VEC = sizeof(TI) == 2 ? 8 : 4, LPH = HD / VEC, HPW = 64 / LPH;  // heads of a wave at once
+    __shared__ __align__(16) float s_x[KA_WG / 64][HPW][HD + 4];
     const KvView &kv = a.kv;
-    const int row = blockIdx.x, tid = threadIdx.x, slot = tid / LPH, d0 = tid % LPH * VEC;
+    const int row = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int slot = lane / LPH, d0 = lane % LPH * VEC;
     const int pos = a.rope ? a.row_pos[row] : 0;
-    if (a.rope && (uint32_t)pos >= (uint32_t)a.n_pos) return;
     const int at = a.k ? a.row_at[row] : -1;
+    if (a.rope && (uint32_t)pos >= (uint32_t)a.n_pos) return;
     const bool store = at >= 0 && at < kv.n_pages * kv.page_tokens;
+    // groups of heads: q's, then k's, then v's
+    const int gq = (a.nh + HPW - 1) / HPW, gk = (kv.nkv + HPW - 1) / HPW, groups = gq + (store ? 2 * gk : 0);
+    const int step = gridDim.y * (KA_WG / 64);
+    struct Head {
+        int kind, h;  // 0 q, 1 k, 2 v; head
+    };
+    auto head_of = [&](int g) {
+        const int kind = g < gq ? 0 : g < gq + gk ? 1 : 2;
+        return Head{kind, (kind == 0 ? g : kind == 1 ? g - gq : g - gq - gk) * HPW + slot};
+    };
+    auto load = [&](int g, float (&x)[VEC]) {
+        const Head o = head_of(g);
+        const TI *p = o.kind == 0   ? (const TI *)a.q + row * a.ldq + (int64_t)min(o.h, a.nh - 1) * HD
+                      : o.kind == 1 ? (const TI *)a.k + row * a.ldk + (int64_t)min(o.h, kv.nkv - 1) * HD
+                                    : (const TI *)a.v + row * a.ldv + (int64_t)min(o.h, kv.nkv - 1) * HD;
+        load_row<TI, VEC>(p + d0, x);
+    };
+    int g = blockIdx.y * (KA_WG / 64) + wave;
+    if (g >= groups) return;
+    float next[VEC];
+    load(g, next);
     // this lane's dims: (cos, sin), the sign of the partner's sine, its dim
     const int half = a.n_rot / 2;
-    double c[VEC], s[VEC];
+    double c[VEC], s[VEC], cw[VEC], sw[VEC];
     int other[VEC];
 #pragma unroll
     for (int e = 0; e < VEC; e++) {
@@ -75,63 +101,78 @@ __global__ void __launch_bounds__(KA_WG) k_kv_append(KvAppendArgs a)
             s[e] = hi ? cs.y : -cs.y;
         }
     }
-    const int heads = a.nh + (store ? 2 * kv.nkv : 0);
-    for (int h0 = 0; h0 < heads; h0 += HEADS) {
-        const int h = h0 + slot;
-        const bool is = h < heads, is_q = h < a.nh, is_v = h >= a.nh + kv.nkv;
+    int kind = -1;
+    for (; g < groups; g += step) {
+        const Head o = head_of(g);
         float x[VEC];
-        if (is) {
-            const TI *p = is_q    ? (const TI *)a.q + row * a.ldq + (int64_t)h * HD
-                          : is_v ? (const TI *)a.v + row * a.ldv + (int64_t)(h - a.nh - kv.nkv) * HD
-                                 : (const TI *)a.k + row * a.ldk + (int64_t)(h - a.nh) * HD;
-            load_row<TI, VEC>(p + d0, x);
-        } else {
 #pragma unroll
-            for (int e = 0; e < VEC; e++) x[e] = 0.0f;
-        }
-        const float *w = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
-        double f = 1.0, ss = 0.0;
+        for (int e = 0; e < VEC; e++) x[e] = next[e];
+        if (g + step < groups) load(g + step, next);
+        const bool is = o.h < (o.kind ? kv.nkv : a.nh);
+        if (o.kind < 2) {
+            const float *w = o.kind ? a.k_norm : a.q_norm;
+            if (o.kind != kind) {  // the norm's weights of the dim and of its partner
+                kind = o.kind;
 #pragma unroll
-        for (int e = 0; e < VEC; e++) ss += (double)x[e] * x[e];
+                for (int e = 0; e < VEC; e++) {
+                    cw[e] = w ? c[e] * w[d0 + e] : c[e];
+                    sw[e] = w ? s[e] * w[other[e]] : s[e];
+                }
+            }
+            double f = 1.0;
+            if (w) {
+                double ss = 0.0;
 #pragma unroll
-        for (int m = 1; m < LPH; m <<= 1) ss += __shfl_xor(ss, m);
-        if (w) f = 1.0 / sqrt(ss * (1.0 / HD) + (double)a.eps);
-        __syncthreads();
+                for (int e = 0; e < VEC; e++) ss += (double)x[e] * x[e];
 #pragma unroll
-        for (int e = 0; e < VEC; e++) s_x[slot][d0 + e] = x[e];
-        __syncthreads();
-        if (!is) continue;
-        if (!is_v) {
-            float y[VEC];
+                for (int m = 1; m < LPH; m <<= 1) ss += __shfl_xor(ss, m);
+                f = 1.0 / sqrt(ss * (1.0 / HD) + (double)a.eps);
+            }
+            float xo[VEC];
+            if (a.interleaved) {
+#pragma unroll
+                for (int e = 0; e < VEC; e++) xo[e] = x[e ^ 1];
+            } else {
+                // (a wave's LDS operations are carried out in order)
+#pragma unroll
+                for (int e = 0; e < VEC; e += 4) *(styx_f4 *)&s_x[wave][slot][d0 + e] = styx_f4{x[e], x[e + 1], x[e + 2], x[e + 3]};
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+                for (int e = 0; e < VEC; e++) xo[e] = s_x[wave][slot][other[e]];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            }
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
-                const double me = w ? x[e] * f * w[d0 + e] : x[e];
-                const float xo = s_x[slot][other[e]];
-                const double you = w ? xo * f * w[other[e]] : xo;
+                const double me = x[e] * cw[e];
                 // (a dim that is not turned keeps its value, whatever it is)
-                float v = (float)(d0 + e < a.n_rot ? me * c[e] + you * s[e] : me);
+                float v = (float)(f * (d0 + e < a.n_rot ? me + xo[e] * sw[e] : me));
                 // (kept apart from a conversion to f16 that may follow:
                 // contracted with it, the f64 value would be rounded to f16 directly)
                 asm volatile("" : "+v"(v));
-                y[e] = v;
+                x[e] = v;
             }
-#pragma unroll
-            for (int e = 0; e < VEC; e++) x[e] = y[e];
         }
-        if (is_q) {
-            store_row<TQ, VEC>((TQ *)a.q_out + row * a.ldo + (int64_t)h * HD + d0, x);
-        } else {
-            TC *pool = (TC *)(is_v ? kv.vpool : kv.kpool);
-            store_row<TC, VEC>(pool + ((int64_t)at * kv.nkv + (h - a.nh) % kv.nkv) * HD + d0, x);
-        }
+        if (!is) continue;
+        if (o.kind == 0)
+            store_row<TQ, VEC>((TQ *)a.q_out + row * a.ldo + (int64_t)o.h * HD + d0, x);
+        else
+            store_row<TC, VEC>((TC *)(o.kind == 1 ? kv.kpool : kv.vpool) + ((int64_t)at * kv.nkv + o.h) * HD + d0, x);
     }
 }
 
-int64_t kv_append_grid(const KvAppendArgs &a) { return a.n_rows; }
+// Workgroups of a row: as many as its heads make where rows are few, so that
+// the chip is filled, else one, whose waves keep the row's sines and cosines.
+static int row_groups(const KvAppendArgs &a)
+{
+    const int vec = a.in_f16 ? 8 : 4, hpw = 64 / (a.kv.hd / vec);
+    const int64_t groups = (a.nh + hpw - 1) / hpw + (a.k ? 2 * ((a.kv.nkv + hpw - 1) / hpw) : 0), most = (groups + 3) / 4;
+    return (int)std::min<int64_t>(std::max<int64_t>(1, std::min<int64_t>(most, 2048 / std::max(a.n_rows, 1))), 65535);
+}
+int64_t kv_append_grid(const KvAppendArgs &a) { return (int64_t)a.n_rows * row_groups(a); }
 
 template <typename TI, typename TQ, typename TC> static void launch_hd(hipStream_t st, const KvAppendArgs &a)
 {
-    const dim3 g((unsigned)kv_append_grid(a)), wg(KA_WG);
+    const dim3 g((unsigned)a.n_rows, (unsigned)row_groups(a)), wg(KA_WG);
     switch (a.kv.hd) {
     case 64: hipLaunchKernelGGL((k_kv_append<TI, TQ, TC, 64>), g, wg, 0, st, a); break;
     case 128: hipLaunchKernelGGL((k_kv_append<TI, TQ, TC, 128>), g, wg, 0, st, a); break;

@@ -11,7 +11,7 @@
 // not depend on an order of execution.
 //
 // Two launches: the sequences by one workgroup (1024 at a time; entries that
-// come back and pages that go out are dealt to its threads, four at a time,
+// come back and pages that go out are dealt to its threads, two at a time,
 // whatever sequence they belong to), then the rows, and where the result goes
 // to arrays of its own the entries and pages that stay, by many.  Bound: the
 // latency of the first launch, whose few reads wait for each other: lengths,
@@ -21,7 +21,7 @@
 
 namespace styx {
 
-constexpr int KP_WG = 1024, KP_WAVES = KP_WG / 64, KP_ROWS = 256, KP_PER = 4;
+constexpr int KP_WG = 1024, KP_WAVES = KP_WG / 64, KP_ROWS = 256, KP_PER = 2;
 
 // Inclusive sums of N numbers over the workgroup's threads, and their totals.
 template <typename T, int N> __device__ __forceinline__ void group_upto(T (&v)[N], T (&total)[N], T (*s_wave)[KP_WAVES])
@@ -86,32 +86,26 @@ __device__ __forceinline__ SeqPlan plan_seq(const KvPlanArgs &a, int b, int64_t 
     return s;
 }
 
-// Places in the table of KP_PER entries from the k-th of the workgroup's
-// sequences' on, -1 past the last: entry k is (its sequence's sum - k) before its
-// sequence's end.
+// Places in the table of every KP_WG-th entry from the k-th of the workgroup's
+// sequences' on, -1 past the last: entry k is (its sequence's sum - k) before
+// its sequence's end.
 __device__ __forceinline__ void deal(int64_t (&e)[KP_PER], const uint32_t *s_upto, const int *s_end, int table_len, int c0, uint32_t k,
                                      uint32_t items)
 {
+    int i[KP_PER];
 #pragma unroll
-    for (int j = 0; j < KP_PER; j++) e[j] = -1;
-    if (k >= items) return;
-    int i = first_above(s_upto, k);
-    uint32_t upto = s_upto[i];
+    for (int j = 0; j < KP_PER; j++) i[j] = first_above(s_upto, min(k + j * KP_WG, items - 1));
 #pragma unroll
-    for (int j = 0; j < KP_PER; j++)
-        if (k + j < items) {
-            if (upto <= k + j) {
-                i = first_above(s_upto, k + j);
-                upto = s_upto[i];
-            }
-            e[j] = (int64_t)(c0 + i) * table_len + s_end[i] - (int)(upto - (k + j));
-        }
+    for (int j = 0; j < KP_PER; j++) {
+        const uint32_t kj = k + j * KP_WG;
+        e[j] = kj < items ? (int64_t)(c0 + i[j]) * table_len + s_end[i[j]] - (int)(s_upto[i[j]] - kj) : -1;
+    }
 }
 
 __global__ void __launch_bounds__(KP_WG) k_kv_plan(KvPlanArgs a)
 {
     __shared__ int64_t s_rows[1][KP_WAVES];
-    __shared__ uint32_t s_wave[2][KP_WAVES], s_upto[KP_WG];
+    __shared__ uint32_t s_wave[KP_PER][KP_WAVES], s_upto[KP_WG];
     __shared__ int s_end[KP_WG];
     const KvView &kv = a.kv;
     const int tid = threadIdx.x;
@@ -133,26 +127,23 @@ __global__ void __launch_bounds__(KP_WG) k_kv_plan(KvPlanArgs a)
         __syncthreads();
         for (uint32_t k0 = 0; k0 < total[0]; k0 += KP_WG * KP_PER) {
             int64_t e[KP_PER];
-            deal(e, s_upto, s_end, kv.table_len, c0, k0 + tid * KP_PER, total[0]);
+            deal(e, s_upto, s_end, kv.table_len, c0, k0 + tid, total[0]);
             int page[KP_PER];
 #pragma unroll
             for (int j = 0; j < KP_PER; j++) page[j] = e[j] >= 0 ? a.in.table[e[j]] : -1;
-            uint32_t good[1] = {0}, found[1];
+            uint32_t at[KP_PER], found[KP_PER];
 #pragma unroll
             for (int j = 0; j < KP_PER; j++) {
                 if (e[j] >= 0) a.out.table[e[j]] = -1;
-                good[0] += (uint32_t)page[j] < (uint32_t)kv.n_pages;
+                at[j] = (uint32_t)page[j] < (uint32_t)kv.n_pages;
             }
-            const uint32_t mine = good[0];
-            group_upto(good, found, s_wave);
-            int64_t to = had + back + good[0] - mine;
+            group_upto(at, found, s_wave);
 #pragma unroll
-            for (int j = 0; j < KP_PER; j++)
-                if ((uint32_t)page[j] < (uint32_t)kv.n_pages) {
-                    if (to < kv.n_pages) a.out.free_pages[to] = page[j];
-                    to++;
-                }
-            back += found[0];
+            for (int j = 0; j < KP_PER; j++) {
+                const int64_t to = had + back + at[j] - 1;
+                if ((uint32_t)page[j] < (uint32_t)kv.n_pages && to < kv.n_pages) a.out.free_pages[to] = page[j];
+                back += found[j];
+            }
         }
     }
     const int had = min(max(top, 0), kv.n_pages), high = (int)min((int64_t)kv.n_pages, had + back);
@@ -185,20 +176,20 @@ __global__ void __launch_bounds__(KP_WG) k_kv_plan(KvPlanArgs a)
             items = i ? s_upto[i - 1] : 0;
         }
         for (uint32_t k0 = 0; k0 < items; k0 += KP_WG * KP_PER) {
-            const uint32_t k = k0 + tid * KP_PER;
+            const uint32_t k = k0 + tid;
             int64_t e[KP_PER];
             deal(e, s_upto, s_end, kv.table_len, c0, k, items);
             int page[KP_PER];
 #pragma unroll
             for (int j = 0; j < KP_PER; j++) {
-                const int at = high - 1 - (int)(taken + k + j);
+                const int at = high - 1 - (int)(taken + k + j * KP_WG);
                 page[j] = e[j] < 0 ? 0 : at < had ? a.in.free_pages[at] : a.out.free_pages[at];
             }
 #pragma unroll
             for (int j = 0; j < KP_PER; j++)
                 if (e[j] >= 0) {
                     a.out.table[e[j]] = page[j];
-                    a.out.free_pages[high - 1 - (int)(taken + k + j)] = -1;
+                    a.out.free_pages[high - 1 - (int)(taken + k + j * KP_WG)] = -1;
                 }
         }
         taken += items;
