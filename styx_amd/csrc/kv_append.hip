@@ -51,7 +51,7 @@ template <typename T, int N> __device__ __forceinline__ void store_row(T *p, con
 }
 
 template <typename TI, typename TQ, typename TC, int HD>
-__global__ void __launch_bounds__(KA_WG) k_kv_append(KvAppendArgs a)
+__global__ void __launch_bounds__(KA_WG, 4) k_kv_append(KvAppendArgs a)
 {
     constexpr int VEC = sizeof(TI) == 2 ? 8 : 4, LPH = HD / VEC, HPW = 64 / LPH;  // heads of a wave at once
     __shared__ __align__(16) float s_x[KA_WG / 64][HPW][HD + 4];
@@ -83,24 +83,11 @@ __global__ void __launch_bounds__(KA_WG) k_kv_append(KvAppendArgs a)
     if (g >= groups) return;
     float next[VEC];
     load(g, next);
-    // this lane's dims: (cos, sin), the sign of the partner's sine, its dim
+    // of this lane's dims: cosine, and the partner's sine with its sign, times
+    // the norm's weights; the partner
+    double c[VEC], s[VEC];
     const int half = a.n_rot / 2;
-    double c[VEC], s[VEC], cw[VEC], sw[VEC];
-    int other[VEC];
-#pragma unroll
-    for (int e = 0; e < VEC; e++) {
-        const int d = d0 + e;
-        c[e] = 1.0;
-        s[e] = 0.0;
-        other[e] = d;
-        if (d < a.n_rot) {
-            const bool hi = a.interleaved ? d & 1 : d >= half;
-            const double2 cs = a.rope[(int64_t)pos * half + (a.interleaved ? d >> 1 : hi ? d - half : d)];
-            other[e] = a.interleaved ? d ^ 1 : hi ? d - half : d + half;
-            c[e] = cs.x;
-            s[e] = hi ? cs.y : -cs.y;
-        }
-    }
+    auto other = [&](int d) { return d >= a.n_rot ? d : a.interleaved ? d ^ 1 : d >= half ? d - half : d + half; };
     int kind = -1;
     for (; g < groups; g += step) {
         const Head o = head_of(g);
@@ -111,13 +98,22 @@ __global__ void __launch_bounds__(KA_WG) k_kv_append(KvAppendArgs a)
         const bool is = o.h < (o.kind ? kv.nkv : a.nh);
         if (o.kind < 2) {
             const float *w = o.kind ? a.k_norm : a.q_norm;
-            if (o.kind != kind) {  // the norm's weights of the dim and of its partner
+            if (o.kind != kind) {
                 kind = o.kind;
 #pragma unroll
                 for (int e = 0; e < VEC; e++) {
-                    cw[e] = w ? c[e] * w[d0 + e] : c[e];
-                    sw[e] = w ? s[e] * w[other[e]] : s[e];
+                    const int d = d0 + e;
+                    double2 cs = {1.0, 0.0};
+                    if (d < a.n_rot) cs = a.rope[(int64_t)pos * half + (a.interleaved ? d >> 1 : d >= half ? d - half : d)];
+                    c[e] = cs.x;
+                    s[e] = (a.interleaved ? d & 1 : d >= half) ? cs.y : -cs.y;
                 }
+                if (w)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) {
+                        c[e] *= w[d0 + e];
+                        s[e] *= w[other(d0 + e)];
+                    }
             }
             double f = 1.0;
             if (w) {
@@ -138,14 +134,14 @@ __global__ void __launch_bounds__(KA_WG) k_kv_append(KvAppendArgs a)
                 for (int e = 0; e < VEC; e += 4) *(styx_f4 *)&s_x[wave][slot][d0 + e] = styx_f4{x[e], x[e + 1], x[e + 2], x[e + 3]};
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-                for (int e = 0; e < VEC; e++) xo[e] = s_x[wave][slot][other[e]];
+                for (int e = 0; e < VEC; e++) xo[e] = s_x[wave][slot][other(d0 + e)];
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             }
 #pragma unroll
             for (int e = 0; e < VEC; e++) {
-                const double me = x[e] * cw[e];
+                const double me = x[e] * c[e];
                 // (a dim that is not turned keeps its value, whatever it is)
-                float v = (float)(f * (d0 + e < a.n_rot ? me + xo[e] * sw[e] : me));
+                float v = (float)(f * (d0 + e < a.n_rot ? me + xo[e] * s[e] : me));
                 // (kept apart from a conversion to f16 that may follow:
                 // contracted with it, the f64 value would be rounded to f16 directly)
                 asm volatile("" : "+v"(v));
