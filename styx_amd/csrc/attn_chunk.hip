@@ -413,11 +413,19 @@ template <int BM, bool TILES> __device__ __forceinline__ Place find_place(const 
 }
 
 // ------------------------------------------------------------- the tiles ---
-// Partial results, of a share's first piece and of its last: sums o, and m and l.
+// A tile that begins in a share and goes on in the next: its pieces, one in
+// each of as many shares, the first at `part0`.  pieces 0: there is none.
+struct alignas(16) Across {
+    int pieces, tile, part0;
+    ChunkSeq s;
+};
+// Partial results, of a share's first piece and of its last (sums o, and m and
+// l), and the tiles that they are of, by share and kv head.
 struct Parts {
     float *o;
     float2 *ml;
-    int rows;  // of a piece
+    Across *across;
+    int rows, shares;  // of a piece; at most
 };
 
 template <typename TQ, typename TC, int HD>
@@ -444,6 +452,7 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD>::NW), 2) k_attn_chunk(A
     const int64_t stride = (int64_t)kv.nkv * La::ROW;
     const char *kp = (const char *)kv.kpool + kvh * La::ROW, *vp = (const char *)kv.vpool + kvh * La::ROW;
     const uint32_t lk = lds_at(&s_k[0][0]), lv = lds_at(&s_v[0][0]);
+    if (threadIdx.x == 0 && nth < parts.shares) parts.across[nth * kv.nkv + kvh].pieces = 0;
     for (bool more = true; more;) {
     // (a lane number that the compiler takes for a new one in every trip: what
     // is computed from it would else be kept in registers over the trips)
@@ -473,6 +482,10 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD>::NW), 2) k_attn_chunk(A
         }
         u += to - it.in;
         more = u < end;
+        if (threadIdx.x == 0 && it.in == 0 && !whole) {
+            const int pieces = (int)((it.before + it.length - 1) / line.share) - nth + 1;
+            parts.across[nth * kv.nkv + kvh] = Across{pieces, it.tile, (int)(part / kv.nkv), s};
+        }
     }
     b0 = uniform(b0);
     b1 = uniform(b1);
@@ -730,8 +743,7 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD>::NW), 2) k_attn_chunk(A
     }
 }
 
-// The pieces of a tile that lies across an end of a share joined, by those of
-// the first such end: ROWS rows a workgroup, four dims a thread, threads beyond
+// The pieces of a tile that lies across ends of shares joined: ROWS rows a workgroup, four dims a thread, threads beyond
 // the rows taking every other piece.
 constexpr int AC_JOIN = 256;
 template <typename TQ, typename TC, int HD, int ROWS>
@@ -743,19 +755,13 @@ __global__ void __launch_bounds__(AC_JOIN) k_attn_chunk_join(AttnChunkArgs a, Pa
     __shared__ styx_f4 s_o[AC_JOIN];
     __shared__ float2 s_ml[AC_JOIN];
     const KvView &kv = a.kv;
-    const Line line = line_of<BM, KT>(a, AC_CUS * W::PER_CU);
     const int w0 = blockIdx.z, kvh = blockIdx.y;
-    const int64_t u = (w0 + 1) * line.share;
-    if (!line.share || u >= line.total) return;
-    const Place it = find_place<BM, false>(a, u);
-    if (it.b < 0 || it.in == 0 || it.before < w0 * line.share) return;
-    const int pieces = (int)((it.before + it.length - 1) / line.share - w0) + 1;
-    // the first piece is its share's last unless the share begins with it
-    const int64_t part0 = 2 * (int64_t)w0 + (it.before > w0 * line.share);
+    const Across it = parts.across[w0 * kv.nkv + kvh];
+    const int pieces = it.pieces, rows = it.s.count * a.gqa - it.tile * BM;
     const int tid = threadIdx.x, d = tid % PER_ROW * 4, in = blockIdx.x * ROWS + tid / PER_ROW % ROWS, group = tid / PER_ROW / ROWS;
+    if (pieces == 0 || (int)blockIdx.x * ROWS >= min(rows, parts.rows)) return;
     const int r = it.tile * BM + in;
-    const bool is = in < parts.rows && r < it.s.count * a.gqa;
-    if (blockIdx.x * ROWS >= parts.rows || it.tile * BM + (int)blockIdx.x * ROWS >= it.s.count * a.gqa) return;
+    const bool is = in < min(rows, parts.rows);
     float m = -INFINITY, l = 0.0f;
     styx_f4 o = {};
     for (int c0 = group; c0 < pieces; c0 += GROUPS * AHEAD) {
@@ -765,7 +771,7 @@ __global__ void __launch_bounds__(AC_JOIN) k_attn_chunk_join(AttnChunkArgs a, Pa
 #pragma unroll
         for (int c = 0; c < AHEAD; c++) {
             const int cc = min(c0 + c * GROUPS, pieces - 1);
-            const int64_t p = ((cc ? 2 * (int64_t)(w0 + cc) : part0) * kv.nkv + kvh) * parts.rows + (is ? in : 0);
+            const int64_t p = ((int64_t)(cc ? 2 * (w0 + cc) : it.part0) * kv.nkv + kvh) * parts.rows + (is ? in : 0);
             ml[c] = parts.ml[p];
             po[c] = *(const styx_f4 *)(parts.o + p * HD + d);
         }
@@ -832,6 +838,7 @@ struct ChunkShape {
     int shares;     // of a kv head, at most
     int rows;       // of a piece's partial results
     int64_t parts(int nkv) const { return 2 * (int64_t)shares * nkv * rows; }
+    int64_t floats(int nkv, int hd) const { return parts(nkv) * (hd + 2) + (int64_t)shares * nkv * (int)(sizeof(Across) / 4); }
 };
 static ChunkShape shape_of(int bm, int per_cu, int n_seq, int nkv, int gqa, int n_rows)
 {
@@ -868,7 +875,7 @@ uint64_t attn_chunk_ws_bytes(int n_seq, int nkv, int hd, int gqa, int n_rows)
         with_kernel(t > 0, t > 1, hd, [&](auto tq, auto tc, auto n) {
             using W = Wave<decltype(tq), decltype(tc), decltype(n)::value>;
             static_assert(W::BM >= 128 && W::PER_CU <= 2, "attn_chunk_grid");
-            floats = std::max(floats, shape_of(W::BM, W::PER_CU, n_seq, nkv, gqa, n_rows).parts(nkv) * (hd + 2));
+            floats = std::max(floats, shape_of(W::BM, W::PER_CU, n_seq, nkv, gqa, n_rows).floats(nkv, hd));
             return 0;
         });
     return 4ull * floats;
@@ -884,7 +891,10 @@ hipError_t launch_attn_chunk(hipStream_t st, AttnChunkArgs a, void *ws)
         constexpr int HD = decltype(hd)::value;
         using W = Wave<TQ, TC, HD>;
         const ChunkShape s = shape_of(W::BM, W::PER_CU, a.kv.n_seq, a.kv.nkv, a.gqa, a.chunk.n_rows);
-        const Parts parts{(float *)ws, (float2 *)((float *)ws + s.parts(a.kv.nkv) * HD), s.rows};
+        // (the tiles first: they want 16 bytes' alignment, and sums of few rows have it behind them)
+        Across *across = (Across *)ws;
+        float *o = (float *)(across + (int64_t)s.shares * a.kv.nkv);
+        const Parts parts{o, (float2 *)(o + s.parts(a.kv.nkv) * HD), across, s.rows, s.shares};
         // rows of a wave in pages one after another, within 32 bits
         constexpr int PER_WAVE = W::KT / W::NW;
         a.runs = a.kv.page_tokens % PER_WAVE == 0 && (int64_t)a.kv.nkv * HD * (int)sizeof(TC) < (1 << 26);
