@@ -330,22 +330,25 @@ template <int HD> struct Wave<float, float, HD> {
 // workgroup by itself.
 constexpr int AC_CUS = 256;
 constexpr int AC_LEAST = 4;   // blocks of a share at least
-constexpr int AC_START = 16;  // what a share's starts, partial results and joining cost, in blocks
+constexpr int AC_TILE = 4;    // what a tile's start costs, in blocks (its rows of q, its first blocks)
+constexpr int AC_START = 16;  // what partial results and joining cost beside that
 
 // A sequence's part of the line: tile t is first + t step long, in slots times
-// rows of a token.
+// rows of a token.  (With a tile's start: of a prompt's many short first tiles a
+// share would else hold a dozen, 4096 tokens, head_dim 256: 351 us, 257 with.)
 struct SeqLine {
     int tiles;
     int64_t first, step;
     __device__ __forceinline__ int64_t upto(int64_t t) const { return t * first + step * (t * (t - 1) / 2); }
 };
-template <int BM> __device__ __forceinline__ SeqLine seq_line(const AttnChunkArgs &a, const ChunkSeq &s)
+template <int BM, int KT> __device__ __forceinline__ SeqLine seq_line(const AttnChunkArgs &a, const ChunkSeq &s)
 {
     if (s.count == 0) return {0, 0, 0};
     const int tiles = (s.count * a.gqa + BM - 1) / BM;
     const int64_t most = (int64_t)a.window * a.gqa + BM;
-    if (a.window && most < ((int64_t)s.len + s.count) * a.gqa) return {tiles, most, 0};
-    return {tiles, (int64_t)s.len * a.gqa + BM, BM};
+    const int64_t start = (int64_t)AC_TILE * KT * a.gqa;
+    if (a.window && most < ((int64_t)s.len + s.count) * a.gqa) return {tiles, most + start, 0};
+    return {tiles, (int64_t)s.len * a.gqa + BM + start, BM};
 }
 struct Line {
     int64_t share, total;  // share 0: by tiles
@@ -355,7 +358,7 @@ template <int BM, int KT> __device__ __forceinline__ Line line_of(const AttnChun
     const int lane = threadIdx.x & 63;
     int64_t tiles = 0, total = 0, longest = 0;
     for (int b0 = 0; b0 < a.kv.n_seq; b0 += 64) {
-        const SeqLine w = seq_line<BM>(a, chunk_seq(a.chunk, a.kv, b0 + lane));
+        const SeqLine w = seq_line<BM, KT>(a, chunk_seq(a.chunk, a.kv, b0 + lane));
         tiles += w.tiles;
         total += w.upto(w.tiles);
         longest = max(longest, w.tiles ? w.upto(w.tiles) - w.upto(w.tiles - 1) : (int64_t)0);
@@ -368,7 +371,7 @@ template <int BM, int KT> __device__ __forceinline__ Line line_of(const AttnChun
     // more of them leave half a tile's time unused at the end.
     const int64_t unit = (int64_t)KT * a.gqa, even = total * a.kv.nkv / slots;
     const int64_t by_tiles = tiles * a.kv.nkv <= slots ? longest : even + total / tiles / 2;
-    if (by_tiles <= even + even / 10 + AC_START * unit + BM) return {0, tiles};
+    if (by_tiles <= even + even / 10 + (AC_START + AC_TILE) * unit + BM) return {0, tiles};
     const int64_t shares = max(slots / a.kv.nkv, 1);
     return {max((total + shares - 1) / shares, AC_LEAST * unit), total};
 }
@@ -380,13 +383,13 @@ struct Place {
     int64_t in, length, before;  // at - before = in, of length
     ChunkSeq s;
 };
-template <int BM, bool TILES> __device__ __forceinline__ Place find_place(const AttnChunkArgs &a, int64_t at)
+template <int BM, int KT, bool TILES> __device__ __forceinline__ Place find_place(const AttnChunkArgs &a, int64_t at)
 {
     const int lane = threadIdx.x & 63;
     int64_t base = 0;
     for (int b0 = 0; b0 < a.kv.n_seq; b0 += 64) {
         const ChunkSeq s = chunk_seq(a.chunk, a.kv, b0 + lane);
-        const SeqLine w = seq_line<BM>(a, s);
+        const SeqLine w = seq_line<BM, KT>(a, s);
         const int64_t mine = TILES ? w.tiles : w.upto(w.tiles), upto = base + wave_upto(mine);
         if (const unsigned long long hit = __ballot(upto > at)) {
             const int l = __builtin_ctzll(hit);
@@ -459,7 +462,7 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD>::NW), 2) k_attn_chunk(A
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));
     const int n = lane & 31, h = lane >> 5;
-    const Place it = line.share ? find_place<BM, false>(a, u) : find_place<BM, true>(a, nth);
+    const Place it = line.share ? find_place<BM, KT, false>(a, u) : find_place<BM, KT, true>(a, nth);
     if (it.b < 0 || (line.share && u >= end)) return;
     const ChunkSeq &s = it.s;
     const int rows = s.count * a.gqa, row0 = it.tile * BM;
