@@ -27,17 +27,7 @@ template <> struct Piece<float, 4> { typedef styx_f4 V; };
 template <> struct Piece<_Float16, 4> { typedef _Float16 V __attribute__((ext_vector_type(4))); };
 template <> struct Piece<_Float16, 8> { typedef h8 V; };
 
-// N consecutive values as floats / from floats, in pieces of 16 bytes at most
-template <typename T, int N> __device__ __forceinline__ void load_row(const T *p, float (&x)[N])
-{
-    constexpr int M = sizeof(T) == 4 ? 4 : N < 8 ? N : 8;
-#pragma unroll
-    for (int i = 0; i < N; i += M) {
-        const auto v = *(const typename Piece<T, M>::V *)(p + i);
-#pragma unroll
-        for (int e = 0; e < M; e++) x[i + e] = (float)v[e];
-    }
-}
+// N consecutive values, and from floats, in pieces of 16 bytes at most
 template <typename T, int N> __device__ __forceinline__ void store_row(T *p, const float (&x)[N])
 {
     constexpr int M = sizeof(T) == 4 ? 4 : N < 8 ? N : 8;
@@ -72,17 +62,17 @@ __global__ void __launch_bounds__(KA_WG, 4) k_kv_append(KvAppendArgs a)
         const int kind = g < gq ? 0 : g < gq + gk ? 1 : 2;
         return Head{kind, (kind == 0 ? g : kind == 1 ? g - gq : g - gq - gk) * HPW + slot};
     };
-    auto load = [&](int g, float (&x)[VEC]) {
-        const Head o = head_of(g);
+    typedef typename Piece<TI, VEC>::V Raw;
+    auto load = [&](int g) {
+        const Head o = head_of(min(g, groups - 1));
         const TI *p = o.kind == 0   ? (const TI *)a.q + row * a.ldq + (int64_t)min(o.h, a.nh - 1) * HD
                       : o.kind == 1 ? (const TI *)a.k + row * a.ldk + (int64_t)min(o.h, kv.nkv - 1) * HD
                                     : (const TI *)a.v + row * a.ldv + (int64_t)min(o.h, kv.nkv - 1) * HD;
-        load_row<TI, VEC>(p + d0, x);
+        return *(const Raw *)(p + d0);
     };
     int g = blockIdx.y * (KA_WG / 64) + wave;
     if (g >= groups) return;
-    float next[VEC];
-    load(g, next);
+    Raw next = load(g);  // (two or three ahead measured the same or slower)
     // of this lane's dims: cosine, and the partner's sine with its sign, times
     // the norm's weights; the partner
     double c[VEC], s[VEC];
@@ -93,8 +83,8 @@ __global__ void __launch_bounds__(KA_WG, 4) k_kv_append(KvAppendArgs a)
         const Head o = head_of(g);
         float x[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; e++) x[e] = next[e];
-        if (g + step < groups) load(g + step, next);
+        for (int e = 0; e < VEC; e++) x[e] = (float)next[e];
+        next = load(g + step);
         const bool is = o.h < (o.kind ? kv.nkv : a.nh);
         if (o.kind < 2) {
             const float *w = o.kind ? a.k_norm : a.q_norm;

@@ -162,6 +162,93 @@ def test_results_repeat(gpu, types):
     assert np.array_equal(a[0], b[0]) and np.array_equal(a[1], b[1])
 
 
+FEW = lambda n: range(n) if n < 12 else sorted({0, 1, n // 3, n // 2, n - 2, n - 1})  # noqa: E731
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("gqa", [1, 5, 16])
+def test_tiles_cut_into_shares(gpu, types, hd, gqa):
+    """Long contexts beside short ones, one token beside many: shares that end inside tiles, hold several, or none."""
+    c = Chunked(np.random.default_rng(hd * gqa), *TYPES[types], [3000, 0, 2500, 700, 1], [1, 90, 40, 3, 1], 2, gqa, hd, 48)
+    check_chunk(c, *run_chunk(gpu, c), tokens=FEW)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_cut_tiles_with_missing_pages_and_values_that_are_not_finite(gpu, types, hd):
+    c = Chunked(np.random.default_rng(hd), *TYPES[types], [3100, 2000], [5, 70], 1, 4, hd, 16)
+    rows = c.rows(1)
+    c.table[0, 20:140] = -1          # whole pieces without a row
+    c.table[0, 194:] = c.n_pages + 3  # the new rows' among them
+    for p in (c.k, c.v):
+        rest = np.ones(len(p), bool)
+        rest[np.concatenate([c.rows(b)[c.rows(b) >= 0] for b in range(2)])] = False
+        p[rest] = np.nan
+    c.v[rows[2040], 0, 3] = np.inf   # seen by the tokens from 40 on
+    out, lse = run_chunk(gpu, c)
+    check_chunk(c, out, lse, tokens=lambda n: range(min(n, 40)))
+    late = out[5 + 40:75].reshape(30, 4, hd)
+    assert not np.isfinite(late[:, :, 3]).any() and np.isfinite(np.delete(late, 3, 2)).all() and np.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("window", [700, 2500])
+def test_cut_tiles_under_a_window(gpu, types, window):
+    c = Chunked(np.random.default_rng(window), *TYPES[types], [4000, 100, 3000], [3, 60, 33], 1, 8, 128, 100, window=window)
+    check_chunk(c, *run_chunk(gpu, c), tokens=FEW)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_many_sequences_with_long_ones_among_them(gpu, types):
+    """More sequences than a wave has lanes, a few of them cut, skipped ones between."""
+    rng = np.random.default_rng(16)
+    lens = [int(n) for n in rng.integers(0, 60, 140)]
+    counts = [int(n) for n in rng.integers(0, 4, 140)]
+    for b in (3, 64, 70, 139):
+        lens[b], counts[b] = 2000 + b, 1 + b % 3
+    lens[5], lens[100] = -1, -1
+    c = Chunked(rng, *TYPES[types], lens, counts, 1, 4, 64, 32)
+    check_chunk(c, *run_chunk(gpu, c))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("nkv", [7, 40, 300, 600])
+def test_many_kv_heads(gpu, types, nkv):
+    """Fewer and fewer shares for a head, down to one."""
+    c = Chunked(np.random.default_rng(nkv), *TYPES[types], [900, 0], [1, 2], nkv, 1, 64, 64)
+    check_chunk(c, *run_chunk(gpu, c))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("scale", [0.0, -0.2, 3.0])
+def test_scales(gpu, types, scale):
+    c = Chunked(np.random.default_rng(17), *TYPES[types], [130], [9], 2, 4, 64, 16, window=50)
+    c.scale = scale
+    c.k = (c.k * 0.2).astype(c.dt)
+    out, lse = run_chunk(gpu, c)
+    c2 = Chunked(np.random.default_rng(17), *TYPES[types], [130], [9], 2, 4, 64, 16, window=50)
+    c2.k, c2.v, c2.table = c.k, c.v, c.table
+    c2.q, c2.scale = (-c.q if scale < 0 else c.q), abs(scale)  # (the bound's sums take a positive scale)
+    check_chunk(c2, out, lse)
+
+
+def test_queries_of_all_sizes_on_a_16_bit_cache(gpu):
+    """f32 queries from 1e-30 to 1e4 and rows of zeros: the pieces' power of two is the row's own."""
+    c = Chunked(np.random.default_rng(18), True, False, [60], [40], 1, 4, 64, 16)
+    size = np.float32(10.0) ** np.random.default_rng(19).uniform(-30, 2, (40, 4)).astype(np.float32)
+    c.q = (c.q.reshape(40, 4, 64) * size[:, :, None]).reshape(40, -1).astype(np.float32)
+    c.q[7] = 0
+    check_chunk(c, *run_chunk(gpu, c))
+
+
+def test_more_rows_than_the_sequences_have(gpu):
+    """A chunk laid out for a larger batch: rows behind the last sequence stay as they are."""
+    for types in TYPES.values():
+        c = Chunked(np.random.default_rng(20), *types, [900, 40], [1, 30], 2, 4, 64, 16, n_rows=5000)
+        check_chunk(c, *run_chunk(gpu, c))
+
+
 def test_offsets_past_32_bits(gpu):
     """Pools of more than 2^32 bytes and 2^31 values: rows at their ends."""
     c = Chunked(np.random.default_rng(14), True, True, [40], [9], 8, 2, 128, 64)

@@ -158,6 +158,39 @@ def test_rows_outside_the_table_or_the_pools(gpu, t):
     r.check(r.call(gpu))
 
 
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("norms", [False, True])
+@pytest.mark.parametrize("t", [L.F32, L.F16])
+def test_values_that_are_not_finite_stay_in_their_head(gpu, inter, norms, t):
+    """Without the norm in their pair, and behind the dims that are turned in their dim."""
+    r = Rows(np.random.default_rng(6), t, t, t, 6, 4, 2, 64, 32, inter, norms=norms)
+    r.qkv[1, 64 + 5] = np.nan       # q head 1, a turned dim
+    r.qkv[2, 40] = np.inf           # q head 0, one that is not
+    r.qkv[3, 4 * 64 + 7] = -np.inf  # k head 0
+    r.qkv[4, 6 * 64 + 9] = np.nan   # v head 0
+    out, kp, vp = r.call(gpu)
+    bad_q, bad_k, bad_v = (~np.isfinite(x.astype(np.float32)) for x in (out.reshape(6, 4, 64), kp[r.row_at], vp[r.row_at]))
+    pair = lambda d: {d, d ^ 1} if inter else {d, (d + 16) % 32}  # noqa: E731
+    # (under the norm NaN takes the whole head, an infinity makes the others 0)
+    whole = set(range(64))
+    for got, row, head, dims in ((bad_q, 1, 1, whole if norms else pair(5)), (bad_q, 2, 0, {40}), (bad_k, 3, 0, pair(7))):
+        assert set(np.nonzero(got[row, head])[0].tolist()) == dims
+        got[row, head] = False
+    assert not bad_q.any() and not bad_k.any()
+    assert np.argwhere(bad_v).tolist() == [[4, 0, 9]]
+
+
+@pytest.mark.parametrize("t", [L.F32, L.F16])
+def test_more_rows_than_workgroups_for_their_heads(gpu, t):
+    r = Rows(np.random.default_rng(7), t, t, t, 2100, 5, 2, 64, 64, False)
+    got = r.call(gpu)
+    keep = np.random.default_rng(8).permutation(2100)[:60]
+    for i in keep:
+        r.near(got[0][i].reshape(5, 64), r.turned(i, "q"), t)
+        r.near(got[1][r.row_at[i]], r.turned(i, "k"), t)
+        assert np.array_equal(got[2][r.row_at[i]], r.part(i, "v"))
+
+
 def test_small_and_zero_rows_under_the_norm(gpu):
     r = Rows(np.random.default_rng(4), L.F32, L.F32, L.F32, 9, 4, 2, 128, 128, False, spread=1e-5)
     r.qkv[4] = 0

@@ -200,6 +200,7 @@ def test_refusals(gpu):
               dict(o=L.KvPages(a[0], *a[5:8])), dict(o=L.KvPages(*a[0:3], a[7])), dict(n=-1), dict(len_=None), dict(new=None),
               dict(pos=None), dict(first=None), dict(count=None), dict(kv=L.KvCache(L.F32, 0, 1, 64, 8, 4, 4, None, None, None)),
               dict(kv=L.KvCache(L.F32, 2, 1, 64, 0, 4, 4, None, None, None)),
-              dict(kv=L.KvCache(L.F32, 2, 1, 64, 1 << 16, 1 << 16, 4, None, None, None))]:
+              dict(kv=L.KvCache(L.F32, 2, 1, 64, 1 << 16, 1 << 16, 4, None, None, None)),
+              dict(kv=L.KvCache(L.F32, 3, 1, 64, 1, 4, 1 << 30, None, None, None))]:
         assert call(**b) == -1, b
     gpu.sync()

@@ -149,6 +149,31 @@ def test_not_finite(gpu, types):
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_scales(gpu, types, scale):
+    c = Chunked(np.random.default_rng(8), *TYPES[types], [130], [9], 2, 4, 64, 16)
+    c.scale = abs(scale)
+    q = c.q
+    c.q = -q if scale < 0 else q
+    lse = lse_of(c)
+    c.q, c.scale = q, scale
+    got = run(gpu, c, lse, 5)
+    c.q, c.scale = (-q if scale < 0 else q), abs(scale)  # (the bound's sums take a positive scale)
+    check(c, lse, 5, got)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+def test_more_work_than_workgroups(gpu, types):
+    """More sequences than a wave has lanes, waiting ones among them, more slots than one round of workgroups takes."""
+    rng = np.random.default_rng(9)
+    lens = [int(n) for n in rng.integers(0, 700, 150)]
+    lens[7] = lens[149] = -1
+    c = Chunked(rng, *TYPES[types], lens, [1] * 150, 12, 1, 64, 64)
+    lse = lse_of(c)
+    check(c, lse, 1, run(gpu, c, lse, 1))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
 def test_results_repeat(gpu, types):
     c = Chunked(np.random.default_rng(6), *TYPES[types], [700, 90], [80, 40], 2, 8, 128, 64)
     lse = lse_of(c)
@@ -170,4 +195,5 @@ def test_refusals(gpu):
               dict(ldq=514), dict(q=q.ptr + 4), dict(window=-1), dict(last=-1), dict(lse=None), dict(acc=None)]:
         assert call(**b) == -1, b
     assert call(pos=None, where=None) == 0
+    assert call(ch=L.KvChunk(1 << 27, ch.first, ch.count, ch.len)) == -1
     gpu.sync()
