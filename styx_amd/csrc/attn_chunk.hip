@@ -88,14 +88,14 @@ template <typename TC> __device__ __forceinline__ uint32_t not_finite(uint32_t v
 // use, the factors' arithmetic between matrix instructions.
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
-template <typename TQ, typename TC, int HD> struct Wave;
+template <typename TQ, typename TC, int HD, bool FEW = false> struct Wave;
 
 // f16 caches: v_mfma_f32_32x32x16_f16.  f32 queries and their factors are two
 // f16 pieces each, hi + lo with |x - hi - lo| <= 2^-22 |x|, queries brought to
 // [2^9, 2^10) by a power of two per row so that the low pieces of all that
 // counts are normal numbers.  f16 queries take factors rounded to f16: an
 // error of at most 2^-11 of each, as large as the output's own rounding.
-template <typename TQ, int HD> struct Wave<TQ, _Float16, HD> {
+template <typename TQ, int HD> struct Wave<TQ, _Float16, HD, false> {
     using TC = _Float16;
     using La = Lay<TC, HD>;
     static constexpr int NP = sizeof(TQ) == 4 ? 2 : 1;  // pieces
@@ -103,6 +103,7 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD> {
     static constexpr int DS = HD == 256 && NP == 2 ? 2 : 1, HW = HD / DS, NK = HW / 16, ND = HW / 32;
     static constexpr int KT = HD == 256 ? 32 : 64;
     static constexpr int NW = DS == 2 ? 8 : 4, PER_CU = 8 / NW, BM = 32 * NW / DS;
+    static constexpr int IDLE = 4, BUSY = 16;  // line_of
     h8 q[NP][NK], p[KT / 32][NP][2];
     f16v s[KT / 32], o[ND];
     float mul, ref, sum[2];  // score to factor: 2^(s mul + ref); the factors' sum
@@ -244,13 +245,15 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD> {
 };
 
 // f32 caches: v_mfma_f32_32x32x2_f32, dims in fours on both sides of the score
-// product for 16-byte reads.
-template <int HD> struct Wave<float, float, HD> {
+// product for 16-byte reads.  FEW: for chunks of at most 64 query rows, which
+// leave two of four waves without any: two waves for each 32 rows.
+template <int HD, bool FEW> struct Wave<float, float, HD, FEW> {
     using TC = float;
     using La = Lay<TC, HD>;
-    static constexpr int DS = HD == 256 ? 2 : 1, HW = HD / DS, NK = HW / 8, ND = HW / 32;
+    static constexpr int DS = HD == 256 || FEW ? 2 : 1, HW = HD / DS, NK = HW / 8, ND = HW / 32;
     static constexpr int KT = 32;
-    static constexpr int NW = HD == 256 ? 8 : 4, PER_CU = 8 / NW, BM = 32 * NW / DS;
+    static constexpr int NW = 4 * DS, PER_CU = 8 / NW, BM = 32 * NW / DS;
+    static constexpr int IDLE = 2, BUSY = 8;
     styx_f4 q[NK];
     f16v s[1], o[ND];
     float mul, ref, sum[2], p[2];
@@ -331,7 +334,6 @@ template <int HD> struct Wave<float, float, HD> {
 constexpr int AC_CUS = 256;
 constexpr int AC_LEAST = 4;   // blocks of a share at least
 constexpr int AC_TILE = 4;    // what a tile's start costs, in blocks (its rows of q, its first blocks)
-constexpr int AC_START = 16;  // what partial results and joining cost beside that
 
 // A sequence's part of the line: tile t is first + t step long, in slots times
 // rows of a token.  (With a tile's start: of a prompt's many short first tiles a
@@ -353,8 +355,9 @@ template <int BM, int KT> __device__ __forceinline__ SeqLine seq_line(const Attn
 struct Line {
     int64_t share, total;  // share 0: by tiles
 };
-template <int BM, int KT> __device__ __forceinline__ Line line_of(const AttnChunkArgs &a, int slots)
+template <typename W> __device__ __forceinline__ Line line_of(const AttnChunkArgs &a)
 {
+    constexpr int BM = W::BM, KT = W::KT, slots = AC_CUS * W::PER_CU;
     const int lane = threadIdx.x & 63;
     int64_t tiles = 0, total = 0, longest = 0;
     for (int b0 = 0; b0 < a.kv.n_seq; b0 += 64) {
@@ -368,10 +371,14 @@ template <int BM, int KT> __device__ __forceinline__ Line line_of(const AttnChun
     longest = uniform(wave_most(longest));
     if (tiles == 0) return {0, 0};
     // What either costs: tiles that all run at once take as long as the longest,
-    // more of them leave half a tile's time unused at the end.
+    // more of them leave half a tile's time unused at the end; shares cost their
+    // partial results and the joining, little on a chip that is mostly idle
+    // (IDLE blocks: one token over 500 slots 12.9 us cut, 16.4 by tiles) and more
+    // where all write at once (BUSY: a prompt of 2048 tokens 74 us cut, 63 by tiles).
     const int64_t unit = (int64_t)KT * a.gqa, even = total * a.kv.nkv / slots;
     const int64_t by_tiles = tiles * a.kv.nkv <= slots ? longest : even + total / tiles / 2;
-    if (by_tiles <= even + even / 10 + (AC_START + AC_TILE) * unit + BM) return {0, tiles};
+    const int start = 8 * tiles * a.kv.nkv <= slots ? W::IDLE : W::BUSY;
+    if (by_tiles <= even + even / 10 + (start + AC_TILE) * unit + BM) return {0, tiles};
     const int64_t shares = max(slots / a.kv.nkv, 1);
     return {max((total + shares - 1) / shares, AC_LEAST * unit), total};
 }
@@ -431,10 +438,10 @@ struct Parts {
     int rows, shares;  // of a piece; at most
 };
 
-template <typename TQ, typename TC, int HD>
-__global__ void __launch_bounds__((64 * Wave<TQ, TC, HD>::NW), 2) k_attn_chunk(AttnChunkArgs a, Parts parts)
+template <typename TQ, typename TC, int HD, bool FEW>
+__global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, FEW>::NW), 2) k_attn_chunk(AttnChunkArgs a, Parts parts)
 {
-    using W = Wave<TQ, TC, HD>;
+    using W = Wave<TQ, TC, HD, FEW>;
     using La = Lay<TC, HD>;
     constexpr int KT = W::KT, DS = W::DS, HW = W::HW, BM = W::BM, ND = W::ND;
     constexpr int NW = W::NW, WG = 64 * NW, BLOCK = KT * La::ROW, PER_WAVE = KT / NW, NI = PER_WAVE / La::RPI;
@@ -448,7 +455,7 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD>::NW), 2) k_attn_chunk(A
     const KvView &kv = a.kv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int dw = wave % DS * HW;  // the wave's first dim
-    const Line line = line_of<BM, KT>(a, AC_CUS * W::PER_CU);
+    const Line line = line_of<W>(a);
     const int kvh = blockIdx.x % kv.nkv, nth = blockIdx.x / kv.nkv;
     int64_t u = nth * line.share;
     const int64_t end = min(u + line.share, line.total);
@@ -884,6 +891,29 @@ uint64_t attn_chunk_ws_bytes(int n_seq, int nkv, int hd, int gqa, int n_rows)
     return 4ull * floats;
 }
 
+template <typename TQ, typename TC, int HD, bool FEW> static void launch_chunk(hipStream_t st, AttnChunkArgs a, void *ws)
+{
+    using W = Wave<TQ, TC, HD, FEW>;
+    const ChunkShape s = shape_of(W::BM, W::PER_CU, a.kv.n_seq, a.kv.nkv, a.gqa, a.chunk.n_rows);
+    // (the tiles first: they want 16 bytes' alignment, and sums of few rows have it behind them)
+    Across *across = (Across *)ws;
+    float *o = (float *)(across + (int64_t)s.shares * a.kv.nkv);
+    const Parts parts{o, (float2 *)(o + s.parts(a.kv.nkv) * HD), across, s.rows, s.shares};
+    // rows of a wave in pages one after another, within 32 bits
+    constexpr int PER_WAVE = W::KT / W::NW;
+    a.runs = a.kv.page_tokens % PER_WAVE == 0 && (int64_t)a.kv.nkv * HD * (int)sizeof(TC) < (1 << 26);
+    const int64_t grid = std::max<int64_t>(s.tiles, (int64_t)s.shares * a.kv.nkv);
+    hipLaunchKernelGGL((k_attn_chunk<TQ, TC, HD, FEW>), dim3((unsigned)grid), dim3(64 * W::NW), 0, st, a, parts);
+    // (tiles of at most IDLE blocks are never cut: line_of)
+    if (s.shares == 1 || a.kv.cap <= W::IDLE * W::KT) return;
+    constexpr int MANY = AC_JOIN / (HD / 4), SOME = MANY > 4 ? 4 : MANY;
+    if (s.rows > 64)
+        hipLaunchKernelGGL((k_attn_chunk_join<TQ, TC, HD, MANY>), dim3((s.rows + MANY - 1) / MANY, a.kv.nkv, s.shares - 1), dim3(AC_JOIN),
+                           0, st, a, parts);
+    else
+        hipLaunchKernelGGL((k_attn_chunk_join<TQ, TC, HD, SOME>), dim3((s.rows + SOME - 1) / SOME, a.kv.nkv, s.shares - 1), dim3(AC_JOIN),
+                           0, st, a, parts);
+}
 hipError_t launch_attn_chunk(hipStream_t st, AttnChunkArgs a, void *ws)
 {
     a.scale = (float)((double)a.scale * 1.4426950408889634);  // log2 e
@@ -892,27 +922,12 @@ hipError_t launch_attn_chunk(hipStream_t st, AttnChunkArgs a, void *ws)
         using TQ = decltype(tq);
         using TC = decltype(tc);
         constexpr int HD = decltype(hd)::value;
-        using W = Wave<TQ, TC, HD>;
-        const ChunkShape s = shape_of(W::BM, W::PER_CU, a.kv.n_seq, a.kv.nkv, a.gqa, a.chunk.n_rows);
-        // (the tiles first: they want 16 bytes' alignment, and sums of few rows have it behind them)
-        Across *across = (Across *)ws;
-        float *o = (float *)(across + (int64_t)s.shares * a.kv.nkv);
-        const Parts parts{o, (float2 *)(o + s.parts(a.kv.nkv) * HD), across, s.rows, s.shares};
-        // rows of a wave in pages one after another, within 32 bits
-        constexpr int PER_WAVE = W::KT / W::NW;
-        a.runs = a.kv.page_tokens % PER_WAVE == 0 && (int64_t)a.kv.nkv * HD * (int)sizeof(TC) < (1 << 26);
-        const int64_t grid = std::max<int64_t>(s.tiles, (int64_t)s.shares * a.kv.nkv);
-        hipLaunchKernelGGL((k_attn_chunk<TQ, TC, HD>), dim3((unsigned)grid), dim3(64 * W::NW), 0, st, a, parts);
-        // (tiles of at most AC_START blocks are never cut: line_of)
-        if (s.shares > 1 && a.kv.cap > AC_START * W::KT) {
-            constexpr int MANY = AC_JOIN / (HD / 4), FEW = MANY > 4 ? 4 : MANY;
-            if (s.rows > 64)
-                hipLaunchKernelGGL((k_attn_chunk_join<TQ, TC, HD, MANY>), dim3((s.rows + MANY - 1) / MANY, a.kv.nkv, s.shares - 1),
-                                   dim3(AC_JOIN), 0, st, a, parts);
-            else
-                hipLaunchKernelGGL((k_attn_chunk_join<TQ, TC, HD, FEW>), dim3((s.rows + FEW - 1) / FEW, a.kv.nkv, s.shares - 1),
-                                   dim3(AC_JOIN), 0, st, a, parts);
-        }
+        if constexpr (sizeof(TC) == 4 && HD == 128)
+            if ((int64_t)a.chunk.n_rows * a.gqa <= 64) {
+                launch_chunk<TQ, TC, HD, true>(st, a, ws);
+                return 0;
+            }
+        launch_chunk<TQ, TC, HD, false>(st, a, ws);
         return 0;
     });
     return hipGetLastError();
