@@ -222,7 +222,7 @@ int styx_op_attn_chunk(styx_gpu *g, const styx_kv_cache *kv, const styx_kv_chunk
     a.nh = nh;
     a.gqa = nh / kv->nkv;
     a.q_f16 = type_q == STYX_F16;
-    a.window = window;
+    a.window = window < a.kv.cap ? window : 0;  // (all of a sequence: none)
     a.q = q;
     a.ldq = ldq;
     a.ldo = ldo;
@@ -252,7 +252,7 @@ int styx_op_kv_weigh(styx_gpu *g, const styx_kv_cache *kv, const styx_kv_chunk *
     a.nh = nh;
     a.gqa = nh / kv->nkv;
     a.q_f16 = type_q == STYX_F16;
-    a.window = window;
+    a.window = window < a.kv.cap ? window : 0;  // (all of a sequence: none)
     a.last = last;
     a.q = q;
     a.ldq = ldq;

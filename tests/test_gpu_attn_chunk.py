@@ -41,7 +41,7 @@ def test_pages_that_end_inside_a_tile(gpu, types, page):
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
-@pytest.mark.parametrize("window", [1, 2, 31, 64, 200, 1 << 30])
+@pytest.mark.parametrize("window", [1, 2, 31, 64, 200, 431, 432, 1 << 30, 2 ** 31 - 1])
 def test_window(gpu, types, window):
     c = Chunked(np.random.default_rng(window % 97), *TYPES[types], [0, 150, 400], [140, 33, 1], 2, 2, 64, 32, window=window)
     check_chunk(c, *run_chunk(gpu, c))

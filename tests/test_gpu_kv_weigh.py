@@ -105,7 +105,7 @@ def test_how_many_tokens_count(gpu, types, last):
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
-@pytest.mark.parametrize("window", [1, 40, 100])
+@pytest.mark.parametrize("window", [1, 40, 100, 2 ** 31 - 1])
 def test_window(gpu, types, window):
     c = Chunked(np.random.default_rng(2), *TYPES[types], [33, 500], [100, 70], 1, 4, 64, 100, window=window)
     lse = lse_of(c)
