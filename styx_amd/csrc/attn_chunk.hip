@@ -755,7 +755,7 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, FEW>::NW), 2) k_attn_ch
 
 // The pieces of a tile that lies across ends of shares joined: ROWS rows a workgroup, four dims a thread, threads beyond
 // the rows taking every other piece.
-constexpr int AC_JOIN = 256;
+constexpr int AC_JOIN = 512;
 template <typename TQ, typename TC, int HD, int ROWS>
 __global__ void __launch_bounds__(AC_JOIN) k_attn_chunk_join(AttnChunkArgs a, Parts parts)
 {
