@@ -153,6 +153,28 @@ def test_a_long_step_of_prompts(gpu):
     assert want["count"].tolist() == [9000, 1, 0, 5003, 17]
 
 
+@pytest.mark.parametrize("wrong", [0.0, 0.3])
+@pytest.mark.parametrize("sizes", [[40000, 0, 3, 1], [17, 16, 15, 0, 33, 20001, 5, 9000], [31] * 900 + [700] * 40])
+def test_many_pages_change_hands(gpu, sizes, wrong):
+    """Ended sequences' pages, entries outside the pool among them, come back and go to as many that begin."""
+    rng = np.random.default_rng(len(sizes))
+    ended, T = len(sizes), max(sizes)
+    B = 2 * ended
+    held = np.zeros(B, int)
+    held[::2] = sizes
+    n_pages = int(held.sum()) + 9
+    table = np.full((B, T), -1)
+    pages, at = rng.permutation(n_pages), 0
+    for b in range(0, B, 2):
+        table[b, :held[b]] = pages[at:at + held[b]]
+        at += held[b]
+    table[rng.random(table.shape) < wrong] = n_pages
+    lens, new = np.where(np.arange(B) % 2 == 0, -1, 0), np.zeros(B, int)
+    new[1::2] = [2 * n - (n % 3 == 1) for n in sizes[::-1]]
+    want = Plan(2, n_pages, T, table, held, pages[at:], 9, lens, new).check(gpu)
+    assert (want["count"][1::2] == new[1::2]).all() == (wrong == 0)
+
+
 def test_what_does_not_fit_is_refused(gpu):
     """Slots past cap, rows past n_rows, lengths past cap, and impossible numbers of pages."""
     big = 2 ** 31 - 1
