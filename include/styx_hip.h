@@ -423,7 +423,8 @@ typedef struct styx_kv_pages {
  * row, -1 for rows of no sequence and of those with count 0.  kv gives n_seq,
  * page_tokens, n_pages and table_len, its pointers are not read.  out's four
  * arrays are in's (in place), or others that overlap none of them; entries
- * past those named stay as they are.  Advance len by count for the next step. */
+ * past those named stay as they are.  n_seq * table_len must be below 2^31.
+ * Advance len by count for the next step.  Allocates nothing. */
 int styx_op_kv_plan(styx_gpu *gpu, const styx_kv_cache *kv, const styx_kv_pages *in,
                     const styx_kv_pages *out, const int32_t *shared, const int32_t *len,
                     const int32_t *n_new, const int32_t *pos, int n_rows, int32_t *first,
@@ -454,7 +455,8 @@ int styx_op_kv_append(styx_gpu *gpu, const styx_kv_cache *kv, int n_rows, const 
  * slots t <= len[b] + i, with window > 0 those of t > len[b] + i - window
  * alone, as far as their pages are in the pool.  q (turned) and out
  * [n_rows][nh*hd] of type_q: STYX_F32, or STYX_F16 for an f16 cache; rows ldq
- * and ldo values apart, 16-byte aligned; nh / nkv from 1 to 16.
+ * and ldo values apart, 16-byte aligned; nh / nkv from 1 to 16, n_rows times it
+ * at most 2^28.
  *   s_t = scale q . K[t], out = sum e^(s_t - M) V[t] / sum e^(s_t - M)
  * lse [n_rows][nh] f32 or NULL: ln of the sum of e^s_t.  A token that sees
  * nothing: out 0, lse -infinity.  Scores, sums and lse are f32; with f16 q the

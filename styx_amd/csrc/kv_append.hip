@@ -11,7 +11,10 @@
 // a wave takes heads of one row, the next under way while one is turned, and
 // keeps the row's sines and cosines.  The partner of a dim is in the same lane
 // where pairs are neighbours, else it is read back from LDS (for a part of a
-// head it may lie anywhere).
+// head it may lie anywhere).  A row's heads go to several workgroups where rows
+// are few: 48 tokens 5.6 us a call.  8192 f16 tokens of
+// 40 heads, 172 MB: 42 us in the kernel (4.1 TB/s), 53 where neither side is in
+// a cache; 4 parts of documents, f32 heads of 256, 125 MB: 27 and 30 us.
 #include <algorithm>
 
 #include "kv_chunk.h"
