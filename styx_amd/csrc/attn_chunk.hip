@@ -104,22 +104,24 @@ template <typename TC> __device__ __forceinline__ uint32_t not_finite(uint32_t v
 // use, the factors' arithmetic between matrix instructions.
 __device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
 
-template <typename TQ, typename TC, int HD, bool FEW = false> struct Wave;
+// RG: groups of 32 rows in a tile.
+template <typename TQ, typename TC, int HD, int RG = 4> struct Wave;
 
 // f16 caches: v_mfma_f32_32x32x16_f16.  f32 queries and their factors are two
 // f16 pieces each, hi + lo with |x - hi - lo| <= 2^-22 |x|, queries brought to
 // [2^9, 2^10) by a power of two per row so that the low pieces of all that
 // counts are normal numbers.  f16 queries take factors rounded to f16: an
 // error of at most 2^-11 of each, as large as the output's own rounding.
-template <typename TQ, int HD> struct Wave<TQ, _Float16, HD, false> {
+template <typename TQ, int HD> struct Wave<TQ, _Float16, HD, 4> {
     using TC = _Float16;
     using La = Lay<TC, HD>;
     static constexpr int NP = sizeof(TQ) == 4 ? 2 : 1;  // pieces
     // waves that share a query's dims, dims of a wave
     static constexpr int DS = HD == 256 && NP == 2 ? 2 : 1, HW = HD / DS, NK = HW / 16, ND = HW / 32;
     static constexpr int KT = HD == 256 ? 32 : 64;
-    static constexpr int NW = DS == 2 ? 8 : 4, PER_CU = 8 / NW, BM = 32 * NW / DS;
-    static constexpr int IDLE = 4, BUSY = 16;  // line_of
+    static constexpr int NW = 4 * DS, PER_CU = 8 / NW, BM = 128;
+    static constexpr int IDLE = 5, BUSY = 16;  // line_of
+    static constexpr float PART = HD / 3000.0f;  // (half to twice of it: within 10%)
     h8 q[NP][NK], p[KT / 32][NP][2];
     f16v s[KT / 32], o[ND];
     float mul, ref, sum[2];  // score to factor: 2^(s mul + ref); the factors' sum
@@ -173,8 +175,10 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD, false> {
         }
     }
     // The scores of 32 slots, with fill(j, N) done behind the j-th of N operands.
-    template <typename F> __device__ __forceinline__ void scores(int kt, const char *kb, F fill)
+    template <typename F> __device__ __forceinline__ void scores(int kt, const char *kb, int d0, F fill)
     {
+        static_assert(DS == 1 || 2 * HW % 256 == 0, "whole permuted pieces");
+        kb += 2 * d0;
         constexpr int AHEAD = 4;
         const int m = lane & 31, h = lane >> 5;
         const f16v zero = {};
@@ -207,8 +211,9 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD, false> {
     }
     // o += factors of 32 slots times V, with fill(j, N) done behind the j-th of N
     // operands; the factors of a step of 16 slots are needed at its first.
-    template <typename F> __device__ __forceinline__ void values(int kt, const char *vb, F fill)
+    template <typename F> __device__ __forceinline__ void values(int kt, const char *vb, int d0, F fill)
     {
+        vb += 2 * d0;
         constexpr int N = 2 * ND, AHEAD = 4;
         const int h = lane >> 5, u = (lane >> 4) & 1, kk = (lane & 15) >> 2;
         // piece of dims 16 u + 4 (lane & 3) .. of the first 32, row kk + 4 (h + 2 r)
@@ -261,15 +266,18 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD, false> {
 };
 
 // f32 caches: v_mfma_f32_32x32x2_f32, dims in fours on both sides of the score
-// product for 16-byte reads.  FEW: for chunks of at most 64 query rows, which
-// leave two of four waves without any: two waves for each 32 rows.
-template <int HD, bool FEW> struct Wave<float, float, HD, FEW> {
+// product for 16-byte reads.  Chunks of at most 64 or 32 query rows would leave
+// two or three of four waves without any: two or four waves take the same rows,
+// each a part of the dims (one token over 2000 slots: 22.3 us with two, 18.3 with
+// four; over 32000 58 and 45).
+template <int HD, int RG> struct Wave<float, float, HD, RG> {
     using TC = float;
     using La = Lay<TC, HD>;
-    static constexpr int DS = HD == 256 || FEW ? 2 : 1, HW = HD / DS, NK = HW / 8, ND = HW / 32;
+    static constexpr int DS = HD == 256 && RG == 4 ? 2 : 4 / RG, HW = HD / DS, NK = HW / 8, ND = HW / 32;
     static constexpr int KT = 32;
-    static constexpr int NW = 4 * DS, PER_CU = 8 / NW, BM = 32 * NW / DS;
-    static constexpr int IDLE = 2, BUSY = 8;
+    static constexpr int NW = RG * DS, PER_CU = HD == 256 || RG < 4 ? 1 : 2, BM = 32 * RG;
+    static constexpr int IDLE = HD == 64 ? 2 : 1, BUSY = 8;
+    static constexpr float PART = 0.025f * RG / 4;
     styx_f4 q[NK];
     f16v s[1], o[ND];
     float mul, ref, sum[2], p[2];
@@ -283,11 +291,12 @@ template <int HD, bool FEW> struct Wave<float, float, HD, FEW> {
 #pragma unroll
         for (int i = 0; i < NK; i++) q[i] = *(const styx_f4 *)(row + 8 * i + 4 * h) * sign;
     }
-    template <typename F> __device__ __forceinline__ void scores(int, const char *kb, F)
+    template <typename F> __device__ __forceinline__ void scores(int, const char *kb, int d0, F)
     {
         const int m = lane & 31, h = lane >> 5;
         const f16v zero = {};
-        const int at = m * La::ROW + ((h ^ La::perm(m)) << 4);
+        const int at = (m * La::ROW + ((h ^ La::perm(m)) << 4)) ^ ((4 * d0) & 255);
+        kb += (4 * d0) & ~255;
         f16v c[2];  // two chains: a product follows the one before on its sum at once otherwise
         constexpr int AHEAD = 2;
         auto read = [&](int i) { return *(const styx_f4 *)(kb + (at ^ ((32 * i) & 255)) + ((32 * i) & ~255)); };
@@ -310,13 +319,14 @@ template <int HD, bool FEW> struct Wave<float, float, HD, FEW> {
         p[i & 1] = exp2_(fmaf(s[0][i], mul, ref));
         sum[i & 1] += p[i & 1];
     }
-    template <typename F> __device__ __forceinline__ void values(int, const char *vb, F fill)
+    template <typename F> __device__ __forceinline__ void values(int, const char *vb, int d0, F fill)
     {
         constexpr int N = 16 * ND, AHEAD = 8;
         const int m = lane & 31, h = lane >> 5;
+        vb += (4 * d0) & ~255;
         auto read = [&](int j) {
             const int d = j % ND, i = j / ND, t = 8 * (i >> 2) + 4 * h + (i & 3);
-            const int at = t * La::ROW + (((m >> 2) ^ La::perm(t)) << 4) + 4 * (m & 3);
+            const int at = (t * La::ROW + (((m >> 2) ^ La::perm(t)) << 4) + 4 * (m & 3)) ^ ((4 * d0) & 255);
             return *(const float *)(vb + (at ^ ((128 * d) & 255)) + ((128 * d) & ~255));
         };
         float v[AHEAD];
@@ -348,25 +358,26 @@ template <int HD, bool FEW> struct Wave<float, float, HD, FEW> {
 // pieces are joined afterwards.  Both are known from the lengths alone, to every
 // workgroup by itself.
 constexpr int AC_CUS = 256;
-constexpr int AC_LEAST = 4;   // blocks of a share at least
 constexpr int AC_TILE = 4;    // what a tile's start costs, in blocks (its rows of q, its first blocks)
 
 // A sequence's part of the line: tile t is first + t step long, in slots times
 // rows of a token.  (With a tile's start: of a prompt's many short first tiles a
 // share would else hold a dozen, 4096 tokens, head_dim 256: 351 us, 257 with.)
 struct SeqLine {
-    int tiles;
+    int tiles, blocks;  // of the longest tile
     int64_t first, step;
     __device__ __forceinline__ int64_t upto(int64_t t) const { return t * first + step * (t * (t - 1) / 2); }
 };
 template <int BM, int KT> __device__ __forceinline__ SeqLine seq_line(const AttnChunkArgs &a, const ChunkSeq &s)
 {
-    if (s.count == 0) return {0, 0, 0};
+    if (s.count == 0) return {0, 0, 0, 0};
     const int tiles = (s.count * a.gqa + BM - 1) / BM;
     const int64_t most = (int64_t)a.window * a.gqa + BM;
     const int64_t start = (int64_t)AC_TILE * KT * a.gqa;
-    if (a.window && most < ((int64_t)s.len + s.count) * a.gqa) return {tiles, most + start, 0};
-    return {tiles, (int64_t)s.len * a.gqa + BM + start, BM};
+    const int end = (s.len + s.count + KT - 1) / KT;
+    if (a.window && most < ((int64_t)s.len + s.count) * a.gqa)
+        return {tiles, min(end, (int)((a.window + (int64_t)BM / a.gqa + KT - 1) / KT) + 1), most + start, 0};
+    return {tiles, end, (int64_t)s.len * a.gqa + BM + start, BM};
 }
 struct Line {
     int64_t share, total;  // share 0: by tiles
@@ -375,12 +386,13 @@ template <typename W> __device__ __forceinline__ Line line_of(const AttnChunkArg
 {
     constexpr int BM = W::BM, KT = W::KT, slots = AC_CUS * W::PER_CU;
     const int lane = threadIdx.x & 63;
-    int64_t tiles = 0, total = 0, longest = 0;
+    int64_t tiles = 0, total = 0;
+    int longest = 0;
     for (int b0 = 0; b0 < a.kv.n_seq; b0 += 64) {
         const SeqLine w = seq_line<BM, KT>(a, chunk_seq(a.chunk, a.kv, b0 + lane));
         tiles += w.tiles;
         total += w.upto(w.tiles);
-        longest = max(longest, w.tiles ? w.upto(w.tiles) - w.upto(w.tiles - 1) : (int64_t)0);
+        longest = max(longest, w.blocks);
     }
     tiles = uniform(wave_total(tiles));
     total = uniform(wave_total(total));
@@ -389,14 +401,22 @@ template <typename W> __device__ __forceinline__ Line line_of(const AttnChunkArg
     // What either costs: tiles that all run at once take as long as the longest,
     // more of them leave half a tile's time unused at the end; shares cost their
     // partial results and the joining, little on a chip that is mostly idle
-    // (IDLE blocks: one token over 500 slots 12.9 us cut, 16.4 by tiles) and more
-    // where all write at once (BUSY: a prompt of 2048 tokens 74 us cut, 63 by tiles).
+    // (IDLE blocks, f16: one token over 400 slots 11.5 us cut, 15.1 by tiles, 20
+    // tokens over 300 slots 19.4 and 14.8) and more where all write at once
+    // (BUSY: a prompt of 2048 tokens 74 us cut, 63 by tiles).
     const int64_t unit = (int64_t)KT * a.gqa, even = total * a.kv.nkv / slots;
-    const int64_t by_tiles = tiles * a.kv.nkv <= slots ? longest : even + total / tiles / 2;
+    const int64_t by_tiles = tiles * a.kv.nkv <= slots ? (longest + AC_TILE) * unit : even + total / tiles / 2;
     const int start = 8 * tiles * a.kv.nkv <= slots ? W::IDLE : W::BUSY;
-    if (by_tiles <= even + even / 10 + (start + AC_TILE) * unit + BM) return {0, tiles};
+    if (by_tiles <= even + even / 10 + (start + AC_TILE) * unit) return {0, tiles};
+    // Shares of fewer blocks only add partial results.  n blocks in shares of l
+    // take the time of l blocks and of n / l partial results, each PART of a
+    // block's for a whole tile: least for l = sqrt(n PART).  (64 f16 tokens over
+    // 2000 slots: 27 us with 4 blocks at least, 39 with one; one token 15.3 and 13.)
+    const float blocks = (float)(total * a.kv.nkv) / (float)unit;
+    const float full = fminf(1.0f, (float)a.chunk.n_rows * a.gqa / ((float)tiles * BM));
+    const int64_t least = max((int)__builtin_amdgcn_sqrtf(blocks * full * W::PART), 1) * unit;
     const int64_t shares = max(slots / a.kv.nkv, 1);
-    return {max((total + shares - 1) / shares, AC_LEAST * unit), total};
+    return {uniform(max((total + shares - 1) / shares, least)), total};
 }
 
 // A tile and what of its length lies before `at`.  TILES: `at` counts tiles, the
@@ -416,7 +436,7 @@ template <int BM, int KT, bool TILES> __device__ __forceinline__ Place find_plac
         const int64_t mine = TILES ? w.tiles : w.upto(w.tiles), upto = base + wave_upto(mine);
         if (const unsigned long long hit = __ballot(upto > at)) {
             const int l = __builtin_ctzll(hit);
-            const SeqLine o{(int)__builtin_amdgcn_readlane(w.tiles, l), of_lane(w.first, l), of_lane(w.step, l)};
+            const SeqLine o{(int)__builtin_amdgcn_readlane(w.tiles, l), 0, of_lane(w.first, l), of_lane(w.step, l)};
             const int64_t start = of_lane(upto, l) - of_lane(mine, l), in = at - start;
             int tile = 0;
             if (TILES)
@@ -454,10 +474,11 @@ struct Parts {
     int rows, shares;  // of a piece; at most
 };
 
-template <typename TQ, typename TC, int HD, bool FEW>
-__global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, FEW>::NW), 2) k_attn_chunk(AttnChunkArgs a, Parts parts)
+template <typename TQ, typename TC, int HD, int RG>
+__global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, RG>::NW), (Wave<TQ, TC, HD, RG>::PER_CU * Wave<TQ, TC, HD, RG>::NW / 4))
+    k_attn_chunk(AttnChunkArgs a, Parts parts)
 {
-    using W = Wave<TQ, TC, HD, FEW>;
+    using W = Wave<TQ, TC, HD, RG>;
     using La = Lay<TC, HD>;
     constexpr int KT = W::KT, DS = W::DS, HW = W::HW, BM = W::BM, ND = W::ND;
     constexpr int NW = W::NW, WG = 64 * NW, BLOCK = KT * La::ROW, PER_WAVE = KT / NW, NI = PER_WAVE / La::RPI;
@@ -466,8 +487,8 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, FEW>::NW), 2) k_attn_ch
     __shared__ __align__(1024) char s_v[2][BLOCK];
     // scores of half the dims; in the block of K where there is no other place
     constexpr int PIECES = 4;
-    constexpr bool APART = 4 * BLOCK + NW * PIECES * 1024 < 150000;
-    __shared__ styx_f4 s_half[DS == 2 && APART ? NW * PIECES : 1][64];
+    constexpr bool APART = 4 * BLOCK + NW * PIECES * 1024 < 150000 / W::PER_CU;
+    __shared__ styx_f4 s_half[DS > 1 && APART ? NW * PIECES : 1][64];
     const KvView &kv = a.kv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int dw = wave % DS * HW;  // the wave's first dim
@@ -528,9 +549,10 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, FEW>::NW), 2) k_attn_ch
     float m = -INFINITY;  // the reference, a whole number
     x.ref = AC_OFF;
     x.sum[0] = x.sum[1] = 0.0f;
-    uint32_t nan_at[HW / 64];  // dims that are NaN whatever the sums are
+    constexpr int NANS = (HW + 63) / 64;
+    uint32_t nan_at[NANS];  // dims that are NaN whatever the sums are
 #pragma unroll
-    for (int w = 0; w < HW / 64; w++) nan_at[w] = 0;
+    for (int w = 0; w < NANS; w++) nan_at[w] = 0;
     x.init((const TQ *)a.q + orow * a.ldq + (int64_t)head * HD + dw, dw, a.scale);
 #pragma unroll
     for (int d = 0; d < ND; d++) x.o[d] = f16v{};
@@ -631,7 +653,7 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, FEW>::NW), 2) k_attn_ch
                         for (int e = 0; e < 4; e++) bad |= (uint32_t) !(fabsf((float)v[e]) < INFINITY) << e;
                         if (bad)
 #pragma unroll
-                            for (int w = 0; w < HW / 64; w++) nan_at[w] |= w == j >> 3 ? (bad & see) << (4 * (j & 7)) : 0;
+                            for (int w = 0; w < NANS; w++) nan_at[w] |= w == j >> 3 ? (bad & see) << (4 * (j & 7)) : 0;
                     }
                 }
                 __syncthreads();
@@ -673,22 +695,22 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, FEW>::NW), 2) k_attn_ch
                 for (int i = 0; i < 16; i++)
                     if (i / (16 / steps) == j) x.factor(kt, i);
             };
-            x.scores(0, kb, nothing);
+            x.scores(0, kb, 0, nothing);
             if (masked) mask(0);
             follow(0);
-            x.scores(1, kb, [&](int j, int steps) { factors(0, j, steps); });
+            x.scores(1, kb, 0, [&](int j, int steps) { factors(0, j, steps); });
             if (masked) mask(1);
             follow(1);
-            x.values(0, vb, [&](int j, int steps) { factors(1, j, steps); });
-            x.values(1, vb, nothing);
+            x.values(0, vb, 0, [&](int j, int steps) { factors(1, j, steps); });
+            x.values(1, vb, 0, nothing);
         } else {
             if constexpr (DS == 1) {
                 if (idle) continue;
-                x.scores(0, kb, nothing);
+                x.scores(0, kb, 0, nothing);
             } else {
-                // each wave of a pair has half the dims: both add the halves up
+                // each of DS waves has a part of the dims: all add the parts up
                 styx_f4 (*half)[64] = APART ? s_half : (styx_f4(*)[64])s_k[buf];
-                if (!idle) x.scores(0, kb + dw * (int)sizeof(TC), nothing);
+                if (!idle) x.scores(0, kb, dw, nothing);
                 if constexpr (!APART) {
                     static_assert(NW * PIECES * 1024 <= BLOCK, "scores in the place of K");
                     __syncthreads();
@@ -701,9 +723,16 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, FEW>::NW), 2) k_attn_ch
                 if (idle) continue;
 #pragma unroll
                 for (int i = 0; i < PIECES; i++) {
-                    const styx_f4 y = half[(wave ^ 1) * PIECES + i][lane];
+                    styx_f4 y = half[(DS == 2 ? wave ^ 1 : wave & -DS) * PIECES + i][lane];
+                    if constexpr (DS == 2) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x.s[0][4 * i + e] += y[e];
+                        for (int e = 0; e < 4; e++) x.s[0][4 * i + e] += y[e];
+                    } else {  // in one order, so that they all have the same sums
+#pragma unroll
+                        for (int w = 1; w < DS; w++) y += half[((wave & -DS) + w) * PIECES + i][lane];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x.s[0][4 * i + e] = y[e];
+                    }
                 }
             }
             if (masked) mask(0);
@@ -712,7 +741,7 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, FEW>::NW), 2) k_attn_ch
             constexpr int LEAD = sizeof(TC) == 2 ? 8 : 1;
 #pragma unroll
             for (int i = 0; i < LEAD; i++) x.factor(0, i);
-            x.values(0, vb + dw * (int)sizeof(TC), [&](int j, int steps) {
+            x.values(0, vb, dw, [&](int j, int steps) {
                 if constexpr (sizeof(TC) == 4) {
                     if (j % (steps / 16) == 0 && j < steps - steps / 16) x.factor(0, j / (steps / 16) + 1);
                 } else {
@@ -879,17 +908,25 @@ static ChunkShape shape_of(int bm, int per_cu, int n_seq, int nkv, int gqa, int 
     s.rows = (int)std::min<int64_t>(bm, (int64_t)n_rows * gqa);
     return s;
 }
-template <typename F> static auto with_kernel(bool f16, bool q16, int hd, F f)
+// f(query type, row type, head_dim, groups of rows) for the kernel of a call
+template <typename F> static auto with_kernel(bool f16, bool q16, int hd, int64_t rows, F f)
 {
-    auto by_hd = [&](auto tq, auto tc) {
-        switch (hd) {
-        case 64: return f(tq, tc, std::integral_constant<int, 64>{});
-        case 128: return f(tq, tc, std::integral_constant<int, 128>{});
-        default: return f(tq, tc, std::integral_constant<int, 256>{});
-        }
+    const auto four = std::integral_constant<int, 4>{};
+    auto by_rows = [&](auto hd) {
+        if constexpr (hd() > 64)
+            if (rows <= 32) return f(float{}, float{}, hd, std::integral_constant<int, 1>{});
+        if (rows <= 64) return f(float{}, float{}, hd, std::integral_constant<int, 2>{});
+        return f(float{}, float{}, hd, four);
     };
-    if (!f16) return by_hd(float{}, float{});
-    return q16 ? by_hd(_Float16{}, _Float16{}) : by_hd(float{}, _Float16{});
+    auto by_type = [&](auto hd) {
+        if (!f16) return by_rows(hd);
+        return q16 ? f(_Float16{}, _Float16{}, hd, four) : f(float{}, _Float16{}, hd, four);
+    };
+    switch (hd) {
+    case 64: return by_type(std::integral_constant<int, 64>{});
+    case 128: return by_type(std::integral_constant<int, 128>{});
+    default: return by_type(std::integral_constant<int, 256>{});
+    }
 }
 // (times 8, so that rows times gqa stay below 2^28)
 int64_t attn_chunk_grid(int n_seq, int nkv, int gqa, int n_rows)
@@ -902,18 +939,18 @@ uint64_t attn_chunk_ws_bytes(int n_seq, int nkv, int hd, int gqa, int n_rows)
     // the types that the call may bring
     int64_t floats = 4;
     for (int t = 0; t < 3; t++)
-        with_kernel(t > 0, t > 1, hd, [&](auto tq, auto tc, auto n) {
-            using W = Wave<decltype(tq), decltype(tc), decltype(n)::value>;
-            static_assert(W::BM >= 128 && W::PER_CU <= 2, "attn_chunk_grid");
+        with_kernel(t > 0, t > 1, hd, (int64_t)n_rows * gqa, [&](auto tq, auto tc, auto n, auto rg) {
+            using W = Wave<decltype(tq), decltype(tc), n(), rg()>;
+            static_assert((W::BM >= 128 || rg() < 4) && W::PER_CU <= 2, "attn_chunk_grid");
             floats = std::max(floats, shape_of(W::BM, W::PER_CU, n_seq, nkv, gqa, n_rows).floats(nkv, hd));
             return 0;
         });
     return 4ull * floats;
 }
 
-template <typename TQ, typename TC, int HD, bool FEW> static void launch_chunk(hipStream_t st, AttnChunkArgs a, void *ws)
+template <typename TQ, typename TC, int HD, int RG> static void launch_chunk(hipStream_t st, AttnChunkArgs a, void *ws)
 {
-    using W = Wave<TQ, TC, HD, FEW>;
+    using W = Wave<TQ, TC, HD, RG>;
     const ChunkShape s = shape_of(W::BM, W::PER_CU, a.kv.n_seq, a.kv.nkv, a.gqa, a.chunk.n_rows);
     // (the tiles first: they want 16 bytes' alignment, and sums of few rows have it behind them)
     Across *across = (Across *)ws;
@@ -923,7 +960,7 @@ template <typename TQ, typename TC, int HD, bool FEW> static void launch_chunk(h
     constexpr int PER_WAVE = W::KT / W::NW;
     a.runs = a.kv.page_tokens % PER_WAVE == 0 && (int64_t)a.kv.nkv * HD * (int)sizeof(TC) < (1 << 26);
     const int64_t grid = std::max<int64_t>(s.tiles, (int64_t)s.shares * a.kv.nkv);
-    hipLaunchKernelGGL((k_attn_chunk<TQ, TC, HD, FEW>), dim3((unsigned)grid), dim3(64 * W::NW), 0, st, a, parts);
+    hipLaunchKernelGGL((k_attn_chunk<TQ, TC, HD, RG>), dim3((unsigned)grid), dim3(64 * W::NW), 0, st, a, parts);
     // (tiles of at most IDLE blocks are never cut: line_of)
     if (s.shares == 1 || a.kv.cap <= W::IDLE * W::KT) return;
     constexpr int MANY = AC_JOIN / (HD / 4), SOME = MANY > 4 ? 4 : MANY;
@@ -938,16 +975,8 @@ hipError_t launch_attn_chunk(hipStream_t st, AttnChunkArgs a, void *ws)
 {
     a.scale = (float)((double)a.scale * 1.4426950408889634);  // log2 e
     a.by_gqa = page_div((uint32_t)a.gqa);
-    with_kernel(a.kv.f16, a.q_f16, a.kv.hd, [&](auto tq, auto tc, auto hd) {
-        using TQ = decltype(tq);
-        using TC = decltype(tc);
-        constexpr int HD = decltype(hd)::value;
-        if constexpr (sizeof(TC) == 4 && HD == 128)
-            if ((int64_t)a.chunk.n_rows * a.gqa <= 64) {
-                launch_chunk<TQ, TC, HD, true>(st, a, ws);
-                return 0;
-            }
-        launch_chunk<TQ, TC, HD, false>(st, a, ws);
+    with_kernel(a.kv.f16, a.q_f16, a.kv.hd, (int64_t)a.chunk.n_rows * a.gqa, [&](auto tq, auto tc, auto hd, auto rg) {
+        launch_chunk<decltype(tq), decltype(tc), hd(), rg()>(st, a, ws);
         return 0;
     });
     return hipGetLastError();

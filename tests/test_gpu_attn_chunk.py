@@ -200,6 +200,28 @@ def test_cut_tiles_under_a_window(gpu, types, window):
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("gqa,counts", [(8, [1, 2, 1]), (8, [3, 1, 4]), (1, [31, 0, 1]), (1, [5, 27, 1]), (16, [2, 1, 1]), (1, [60, 5, 0])])
+@pytest.mark.parametrize("window", [0, 45, 900])
+def test_few_rows(gpu, types, hd, gqa, counts, window):
+    """Calls of 32, 33, 64, 65 rows and fewer: whole contexts and cut ones, missing pages, unseen values that are not finite."""
+    lens = [40, 2100, 333]
+    c = Chunked(np.random.default_rng(hd + gqa + sum(counts)), *TYPES[types], lens, counts, 2, gqa, hd, 24, window=window)
+    c.table[1, 3:60] = -1
+    for p in (c.k, c.v):
+        rest = np.ones(len(p), bool)
+        rest[np.concatenate([c.rows(b)[c.rows(b) >= 0] for b in range(3)])] = False
+        p[rest] = np.nan
+    late = c.rows(0)[lens[0] + counts[0] - 1]  # seen by the first sequence's last token alone
+    c.v[late, 1, hd - 1] = np.inf
+    out, lse = run_chunk(gpu, c)
+    assert not np.isfinite(out[counts[0] - 1].reshape(2, gqa, hd)[1, :, hd - 1]).any()
+    c.v[late, 1, hd - 1] = 0
+    out[counts[0] - 1].reshape(2, gqa, hd)[1, :, hd - 1] = run_chunk(gpu, c)[0][counts[0] - 1].reshape(2, gqa, hd)[1, :, hd - 1]
+    check_chunk(c, out, lse, tokens=FEW)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
 def test_many_sequences_with_long_ones_among_them(gpu, types):
     """More sequences than a wave has lanes, a few of them cut, skipped ones between."""
     rng = np.random.default_rng(16)
