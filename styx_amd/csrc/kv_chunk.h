@@ -82,7 +82,8 @@ struct KvWeighArgs {
     const float *lse, *acc_in;
     float *acc_out;
     int32_t *slot_pos;
-    PageDiv by_gqa;  // (filled by the launch)
+    PageDiv by_gqa;  // (filled by the launch, as is few)
+    int few;         // blocks of 32 slots for which a workgroup's waves share a block
 };
 int64_t kv_weigh_grid(const KvWeighArgs &a);
 hipError_t launch_kv_weigh(hipStream_t st, KvWeighArgs a);

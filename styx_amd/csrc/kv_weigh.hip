@@ -27,6 +27,14 @@
 namespace styx {
 
 constexpr int KW_ROWS = 32;
+// Where blocks of 32 slots are few, the waves of a workgroup take one of them
+// together, each other tiles of query rows, read as they lie, and add their sums
+// up in order: half of KW_FEW blocks at most, all of it where there are 8 tiles
+// and more and no pieces to form of each (launch_kv_weigh).  One conversation of
+// 4000 slots over 4 kv heads, 64 tokens: 500 blocks, f16 15 us, 22 without,
+// f32 32 and 49, heads of 256 47 and 92; f32 queries on f16 rows 38 and 33; 16
+// tokens over 2000 f32 slots 8.7 and 15.9.  With 1024 blocks and 4 tiles 17.8 and 9.4.
+constexpr int KW_FEW = 512;
 // Waves of a workgroup, all of which read its tiles: f16 products are so fast
 // that fetching the tiles counts (64 tokens over 32768 slots: 8 waves 31 us, 4
 // waves 35, 2 waves 36), f32 ones are not, and smaller workgroups fill the chip
@@ -47,14 +55,31 @@ template <typename T, int HD> struct RowLay {
     }
 };
 
-template <typename TQ, typename TC, int HD>
-__global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), HD == 256 && sizeof(TQ) == 4 ? 2 : 3) k_kv_weigh(KvWeighArgs a)
+// f32 queries on f16 rows are two f16 pieces, brought to [2^9, 2^10) by a power
+// of two per row (m: its largest value), as in the attention.
+__device__ __forceinline__ float up_of(float m)
 {
-    // f32 queries on f16 rows are two f16 pieces, brought to [2^9, 2^10) by a
-    // power of two per row, as in the attention
+    const int e = m > 0.0f && m < INFINITY ? (int)((__float_as_uint(m) >> 23) & 255) - 127 : 9;
+    return e < -100 ? ldexpf(1.0f, 109) : ldexpf(1.0f, 9 - e);
+}
+__device__ __forceinline__ void pieces(const float *v, float up, h8 &hi, h8 &lo)
+{
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const float y = v[e] * up;
+        hi[e] = (_Float16)y;
+        lo[e] = (_Float16)(y - (float)hi[e]);
+    }
+}
+
+// Waves of a SIMD: two workgroups of f16 rows a CU, but for heads of 256.
+template <typename TQ, typename TC, int HD> constexpr int KW_SIMD = HD == 256 && sizeof(TQ) == 4 ? 2 : sizeof(TC) == 2 && HD <= 128 ? 4 : 3;
+template <typename TQ, typename TC, int HD>
+__global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), (KW_SIMD<TQ, TC, HD>)) k_kv_weigh(KvWeighArgs a)
+{
     constexpr int NP = sizeof(TQ) == 4 && sizeof(TC) == 2 ? 2 : 1;
     using La = RowLay<TC, HD>;
-    constexpr int KW_WG = 64 * kw_waves(sizeof(TC) == 2, HD), KW_KEYS = KW_WG / 2;
+    constexpr int KW_NW = kw_waves(sizeof(TC) == 2, HD), KW_WG = 64 * KW_NW;
     constexpr int NK = sizeof(TC) == 2 ? HD / 16 : HD / 8;  // operands of a row
     constexpr int PER = KW_ROWS * HD / KW_WG;               // values of a thread in a tile
     constexpr int TPR = HD / PER;                           // threads of a row
@@ -63,19 +88,38 @@ __global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), HD == 256 
     __shared__ __align__(16) char s_q[2][NP][KW_ROWS * La::ROW];
     __shared__ __align__(16) float s_lse[2][KW_ROWS], s_mul[2][KW_ROWS];
     __shared__ __align__(16) int s_at[2][KW_ROWS];
+    // of each wave's own tile; sums by wave
+    __shared__ __align__(16) float s_own[KW_NW][2][KW_ROWS];
+    __shared__ __align__(16) int s_own_at[KW_NW][KW_ROWS];
+    __shared__ float s_sum[KW_NW][KW_ROWS];
     const KvView &kv = a.kv;
-    const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, h = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t stride = (int64_t)kv.nkv * HD;
+    bool few = a.few != 0;
+    if (few) {
+        int blocks = 0;  // up to one more than KW_FEW
+        for (int b0 = 0; b0 < kv.n_seq; b0 += 64) {
+            const ChunkSeq mine = chunk_seq(a.chunk, kv, b0 + lane);
+            blocks = min(blocks + (mine.count ? min((mine.len + mine.count + 31) / 32, KW_FEW + 1) : 0), KW_FEW + 1);
+        }
+        few = (int64_t)of_lane(wave_total((uint32_t)blocks), 0) * kv.nkv <= a.few;
+    }
+    const int keys = few ? 32 : 32 * KW_NW;
     for (int64_t item = blockIdx.x;; item += gridDim.x) {
-        // the sequence and its KW_KEYS slots
+        // (numbers that the compiler takes for new ones in every trip: what is
+        // computed from them would else be kept in registers over the trips)
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        const int n = tid & 31, h = tid >> 5 & 1;
+        // the sequence and its slots
         const int kvh = (int)(item % kv.nkv);
         int64_t nth = item / kv.nkv;
         int b = -1;
         ChunkSeq s{};
         for (int b0 = 0; b0 < kv.n_seq && b < 0; b0 += 64) {
             const ChunkSeq mine = chunk_seq(a.chunk, kv, b0 + lane);
-            const int64_t tiles = mine.count ? ((int64_t)mine.len + mine.count + KW_KEYS - 1) / KW_KEYS : 0, upto = wave_upto(tiles);
+            const int64_t tiles = mine.count ? ((int64_t)mine.len + mine.count + keys - 1) / keys : 0, upto = wave_upto(tiles);
             if (const unsigned long long hit = __ballot(upto > nth)) {
                 const int l = __builtin_ctzll(hit);
                 b = b0 + l;
@@ -87,8 +131,8 @@ __global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), HD == 256 
             }
         }
         if (b < 0) return;
-        const int k0 = (int)nth * KW_KEYS, slots = s.len + s.count;
-        const int t = k0 + 32 * wave + n;  // this lane's slot
+        const int k0 = (int)nth * keys, slots = s.len + s.count;
+        const int w0 = k0 + (few ? 0 : 32 * wave), t = w0 + n;  // this lane's slot
         const int row = t < slots ? kv.row(kv.table + (int64_t)b * kv.table_len, t) : -1;
         Op k[NK];
         const TC *kp = (const TC *)kv.kpool + max(row, 0) * stride + kvh * HD + (sizeof(TC) == 2 ? 8 : 4) * h;
@@ -96,7 +140,7 @@ __global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), HD == 256 
         for (int i = 0; i < NK; i++) k[i] = *(const Op *)(kp + (sizeof(TC) == 2 ? 16 : 8) * i);
         // tokens that count and see any of these slots, and their rows
         const int i0 = max(max(s.count - min(a.last, s.count), k0 - s.len), 0);
-        const int i1 = a.window ? (int)max((int64_t)i0, min((int64_t)s.count, (int64_t)k0 + KW_KEYS - 1 + a.window - s.len)) : s.count;
+        const int i1 = a.window ? (int)max((int64_t)i0, min((int64_t)s.count, (int64_t)k0 + keys - 1 + a.window - s.len)) : s.count;
         const int r0 = i0 * a.gqa, r1 = max(i0, i1) * a.gqa;
         // a thread's part of a row of the next tile
         __align__(16) TQ in[PER];
@@ -119,18 +163,12 @@ __global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), HD == 256 
                 for (int i = 0; i < PER; i++) m = fmaxf(m, fabsf((float)in[i]));
 #pragma unroll
                 for (int d = 1; d < TPR; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-                const int e = m > 0.0f && m < INFINITY ? (int)((__float_as_uint(m) >> 23) & 255) - 127 : 9;
-                const float up = e < -100 ? ldexpf(1.0f, 109) : ldexpf(1.0f, 9 - e);
+                const float up = up_of(m);
                 mul /= up;
 #pragma unroll
                 for (int i = 0; i < PER; i += 8) {
                     h8 hi, lo;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float y = (float)in[i + e] * up;
-                        hi[e] = (_Float16)y;
-                        lo[e] = (_Float16)(y - (float)hi[e]);
-                    }
+                    pieces((const float *)in + i, up, hi, lo);
                     *(h8 *)(s_q[buf][0] + La::at(mr, 2 * (md + i))) = hi;
                     *(h8 *)(s_q[buf][NP - 1] + La::at(mr, 2 * (md + i))) = lo;
                 }
@@ -148,8 +186,34 @@ __global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), HD == 256 
             }
         };
         float sum[2] = {};
+        auto add = [&](const f16v &x, int base, const float *s_l, const float *s_m, const int *s_a) {
+            // whether every row of the tile sees all of the wave's slots
+            const bool whole = base + KW_ROWS <= r1 && w0 + 31 <= s.len + a.by_gqa.of(base) &&
+                               (!a.window || w0 > s.len + a.by_gqa.of(base + KW_ROWS - 1) - a.window);
+            float w[16];
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int r = 2 * i + 4 * h;
+                const styx_f4 lse = *(const styx_f4 *)&s_l[r], mul = *(const styx_f4 *)&s_m[r];
+#pragma unroll
+                for (int e = 0; e < 4; e++) w[i + e] = __builtin_amdgcn_exp2f(fmaf(x[i + e], mul[e], -lse[e]));
+            }
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int at = s_a[8 * (i >> 2) + 4 * h + (i & 3)];
+                    const bool see = (t <= at) & ((a.window == 0) | (t > at - a.window));
+                    w[i] = see ? w[i] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+                sum[0] += w[i];
+                sum[1] += w[i + 1];
+            }
+        };
         __syncthreads();  // (the last item's tiles are read no more)
-        if (r0 < r1) {
+        if (r0 < r1 && !few) {
             ask(r0);
             put(0, r0);
             // (here, so that no trip waits for them, and with them for the next tile)
@@ -157,7 +221,7 @@ __global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), HD == 256 
             for (int i = 0; i < NK; i++) asm volatile("" : "+v"(k[i]));
             if (r0 + KW_ROWS < r1) ask(r0 + KW_ROWS);
         }
-        for (int base = r0, buf = 0; base < r1; base += KW_ROWS, buf ^= 1) {
+        for (int base = few ? r1 : r0, buf = 0; base < r1; base += KW_ROWS, buf ^= 1) {
             __syncthreads();
             f16v x = {};
 #pragma unroll
@@ -176,35 +240,77 @@ __global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), HD == 256 
                 put(buf ^ 1, base + KW_ROWS);
                 if (base + 2 * KW_ROWS < r1) ask(base + 2 * KW_ROWS);
             }
-            // whether every row of the tile sees all of the wave's slots
-            const int w0 = k0 + 32 * wave;
-            const bool whole = base + KW_ROWS <= r1 && w0 + 31 <= s.len + a.by_gqa.of(base) &&
-                               (!a.window || w0 > s.len + a.by_gqa.of(base + KW_ROWS - 1) - a.window);
-            float w[16];
+            add(x, base, s_lse[buf], s_mul[buf], s_at[buf]);
+        }
+        for (int base = few ? r0 + KW_ROWS * wave : r1; base < r1; base += KW_ROWS * KW_NW) {
+            // row n of a tile of the wave's own, as it lies
+            const int r = min(base + n, r1 - 1), tok = a.by_gqa.of(r), head = kvh * a.gqa + (r - tok * a.gqa);
+            const TQ *p = (const TQ *)a.q + (int64_t)(s.first + tok) * a.ldq + (int64_t)head * HD + (sizeof(TC) == 2 ? 8 : 4) * h;
+            const float lse = a.lse[(int64_t)(s.first + tok) * a.nh + head];
+            constexpr int AHEAD = sizeof(TQ) == 2 ? (NK < 8 ? NK : 8) : NP == 2 || HD == 256 ? 2 : 4;
+            struct Raw {
+                Op v[sizeof(TQ) == 4 && NP == 2 ? 2 : 1];
+            };
+            auto read = [&](int i) { return *(const Raw *)(p + (sizeof(TC) == 2 ? 16 : 8) * i); };
+            float mul = a.scale, up = 1.0f;
+            if constexpr (NP == 2) {
+                float m = 0.0f;
+#pragma unroll 2
+                for (int i = 0; i < NK; i++) {
+                    const Raw y = read(i);
+                    const float *f = (const float *)&y;
 #pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const int r = 2 * i + 4 * h;
-                const styx_f4 lse = *(const styx_f4 *)&s_lse[buf][r], mul = *(const styx_f4 *)&s_mul[buf][r];
-#pragma unroll
-                for (int e = 0; e < 4; e++) w[i + e] = __builtin_amdgcn_exp2f(fmaf(x[i + e], mul[e], -lse[e]));
-            }
-            if (!whole) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int at = s_at[buf][8 * (i >> 2) + 4 * h + (i & 3)];
-                    const bool see = (t <= at) & ((a.window == 0) | (t > at - a.window));
-                    w[i] = see ? w[i] : 0.0f;
+                    for (int e = 0; e < 8; e++) m = fmaxf(m, fabsf(f[e]));
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                m = fmaxf(m, __shfl_xor(m, 32));
+                up = up_of(m);
+                mul /= up;
             }
+            if (h == 0) {
+                s_own[wave][0][n] = base + n < r1 && lse != -INFINITY ? lse * 1.44269504f : INFINITY;
+                s_own[wave][1][n] = mul;
+                s_own_at[wave][n] = base + n < r1 ? s.len + tok : -1;
+            }
+            Raw y[AHEAD];
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-                sum[0] += w[i];
-                sum[1] += w[i + 1];
+            for (int i = 0; i < AHEAD; i++) y[i] = read(i);
+            f16v x = {};
+#pragma unroll
+            for (int i = 0; i < NK; i++) {
+                const Raw q = y[i % AHEAD];
+                if (i + AHEAD < NK) y[i % AHEAD] = read(i + AHEAD);
+                if constexpr (NP == 2) {
+                    h8 hi, lo;
+                    pieces((const float *)&q, up, hi, lo);
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(hi, k[i], x, 0, 0, 0);
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(lo, k[i], x, 0, 0, 0);
+                } else if constexpr (sizeof(TC) == 2) {
+                    x = __builtin_amdgcn_mfma_f32_32x32x16_f16(q.v[0], k[i], x, 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x = __builtin_amdgcn_mfma_f32_32x32x2f32(q.v[0][e], k[i][e], x, 0, 0, 0);
+                }
+                // (loads stay AHEAD: all at once they cost registers, and the
+                // long calls the second workgroup of a CU)
+                __builtin_amdgcn_sched_barrier(0);
             }
+            // (a wave's LDS operations are carried out in order)
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            add(x, base, s_own[wave][0], s_own[wave][1], s_own_at[wave]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
         float all = sum[0] + sum[1];
         const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(all), __float_as_uint(all), false, false);
         all = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+        if (few) {
+            if (h == 0) s_sum[wave][n] = all;
+            __syncthreads();
+            if (wave) continue;
+            all = s_sum[0][n];
+#pragma unroll
+            for (int w = 1; w < KW_NW; w++) all += s_sum[w][n];
+        }
         if (h == 0 && t < slots) {
             const int64_t at = ((int64_t)b * kv.nkv + kvh) * kv.cap + t;
             a.acc_out[at] = (a.acc_in && t < s.len ? a.decay * a.acc_in[at] : 0.0f) + (row >= 0 ? all : 0.0f);
@@ -215,9 +321,8 @@ __global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), HD == 256 
 
 int64_t kv_weigh_grid(const KvWeighArgs &a)
 {
-    const int KW_KEYS = 32 * kw_waves(a.kv.f16, a.kv.hd);
-    const int64_t tiles = ((int64_t)a.kv.cap + KW_KEYS - 1) / KW_KEYS;
-    return std::min<int64_t>(tiles * a.kv.n_seq * a.kv.nkv, 4096);
+    const int64_t heads = (int64_t)a.kv.n_seq * a.kv.nkv, blocks = ((int64_t)a.kv.cap + 31) / 32 * heads;
+    return std::min<int64_t>(blocks, std::max<int64_t>(KW_FEW, std::min<int64_t>(4096, blocks / kw_waves(a.kv.f16, a.kv.hd) + heads)));
 }
 
 template <typename TQ, typename TC> static void launch_hd(hipStream_t st, const KvWeighArgs &a)
@@ -233,6 +338,8 @@ hipError_t launch_kv_weigh(hipStream_t st, KvWeighArgs a)
 {
     a.scale = (float)((double)a.scale * 1.4426950408889634);  // log2 e
     a.by_gqa = page_div((uint32_t)a.gqa);
+    const int64_t rows = (int64_t)std::min(a.last, a.chunk.n_rows) * a.gqa;
+    a.few = rows <= KW_ROWS ? 0 : (!a.kv.f16 || a.q_f16) && rows >= 8 * KW_ROWS ? KW_FEW : KW_FEW / 2;
     if (!a.kv.f16)
         launch_hd<float, float>(st, a);
     else if (a.q_f16)

@@ -174,6 +174,29 @@ def test_more_work_than_workgroups(gpu, types):
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 45])
+def test_many_blocks_of_slots(gpu, types, hd, window):
+    """More than 512 blocks of 32 slots, each a wave's; missing pages, unseen rows that are not finite, several tiles of rows."""
+    c = Chunked(np.random.default_rng(hd), *TYPES[types], [500, 33, 0], [12, 5, 70], 40, 3, hd, 24, window=window)
+    c.table[0, 4:6] = -1
+    rest = np.ones(len(c.k), bool)
+    rest[np.concatenate([c.rows(b)[c.rows(b) >= 0] for b in range(3)])] = False
+    c.k[rest] = np.nan
+    lse = lse_of(c)
+    check(c, lse, 30, run(gpu, c, lse, 30))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("lens,nkv", [([1000, 2900], 2), ([1000, 3200], 2), ([1000, 7000], 2), ([1000, 7300], 2)])
+def test_blocks_shared_by_waves_or_not(gpu, types, lens, nkv):
+    """Just fewer and just more blocks than waves share them for: the same weights to rounding."""
+    c = Chunked(np.random.default_rng(17), *TYPES[types], lens, [11, 30], nkv, 12, 64, 100)
+    lse = lse_of(c)
+    check(c, lse, 25, run(gpu, c, lse, 25))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
 def test_results_repeat(gpu, types):
     c = Chunked(np.random.default_rng(6), *TYPES[types], [700, 90], [80, 40], 2, 8, 128, 64)
     lse = lse_of(c)
