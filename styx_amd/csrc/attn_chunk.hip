@@ -266,16 +266,16 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD, 4> {
 };
 
 // f32 caches: v_mfma_f32_32x32x2_f32, dims in fours on both sides of the score
-// product for 16-byte reads.  Chunks of at most 64 or 32 query rows would leave
+// product for 16-byte reads.  Sequences of at most 64 or 32 query rows would leave
 // two or three of four waves without any: two or four waves take the same rows,
 // each a part of the dims (one token over 2000 slots: 22.3 us with two, 18.3 with
-// four; over 32000 58 and 45).
+// four; over 32000 58 and 45; more: with_kernel).
 template <int HD, int RG> struct Wave<float, float, HD, RG> {
     using TC = float;
     using La = Lay<TC, HD>;
     static constexpr int DS = HD == 256 && RG == 4 ? 2 : 4 / RG, HW = HD / DS, NK = HW / 8, ND = HW / 32;
     static constexpr int KT = 32;
-    static constexpr int NW = RG * DS, PER_CU = HD == 256 || RG < 4 ? 1 : 2, BM = 32 * RG;
+    static constexpr int NW = RG * DS, PER_CU = HD == 64 || (HD == 128 && RG == 4) ? 2 : 1, BM = 32 * RG;
     static constexpr int IDLE = HD == 64 ? 2 : 1, BUSY = 8;
     static constexpr float PART = 0.025f * RG / 4;
     styx_f4 q[NK];
@@ -462,7 +462,7 @@ template <int BM, int KT, bool TILES> __device__ __forceinline__ Place find_plac
 // A tile that begins in a share and goes on in the next: its pieces, one in
 // each of as many shares, the first at `part0`.  pieces 0: there is none.
 struct alignas(16) Across {
-    int pieces, tile, part0;
+    int pieces, row0, part0;
     ChunkSeq s;
 };
 // Partial results, of a share's first piece and of its last (sums o, and m and
@@ -531,7 +531,7 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, RG>::NW), (Wave<TQ, TC,
         more = u < end;
         if (threadIdx.x == 0 && it.in == 0 && !whole) {
             const int pieces = (int)((it.before + it.length - 1) / line.share) - nth + 1;
-            parts.across[nth * kv.nkv + kvh] = Across{pieces, it.tile, (int)(part / kv.nkv), s};
+            parts.across[nth * kv.nkv + kvh] = Across{pieces, row0, (int)(part / kv.nkv), s};
         }
     }
     b0 = uniform(b0);
@@ -808,19 +808,18 @@ constexpr int AC_JOIN = 512;
 template <typename TQ, typename TC, int HD, int ROWS>
 __global__ void __launch_bounds__(AC_JOIN) k_attn_chunk_join(AttnChunkArgs a, Parts parts)
 {
-    using W = Wave<TQ, TC, HD>;
-    constexpr int KT = W::KT, BM = W::BM, PER_ROW = HD / 4, GROUPS = AC_JOIN / PER_ROW / ROWS, AHEAD = 4;
+    constexpr int PER_ROW = HD / 4, GROUPS = AC_JOIN / PER_ROW / ROWS, AHEAD = 4;
     static_assert(GROUPS >= 1, "threads for the rows");
     __shared__ styx_f4 s_o[AC_JOIN];
     __shared__ float2 s_ml[AC_JOIN];
     const KvView &kv = a.kv;
     const int w0 = blockIdx.z, kvh = blockIdx.y;
     const Across it = parts.across[w0 * kv.nkv + kvh];
-    const int pieces = it.pieces, rows = it.s.count * a.gqa - it.tile * BM;
+    const int pieces = it.pieces, rows = min(it.s.count * a.gqa - it.row0, parts.rows);
     const int tid = threadIdx.x, d = tid % PER_ROW * 4, in = blockIdx.x * ROWS + tid / PER_ROW % ROWS, group = tid / PER_ROW / ROWS;
-    if (pieces == 0 || (int)blockIdx.x * ROWS >= min(rows, parts.rows)) return;
-    const int r = it.tile * BM + in;
-    const bool is = in < min(rows, parts.rows);
+    if (pieces == 0 || (int)blockIdx.x * ROWS >= rows) return;
+    const int r = it.row0 + in;
+    const bool is = in < rows;
     float m = -INFINITY, l = 0.0f;
     styx_f4 o = {};
     for (int c0 = group; c0 < pieces; c0 += GROUPS * AHEAD) {
@@ -908,14 +907,24 @@ static ChunkShape shape_of(int bm, int per_cu, int n_seq, int nkv, int gqa, int 
     s.rows = (int)std::min<int64_t>(bm, (int64_t)n_rows * gqa);
     return s;
 }
-// f(query type, row type, head_dim, groups of rows) for the kernel of a call
-template <typename F> static auto with_kernel(bool f16, bool q16, int hd, int64_t rows, F f)
+// f(query type, row type, head_dim, groups of rows) for the kernel of a call with
+// so many rows.  The fewer groups a tile has the more tiles there are, and the
+// more often a slot is read.  What a sequence has is known to the device alone:
+// the sequences' average counts, and a total that one sequence may have alone.
+// One token for each of 24 over 2000 slots, heads of 128, 1 / 2 / 4 groups: 65 /
+// 88 / 81 us; 16 tokens of one 23 / 23 / 30, 128 of one 85 / 71 / 81, 32 for each
+// of 16 over 500 slots 88 / 67 / 88; a prompt of 512 54 / 61 / 51, of 1024 166 /
+// 125 / 110.  Heads of 64: 128 tokens of one - / 42 / 50, a prompt of 1024 - / 71
+// / 68.  Heads of 256: 64 of one 73 / 67 / 78, 128 of one 132 / 112 / 106.
+template <typename F> static auto with_kernel(bool f16, bool q16, int hd, int n_seq, int64_t rows, F f)
 {
     const auto four = std::integral_constant<int, 4>{};
     auto by_rows = [&](auto hd) {
+        const int64_t each = rows <= 4096 ? n_seq : 0;
         if constexpr (hd() > 64)
-            if (rows <= 32) return f(float{}, float{}, hd, std::integral_constant<int, 1>{});
-        if (rows <= 64) return f(float{}, float{}, hd, std::integral_constant<int, 2>{});
+            if (rows <= 32 * each) return f(float{}, float{}, hd, std::integral_constant<int, 1>{});
+        if (rows <= (hd() == 256 ? 512 : 1024) || rows <= 256 * each)
+            return f(float{}, float{}, hd, std::integral_constant<int, 2>{});
         return f(float{}, float{}, hd, four);
     };
     auto by_type = [&](auto hd) {
@@ -939,7 +948,7 @@ uint64_t attn_chunk_ws_bytes(int n_seq, int nkv, int hd, int gqa, int n_rows)
     // the types that the call may bring
     int64_t floats = 4;
     for (int t = 0; t < 3; t++)
-        with_kernel(t > 0, t > 1, hd, (int64_t)n_rows * gqa, [&](auto tq, auto tc, auto n, auto rg) {
+        with_kernel(t > 0, t > 1, hd, n_seq, (int64_t)n_rows * gqa, [&](auto tq, auto tc, auto n, auto rg) {
             using W = Wave<decltype(tq), decltype(tc), n(), rg()>;
             static_assert((W::BM >= 128 || rg() < 4) && W::PER_CU <= 2, "attn_chunk_grid");
             floats = std::max(floats, shape_of(W::BM, W::PER_CU, n_seq, nkv, gqa, n_rows).floats(nkv, hd));
@@ -975,7 +984,7 @@ hipError_t launch_attn_chunk(hipStream_t st, AttnChunkArgs a, void *ws)
 {
     a.scale = (float)((double)a.scale * 1.4426950408889634);  // log2 e
     a.by_gqa = page_div((uint32_t)a.gqa);
-    with_kernel(a.kv.f16, a.q_f16, a.kv.hd, (int64_t)a.chunk.n_rows * a.gqa, [&](auto tq, auto tc, auto hd, auto rg) {
+    with_kernel(a.kv.f16, a.q_f16, a.kv.hd, a.kv.n_seq, (int64_t)a.chunk.n_rows * a.gqa, [&](auto tq, auto tc, auto hd, auto rg) {
         launch_chunk<decltype(tq), decltype(tc), hd(), rg()>(st, a, ws);
         return 0;
     });
