@@ -116,8 +116,11 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD, 4> {
     using TC = _Float16;
     using La = Lay<TC, HD>;
     static constexpr int NP = sizeof(TQ) == 4 ? 2 : 1;  // pieces
-    // waves that share a query's dims, dims of a wave
-    static constexpr int DS = HD == 256 && NP == 2 ? 2 : 1, HW = HD / DS, NK = HW / 16, ND = HW / 32;
+    // waves that share a query's dims, dims of a wave (f16 queries with heads of
+    // 256: with one, registers spill.  A prompt of 2048 tokens, 16 heads, 92 us,
+    // 118 with one; single tokens of 16 sequences over 4000 slots 33 and 45; four
+    // chunks of 256 tokens behind 8000 slots 231 and 214)
+    static constexpr int DS = HD == 256 ? 2 : 1, HW = HD / DS, NK = HW / 16, ND = HW / 32;
     static constexpr int KT = HD == 256 ? 32 : 64;
     static constexpr int NW = 4 * DS, PER_CU = 8 / NW, BM = 128;
     static constexpr int IDLE = 5, BUSY = 16;  // line_of

@@ -12,9 +12,9 @@
 // (its other half, lane ^ 32, the other 16): weights are summed lane by lane.
 //
 // Bound: products and exponentials, a score costing 256 FLOP and one exponential
-// at head_dim 128.  64 tokens of 32 f16 heads over 32768 slots, 17 GFLOP: 32 us,
+// at head_dim 128.  64 tokens of 32 f16 heads over 32768 slots, 17 GFLOP: 33 us,
 // where a tile's products and its factors take about the same time, one after
-// the other.  16 conversations, 16 tokens of 64 f32 heads each, 4.3 GFLOP: 61 us,
+// the other.  16 conversations, 16 tokens of 64 f32 heads each, 4.3 GFLOP: 63 us,
 // where products alone would take 28; 540 workgroups of equal length for 256
 // CUs, so that some CUs take three and most two.  Smaller workgroups even that
 // out, but each fetches all query rows (kw_waves).
