@@ -490,7 +490,7 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, RG>::NW), (Wave<TQ, TC,
     __shared__ __align__(1024) char s_v[2][BLOCK];
     // scores of half the dims; in the block of K where there is no other place
     constexpr int PIECES = 4;
-    constexpr bool APART = 4 * BLOCK + NW * PIECES * 1024 < 150000 / W::PER_CU;
+    constexpr bool APART = 4 * BLOCK + NW * PIECES * 1024 <= 163840 / W::PER_CU;
     __shared__ styx_f4 s_half[DS > 1 && APART ? NW * PIECES : 1][64];
     const KvView &kv = a.kv;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -643,7 +643,20 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, RG>::NW), (Wave<TQ, TC,
 #pragma unroll
                 for (int e = 0; e < 4; e++) odd |= not_finite<TC>(v[e]) != 0;
             }
-            if (__syncthreads_or(odd)) {
+            bool any;
+            if constexpr (DS > 1 && APART) {
+                // (in the place of the scores: those of the last block have been
+                // read, and there may be no more LDS)
+                int *const odds = (int *)s_half;
+                const bool mine_odd = __ballot(odd) != 0;
+                if (lane == 0) odds[wave] = mine_odd;
+                __syncthreads();
+                any = __ballot(lane < NW && odds[lane & (NW - 1)]) != 0;
+                __syncthreads();
+            } else {
+                any = __syncthreads_or(odd) != 0;
+            }
+            if (any) {
 #pragma unroll 1
                 for (int t = 0; t < KT; t++) {
                     const uint32_t see = 0u - (vis[KT == 64 ? t >> 5 : 0] >> (t & 31) & 1);
