@@ -123,7 +123,7 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD, 4> {
     static constexpr int DS = HD == 256 ? 2 : 1, HW = HD / DS, NK = HW / 16, ND = HW / 32;
     static constexpr int KT = HD == 256 ? 32 : 64;
     static constexpr int NW = 4 * DS, PER_CU = 8 / NW, BM = 128;
-    static constexpr int IDLE = 5, BUSY = 16;  // line_of
+    static constexpr int IDLE = 5, BUSY = 16, ALONE = 0;  // line_of
     static constexpr float PART = HD / 3000.0f;  // (half to twice of it: within 10%)
     h8 q[NP][NK], p[KT / 32][NP][2];
     f16v s[KT / 32], o[ND];
@@ -278,8 +278,8 @@ template <int HD, int RG> struct Wave<float, float, HD, RG> {
     using La = Lay<TC, HD>;
     static constexpr int DS = HD == 256 && RG == 4 ? 2 : 4 / RG, HW = HD / DS, NK = HW / 8, ND = HW / 32;
     static constexpr int KT = 32;
-    static constexpr int NW = RG * DS, PER_CU = HD == 64 || (HD == 128 && RG == 4) ? 2 : 1, BM = 32 * RG;
-    static constexpr int IDLE = HD == 64 ? 2 : 1, BUSY = 8;
+    static constexpr int NW = RG * DS, PER_CU = HD == 256 ? 1 : 2, BM = 32 * RG;
+    static constexpr int IDLE = HD == 64 ? 2 : 1, BUSY = 8, ALONE = PER_CU == 2 ? 12 : 0;
     static constexpr float PART = 0.025f * RG / 4;
     styx_f4 q[NK];
     f16v s[1], o[ND];
@@ -418,7 +418,10 @@ template <typename W> __device__ __forceinline__ Line line_of(const AttnChunkArg
     const float blocks = (float)(total * a.kv.nkv) / (float)unit;
     const float full = fminf(1.0f, (float)a.chunk.n_rows * a.gqa / ((float)tiles * BM));
     const int64_t least = max((int)__builtin_amdgcn_sqrtf(blocks * full * W::PART), 1) * unit;
-    const int64_t shares = max(slots / a.kv.nkv, 1);
+    // Of two workgroups of f32 products on a CU each takes twice the time: one
+    // where it has fewer than ALONE blocks (8 tokens over 2000 slots 20 us, 22 with
+    // two; single tokens of 24 sequences over 2000 slots, 23 blocks, 65 and 52).
+    const int64_t shares = max((blocks < W::ALONE * AC_CUS ? AC_CUS : slots) / a.kv.nkv, 1);
     return {uniform(max((total + shares - 1) / shares, least)), total};
 }
 
@@ -927,19 +930,20 @@ static ChunkShape shape_of(int bm, int per_cu, int n_seq, int nkv, int gqa, int 
 // so many rows.  The fewer groups a tile has the more tiles there are, and the
 // more often a slot is read.  What a sequence has is known to the device alone:
 // the sequences' average counts, and a total that one sequence may have alone.
-// One token for each of 24 over 2000 slots, heads of 128, 1 / 2 / 4 groups: 65 /
-// 88 / 81 us; 16 tokens of one 23 / 23 / 30, 128 of one 85 / 71 / 81, 32 for each
-// of 16 over 500 slots 88 / 67 / 88; a prompt of 512 54 / 61 / 51, of 1024 166 /
-// 125 / 110.  Heads of 64: 128 tokens of one - / 42 / 50, a prompt of 1024 - / 71
-// / 68.  Heads of 256: 64 of one 73 / 67 / 78, 128 of one 132 / 112 / 106.
+// One token for each of 24 over 2000 slots, heads of 128, 1 / 2 / 4 groups: 53 /
+// 72 / 82 us; 16 tokens of one over 500 17 / 20 / 22, 64 of one over 2000 44 / 43 /
+// 48, 128 of one 71 / 66 / 65; a prompt of 512 50 / 55 / 50, of 1024 124 / 119 /
+// 111.  Heads of 64: 16 tokens of one over 2000 - / 19 / 22, 128 of one - / 45 / 43.
+// Heads of 256: 64 of one 74 / 67 / 77, 128 of one 134 / 114 / 105, 32 for each of 16
+// over 500 138 / 107 / 160.
 template <typename F> static auto with_kernel(bool f16, bool q16, int hd, int n_seq, int64_t rows, F f)
 {
     const auto four = std::integral_constant<int, 4>{};
     auto by_rows = [&](auto hd) {
         const int64_t each = rows <= 4096 ? n_seq : 0;
         if constexpr (hd() > 64)
-            if (rows <= 32 * each) return f(float{}, float{}, hd, std::integral_constant<int, 1>{});
-        if (rows <= (hd() == 256 ? 512 : 1024) || rows <= 256 * each)
+            if (rows <= 128 || rows <= 32 * each) return f(float{}, float{}, hd, std::integral_constant<int, 1>{});
+        if (rows <= 512 || rows <= (hd() == 256 ? 256 : 64) * each)
             return f(float{}, float{}, hd, std::integral_constant<int, 2>{});
         return f(float{}, float{}, hd, four);
     };
