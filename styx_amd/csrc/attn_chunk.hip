@@ -552,7 +552,10 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, RG>::NW), (Wave<TQ, TC,
     const int r = min(wrow0 + n, rows - 1), tok = a.by_gqa.of(r), head = kvh * a.gqa + (r - tok * a.gqa);
     const int at = wrow0 + n < rows ? s.len + tok : -1;  // last slot seen, -1: no such row
     const int64_t orow = s.first + tok;                  // row of q and out
-    float m = -INFINITY;  // the reference, a whole number
+    // the reference: a whole number, or the first block's largest score, whose
+    // factor then has no rounding to f16 (a token that sees one slot gets its V)
+    constexpr bool ONE = sizeof(TQ) == 2;
+    float m = -INFINITY;
     x.ref = AC_OFF;
     x.sum[0] = x.sum[1] = 0.0f;
     constexpr int NANS = (HW + 63) / 64;
@@ -697,7 +700,8 @@ __global__ void __launch_bounds__((64 * Wave<TQ, TC, HD, RG>::NW), (Wave<TQ, TC,
             for (int i = 0; i < 16; i += 2) mx = fmaxf(fmaxf(mx, x.s[kt][i]), x.s[kt][i + 1]);
             mx = fmaxf(mx, other_half(mx)) * x.mul;
             if (__ballot(mx > m + AC_LAG)) {
-                const float mn = fmaxf(m, ceilf(mx));
+                // (by whole numbers, so that sums are multiplied by powers of two)
+                const float mn = !ONE ? fmaxf(m, ceilf(mx)) : m == -INFINITY ? mx : m + fmaxf(ceilf(mx - m), 0.0f);
                 if (mn != -INFINITY) {
                     x.rescale(exp2_(m - mn), kt > 0);
                     x.ref = AC_OFF - mn;

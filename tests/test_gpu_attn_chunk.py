@@ -7,7 +7,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from chunk_cases import Chunked, check_chunk, run_chunk
+from chunk_cases import E, Chunked, check_chunk, run_chunk
 from styx_amd import _lib as L
 
 pytestmark = pytest.mark.gpu
@@ -143,6 +143,26 @@ def test_values_that_are_not_finite_reach_the_outputs(gpu, types, count):
     c.k[rows[40], 0, 3] = np.nan
     out, lse = run_chunk(gpu, c)
     assert np.isnan(out).all() and np.isnan(lse).all()
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("lens,counts,window", [([0, 0, 0], [1, 1, 1], 0), ([200, 0, 2000], [70, 33, 3], 1)])
+def test_one_slot_gives_its_value(gpu, types, hd, lens, counts, window):
+    """A weight of 1 is no rounding: 16-bit outputs are the slot's V itself, 32-bit ones to the quotient of two sums."""
+    c = Chunked(np.random.default_rng(hd), *TYPES[types], lens, counts, 2, 4, hd, 16, window=window)
+    out, lse = run_chunk(gpu, c)
+    check_chunk(c, out, lse, tokens=FEW)
+    for b in range(3):
+        rows = c.rows(b)
+        for i in range(counts[b]):
+            want = np.repeat(c.v[rows[lens[b] + i]], 4, 0)
+            got = out[c.first[b] + i].reshape(8, hd)
+            if c.q16:
+                assert np.array_equal(got, want), (b, i)
+            else:  # a factor's own pieces or bits, over it: 2^-22 and two roundings
+                want = want.astype(np.float64)
+                assert (np.abs(got - want) <= (2.0 ** -22 + 4 * E) * np.abs(want)).all(), (b, i)
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
