@@ -19,7 +19,7 @@
 // clock is what holds it: 1.85 GHz under these products, and with q, K and V all
 // 0 the same launch takes 455 us.  f32 queries on f16 rows, 406 GFLOP in two
 // pieces: 458 us, 886 TFLOP/s.  f32, three documents, heads of 256, 211 GFLOP:
-// 1.78 ms, 119 of 152 TFLOP/s.  f16 heads of 64 under a window of 1024, 21 GFLOP:
+// 1.75 ms, 121 of 152 TFLOP/s.  f16 heads of 64 under a window of 1024, 21 GFLOP:
 // 49 us; a score costs 256 FLOP there and its exponential, maximum, sum and
 // rounding more time than they.
 //
