@@ -459,8 +459,10 @@ int styx_op_kv_append(styx_gpu *gpu, const styx_kv_cache *kv, int n_rows, const 
  * at most 2^28.
  *   s_t = scale q . K[t], out = sum e^(s_t - M) V[t] / sum e^(s_t - M)
  * lse [n_rows][nh] f32 or NULL: ln of the sum of e^s_t.  A token that sees
- * nothing: out 0, lse -infinity.  Scores, sums and lse are f32; with f16 q the
- * factors are rounded to f16 on their way to V, with f32 q they are not.  A
+ * nothing: out 0, lse -infinity.  Scores, sums and lse are f32.  On their way to
+ * V the factors e^(s_t - M) are f32 for an f32 cache; for an f16 cache they are
+ * off by at most 2^-11 of themselves with f16 q, 2^-22 with f32 q (which is
+ * rounded to 22 bits, too), and 2^-30 of the token's largest factor.  A
  * score that is NaN or +infinity makes the outputs of its token and head NaN
  * (with f32 q on an f16 cache one of -infinity, too); a V value that is not
  * finite makes its dimension infinite or NaN where the token sees the row.

@@ -253,7 +253,8 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD, 4> {
         }
     }
     // All but the scores times c, a power of two; `pending`: factors of the first
-    // 32 slots that have not met V.
+    // 32 slots that have not met V.  Those in f32, as c need not be an f16 number:
+    // below 2^-24 it would be 0, where a factor of up to 2^15 times it is one.
     __device__ __forceinline__ void rescale(float c, bool pending)
     {
         sum[0] *= c;
@@ -262,9 +263,14 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD, 4> {
         for (int d = 0; d < ND; d++) o[d] *= c;
         if (pending)
 #pragma unroll
-            for (int y = 0; y < NP; y++)
-#pragma unroll
-                for (int k = 0; k < 2; k++) p[0][y][k] *= (_Float16)c;
+            for (int i = 0; i < 16; i++) {
+                float f = (float)p[0][0][i >> 3][i & 7];
+                if constexpr (NP == 2) f += (float)p[0][1][i >> 3][i & 7];
+                f *= c;
+                const _Float16 hi = (_Float16)f;
+                p[0][0][i >> 3][i & 7] = hi;
+                if constexpr (NP == 2) p[0][1][i >> 3][i & 7] = (_Float16)(f - (float)hi);
+            }
     }
 };
 

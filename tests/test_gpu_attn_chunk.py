@@ -7,7 +7,7 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from chunk_cases import E, Chunked, check_chunk, run_chunk
+from chunk_cases import E, E16, TINY16, Chunked, check_chunk, run_chunk
 from styx_amd import _lib as L
 
 pytestmark = pytest.mark.gpu
@@ -172,6 +172,43 @@ def test_large_and_equal_scores(gpu, types):
     c.q = (c.q * 40).astype(c.qt)
     c.q[30:] = 0
     check_chunk(c, *run_chunk(gpu, c))
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("start", [0, 32, 64])
+@pytest.mark.parametrize("slots", [130, 6000])
+@pytest.mark.parametrize("sizes", [(1, 0.5, 1, 1.25), (1, 0.5, 1, 0.75)])
+def test_a_score_far_above_those_before_it(gpu, types, hd, start, slots, sizes):
+    """Slots with scores of 0, 32 of 7.75 (in units of ln 2), one of `jump`, the rest of -60: V is 1 in the 32 alone, so
+    that the outputs are nothing but their small weights, whatever part of a block the large score comes in.  Queries of
+    `sizes`: 1.25 moves the reference for the 32, too (7.75 times it is more than 8).
+
+    Weights as in Chunked.attend; with 16-bit rows a factor is also off by half of f16's smallest step when it is formed
+    and once more when the large score moves the reference: 2 TINY16, where the largest factor is 2^6 at least."""
+    for jump in (9, 15, 23.5, 24, 24.5, 25.5, 26.5, 33):
+        c = Chunked(np.random.default_rng(1), *TYPES[types], [slots - 4], [4], 2, 4, hd, 16)
+        c.scale = float(np.float32(np.log(2)))
+        s = np.full(slots, -60.0)
+        s[:start], s[start:start + 32], s[start + 32] = 0, 7.75, jump
+        rows = c.rows(0)
+        c.q[:], c.k[:], c.v[:] = 0, 0, 0
+        c.q.reshape(4, 8, hd)[:, :, 0] = sizes * 2
+        c.k[rows, :, 0] = s[:, None]
+        c.v[rows[start:start + 32]] = 1
+        out, lse = run_chunk(gpu, c)
+        for i, j in ((0, 0), (3, 1)):
+            want, _, want_lse, tol_lse = c.attend(0, i, j)
+            x, ds, see = c.scores(0, i, j, rows)
+            tot = np.exp(x - x.max(1, keepdims=True)).sum(1, keepdims=True)
+            tol = (2 * ds.max(1, keepdims=True) + 2 * (see.sum() + 40) * E) * want + 1e-30
+            if c.f16:
+                tol = tol + 2 * TINY16 * 2.0 ** -6 * 32 / tot
+            if c.q16:
+                tol = tol + E16 * want + E16 * want + TINY16
+            got = out[i].reshape(8, hd)[4 * j:4 * j + 4].astype(np.float64)
+            assert (np.abs(got - want) <= tol).all(), (jump, i, j, got[:, 0], want[:, 0], tol[:, 0])
+            assert (np.abs(lse[i, 4 * j:4 * j + 4] - want_lse) <= tol_lse).all(), (jump, i, j)
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
