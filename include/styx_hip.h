@@ -442,8 +442,9 @@ typedef struct styx_rope {
  * hold all three); q_norm, k_norm [hd] or NULL; rope NULL: no rotation.
  * q_out [n_rows][nh*hd] of type_q, rows ldo apart; it may be q itself.  k and
  * v NULL: q alone; q and q_out NULL: k and v alone.  A row whose row_pos is
- * outside the rope table is skipped; one whose row_at is outside the pools
- * has its q turned and no K and V.  Normalised and turned in f64, rounded to
+ * below 0 or outside the rope table is skipped (row_pos NULL, without a table
+ * alone: none is); one whose row_at is outside the pools has its q turned and no
+ * K and V.  Normalised and turned in f64, rounded to
  * f32 and from there to the type.  Two rows may not have one row_at.  Rows must
  * be 16-byte aligned.  The cache's page table is not read.  Allocates nothing. */
 int styx_op_kv_append(styx_gpu *gpu, const styx_kv_cache *kv, int n_rows, const int32_t *row_pos,

@@ -54,9 +54,10 @@ __global__ void __launch_bounds__(KA_WG, 4) k_kv_append(KvAppendArgs a)
     const KvView &kv = a.kv;
     const int row = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int slot = lane / LPH, d0 = lane % LPH * VEC;
-    const int pos = a.rope ? a.row_pos[row] : 0;
+    const int pos = a.row_pos ? a.row_pos[row] : 0;
     const int at = a.k ? a.row_at[row] : -1;
-    if (a.rope && (uint32_t)pos >= (uint32_t)a.n_pos) return;
+    // (a row of no sequence has a position below 0, with a table or without)
+    if (a.rope ? (uint32_t)pos >= (uint32_t)a.n_pos : pos < 0) return;
     const bool store = at >= 0 && at < kv.n_pages * kv.page_tokens;
     // groups of heads: q's, then k's, then v's
     const int gq = (a.nh + HPW - 1) / HPW, gk = (kv.nkv + HPW - 1) / HPW, groups = gq + (store ? 2 * gk : 0);

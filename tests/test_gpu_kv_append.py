@@ -158,6 +158,32 @@ def test_rows_outside_the_table_or_the_pools(gpu, t):
     r.check(r.call(gpu))
 
 
+@pytest.mark.parametrize("t", [L.F32, L.F16])
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("norms", [False, True])
+def test_rows_of_no_sequence_without_positions(gpu, t, in_place, norms):
+    """No table: a row whose position is negative, as a plan marks rows of no sequence and of those that got no pages,
+    is left all the same (in place it is asked for again, and a norm must not be applied twice)."""
+    r = Rows(np.random.default_rng(9), t, t, t, 12, 4, 2, 64, 0, False, norms=norms, pad=8)
+    r.row_pos[[0, 5, 11]] = [-1, -7, -2 ** 31]
+    r.row_pos[3] = 2 ** 31 - 1  # (there is no table that it could be outside of)
+    r.row_at[[0, 5]] = -1       # (the last one's place is a row of the pools)
+    r.row_at[4] = -1
+    out, kp, vp = r.call(gpu, in_place=in_place, ldo=4 * 64 + 8)
+    left = np.ones(len(kp), bool)
+    for i in range(12):
+        if i in (0, 5, 11):
+            assert np.array_equal(out[i], r.qkv[i]) if in_place else (out[i] == 7.5).all(), i
+            continue
+        r.near(out[i, :256].reshape(4, 64), r.turned(i, "q"), t)
+        if i != 4:
+            left[r.row_at[i]] = False
+            r.near(kp[r.row_at[i]], r.turned(i, "k"), t)
+            assert np.array_equal(vp[r.row_at[i]], r.part(i, "v"))
+    for p, before in zip((kp, vp), r.pools):
+        assert np.array_equal(p[left], before[left])
+
+
 @pytest.mark.parametrize("inter", [False, True])
 @pytest.mark.parametrize("norms", [False, True])
 @pytest.mark.parametrize("t", [L.F32, L.F16])
