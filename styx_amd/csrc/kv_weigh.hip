@@ -179,16 +179,17 @@ __global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), (KW_SIMD<T
             }
             if (tid % TPR == 0) {
                 const int r = base + mr;
-                // a token that sees nothing has no weights
-                s_lse[buf][mr] = r < r1 && in_lse != -INFINITY ? in_lse * 1.44269504f : INFINITY;
+                // a token that sees nothing has no weights: none that are NaN, either
+                const bool counts = r < r1 && in_lse != -INFINITY;
+                s_lse[buf][mr] = counts ? in_lse * 1.44269504f : INFINITY;
                 s_mul[buf][mr] = mul;
-                s_at[buf][mr] = r < r1 ? s.len + a.by_gqa.of(r) : -1;
+                s_at[buf][mr] = counts ? s.len + a.by_gqa.of(r) : -1;
             }
         };
         float sum[2] = {};
-        auto add = [&](const f16v &x, int base, const float *s_l, const float *s_m, const int *s_a) {
-            // whether every row of the tile sees all of the wave's slots
-            const bool whole = base + KW_ROWS <= r1 && w0 + 31 <= s.len + a.by_gqa.of(base) &&
+        auto add = [&](const f16v &x, int base, bool all, const float *s_l, const float *s_m, const int *s_a) {
+            // whether every row of the tile counts and sees all of the wave's slots
+            const bool whole = all && w0 + 31 <= s.len + a.by_gqa.of(base) &&
                                (!a.window || w0 > s.len + a.by_gqa.of(base + KW_ROWS - 1) - a.window);
             float w[16];
 #pragma unroll
@@ -223,6 +224,7 @@ __global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), (KW_SIMD<T
         }
         for (int base = few ? r1 : r0, buf = 0; base < r1; base += KW_ROWS, buf ^= 1) {
             __syncthreads();
+            const int last = s_at[buf][n];
             f16v x = {};
 #pragma unroll
             for (int i = 0; i < NK; i++) {
@@ -240,7 +242,7 @@ __global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), (KW_SIMD<T
                 put(buf ^ 1, base + KW_ROWS);
                 if (base + 2 * KW_ROWS < r1) ask(base + 2 * KW_ROWS);
             }
-            add(x, base, s_lse[buf], s_mul[buf], s_at[buf]);
+            add(x, base, __ballot(last < 0) == 0, s_lse[buf], s_mul[buf], s_at[buf]);
         }
         for (int base = few ? r0 + KW_ROWS * wave : r1; base < r1; base += KW_ROWS * KW_NW) {
             // row n of a tile of the wave's own, as it lies
@@ -268,9 +270,10 @@ __global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), (KW_SIMD<T
                 mul /= up;
             }
             if (h == 0) {
-                s_own[wave][0][n] = base + n < r1 && lse != -INFINITY ? lse * 1.44269504f : INFINITY;
+                const bool counts = base + n < r1 && lse != -INFINITY;
+                s_own[wave][0][n] = counts ? lse * 1.44269504f : INFINITY;
                 s_own[wave][1][n] = mul;
-                s_own_at[wave][n] = base + n < r1 ? s.len + tok : -1;
+                s_own_at[wave][n] = counts ? s.len + tok : -1;
             }
             Raw y[AHEAD];
 #pragma unroll
@@ -297,7 +300,7 @@ __global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), (KW_SIMD<T
             }
             // (a wave's LDS operations are carried out in order)
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            add(x, base, s_own[wave][0], s_own[wave][1], s_own_at[wave]);
+            add(x, base, __ballot(s_own_at[wave][n] < 0) == 0, s_own[wave][0], s_own[wave][1], s_own_at[wave]);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
         float all = sum[0] + sum[1];

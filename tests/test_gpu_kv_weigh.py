@@ -149,6 +149,25 @@ def test_not_finite(gpu, types):
 
 
 @pytest.mark.parametrize("types", sorted(TYPES))
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("lens,counts,gqa", [([70], [10], 4), ([3000, 40], [60, 5], 8), ([40000], [40], 4)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf])
+def test_a_token_without_weights_adds_nothing_whatever_its_query_holds(gpu, types, hd, lens, counts, gqa, bad):
+    """Tokens with lse -infinity whose q is not finite: the others' weights alone, where waves share blocks of slots and not."""
+    c = Chunked(np.random.default_rng(hd), *TYPES[types], lens, counts, 1, gqa, hd, 16)
+    q = c.q.copy()
+    lse = np.full((c.n_rows, c.nh), 4, np.float32)
+    dead = [0, 3, counts[0] - 1]
+    lse[dead] = -np.inf
+    c.q[dead] = bad
+    got = run(gpu, c, lse, 1000, with_acc=False)
+    assert np.isfinite(got[4]).all()
+    c.q = q
+    lse[dead] = 1e5  # (e^-1e5 is 0, too; check's bound would be 0 times infinity)
+    check(c, lse, max(counts), got, with_acc=False)
+
+
+@pytest.mark.parametrize("types", sorted(TYPES))
 @pytest.mark.parametrize("scale", [0.0, -0.2])
 def test_scales(gpu, types, scale):
     c = Chunked(np.random.default_rng(8), *TYPES[types], [130], [9], 2, 4, 64, 16)
