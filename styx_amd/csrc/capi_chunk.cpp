@@ -4,7 +4,6 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
-#include <vector>
 
 #include "capi.h"
 #include "kv_chunk.h"
@@ -64,32 +63,35 @@ int styx_rope_table_scaled(float base, int n_rot, int n_pos, const styx_rope_sca
     const double pi2 = 6.283185307179586476925286766559, factor = z.factor;
     double b = base, gain = z.gain != 0.0f ? z.gain : 1.0;
     if (z.kind == STYX_ROPE_BASE) b = base * std::pow(factor, (double)n_rot / (n_rot - 2));
-    std::vector<double> f(half);
     const double ts = std::pow(b, -2.0 / (double)n_rot);
-    for (int i = 0; i < half; i++) f[i] = std::pow(ts, (double)i);
-    if (z.kind == STYX_ROPE_LINEAR)
-        for (double &x : f) x /= factor;
+    double low = 0.0, high = 0.0;  // PARTS: the ramp's pairs
     if (z.kind == STYX_ROPE_PARTS) {
         // the pair that makes `turns` turns over n_orig positions
         auto pair_of = [&](double turns) { return n_rot * std::log(z.n_orig / (turns * pi2)) / (2.0 * std::log(b)); };
-        const double low = std::max(0.0, std::floor(pair_of(fast)));
-        double high = std::min(n_rot - 1.0, std::ceil(pair_of(slow)));
+        low = std::max(0.0, std::floor(pair_of(fast)));
+        high = std::min(n_rot - 1.0, std::ceil(pair_of(slow)));
         if (high <= low) high = low + 0.001;  // a step
-        for (int i = 0; i < half; i++) {
-            const double r = std::min(1.0, std::max(0.0, (i - low) / (high - low)));
-            f[i] = f[i] * (1.0 - r) + f[i] / factor * r;
-        }
         if (z.gain == 0.0f && factor > 1.0) gain = 0.1 * std::log(factor) + 1.0;
     }
-    if (z.kind == STYX_ROPE_BANDS)
-        for (double &x : f) {
-            const double turns = z.n_orig * x / pi2;
-            const double r = std::min(1.0, std::max(0.0, (turns - slow) / (fast - slow)));
-            x = x / factor * (1.0 - r) + x * r;
+    // The frequencies lie in the table's first row until that, the last, is
+    // written: there is no other memory, whose allocation could throw.
+    for (int i = 0; i < half; i++) {
+        double f = std::pow(ts, (double)i);
+        if (z.kind == STYX_ROPE_LINEAR) f /= factor;
+        if (z.kind == STYX_ROPE_PARTS) {
+            const double r = std::min(1.0, std::max(0.0, (i - low) / (high - low)));
+            f = f * (1.0 - r) + f / factor * r;
         }
-    for (int p = 0; p < n_pos; p++)
+        if (z.kind == STYX_ROPE_BANDS) {
+            const double turns = z.n_orig * f / pi2;
+            const double r = std::min(1.0, std::max(0.0, (turns - slow) / (fast - slow)));
+            f = f / factor * (1.0 - r) + f * r;
+        }
+        out[(size_t)i * 2] = f;
+    }
+    for (int p = n_pos - 1; p >= 0; p--)
         for (int i = 0; i < half; i++) {
-            const double th = (double)p * f[i];
+            const double th = (double)p * out[(size_t)i * 2];
             out[((size_t)p * half + i) * 2] = gain * std::cos(th);
             out[((size_t)p * half + i) * 2 + 1] = gain * std::sin(th);
         }

@@ -8,6 +8,8 @@ import json
 import math
 import shutil
 import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -15,6 +17,7 @@ import pytest
 from styx_amd import _lib as L, rope_table
 from test_abi_drift import HDR, rust_layout, rust_structs
 
+ROOT = Path(__file__).resolve().parent.parent
 STRUCTS = {"styx_kv_chunk": "KvChunk", "styx_kv_pages": "KvPages", "styx_rope": "Rope", "styx_rope_scaling": "RopeScaling"}
 
 
@@ -120,3 +123,30 @@ def test_entry_points_refuse_a_null_gpu():
     assert lib.styx_op_kv_append(None, None, 0, None, None, 0, 0, None, 0, None, 0, None, 0, None, None, 0.0, None, 0, None, 0) == -1
     assert lib.styx_op_attn_chunk(None, None, None, 0, 0, None, 0, 0.0, 0, None, 0, None, None, 0) == -1
     assert lib.styx_op_kv_weigh(None, None, None, None, 0, 0, None, 0, 0.0, 0, None, 0, 0.0, None, None, None) == -1
+
+
+def test_a_rope_table_needs_no_memory_of_its_own():
+    """The call returns, and right, in a process that can allocate no more (an exception that leaves a C function ends
+    the process)."""
+    src = """
+import resource, numpy as np
+from styx_amd import _lib as L
+lib = L.load()
+n_rot = 1 << 23  # 2^22 pairs: 32 MiB of frequencies
+out, ref = np.zeros((2, n_rot // 2, 2)), np.zeros((2, 32, 2))
+s = L.RopeScaling(L.ROPE_LINEAR, 4.0, 0, 0.0, 0.0, 0.0)
+call = lambda n, o: lib.styx_rope_table_scaled(1e4, n, 2, L.C.byref(s), o.ctypes.data)
+assert call(64, ref) == 0
+used = int(open("/proc/self/statm").read().split()[0]) * resource.getpagesize()
+limit = resource.getrlimit(resource.RLIMIT_AS)
+resource.setrlimit(resource.RLIMIT_AS, (used + (8 << 20), limit[1]))
+rc = call(n_rot, out)
+resource.setrlimit(resource.RLIMIT_AS, limit)
+assert rc == 0
+assert (out[0] == [1.0, 0.0]).all() and np.abs(out[1, 0] - [np.cos(0.25), np.sin(0.25)]).max() < 1e-15
+f = 0.25 * 1e4 ** (-2.0 * (n_rot // 4) / n_rot)
+assert np.abs(out[1, n_rot // 4] - [np.cos(f), np.sin(f)]).max() < 1e-9
+print("done")
+"""
+    r = subprocess.run([sys.executable, "-c", src], capture_output=True, text=True, cwd=ROOT, timeout=100)
+    assert r.returncode == 0 and "done" in r.stdout, (r.returncode, r.stderr[-500:])
