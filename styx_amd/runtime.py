@@ -318,6 +318,11 @@ class KvBatch:
                 b.free()
         return ch
 
+    def _check(self, ch: "Chunk") -> None:
+        """A chunk's arrays have an entry for each of its own batch's sequences."""
+        if ch.n_seq != self.n_seq:
+            raise ValueError(f"a chunk of {ch.n_seq} sequences in a batch of {self.n_seq}")
+
     def _rows(self, name: str, b, type_: int, n_rows: int, heads: int, ld) -> int:
         """Values from one row to the next, after a check of the buffer's size."""
         ld, es = ld or heads * self.hd, 2 if type_ == L.F16 else 4
@@ -331,6 +336,7 @@ class KvBatch:
                type_in: int = L.F32, type_q: int = L.F32, ldq=None, ldk=None, ldv=None, ldo=None) -> None:
         """styx_op_kv_append of the chunk's rows; q, k, v and q_out are buffers
         or (buffer, byte offset), ld* the values from one row to the next."""
+        self._check(ch)
         n_rot = self.hd if n_rot is None else n_rot
         if rope is not None and rope.nbytes < 8 * n_pos * n_rot:
             raise ValueError(f"rope: {rope.nbytes} bytes, {8 * n_pos * n_rot} needed")
@@ -350,6 +356,7 @@ class KvBatch:
                      type_q: int = L.F32, ldq=None, ldo=None) -> None:
         """styx_op_attn_chunk of the chunk's rows; q and out are buffers or
         (buffer, byte offset)."""
+        self._check(ch)
         at = lambda b: b[0].ptr + b[1] if isinstance(b, tuple) else b.ptr  # noqa: E731
         ldq, ldo = (self._rows(name, b, type_q, ch.n_rows, nh, ld) for name, b, ld in (("q", q, ldq), ("out", out, ldo)))
         if lse is not None and lse.nbytes < 4 * ch.n_rows * nh:
@@ -365,6 +372,7 @@ class KvBatch:
         tokens, and the new rows' positions."""
         if not self.scored:
             raise ValueError("a cache without scores has nothing to add to")
+        self._check(ch)
         ldq = self._rows("q", q, type_q, ch.n_rows, nh, ldq)
         if lse.nbytes < 4 * ch.n_rows * nh:
             raise ValueError(f"lse: {lse.nbytes} bytes, {4 * ch.n_rows * nh} needed")

@@ -14,7 +14,7 @@ from pathlib import Path
 import numpy as np
 import pytest
 
-from styx_amd import _lib as L, rope_table
+from styx_amd import Chunk, KvBatch, _lib as L, rope_table
 from test_abi_drift import HDR, rust_layout, rust_structs
 
 ROOT = Path(__file__).resolve().parent.parent
@@ -150,3 +150,48 @@ print("done")
 """
     r = subprocess.run([sys.executable, "-c", src], capture_output=True, text=True, cwd=ROOT, timeout=100)
     assert r.returncode == 0 and "done" in r.stdout, (r.returncode, r.stderr[-500:])
+
+
+class Held:
+    """A buffer that is there, or was freed."""
+    ptr, nbytes = 4096, 1 << 20
+
+    def __init__(self):
+        self.h = 1
+
+    def free(self):
+        self.h = None
+
+
+def batch_and_chunk(n_seq, n_seq_chunk):
+    """A KvBatch and a Chunk of a batch of other sequences, without a GPU; a call that gets as far as the library counts."""
+    kv, other, reached = KvBatch.__new__(KvBatch), KvBatch.__new__(KvBatch), []
+
+    class Gpu:
+        h = None
+        buffer = staticmethod(lambda nbytes: Held())
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: reached.append(name) or 0
+    for x, n in ((kv, n_seq), (other, n_seq_chunk)):
+        x.gpu, x.lib, x.n_seq, x.nkv, x.hd, x.scored, x._ws = Gpu(), Lib(), n, 1, 64, True, Held()
+        x.c = L.KvCache(L.F32, n, 1, 64, 16, 4, 4, 4096, 4096, 4096)
+        x.kpool, x.vpool, x.table, x.len, x.pos, x.acc, x.slot_pos = (Held() for _ in range(7))
+        x.held = x.free_pages = x.n_free = None
+    return kv, Chunk(other, 3), reached
+
+
+CALLS = {"append": lambda kv, ch, b: kv.append(ch, 1, b, b, b, b, None),
+         "attend_chunk": lambda kv, ch, b: kv.attend_chunk(ch, 1, b, b, 1.0),
+         "weigh": lambda kv, ch, b: kv.weigh(ch, 1, b, b, 1.0, 1)}
+
+
+@pytest.mark.parametrize("call", sorted(CALLS))
+@pytest.mark.parametrize("n_seq,n_seq_chunk", [(4, 2), (2, 4)])
+def test_a_chunk_of_other_sequences_is_refused(call, n_seq, n_seq_chunk):
+    """Its arrays have as many entries as its own batch has sequences: a larger batch would read behind them."""
+    kv, ch, reached = batch_and_chunk(n_seq, n_seq_chunk)
+    with pytest.raises(ValueError, match="sequences"):
+        CALLS[call](kv, ch, Held())
+    assert not reached
