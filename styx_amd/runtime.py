@@ -319,7 +319,9 @@ class KvBatch:
         return ch
 
     def _check(self, ch: "Chunk") -> None:
-        """A chunk's arrays have an entry for each of its own batch's sequences."""
+        """A chunk's arrays have an entry for each of its own batch's sequences, and must still be there."""
+        if not all(b.h for b in (ch.first, ch.count, ch.len, ch.row_seq, ch.row_pos, ch.row_at)):
+            raise ValueError("the chunk, or the batch that planned it, was freed")
         if ch.n_seq != self.n_seq:
             raise ValueError(f"a chunk of {ch.n_seq} sequences in a batch of {self.n_seq}")
 
@@ -398,7 +400,8 @@ class Chunk:
         self.n_rows, self.n_seq = n_rows, kv.n_seq
         self.first, self.count = (kv.gpu.buffer(max(4 * kv.n_seq, 16)) for _ in range(2))
         self.row_seq, self.row_pos, self.row_at = (kv.gpu.buffer(max(4 * n_rows, 16)) for _ in range(3))
-        self.c = L.KvChunk(n_rows, self.first.ptr, self.count.ptr, kv.len.ptr)
+        self.len = kv.len
+        self.c = L.KvChunk(n_rows, self.first.ptr, self.count.ptr, self.len.ptr)
 
     def counts(self) -> np.ndarray:
         """New tokens of each sequence that got its pages."""

@@ -195,3 +195,20 @@ def test_a_chunk_of_other_sequences_is_refused(call, n_seq, n_seq_chunk):
     with pytest.raises(ValueError, match="sequences"):
         CALLS[call](kv, ch, Held())
     assert not reached
+
+
+@pytest.mark.parametrize("call", sorted(CALLS))
+@pytest.mark.parametrize("freed", ["chunk", "batch"])
+def test_a_freed_chunk_is_refused(call, freed):
+    """And one whose lengths were freed with the batch that planned it."""
+    kv, ch, reached = batch_and_chunk(4, 4)
+    CALLS[call](kv, ch, Held())
+    assert any("styx_op" in name for name in reached)
+    reached.clear()
+    if freed == "chunk":
+        ch.free()
+    else:
+        ch.len.free()
+    with pytest.raises(ValueError, match="freed"):
+        CALLS[call](kv, ch, Held())
+    assert not reached
