@@ -404,9 +404,11 @@ typedef struct styx_kv_pages {
     int32_t *free_pages; /* [n_pages] */
     int32_t *n_free;     /* [1] */
 } styx_kv_pages;
-/* Page tables and row maps of a step.  Sequence b has len[b] rows (-1: it has
- * ended, or waits) and asks for n_new[b] more (a negative number is 0) from
- * position pos[b] on.  first[b] is the sum of n_new before b.  In this order:
+/* Page tables and row maps of a step.  Sequence b has len[b] rows and asks for
+ * n_new[b] more (a negative number is 0) from position pos[b] on.  len[b] = -1:
+ * there is no sequence, it has ended or not begun, and its pages go back; one
+ * that only pauses keeps its length and asks for 0.  first[b] is the sum of
+ * n_new before b.  In this order:
  *   pages past those that the rows fill, new ones included, and past the
  *   first shared[b] (pages of another's; NULL: none) go to the stack, sequence
  *   by sequence, in the order of the table; their entries become -1.  Entries
@@ -424,6 +426,9 @@ typedef struct styx_kv_pages {
  * page_tokens, n_pages and table_len, its pointers are not read.  out's four
  * arrays are in's (in place), or others that overlap none of them; entries
  * past those named stay as they are.  n_seq * table_len must be below 2^31.
+ * Entries of shared pages stay, with held, where a sequence has ended, too:
+ * whoever put them there takes them out before its place is used again, else
+ * they are the next sequence's own.
  * Advance len by count for the next step.  Allocates nothing. */
 int styx_op_kv_plan(styx_gpu *gpu, const styx_kv_cache *kv, const styx_kv_pages *in,
                     const styx_kv_pages *out, const int32_t *shared, const int32_t *len,
@@ -446,7 +451,8 @@ typedef struct styx_rope {
  * alone: none is); one whose row_at is outside the pools has its q turned and no
  * K and V.  Normalised and turned in f64, rounded to
  * f32 and from there to the type.  Two rows may not have one row_at.  Rows must
- * be 16-byte aligned.  The cache's page table is not read.  Allocates nothing. */
+ * be 16-byte aligned, n_rows below 2^24.  The cache's page table is not read
+ * (NULL is refused all the same).  Allocates nothing. */
 int styx_op_kv_append(styx_gpu *gpu, const styx_kv_cache *kv, int n_rows, const int32_t *row_pos,
                       const int32_t *row_at, int nh, int type_in, const void *q, int64_t ldq,
                       const void *k, int64_t ldk, const void *v, int64_t ldv, const float *q_norm,
@@ -456,8 +462,8 @@ int styx_op_kv_append(styx_gpu *gpu, const styx_kv_cache *kv, int n_rows, const 
  * slots t <= len[b] + i, with window > 0 those of t > len[b] + i - window
  * alone, as far as their pages are in the pool.  q (turned) and out
  * [n_rows][nh*hd] of type_q: STYX_F32, or STYX_F16 for an f16 cache; rows ldq
- * and ldo values apart, 16-byte aligned; nh / nkv from 1 to 16, n_rows times it
- * at most 2^28.
+ * and ldo values apart, 16-byte aligned; nh / nkv from 1 to 16, n_rows * nh +
+ * 128 * nkv * (n_seq + 1) at most 2^28.
  *   s_t = scale q . K[t], out = sum e^(s_t - M) V[t] / sum e^(s_t - M)
  * lse [n_rows][nh] f32 or NULL: ln of the sum of e^s_t.  A token that sees
  * nothing: out 0, lse -infinity.  Scores, sums and lse are f32.  On their way to
@@ -485,8 +491,9 @@ uint64_t styx_op_attn_chunk_ws_bytes(const styx_kv_cache *kv, int n_rows, int nh
  * [n_seq][nkv][cap], acc_in NULL: zeros; it may be acc_out); slots past them
  * stay as they are.  A token with lse -infinity adds nothing, one with a NaN
  * makes what it sees NaN.  slot_pos [n_seq][nkv][cap] or NULL: the new slots
- * get pos[b] + i.  With one token per sequence and last 1 this is what
- * styx_op_attn_decode_batch adds.  Allocates nothing. */
+ * get pos[b] + i.  n_rows * nh / nkv at most 2^28.  With one token per
+ * sequence and last 1 this is what styx_op_attn_decode_batch adds.  Allocates
+ * nothing. */
 int styx_op_kv_weigh(styx_gpu *gpu, const styx_kv_cache *kv, const styx_kv_chunk *chunk,
                      const int32_t *pos, int nh, int type_q, const void *q, int64_t ldq,
                      float scale, int window, const float *lse, int last, float decay,

@@ -117,6 +117,15 @@ def test_workspace_sizes():
         assert lib.styx_op_attn_chunk_ws_bytes(*args) == 0, args[1:]
 
 
+@pytest.mark.parametrize("nkv,gqa,n_seq", [(1, 1, 1), (1, 16, 1), (4, 8, 24), (2, 3, 1000), (8, 16, 200000)])
+def test_the_largest_attention_is_as_large_as_the_header_says(nkv, gqa, n_seq):
+    kv = C.byref(L.KvCache(L.F16, n_seq, nkv, 128, 16, 100, 20, None, None, None))
+    most = (2 ** 28 - 128 * nkv * (n_seq + 1)) // (nkv * gqa)
+    size = L.load().styx_op_attn_chunk_ws_bytes
+    assert size(kv, most, nkv * gqa) > 0
+    assert size(kv, most + 128 * (n_seq + 2), nkv * gqa) == 0
+
+
 def test_entry_points_refuse_a_null_gpu():
     lib = L.load()
     assert lib.styx_op_kv_plan(*[None] * 8, 0, *[None] * 5) == -1
