@@ -15,13 +15,14 @@
 //
 // Bound: the matrix cores, and for narrow heads the exponentials beside them.
 // 32 query heads over 4 kv heads of 128, f16, a prompt of 8192 tokens (550
-// GFLOP): 580 us, 950 of the 1146 TFLOP/s that a product of 8192^3 reaches.  The
-// clock is what holds it: 1.85 GHz under these products, and with q, K and V all
-// 0 the same launch takes 455 us.  f32 queries on f16 rows, 406 GFLOP in two
-// pieces: 458 us, 886 TFLOP/s.  f32, three documents, heads of 256, 211 GFLOP:
-// 1.75 ms, 121 of 152 TFLOP/s.  f16 heads of 64 under a window of 1024, 21 GFLOP:
-// 49 us; a score costs 256 FLOP there and its exponential, maximum, sum and
-// rounding more time than they.
+// GFLOP): 600 us, 915 of the 1146 TFLOP/s that a product of 8192^3 reaches.  Half
+// of a CU's cycles have a product under way, and the clock is at 1.77 to 1.85 GHz
+// under them: with q, K and V all 0 the same launch takes as many cycles, at up to
+// 2.4 GHz, and 450 us.  f32 queries on f16 rows, 406 GFLOP in two pieces: 473 us,
+// 860 TFLOP/s.  f32, three documents, heads of 256, 211 GFLOP: 1.75 ms, 121 of 152
+// TFLOP/s.  f16 heads of 64 under a window of 1024, 21 GFLOP: 50 us; a score costs
+// 256 FLOP there and its exponential, maximum, sum and rounding more time than
+// they, which explains about half of the distance to the products' 18.
 //
 // Why 32 rows a wave: their queries, sums and scores stay in 256 registers; 64
 // rows moved sums between register files in every block (1494 us).  Why four
@@ -117,9 +118,11 @@ template <typename TQ, int HD> struct Wave<TQ, _Float16, HD, 4> {
     using La = Lay<TC, HD>;
     static constexpr int NP = sizeof(TQ) == 4 ? 2 : 1;  // pieces
     // waves that share a query's dims, dims of a wave (f16 queries with heads of
-    // 256: with one, registers spill.  A prompt of 2048 tokens, 16 heads, 92 us,
-    // 118 with one; single tokens of 16 sequences over 4000 slots 33 and 45; four
-    // chunks of 256 tokens behind 8000 slots 231 and 214)
+    // 256: with one, registers spill; with two, both form all factors.  Neither
+    // wins everywhere.  16 heads, a prompt of 2048 tokens 95 us with two, 122 with
+    // one, single tokens of 16 sequences over 4000 slots 40 and 56; but a prompt of
+    // 4096 270 and 265, eight of 512 74 and 65, four chunks of 256 tokens behind
+    // 8000 slots 233 and 220)
     static constexpr int DS = HD == 256 ? 2 : 1, HW = HD / DS, NK = HW / 16, ND = HW / 32;
     static constexpr int KT = HD == 256 ? 32 : 64;
     static constexpr int NW = 4 * DS, PER_CU = 8 / NW, BM = 128;
@@ -371,7 +374,8 @@ constexpr int AC_TILE = 4;    // what a tile's start costs, in blocks (its rows 
 
 // A sequence's part of the line: tile t is first + t step long, in slots times
 // rows of a token.  (With a tile's start: of a prompt's many short first tiles a
-// share would else hold a dozen, 4096 tokens, head_dim 256: 351 us, 257 with.)
+// share would else hold a dozen.  4096 tokens, head_dim 256, with a wave to every
+// 32 rows: 351 us, 257 with.)
 struct SeqLine {
     int tiles, blocks;  // of the longest tile
     int64_t first, step;
@@ -940,6 +944,9 @@ static ChunkShape shape_of(int bm, int per_cu, int n_seq, int nkv, int gqa, int 
 // so many rows.  The fewer groups a tile has the more tiles there are, and the
 // more often a slot is read.  What a sequence has is known to the device alone:
 // the sequences' average counts, and a total that one sequence may have alone.
+// (Places of the batch that hold no sequence, or one that asks for nothing, count
+// among the sequences: in a large batch a single chunk of some hundred rows gets
+// smaller tiles than it would alone.)
 // One token for each of 24 over 2000 slots, heads of 128, 1 / 2 / 4 groups: 53 /
 // 72 / 82 us; 16 tokens of one over 500 17 / 20 / 22, 64 of one over 2000 44 / 43 /
 // 48, 128 of one 71 / 66 / 65; a prompt of 512 50 / 55 / 50, of 1024 124 / 119 /

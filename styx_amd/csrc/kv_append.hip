@@ -4,17 +4,23 @@
 //   x^ = x / sqrt(mean x^2 + eps) * w, then for each pair (a, b) of the first
 //   n_rot dims, (i, i + n_rot/2) or (2i, 2i+1), with (c, s) = table[pos][i]:
 //   a' = a c - b s, b' = a s + b c
-// in f64 to the end and rounded to f32 and then to the type, so that a cache
-// holds the same bits whatever the order of a sum.
+// in f64 to the end and rounded to f32 and then to the type.  Another order of
+// the f64 sums (the single-token operator's) gives the same bits but for the rare
+// value that lies at a rounding's border, which is a step of the type away.
 //
 // Bound: HBM, each value read once and written once.  A head is 16 bytes a lane;
 // a wave takes heads of one row, the next under way while one is turned, and
 // keeps the row's sines and cosines.  The partner of a dim is in the same lane
 // where pairs are neighbours, else it is read back from LDS (for a part of a
 // head it may lie anywhere).  A row's heads go to several workgroups where rows
-// are few: 48 tokens 5.6 us a call.  8192 f16 tokens of
-// 40 heads, 172 MB: 42 us in the kernel (4.1 TB/s), 53 where neither side is in
-// a cache; 4 parts of documents, f32 heads of 256, 125 MB: 27 and 30 us.
+// are few: 48 tokens 5.5 us a call.  8192 f16 tokens of
+// 40 heads, 172 MB: 41 us in the kernel (4.2 TB/s), 51 where neither side is in
+// a cache; 4 parts of documents, f32 heads of 256, 125 MB: 27 and 30 us.  A
+// workgroup lives for a row, whose position, angles and turn wait for one
+// another, so that few bytes are under way.  By types, 8192 tokens as above
+// under norms, all of each head turned: f32 to f16 69 us, to an f16 cache and
+// f32 queries 76, f16 to an f16 cache and f32 queries 120 (a lane then stores 32
+// bytes in two pieces, lines half by half); 56, 70 and 52 at a copy's rate.
 // Loads and stores are plain: with non-temporal loads the prompt takes 50 us from
 // memory, but 49 instead of 41 where the Infinity Cache holds what the product
 // before has just written, as it does in use.

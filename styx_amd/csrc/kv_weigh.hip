@@ -13,11 +13,15 @@
 //
 // Bound: products and exponentials, a score costing 256 FLOP and one exponential
 // at head_dim 128.  64 tokens of 32 f16 heads over 32768 slots, 17 GFLOP: 33 us,
-// where a tile's products and its factors take about the same time, one after
-// the other.  16 conversations, 16 tokens of 64 f32 heads each, 4.3 GFLOP: 63 us,
-// where products alone would take 28; 540 workgroups of equal length for 256
-// CUs, so that some CUs take three and most two.  Smaller workgroups even that
-// out, but each fetches all query rows (kw_waves).
+// 15 for the products; f32 queries on them 51, 30 for two pieces.  16
+// conversations, 16 tokens of 64 f32 heads each, 4.3 GFLOP: 63 us, 28 for the
+// products.  What is lost is waits: as built, each operand of a tile is read from
+// LDS right before the product that takes it (four products for f32), which waits
+// for it, in one chain of sums, and a tile's factors follow its products in the
+// same wave.  For the f32 batch 540 workgroups of equal length for 256 CUs, so
+// that some take three and most two, make 28 into 40.  Smaller workgroups even
+// that out, but each fetches all query rows (kw_waves).  One token for each of 24
+// sequences over 8192 f16 slots, 208 MB: 61 us, 45 at a copy's rate.
 #include <algorithm>
 #include <type_traits>
 
@@ -217,7 +221,9 @@ __global__ void __launch_bounds__(64 * kw_waves(sizeof(TC) == 2, HD), (KW_SIMD<T
         if (r0 < r1 && !few) {
             ask(r0);
             put(0, r0);
-            // (here, so that no trip waits for them, and with them for the next tile)
+            // (waited for here.  The loop as built counts these loads down once more
+            // before its products, as the branch past this one reaches it, too; what
+            // it then waits for with them, the next tile's rows, it stages next)
 #pragma unroll
             for (int i = 0; i < NK; i++) asm volatile("" : "+v"(k[i]));
             if (r0 + KW_ROWS < r1) ask(r0 + KW_ROWS);
